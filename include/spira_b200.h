@@ -496,6 +496,91 @@ int spira_b200_conv_ws_static(const void *feats, const void *weights, const void
                               int swap, int64_t num_sources, int64_t num_targets, int K, int c_in, int c_out, void *out,
                               int32_t *status, void *stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Expert feed-forward blocks over voxel rows: routing, row exchange, ragged products, norms with gate and residual.
+ * No reference counterpart (the reference stops at convolutions, BatchNorm and ReLU, spira/nn/).
+ * Element types of rows: */
+#define SPIRA_B200_F16 0
+#define SPIRA_B200_BF16 1
+#define SPIRA_B200_F32 2
+
+/* The k experts of every row of logits[n][experts] (rows `row_stride` elements apart): the k largest, ties to the lowest
+ * index, -inf never (chosen = -1, weight 0).  weights[n][k] fp32: softmax over the chosen (renormalize != 0) or over all
+ * experts.  slots[n][k]: place of every (row, j) in the order (expert, row, j), -1 where there is none; order[n * k]: the
+ * inverse, row * k + j of every place, -1 behind the last; offsets[experts + 1]: first place of every expert.
+ * experts <= 512, k <= min(experts, 32).  The result is a function of the logits alone (no dependence on scheduling).
+ * A NaN counts as the largest logit and makes the row's weights NaN. */
+int spira_b200_expert_route_workspace(int64_t n, int experts, int k, size_t *bytes);
+int spira_b200_expert_route(const void *logits, int dtype, int64_t n, int64_t row_stride, int experts, int k, int renormalize,
+                            float *weights, int32_t *chosen, int32_t *slots, int32_t *order, int32_t *offsets, void *workspace,
+                            size_t workspace_bytes, void *stream);
+/* dlogits[n][experts] (in the logits' type) from dweights (element (t, j) at t * dweights_row + j * dweights_col). */
+int spira_b200_expert_route_backward(const void *logits, int dtype, int64_t n, int64_t row_stride, int experts, int k,
+                                     int renormalize, const float *weights, const int32_t *chosen, const float *dweights,
+                                     int64_t dweights_row, int64_t dweights_col, void *dlogits, void *stream);
+
+/* rows[slots[t][j]] = x[t]; rows behind offsets[experts] are zero.  rows is [n * k][channels].  Places outside
+ * [0, n * k) are skipped, here and below. */
+int spira_b200_expert_dispatch(const void *x, int dtype, int64_t n, int64_t x_stride, int channels, const int32_t *slots, int k,
+                               const int32_t *offsets, int experts, void *rows, void *stream);
+/* out[t] = sum over j of weights[t][j] * rows[slots[t][j]] (fp32 sum in the order of j; weights == NULL: ones). */
+int spira_b200_expert_combine(const void *rows, int dtype, int64_t n, int64_t row_stride, int channels, const float *weights,
+                              int64_t weights_row, int64_t weights_col, const int32_t *slots, int k, void *out, void *stream);
+/* drows[slots[t][j]] = weights[t][j] * dout[t] (zero behind offsets[experts]), dweights[t][j] = <dout[t], rows[slots[t][j]]>;
+ * either may be NULL. */
+int spira_b200_expert_combine_backward(const void *rows, const void *dout, int dtype, int64_t n, int64_t row_stride,
+                                       int64_t dout_stride, int channels, const float *weights, int64_t weights_row,
+                                       int64_t weights_col, const int32_t *slots, int k, const int32_t *offsets, int experts,
+                                       void *drows, float *dweights, void *stream);
+
+/* Ragged products: group e holds the rows [offsets[e], offsets[e + 1]) of x[n][c_in] and has the matrix weight[e][c_in][c_out].
+ *   spira_b200_grouped_linear      y[r] = relu?(x[r] W[e] + bias[e]); rows outside every group are zero
+ *   spira_b200_grouped_linear_dz   dz = dy (y > 0) (dz may be NULL: no ReLU), dbias[e] = column sums of dz (may be NULL);
+ *                                  dz is written for the rows of groups only
+ *   spira_b200_grouped_linear_dx   dx[r] = dy[r] W[e]^T (pass dz as dy); rows outside every group are zero
+ *   spira_b200_grouped_linear_dw   dweight[e] = x_e^T dy_e (zero for an empty group)
+ * fp16 or bf16 in and out, fp32 sums, one rounding.  Offsets are read on the device; an entry counts as the largest of
+ * those before it and as n at most, so a bad list cannot reach outside the tensors.  x and dy have unit column stride and
+ * rows `x_stride` / `dy_stride` elements apart; everything else is dense. */
+typedef struct spira_b200_grouped_desc {
+  int32_t dtype, experts, c_in, c_out, relu, reserved;
+  int64_t n, x_stride, dy_stride;
+  const int32_t *offsets;
+  const void *x, *weight, *bias, *dy;
+  void *y, *dz, *dx, *dweight, *dbias;
+} spira_b200_grouped_desc;
+int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, int32_t *status, void *stream);
+int spira_b200_grouped_linear_dz_workspace(const spira_b200_grouped_desc *desc, size_t *bytes);
+int spira_b200_grouped_linear_dz(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
+int spira_b200_grouped_linear_dx(const spira_b200_grouped_desc *desc, int32_t *status, void *stream);
+int spira_b200_grouped_linear_dw_workspace(const spira_b200_grouped_desc *desc, size_t *bytes);
+int spira_b200_grouped_linear_dw(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status,
+                                 void *stream);
+
+/* Norms around a block, its gate and the residual, in one pass over the rows:
+ *   p = post ? norm(block) * post_weight + post_bias : block
+ *   stream = residual_scale * x + block_scale * gate * p          (block == NULL: the stream is x)
+ *   normed = norm(stream) * weight + bias                          (pre != 0)
+ * norm: v / sqrt(mean(v^2) + eps), or with `layer` != 0 (v - mean) / sqrt(var + eps); statistics in fp32 on unrounded
+ * values.  gate_kind: 0 none, 1 [channels] (a parameter), 2 [n][1], 3 [n][channels] (rows' type).  Parameters are all of
+ * the rows' type or all fp32 (`params_f32`); any of them may be NULL.  channels <= 8192.
+ * The backward call reads x, block, gate and `stats` ([n][4] fp32, written by the forward call where given) and the
+ * gradients dstream / dnormed (dstream may be NULL; dnormed only if pre == 0).  Gradients that are NULL are not computed;
+ * parameter gradients (dgate for gate_kind 1) have the parameters' type and need the workspace. */
+typedef struct spira_b200_norm_desc {
+  int32_t dtype, params_f32, channels, layer, pre, post, gate_kind, reserved;
+  float residual_scale, block_scale, eps, reserved_f;
+  int64_t n, x_stride, block_stride, gate_stride, dstream_stride, dnormed_stride;
+  const void *x, *block, *gate, *weight, *bias, *post_weight, *post_bias;
+  void *stream, *normed;
+  float *stats;
+  const void *dstream, *dnormed;
+  void *dx, *dblock, *dgate, *dweight, *dbias, *dpost_weight, *dpost_bias;
+} spira_b200_norm_desc;
+int spira_b200_residual_norm(const spira_b200_norm_desc *desc, void *stream);
+int spira_b200_residual_norm_backward_workspace(const spira_b200_norm_desc *desc, size_t *bytes);
+int spira_b200_residual_norm_backward(const spira_b200_norm_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -76,6 +76,28 @@ class TapeSlot(C.Structure):
     _fields_ = [("rows", c_int64), ("channels", c_int32), ("buffer", c_int32), ("ptr", c_void_p)]
 
 
+class GroupedDesc(C.Structure):
+    """Mirror of ``spira_b200_grouped_desc`` (include/spira_b200.h)."""
+    _fields_ = [("dtype", c_int32), ("experts", c_int32), ("c_in", c_int32), ("c_out", c_int32), ("relu", c_int32), ("reserved", c_int32),
+                ("n", c_int64), ("x_stride", c_int64), ("dy_stride", c_int64), ("offsets", c_void_p),
+                ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("dy", c_void_p),
+                ("y", c_void_p), ("dz", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p)]
+
+
+class NormDesc(C.Structure):
+    """Mirror of ``spira_b200_norm_desc`` (include/spira_b200.h)."""
+    _fields_ = [("dtype", c_int32), ("params_f32", c_int32), ("channels", c_int32), ("layer", c_int32), ("pre", c_int32), ("post", c_int32),
+                ("gate_kind", c_int32), ("reserved", c_int32),
+                ("residual_scale", C.c_float), ("block_scale", C.c_float), ("eps", C.c_float), ("reserved_f", C.c_float),
+                ("n", c_int64), ("x_stride", c_int64), ("block_stride", c_int64), ("gate_stride", c_int64), ("dstream_stride", c_int64),
+                ("dnormed_stride", c_int64),
+                ("x", c_void_p), ("block", c_void_p), ("gate", c_void_p), ("weight", c_void_p), ("bias", c_void_p),
+                ("post_weight", c_void_p), ("post_bias", c_void_p), ("stream", c_void_p), ("normed", c_void_p), ("stats", c_void_p),
+                ("dstream", c_void_p), ("dnormed", c_void_p), ("dx", c_void_p), ("dblock", c_void_p), ("dgate", c_void_p),
+                ("dweight", c_void_p), ("dbias", c_void_p), ("dpost_weight", c_void_p), ("dpost_bias", c_void_p)]
+
+
+F16, BF16, F32 = 0, 1, 2
 TAPE_CONV, TAPE_IDENTITY, TAPE_POINTWISE = 0, 1, 2
 LAYOUT_OS, LAYOUT_WS = 0, 1
 KERNEL_NAMES = {0: "conv_os_simt_kernel", 1: "conv_os_stem_kernel", 2: "conv_tc_kernel<OS>", 3: "conv_os_n256_kernel",
@@ -137,6 +159,24 @@ SIGNATURES = {
     "spira_b200_conv_ws_static": [c_void_p, c_void_p, c_void_p, C.POINTER(Epilogue), c_void_p, c_void_p, c_void_p, c_void_p,
                                   c_int, c_int64, c_int, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p,
                                   c_void_p],
+    "spira_b200_expert_route_workspace": [c_int64, c_int, c_int, C.POINTER(c_size_t)],
+    "spira_b200_expert_route": [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_size_t, c_void_p],
+    "spira_b200_expert_route_backward": [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64,
+                                         c_int64, c_void_p, c_void_p],
+    "spira_b200_expert_dispatch": [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p],
+    "spira_b200_expert_combine": [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p],
+    "spira_b200_expert_combine_backward": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
+                                           c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
+    "spira_b200_grouped_linear": [C.POINTER(GroupedDesc), c_void_p, c_void_p],
+    "spira_b200_grouped_linear_dz_workspace": [C.POINTER(GroupedDesc), C.POINTER(c_size_t)],
+    "spira_b200_grouped_linear_dz": [C.POINTER(GroupedDesc), c_void_p, c_size_t, c_void_p],
+    "spira_b200_grouped_linear_dx": [C.POINTER(GroupedDesc), c_void_p, c_void_p],
+    "spira_b200_grouped_linear_dw_workspace": [C.POINTER(GroupedDesc), C.POINTER(c_size_t)],
+    "spira_b200_grouped_linear_dw": [C.POINTER(GroupedDesc), c_void_p, c_size_t, c_void_p, c_void_p],
+    "spira_b200_residual_norm": [C.POINTER(NormDesc), c_void_p],
+    "spira_b200_residual_norm_backward_workspace": [C.POINTER(NormDesc), C.POINTER(c_size_t)],
+    "spira_b200_residual_norm_backward": [C.POINTER(NormDesc), c_void_p, c_size_t, c_void_p],
 }
 STATIC_SCRATCH_FLOATS = 4 * 1024 * 1024
 EXPORTS = sorted(list(SIGNATURES) + ["spira_b200_last_error"])
@@ -177,6 +217,9 @@ KERNELS_PER_CALL = {
     "spira_b200_kmap_masks": 1, "spira_b200_kmap_masks_half": 1, "spira_b200_kmap_lists_from_masks": 3, "spira_b200_convert_transposed_os": 1, "spira_b200_transpose_map": 1,
     "spira_b200_pack_weights": 1, "spira_b200_conv_os": 1, "spira_b200_conv_os_grouped": 1, "spira_b200_conv_os_split": 1,
     "spira_b200_kmap_group": 2,
+    "spira_b200_expert_route": 1, "spira_b200_expert_route_backward": 1, "spira_b200_expert_dispatch": 1, "spira_b200_expert_combine": 1,
+    "spira_b200_expert_combine_backward": 1, "spira_b200_grouped_linear": 1, "spira_b200_grouped_linear_dz": 1,
+    "spira_b200_grouped_linear_dx": 1, "spira_b200_grouped_linear_dw": 1, "spira_b200_residual_norm": 1, "spira_b200_residual_norm_backward": 1,
     "spira_b200_conv_ws": 2, "spira_b200_conv_ws_fused": 1, "spira_b200_conv_ws_static": 2,
 }
 launch_count = 0          # kernels launched through `call` since import (or since it was last reset by the caller)

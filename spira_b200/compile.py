@@ -68,6 +68,11 @@ class Recorder:
         o = self.slot(output._features, output._stride, create=True)
         self.ops.append(("cat", ins, o))
 
+    def call(self, fn, inputs, outputs):
+        """``outputs = fn(*inputs)`` on feature tensors, for functions of several tensors or with several results."""
+        ins = [self.slot(x._features) for x in inputs]
+        self.ops.append(("call", fn, ins, [self.slot(y._features, y._stride, create=True) for y in outputs]))
+
     def add(self, a: SparseTensor, b: SparseTensor, output: SparseTensor):
         o = self.slot(output._features, output._stride, create=True)
         self.ops.append(("add", self.slot(a._features), self.slot(b._features), o))
@@ -104,6 +109,8 @@ class CompiledModel:
                 self.ops.append((1,) + op[1:])
             elif op[0] == "cat":
                 self.ops.append((2,) + op[1:])
+            elif op[0] == "call":
+                self.ops.append((4,) + op[1:])
             else:
                 self.ops.append((3,) + op[1:])
 
@@ -195,6 +202,9 @@ class CompiledModel:
                 slots[op[5]] = op[1](slots[op[4]], *op[2], **op[3])
             elif kind == 2:
                 slots[op[2]] = torch.cat([slots[j] for j in op[1]], dim=1)
+            elif kind == 4:
+                for o, y in zip(op[3], op[1](*(slots[j] for j in op[2]))):
+                    slots[o] = y
             else:
                 slots[op[3]] = slots[op[1]] + slots[op[2]]
 

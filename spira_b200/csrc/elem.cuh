@@ -1,0 +1,54 @@
+// Element types of the row-wise operators (fp16, bf16, fp32): conversion, 16-byte vectors, dispatch on the type code.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "common.cuh"
+
+namespace sb {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N consecutive elements as one aligned access of N * sizeof(T) bytes.
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(const T *p, float (&f)[N]) {
+  const Vec<T, N> r = *reinterpret_cast<const Vec<T, N> *>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = to_f32(r.v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f32(T *p, const float (&f)[N]) {
+  Vec<T, N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(f[i]);
+  *reinterpret_cast<Vec<T, N> *>(p) = r;
+}
+
+inline int elem_size(int dtype) { return dtype == SPIRA_B200_F32 ? 4 : 2; }
+
+// Runs BODY with T = the element type of the code.
+#define SB_DISPATCH_ELEM(dtype, T, ...)                              \
+  [&]() -> int {                                                     \
+    if ((dtype) == SPIRA_B200_F16) { using T = __half; __VA_ARGS__ } \
+    if ((dtype) == SPIRA_B200_BF16) { using T = __nv_bfloat16; __VA_ARGS__ } \
+    using T = float; __VA_ARGS__                                     \
+  }()
+
+}  // namespace sb

@@ -1,0 +1,611 @@
+// Routing of rows to experts and moving them there and back.
+//
+//   route     the k experts of every row (the k largest logits), their weights, and the place of every (row, expert) pair
+//             in expert order: a stable counting sort by expert
+//   dispatch  rows[slots[t][j]] = x[t]
+//   combine   out[t] = sum_j weights[t][j] * rows[slots[t][j]]
+//
+// Every result is a function of the inputs alone: counts are integers, places follow from counts and ranks, sums run over
+// j in order.  All of it is bound by memory (or, for a few rows, by the launch).
+#include <cfloat>
+#include <cmath>
+
+#include "common.cuh"
+#include "elem.cuh"
+
+namespace sb {
+
+constexpr int kMaxExperts = 512;
+constexpr int kMaxTopK = 32;
+constexpr int kRouteThreads = 512;
+constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kSmallRouteEntries = 4096;   // (row, expert) pairs up to which one CTA does everything in one launch
+
+// Order of logits as unsigned numbers: -inf < ... < +inf < NaN, -0 = +0.  kGone (a number below every logit but equal to
+// nothing) marks what is masked (-inf) or chosen already.
+constexpr uint32_t kGone = 0;
+__device__ __forceinline__ uint32_t logit_key(float v) {
+  if (v != v) return 0xffffffffu;
+  if (v == -INFINITY) return kGone;
+  const uint32_t b = __float_as_uint(v + 0.f);   // -0 + 0 = +0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_logit(uint32_t k) {
+  if (k == 0xffffffffu) return NAN;
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// One row on G neighbouring lanes, EPL consecutive experts per lane (G * EPL >= experts).  Few lanes with many experts
+// each keep the number of shuffles small: at 64 experts and k = 4, 4 lanes x 16 experts execute a quarter of the
+// instructions of 32 lanes x 2.
+template <typename T, int G, int EPL>
+__device__ __forceinline__ void route_row(const T *logits, int64_t row_stride, bool vec_ok, int64_t row, bool live, int experts, int k,
+                                          int renormalize, float *weights, int32_t *chosen, int *hist) {
+  const int g = threadIdx.x & (G - 1);
+  uint32_t key[EPL];
+  float total = 0.f;
+  const T *src = logits + row * row_stride + g * EPL;
+  if constexpr (EPL * sizeof(T) >= 16) {
+    if (live && vec_ok && (g + 1) * EPL <= experts) {
+      constexpr int V = 16 / sizeof(T);
+#pragma unroll
+      for (int i = 0; i < EPL; i += V) {
+        float f[V];
+        load_f32<T, V>(src + i, f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) key[i + j] = logit_key(f[j]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) key[i] = live && g * EPL + i < experts ? logit_key(to_f32(src[i])) : kGone;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) key[i] = live && g * EPL + i < experts ? logit_key(to_f32(src[i])) : kGone;
+  }
+  float top = 0.f, sum = 0.f;
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = kGone;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (key[i] > best) { best = key[i]; at = i; }     // (strict: the lowest index of equal logits)
+    int e = g * EPL + at;
+#pragma unroll
+    for (int d = 1; d < G; d *= 2) {
+      const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, d, G);
+      const int oe = __shfl_xor_sync(0xffffffffu, e, d, G);
+      if (ob > best || (ob == best && oe < e)) { best = ob; e = oe; }
+    }
+    if (j == 0) {
+      top = best == kGone ? 0.f : key_logit(best);
+      if (!renormalize) {      // the softmax runs over all experts: while every logit is still there
+#pragma unroll
+        for (int i = 0; i < EPL; ++i)
+          if (key[i] != kGone) total += expf(key_logit(key[i]) - top);
+#pragma unroll
+        for (int d = 1; d < G; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d, G);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (g * EPL + i == e) key[i] = kGone;
+    const float score = best == kGone ? 0.f : expf(key_logit(best) - top);
+    sum += score;
+    if (live && g == 0) {
+      weights[row * k + j] = score;                    // divided below, once the sum is known
+      chosen[row * k + j] = best == kGone ? -1 : e;
+      if (best != kGone) atomicAdd(hist + e, 1);
+    }
+  }
+  if (live && g == 0) {
+    const float denom = renormalize ? sum : total;
+    for (int j = 0; j < k; ++j)
+      if (chosen[row * k + j] >= 0) weights[row * k + j] = weights[row * k + j] / denom;
+  }
+}
+
+template <typename T, int G, int EPL>
+__device__ __forceinline__ void route_rows(const T *logits, int64_t row_stride, int64_t r0, int64_t r1, int experts, int k, int renormalize,
+                                           float *weights, int32_t *chosen, int *hist) {
+  const bool vec_ok = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && row_stride * sizeof(T) % 16 == 0;
+  constexpr int kRows = kRouteThreads / G;
+  for (int64_t r = r0; r < r1; r += kRows) {
+    const int64_t row = r + threadIdx.x / G;
+    route_row<T, G, EPL>(logits, row_stride, vec_ok, row, row < r1, experts, k, renormalize, weights, chosen, hist);
+  }
+}
+
+// Places of the entries [n0, n1) (entry = row * k + j) of one CTA's rows: `base[e]` is the place of the CTA's first entry
+// of expert e.  Warps take consecutive pieces; a piece is ranked 32 entries at a time.
+__device__ __forceinline__ void place_entries(const int32_t *chosen, int64_t n0, int64_t n1, int experts, const int *base, int *warp_base,
+                                              int32_t *slots, int32_t *order) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t piece = ((n1 - n0 + kRouteWarps * 32 - 1) / (kRouteWarps * 32)) * 32;
+  const int64_t p0 = n0 + piece * warp < n1 ? n0 + piece * warp : n1, p1 = p0 + piece < n1 ? p0 + piece : n1;
+  int *mine = warp_base + warp * experts;
+  for (int e = lane; e < experts; e += 32) mine[e] = 0;
+  __syncwarp();
+  for (int64_t i = p0 + lane; i < p1; i += 32) {
+    const int e = chosen[i];
+    if (e >= 0) atomicAdd(mine + e, 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kRouteThreads) {
+    int at = base[e];
+    for (int w = 0; w < kRouteWarps; ++w) {
+      const int c = warp_base[w * experts + e];
+      warp_base[w * experts + e] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  for (int64_t i = p0; i < p1; i += 32) {
+    const bool in = i + lane < p1;
+    const int e = in ? chosen[i + lane] : -1;
+    const uint32_t peers = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(peers & ((1u << lane) - 1u));
+    int slot = -1;
+    if (e >= 0) slot = mine[e] + rank;
+    __syncwarp();
+    if (e >= 0 && rank == 0) mine[e] += __popc(peers);
+    __syncwarp();
+    if (in) {
+      slots[i + lane] = slot;
+      if (slot >= 0) order[slot] = static_cast<int32_t>(i + lane);
+    }
+  }
+}
+
+// Exclusive prefix of totals[0..experts) into first[0..experts] by one warp.
+__device__ __forceinline__ void scan_experts(const int *totals, int *first, int experts) {
+  const int lane = threadIdx.x & 31;
+  int run = 0;
+  for (int e0 = 0; e0 < experts; e0 += 32) {
+    int v = e0 + lane < experts ? totals[e0 + lane] : 0;
+    const int own = v;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += o;
+    }
+    if (e0 + lane < experts) first[e0 + lane] = run + v - own;
+    run += __shfl_sync(0xffffffffu, v, 31);
+  }
+  if (lane == 0) first[experts] = run;
+}
+
+struct RouteParams {
+  const void *logits;
+  int64_t n, row_stride, rows_per_cta;
+  int experts, k, renormalize;
+  float *weights;
+  int32_t *chosen, *slots, *order, *offsets;
+  int *block_hist;      // [CTAs][experts]
+};
+
+// Few rows: everything in one CTA and one launch.
+template <typename T, int G, int EPL>
+__global__ void __launch_bounds__(kRouteThreads) route_small_kernel(const RouteParams P) {
+  extern __shared__ int route_smem[];
+  int *hist = route_smem, *first = hist + P.experts, *warp_base = first + P.experts + 1;
+  pdl_trigger();
+  for (int e = threadIdx.x; e < P.experts; e += kRouteThreads) hist[e] = 0;
+  pdl_wait();
+  __syncthreads();
+  route_rows<T, G, EPL>(static_cast<const T *>(P.logits), P.row_stride, 0, P.n, P.experts, P.k, P.renormalize, P.weights, P.chosen, hist);
+  __syncthreads();
+  if (threadIdx.x < 32) scan_experts(hist, first, P.experts);
+  __syncthreads();
+  place_entries(P.chosen, 0, P.n * P.k, P.experts, first, warp_base, P.slots, P.order);
+  for (int e = threadIdx.x; e <= P.experts; e += kRouteThreads) P.offsets[e] = first[e];
+  for (int64_t i = first[P.experts] + threadIdx.x; i < P.n * P.k; i += kRouteThreads) P.order[i] = -1;
+}
+
+template <typename T, int G, int EPL>
+__global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteParams P) {
+  extern __shared__ int route_smem[];
+  pdl_trigger();
+  for (int e = threadIdx.x; e < P.experts; e += kRouteThreads) route_smem[e] = 0;
+  pdl_wait();
+  __syncthreads();
+  const int64_t r0 = blockIdx.x * P.rows_per_cta, r1 = r0 + P.rows_per_cta < P.n ? r0 + P.rows_per_cta : P.n;
+  route_rows<T, G, EPL>(static_cast<const T *>(P.logits), P.row_stride, r0, r1, P.experts, P.k, P.renormalize, P.weights, P.chosen, route_smem);
+  __syncthreads();
+  for (int e = threadIdx.x; e < P.experts; e += kRouteThreads) P.block_hist[static_cast<int64_t>(blockIdx.x) * P.experts + e] = route_smem[e];
+}
+
+// Every CTA adds up the histograms by itself (CTAs x experts numbers from L2) instead of waiting for a scan launch.
+__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteParams P) {
+  extern __shared__ int route_smem[];
+  int *totals = route_smem, *before = totals + P.experts, *first = before + P.experts, *warp_base = first + P.experts + 1;
+  pdl_trigger();
+  for (int e = threadIdx.x; e < P.experts; e += kRouteThreads) totals[e] = before[e] = 0;
+  pdl_wait();
+  __syncthreads();
+  const int G = gridDim.x;
+  // a thread keeps to one expert where it can: few shared-memory additions
+  const int lanes = P.experts < kRouteThreads ? kRouteThreads / P.experts : 1;
+  for (int e = threadIdx.x % P.experts, part = threadIdx.x / P.experts; part < lanes && e < P.experts; part += lanes) {
+    int all = 0, mine = 0;
+#pragma unroll 8
+    for (int b = part; b < G; b += lanes) {
+      const int c = P.block_hist[static_cast<int64_t>(b) * P.experts + e];
+      all += c;
+      if (b < static_cast<int>(blockIdx.x)) mine += c;
+    }
+    atomicAdd(totals + e, all);
+    atomicAdd(before + e, mine);
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) scan_experts(totals, first, P.experts);
+  __syncthreads();
+  for (int e = threadIdx.x; e < P.experts; e += kRouteThreads) before[e] += first[e];
+  __syncthreads();
+  const int64_t r0 = blockIdx.x * P.rows_per_cta, r1 = r0 + P.rows_per_cta < P.n ? r0 + P.rows_per_cta : P.n;
+  place_entries(P.chosen, r0 * P.k, r1 * P.k, P.experts, before, warp_base, P.slots, P.order);
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= P.experts; e += kRouteThreads) P.offsets[e] = first[e];
+  const int64_t total = P.n * P.k;
+  for (int64_t i = first[P.experts] + static_cast<int64_t>(blockIdx.x) * kRouteThreads + threadIdx.x; i < total;
+       i += static_cast<int64_t>(G) * kRouteThreads)
+    P.order[i] = -1;
+}
+
+// dlogits: with u_j = dweights of the chosen experts and dot = sum_j u_j w_j,
+//   softmax over the chosen:  d[e_j] = w_j (u_j - dot), 0 elsewhere
+//   softmax over all:         d[e] = p_e ([e chosen] u_e - dot),  p_e = exp(l_e - max) / sum
+template <typename T, int G>
+__global__ void __launch_bounds__(256) route_backward_kernel(const T *logits, int64_t n, int64_t row_stride, int experts, int k, int renormalize,
+                                                             const float *weights, const int32_t *chosen, const float *dweights,
+                                                             int64_t dw_row, int64_t dw_col, T *dlogits) {
+  pdl_trigger();
+  pdl_wait();
+  const int g = threadIdx.x & (G - 1);
+  constexpr int kRows = 256 / G;
+  const int64_t groups = (n + kRows - 1) / kRows;
+  for (int64_t b = blockIdx.x; b < groups; b += gridDim.x) {
+    const int64_t row = b * kRows + threadIdx.x / G;
+    const bool live = row < n;
+    float dot = 0.f;
+    if (live)
+      for (int j = 0; j < k; ++j)
+        if (chosen[row * k + j] >= 0) dot += dweights[row * dw_row + j * dw_col] * weights[row * k + j];
+    float top = -INFINITY, total = 0.f;
+    bool nan = false;
+    if (!renormalize) {
+      for (int e = g; live && e < experts; e += G) {
+        const float v = to_f32(logits[row * row_stride + e]);
+        nan |= v != v;
+        top = fmaxf(top, v);
+      }
+#pragma unroll
+      for (int d = 1; d < G; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d, G));
+      for (int e = g; live && e < experts; e += G) {
+        const float v = to_f32(logits[row * row_stride + e]);
+        if (v > -INFINITY) total += expf(v - top);
+      }
+      if (nan) total = NAN;
+#pragma unroll
+      for (int d = 1; d < G; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d, G);
+    }
+    for (int e = g; live && e < experts; e += G) {
+      float u = 0.f, w = 0.f;
+      for (int j = 0; j < k; ++j)
+        if (chosen[row * k + j] == e) { u = dweights[row * dw_row + j * dw_col]; w = weights[row * k + j]; }
+      float d;
+      if (renormalize) {
+        d = w == 0.f ? 0.f : w * (u - dot);
+      } else {
+        const float v = to_f32(logits[row * row_stride + e]);
+        const float p = v == -INFINITY ? 0.f : expf(v - top) / total;
+        d = v == -INFINITY ? 0.f : p * (u - dot);
+      }
+      dlogits[row * experts + e] = from_f32<T>(d);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ rows to experts and back
+// A thread moves V elements of one row; the threads of a row are neighbours, so reads and writes are whole lines whatever
+// order the places come in.  Row indices outside [0, rows) are skipped (they come from memory, not from the host).
+struct MoveParams {
+  const void *x, *y;
+  const float *weights;
+  const int32_t *slots, *offsets;
+  void *out;
+  float *dweights;
+  int64_t n, x_stride, y_stride, w_row, w_col;
+  int channels, k, experts;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void zero_tail(const MoveParams &P, T *rows, int vecs) {
+  const int64_t total = P.n * P.k;
+  int64_t tail = P.offsets[P.experts];
+  tail = tail < 0 ? 0 : tail > total ? total : tail;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * blockDim.x, work = (total - tail) * vecs;
+  const float zero[V] = {};
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < work; i += threads)
+    store_f32<T, V>(rows + (tail + i / vecs) * P.channels + (i % vecs) * V, zero);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256) dispatch_kernel(const MoveParams P) {
+  pdl_trigger();
+  pdl_wait();
+  const int vecs = P.channels / V;
+  const int64_t work = P.n * vecs, total = P.n * P.k;
+  T *rows = static_cast<T *>(P.out);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < work; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / vecs;
+    const int c = static_cast<int>(i - row * vecs) * V;
+    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.x) + row * P.x_stride + c);
+    for (int j = 0; j < P.k; ++j) {
+      const int64_t slot = P.slots[row * P.k + j];
+      if (slot >= 0 && slot < total) *reinterpret_cast<Vec<T, V> *>(rows + slot * P.channels + c) = v;
+    }
+  }
+  zero_tail<T, V>(P, rows, vecs);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256) combine_kernel(const MoveParams P) {
+  pdl_trigger();
+  pdl_wait();
+  const int vecs = P.channels / V;
+  const int64_t work = P.n * vecs, total = P.n * P.k;
+  const T *rows = static_cast<const T *>(P.y);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < work; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / vecs;
+    const int c = static_cast<int>(i - row * vecs) * V;
+    float acc[V] = {};
+    for (int j0 = 0; j0 < P.k; j0 += 4) {       // four rows on their way at a time
+      Vec<T, V> v[4];
+      float w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = 0.f;
+        const int64_t slot = j0 + j < P.k ? P.slots[row * P.k + j0 + j] : -1;
+        const bool there = slot >= 0 && slot < total;
+        if (there) {
+          w[j] = P.weights ? P.weights[row * P.w_row + (j0 + j) * P.w_col] : 1.f;
+          v[j] = *reinterpret_cast<const Vec<T, V> *>(rows + slot * P.y_stride + c);
+        } else {
+          v[j] = Vec<T, V>{};
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = fmaf(w[j], to_f32(v[j].v[e]), acc[e]);
+    }
+    store_f32<T, V>(static_cast<T *>(P.out) + row * P.channels + c, acc);
+  }
+}
+
+// drows[slot] = w dout[t], dweights[t][j] = <dout[t], rows[slot]>: G lanes per row of `dout`.
+template <typename T, int V, int G>
+__global__ void __launch_bounds__(256) combine_backward_kernel(const MoveParams P) {
+  pdl_trigger();
+  pdl_wait();
+  const int g = threadIdx.x & (G - 1);
+  const int vecs = P.channels / V;
+  constexpr int kRows = 256 / G;
+  const int64_t total = P.n * P.k, groups = (P.n + kRows - 1) / kRows;
+  const T *dout = static_cast<const T *>(P.x), *rows = static_cast<const T *>(P.y);
+  T *drows = static_cast<T *>(P.out);
+  for (int64_t b = blockIdx.x; b < groups; b += gridDim.x) {
+    const int64_t row = b * kRows + threadIdx.x / G;
+    const bool live = row < P.n;
+    for (int j = 0; j < P.k; ++j) {
+      const int64_t slot = live ? P.slots[row * P.k + j] : -1;
+      const bool there = slot >= 0 && slot < total;
+      float dot = 0.f;
+      if (there) {
+        const float w = P.weights ? P.weights[row * P.w_row + j * P.w_col] : 1.f;
+        for (int i = g; i < vecs; i += G) {
+          float d[V], y[V];
+          load_f32<T, V>(dout + row * P.x_stride + i * V, d);
+          if (P.dweights) {
+            load_f32<T, V>(rows + slot * P.y_stride + i * V, y);
+#pragma unroll
+            for (int e = 0; e < V; ++e) dot = fmaf(d[e], y[e], dot);
+          }
+          if (drows) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] *= w;
+            store_f32<T, V>(drows + slot * P.channels + i * V, d);
+          }
+        }
+      }
+      if (P.dweights) {
+#pragma unroll
+        for (int d = 1; d < G; d *= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d, G);
+        if (live && g == 0) P.dweights[row * P.k + j] = dot;
+      }
+    }
+  }
+  if (drows) zero_tail<T, V>(P, drows, vecs);
+}
+
+static unsigned capped_blocks(int64_t work, int per_cta, int ctas_per_sm) {
+  const int64_t want = div_up(work, per_cta), cap = static_cast<int64_t>(sm_count()) * ctas_per_sm;
+  return static_cast<unsigned>(want < 1 ? 1 : want < cap ? want : cap);
+}
+
+static int route_rows_per_cta(int64_t n, int64_t *rows_per_cta) {
+  const int64_t ctas = sm_count();
+  int64_t r = div_up(n, ctas);
+  r = div_up(r, 64) * 64;
+  *rows_per_cta = r;
+  return static_cast<int>(div_up(n, r));
+}
+
+static size_t place_smem(int experts) { return static_cast<size_t>(3 * experts + 1 + kRouteWarps * experts) * 4; }
+
+template <typename T, int G, int EPL>
+static int launch_route(RouteParams &P, cudaStream_t st) {
+  if (P.n * P.k <= kSmallRouteEntries) {
+    SB_CHECK_CUDA(launch_dependent(route_small_kernel<T, G, EPL>, dim3(1), dim3(kRouteThreads), place_smem(P.experts), st, P));
+    return SPIRA_B200_OK;
+  }
+  const int ctas = route_rows_per_cta(P.n, &P.rows_per_cta);
+  SB_CHECK_CUDA(launch_dependent(route_choose_kernel<T, G, EPL>, dim3(ctas), dim3(kRouteThreads), static_cast<size_t>(P.experts) * 4, st, P));
+  SB_CHECK_CUDA(launch_dependent(route_place_kernel, dim3(ctas), dim3(kRouteThreads), place_smem(P.experts), st, P));
+  return SPIRA_B200_OK;
+}
+
+template <typename T>
+static int launch_route_lanes(RouteParams &P, cudaStream_t st) {
+  if (P.experts <= 8) return launch_route<T, 2, 4>(P, st);
+  if (P.experts <= 16) return launch_route<T, 2, 8>(P, st);
+  if (P.experts <= 32) return launch_route<T, 4, 8>(P, st);
+  if (P.experts <= 64) return launch_route<T, 4, 16>(P, st);
+  if (P.experts <= 128) return launch_route<T, 8, 16>(P, st);
+  if (P.experts <= 256) return launch_route<T, 16, 16>(P, st);
+  return launch_route<T, 32, 16>(P, st);
+}
+
+static int check_route(const char *what, int dtype, int64_t n, int64_t row_stride, int experts, int k) {
+  SB_CHECK_ARG(dtype >= SPIRA_B200_F16 && dtype <= SPIRA_B200_F32, "%s: unknown element type %d", what, dtype);
+  SB_CHECK_ARG(experts >= 1 && experts <= kMaxExperts, "%s: experts=%d must be 1 to %d", what, experts, kMaxExperts);
+  SB_CHECK_ARG(k >= 1 && k <= kMaxTopK && k <= experts, "%s: top_k=%d must be 1 to min(experts, %d)", what, k, kMaxTopK);
+  SB_CHECK_ARG(n >= 0 && n * k < (int64_t(1) << 31), "%s: %lld rows x %d experts are out of range", what, (long long)n, k);
+  SB_CHECK_ARG(row_stride >= experts || n <= 1, "%s: row stride %lld is smaller than experts=%d", what, (long long)row_stride, experts);
+  return SPIRA_B200_OK;
+}
+
+static int check_move(const char *what, const MoveParams &P, int dtype, int64_t stride_a, int64_t stride_b) {
+  SB_CHECK_ARG(dtype >= SPIRA_B200_F16 && dtype <= SPIRA_B200_F32, "%s: unknown element type %d", what, dtype);
+  SB_CHECK_ARG(P.k >= 1 && P.k <= kMaxTopK, "%s: top_k=%d must be 1 to %d", what, P.k, kMaxTopK);
+  SB_CHECK_ARG(P.n >= 0 && P.n * P.k < (int64_t(1) << 31), "%s: %lld rows x %d experts are out of range", what, (long long)P.n, P.k);
+  SB_CHECK_ARG(P.channels >= 1 && P.channels <= (1 << 20), "%s: channels=%d out of range", what, P.channels);
+  SB_CHECK_ARG(stride_a >= 0 && stride_b >= 0, "%s: negative row stride", what);
+  return SPIRA_B200_OK;
+}
+
+// 16-byte accesses need every row of every tensor to start on a 16-byte boundary.
+static bool rows_aligned(const void *p, int64_t stride, int size) {
+  return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0);
+}
+
+template <typename T, int V>
+static int launch_combine_backward(const MoveParams &P, cudaStream_t st) {
+  const int vecs = P.channels / V;
+  const int lanes = vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
+  const unsigned blocks = capped_blocks(P.n * lanes, 256, 16);
+  if (lanes == 4) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 4>, dim3(blocks), dim3(256), 0, st, P));
+  else if (lanes == 8) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 8>, dim3(blocks), dim3(256), 0, st, P));
+  else if (lanes == 16) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 16>, dim3(blocks), dim3(256), 0, st, P));
+  else SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 32>, dim3(blocks), dim3(256), 0, st, P));
+  return SPIRA_B200_OK;
+}
+
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" int spira_b200_expert_route_workspace(int64_t n, int experts, int k, size_t *bytes) {
+  int rc = check_route("expert_route", SPIRA_B200_F32, n, experts, experts, k);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(bytes, "expert_route: null pointer");
+  int64_t rows;
+  *bytes = n * k <= kSmallRouteEntries ? 0 : static_cast<size_t>(route_rows_per_cta(n, &rows)) * experts * 4;
+  return SPIRA_B200_OK;
+}
+
+extern "C" int spira_b200_expert_route(const void *logits, int dtype, int64_t n, int64_t row_stride, int experts, int k, int renormalize,
+                                       float *weights, int32_t *chosen, int32_t *slots, int32_t *order, int32_t *offsets, void *workspace,
+                                       size_t workspace_bytes, void *stream) {
+  int rc = check_route("expert_route", dtype, n, row_stride, experts, k);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(offsets && (n == 0 || (logits && weights && chosen && slots && order)), "expert_route: null pointer");
+  size_t need = 0;
+  rc = spira_b200_expert_route_workspace(n, experts, k, &need);
+  if (rc != SPIRA_B200_OK) return rc;
+  if (workspace_bytes < need || (need && !workspace))
+    return fail(SPIRA_B200_ERR_WORKSPACE, "expert_route: workspace of %zu bytes is smaller than %zu", workspace_bytes, need);
+  RouteParams P{logits, n, row_stride, 0, experts, k, renormalize != 0, weights, chosen, slots, order, offsets, static_cast<int *>(workspace)};
+  return SB_DISPATCH_ELEM(dtype, T, return launch_route_lanes<T>(P, as_stream(stream)););
+}
+
+extern "C" int spira_b200_expert_route_backward(const void *logits, int dtype, int64_t n, int64_t row_stride, int experts, int k,
+                                                int renormalize, const float *weights, const int32_t *chosen, const float *dweights,
+                                                int64_t dweights_row, int64_t dweights_col, void *dlogits, void *stream) {
+  int rc = check_route("expert_route_backward", dtype, n, row_stride, experts, k);
+  if (rc != SPIRA_B200_OK || n == 0) return rc;
+  SB_CHECK_ARG(logits && weights && chosen && dweights && dlogits, "expert_route_backward: null pointer");
+  cudaStream_t st = as_stream(stream);
+  return SB_DISPATCH_ELEM(dtype, T, {
+    const T *l = static_cast<const T *>(logits);
+    T *d = static_cast<T *>(dlogits);
+    if (experts <= 16) {
+      SB_CHECK_CUDA(launch_dependent(route_backward_kernel<T, 8>, dim3(capped_blocks(n * 8, 256, 16)), dim3(256), 0, st, l, n, row_stride, experts, k,
+                                     renormalize != 0 ? 1 : 0, weights, chosen, dweights, dweights_row, dweights_col, d));
+    } else {
+      SB_CHECK_CUDA(launch_dependent(route_backward_kernel<T, 32>, dim3(capped_blocks(n * 32, 256, 16)), dim3(256), 0, st, l, n, row_stride, experts, k,
+                                     renormalize != 0 ? 1 : 0, weights, chosen, dweights, dweights_row, dweights_col, d));
+    }
+    return SPIRA_B200_OK;
+  });
+}
+
+extern "C" int spira_b200_expert_dispatch(const void *x, int dtype, int64_t n, int64_t x_stride, int channels, const int32_t *slots, int k,
+                                          const int32_t *offsets, int experts, void *rows, void *stream) {
+  MoveParams P{};
+  P.x = x; P.slots = slots; P.offsets = offsets; P.out = rows;
+  P.n = n; P.x_stride = x_stride; P.channels = channels; P.k = k; P.experts = experts;
+  int rc = check_move("expert_dispatch", P, dtype, x_stride, 0);
+  if (rc != SPIRA_B200_OK || n == 0) return rc;
+  SB_CHECK_ARG(x && slots && offsets && rows && experts >= 1, "expert_dispatch: null pointer");
+  const int size = elem_size(dtype);
+  const bool wide = channels * size % 16 == 0 && rows_aligned(x, x_stride, size) && rows_aligned(rows, channels, size);
+  cudaStream_t st = as_stream(stream);
+  return SB_DISPATCH_ELEM(dtype, T, {
+    constexpr int V = 16 / sizeof(T);
+    if (wide) SB_CHECK_CUDA(launch_dependent(dispatch_kernel<T, V>, dim3(capped_blocks(n * (channels / V), 256, 16)), dim3(256), 0, st, P));
+    else SB_CHECK_CUDA(launch_dependent(dispatch_kernel<T, 1>, dim3(capped_blocks(n * channels, 256, 16)), dim3(256), 0, st, P));
+    return SPIRA_B200_OK;
+  });
+}
+
+extern "C" int spira_b200_expert_combine(const void *rows, int dtype, int64_t n, int64_t row_stride, int channels, const float *weights,
+                                         int64_t weights_row, int64_t weights_col, const int32_t *slots, int k, void *out, void *stream) {
+  MoveParams P{};
+  P.y = rows; P.weights = weights; P.slots = slots; P.out = out; P.w_row = weights_row; P.w_col = weights_col;
+  P.n = n; P.y_stride = row_stride; P.channels = channels; P.k = k;
+  int rc = check_move("expert_combine", P, dtype, row_stride, 0);
+  if (rc != SPIRA_B200_OK || n == 0) return rc;
+  SB_CHECK_ARG(rows && slots && out, "expert_combine: null pointer");
+  const int size = elem_size(dtype);
+  const bool wide = channels * size % 16 == 0 && rows_aligned(rows, row_stride, size) && rows_aligned(out, channels, size);
+  cudaStream_t st = as_stream(stream);
+  return SB_DISPATCH_ELEM(dtype, T, {
+    constexpr int V = 16 / sizeof(T);
+    if (wide) SB_CHECK_CUDA(launch_dependent(combine_kernel<T, V>, dim3(capped_blocks(n * (channels / V), 256, 16)), dim3(256), 0, st, P));
+    else SB_CHECK_CUDA(launch_dependent(combine_kernel<T, 1>, dim3(capped_blocks(n * channels, 256, 16)), dim3(256), 0, st, P));
+    return SPIRA_B200_OK;
+  });
+}
+
+extern "C" int spira_b200_expert_combine_backward(const void *rows, const void *dout, int dtype, int64_t n, int64_t row_stride, int64_t dout_stride,
+                                                  int channels, const float *weights, int64_t weights_row, int64_t weights_col,
+                                                  const int32_t *slots, int k, const int32_t *offsets, int experts, void *drows,
+                                                  float *dweights, void *stream) {
+  MoveParams P{};
+  P.x = dout; P.y = rows; P.weights = weights; P.slots = slots; P.offsets = offsets; P.out = drows; P.dweights = dweights;
+  P.n = n; P.x_stride = dout_stride; P.y_stride = row_stride; P.w_row = weights_row; P.w_col = weights_col;
+  P.channels = channels; P.k = k; P.experts = experts;
+  int rc = check_move("expert_combine_backward", P, dtype, row_stride, dout_stride);
+  if (rc != SPIRA_B200_OK || n == 0) return rc;
+  SB_CHECK_ARG(dout && slots && offsets && experts >= 1 && (rows || !dweights) && (drows || dweights), "expert_combine_backward: null pointer");
+  const int size = elem_size(dtype);
+  const bool wide = channels * size % 16 == 0 && rows_aligned(rows, row_stride, size) && rows_aligned(dout, dout_stride, size) &&
+                    rows_aligned(drows, channels, size);
+  cudaStream_t st = as_stream(stream);
+  return SB_DISPATCH_ELEM(dtype, T, {
+    if (wide) return launch_combine_backward<T, 16 / static_cast<int>(sizeof(T))>(P, st);
+    return launch_combine_backward<T, 1>(P, st);
+  });
+}

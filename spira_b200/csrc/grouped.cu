@@ -1,0 +1,391 @@
+// Ragged products of grouped rows with one weight matrix per group (the experts of a mixture):
+//
+//   y[r]  = relu?(x[r] W[e] + b[e])      rows r of group e
+//   dz    = dy (y > 0)                    db[e] = sum over the group's rows of dz
+//   dx[r] = dz[r] W[e]^T                  dW[e] = x_e^T dz_e
+//
+// Rows outside every group are zero in y and dx.  Group boundaries are read on the device; the host only knows upper
+// bounds of the tile counts.  Sums over a group's rows are split into pieces that are added in a fixed order.
+//
+// `grouped_any_kernel` takes every channel count, stride and alignment: 64 x 64 tiles, element-wise loads into shared
+// memory, warp-level MMAs with fp32 accumulation.
+#include "common.cuh"
+#include "elem.cuh"
+#include "grouped.cuh"
+
+namespace sb {
+
+constexpr int kATile = 64, kAK = 32, kALd = kAK + 8;     // (row stride of 80 bytes: conflict-free fragment loads)
+constexpr int kAThreads = 128;
+constexpr int kForward = 0, kDx = 1, kDw = 2;
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+struct GroupedParams {
+  const void *a, *b, *bias;       // forward: x, W; dx: dz, W; dW: x, dz
+  const int32_t *offsets;
+  void *out;
+  float *partial;                 // dW with several pieces per group: [pieces][c_in][c_out]
+  int64_t a_stride, b_stride;
+  int n, experts, c_in, c_out, relu, piece;
+};
+
+template <typename T>
+__device__ __forceinline__ void zero_outside(T *out, int channels, int n, const int32_t *offsets, int experts) {
+  int first, last;
+  group_span(offsets, experts, n, first, last);
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * gridDim.y * blockDim.x;
+  const int64_t me = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x;
+  for (int64_t i = me; i < static_cast<int64_t>(first) * channels; i += threads) out[i] = from_f32<T>(0.f);
+  for (int64_t i = static_cast<int64_t>(last) * channels + me; i < static_cast<int64_t>(n) * channels; i += threads) out[i] = from_f32<T>(0.f);
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kAThreads) grouped_any_kernel(const __grid_constant__ GroupedParams P) {
+  __shared__ __align__(16) T sa[kATile * kALd], sb_[kATile * kALd];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (MODE != kDw) zero_outside(static_cast<T *>(P.out), MODE == kForward ? P.c_out : P.c_in, P.n, P.offsets, P.experts);
+  int expert, m0, n0, m_end, n_end, k_begin, k_end;
+  int64_t unit = 0;
+  if (MODE == kDw) {
+    // one piece of one group's rows, one tile of the weight matrix (piece == 0: the whole group)
+    if (P.piece == 0) {
+      expert = blockIdx.x;
+      int lo = clamped_offset(P.offsets, 0, P.n), hi = lo;
+      for (int e = 1; e <= expert + 1; ++e) {
+        if (e == expert + 1) lo = hi;
+        const int v = clamped_offset(P.offsets, e, P.n);
+        hi = v > hi ? v : hi;
+      }
+      k_begin = lo;
+      k_end = hi;
+    } else {
+      const GroupTile t = find_group_tile(P.offsets, P.experts, P.n, P.piece, blockIdx.x);
+      if (t.expert < 0) return;
+      expert = t.expert;
+      unit = blockIdx.x;
+      k_begin = t.begin + t.index * P.piece;
+      k_end = k_begin + P.piece < t.end ? k_begin + P.piece : t.end;
+    }
+    const int m_tiles = (P.c_in + kATile - 1) / kATile;
+    m0 = static_cast<int>(blockIdx.y) % m_tiles * kATile;
+    n0 = static_cast<int>(blockIdx.y) / m_tiles * kATile;
+    m_end = P.c_in;
+    n_end = P.c_out;
+  } else {
+    const GroupTile t = find_group_tile(P.offsets, P.experts, P.n, kATile, blockIdx.x);
+    if (t.expert < 0) return;
+    expert = t.expert;
+    m0 = t.begin + t.index * kATile;
+    m_end = t.end;
+    n0 = blockIdx.y * kATile;
+    n_end = MODE == kForward ? P.c_out : P.c_in;
+    k_begin = 0;
+    k_end = MODE == kForward ? P.c_in : P.c_out;
+  }
+  const T zero = from_f32<T>(0.f);
+  const T *A = static_cast<const T *>(P.a);
+  const T *B = static_cast<const T *>(P.b);
+  if (MODE != kDw) B += static_cast<int64_t>(expert) * P.c_in * P.c_out;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
+  float acc[2][4][4] = {};
+  for (int k0 = k_begin; k0 < k_end; k0 += kAK) {
+    // neighbouring threads follow the direction in which the source is contiguous
+    for (int i = tid; i < kATile * kAK; i += kAThreads) {
+      const int m = MODE == kDw ? i % kATile : i / kAK, k = MODE == kDw ? i / kATile : i % kAK;
+      T v = zero;
+      if (m0 + m < m_end && k0 + k < k_end)
+        v = MODE == kDw ? A[static_cast<int64_t>(k0 + k) * P.a_stride + m0 + m] : A[static_cast<int64_t>(m0 + m) * P.a_stride + k0 + k];
+      sa[m * kALd + k] = v;
+    }
+    for (int i = tid; i < kATile * kAK; i += kAThreads) {
+      const int n = MODE == kDx ? i / kAK : i % kATile, k = MODE == kDx ? i % kAK : i / kATile;
+      T v = zero;
+      if (n0 + n < n_end && k0 + k < k_end) {
+        if (MODE == kForward) v = B[static_cast<int64_t>(k0 + k) * P.c_out + n0 + n];
+        else if (MODE == kDx) v = B[static_cast<int64_t>(n0 + n) * P.c_out + k0 + k];
+        else v = B[static_cast<int64_t>(k0 + k) * P.b_stride + n0 + n];
+      }
+      sb_[n * kALd + k] = v;
+    }
+    __syncthreads();
+    const uint32_t *a32 = reinterpret_cast<const uint32_t *>(sa), *b32 = reinterpret_cast<const uint32_t *>(sb_);
+#pragma unroll
+    for (int ks = 0; ks < kAK / 16; ++ks) {
+      uint32_t a[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t *p = a32 + (wm + 16 * i + g) * (kALd / 2) + ks * 8 + t4;
+        a[i][0] = p[0];
+        a[i][1] = p[8 * (kALd / 2)];
+        a[i][2] = p[4];
+        a[i][3] = p[8 * (kALd / 2) + 4];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t *p = b32 + (wn + 8 * j + g) * (kALd / 2) + ks * 8 + t4;
+        const uint32_t b0 = p[0], b1 = p[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) mma_16816<T>(acc[i][j], a[i], b0, b1);
+      }
+    }
+    __syncthreads();
+  }
+  T *out = static_cast<T *>(P.out);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int m = m0 + wm + 16 * i + g + 8 * (q >> 1), n = n0 + wn + 8 * j + 2 * t4 + (q & 1);
+        if (m >= m_end || n >= n_end) continue;
+        float v = acc[i][j][q];
+        if (MODE == kForward) {
+          if (P.bias) v += to_f32(static_cast<const T *>(P.bias)[static_cast<int64_t>(expert) * P.c_out + n]);
+          if (P.relu) v = v < 0.f ? 0.f : v;          // (a NaN stays)
+          out[static_cast<int64_t>(m) * P.c_out + n] = from_f32<T>(v);
+        } else if (MODE == kDx) {
+          out[static_cast<int64_t>(m) * P.c_in + n] = from_f32<T>(v);
+        } else if (P.piece == 0) {
+          out[(static_cast<int64_t>(expert) * P.c_in + m) * P.c_out + n] = from_f32<T>(v);
+        } else {
+          P.partial[(unit * P.c_in + m) * P.c_out + n] = v;
+        }
+      }
+}
+
+// out[e][i] = sum over the pieces of group e, in order, of partial[piece][i]
+template <typename T>
+__global__ void __launch_bounds__(256) grouped_sum_kernel(const float *partial, const int32_t *offsets, int n, int experts, int piece, int64_t size, T *out) {
+  __shared__ int span[2];
+  pdl_trigger();
+  pdl_wait();
+  const int e = blockIdx.y;
+  if (threadIdx.x == 0) {
+    int hi = clamped_offset(offsets, 0, n), first = 0, mine = 0;
+    for (int i = 0; i <= e; ++i) {
+      const int lo = hi, v = clamped_offset(offsets, i + 1, n);
+      hi = v > hi ? v : hi;
+      first += mine;
+      mine = (hi - lo + piece - 1) / piece;
+    }
+    span[0] = first;
+    span[1] = mine;
+  }
+  __syncthreads();
+  const int64_t first = span[0];
+  const int count = span[1];
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < size; i += static_cast<int64_t>(gridDim.x) * 256) {
+    float t = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < count; ++p) t += partial[(first + p) * size + i];
+    out[e * size + i] = from_f32<T>(t);
+  }
+}
+
+// dz = dy (y > 0) where a ReLU followed (dz != NULL), and partial column sums over pieces of a group's rows.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) grouped_dz_kernel(const T *dy, int64_t dy_stride, const T *y, T *dz, float *partial, const int32_t *offsets,
+                                                         int n, int experts, int c_out, int piece) {
+  __shared__ float sums[256 * V];
+  pdl_trigger();
+  pdl_wait();
+  const GroupTile t = find_group_tile(offsets, experts, n, piece, blockIdx.x);
+  if (t.expert < 0) return;
+  const int r0 = t.begin + t.index * piece, r1 = r0 + piece < t.end ? r0 + piece : t.end;
+  const int vecs = c_out / V, wide = vecs - static_cast<int>(blockIdx.y) * 256 < 256 ? vecs - static_cast<int>(blockIdx.y) * 256 : 256;
+  const int lanes = 256 / wide;                 // rows in parallel
+  const int lane = threadIdx.x / wide, c = (blockIdx.y * 256 + threadIdx.x % wide) * V;
+  float sum[V] = {};
+  if (lane < lanes)
+    for (int r = r0 + lane; r < r1; r += lanes) {
+      float d[V];
+      load_f32<T, V>(dy + r * dy_stride + c, d);
+      if (dz) {
+        float f[V];
+        load_f32<T, V>(y + static_cast<int64_t>(r) * c_out + c, f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[i] = f[i] > 0.f ? d[i] : 0.f;
+        store_f32<T, V>(dz + static_cast<int64_t>(r) * c_out + c, d);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] += d[i];
+    }
+  if (partial == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sums[threadIdx.x * V + i] = sum[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < wide * V; i += 256) {
+    float s = 0.f;
+    for (int l = 0; l < lanes; ++l) s += sums[(l * wide) * V + i];
+    partial[static_cast<int64_t>(blockIdx.x) * c_out + blockIdx.y * 256 * V + i] = s;
+  }
+}
+
+constexpr int kDzPiece = 256;
+
+static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Rows of a group that one CTA of the weight gradient adds up (0: all of them).  Splitting fills the SMs when the weight
+// matrices have few tiles, at the price of fp32 partial sums: about two CTAs per SM, at least 256 rows each.
+static int dw_piece(int64_t n, int experts, int64_t tiles) {
+  if (tiles * experts >= sm_count() || n <= 256) return 0;
+  const int64_t pieces = div_up(2 * static_cast<int64_t>(sm_count()), tiles);
+  int64_t piece = div_up(div_up(n, pieces), 64) * 64;
+  if (piece < 256) piece = 256;
+  return piece >= n ? 0 : static_cast<int>(piece);
+}
+
+static int64_t any_tiles(int c_in, int c_out) { return div_up(c_in, kATile) * div_up(c_out, kATile); }
+
+static int grouped_check(const char *what, const spira_b200_grouped_desc *D) {
+  SB_CHECK_ARG(D, "%s: null descriptor", what);
+  SB_CHECK_ARG(D->dtype == SPIRA_B200_F16 || D->dtype == SPIRA_B200_BF16, "%s: element type %d is neither fp16 nor bf16", what, D->dtype);
+  SB_CHECK_ARG(D->n >= 0 && D->n < (int64_t(1) << 31) - 4096, "%s: n=%lld out of range", what, (long long)D->n);
+  SB_CHECK_ARG(D->experts >= 1 && D->experts <= kMaxGroups, "%s: experts=%d must be 1 to %d", what, D->experts, kMaxGroups);
+  SB_CHECK_ARG(D->c_in >= 1 && D->c_in <= 65536 && D->c_out >= 1 && D->c_out <= 65536, "%s: channels %d -> %d out of range", what, D->c_in, D->c_out);
+  SB_CHECK_ARG(D->x_stride >= 0 && D->dy_stride >= 0, "%s: negative row stride", what);
+  SB_CHECK_ARG(D->n == 0 || D->offsets, "%s: null pointer", what);
+  return SPIRA_B200_OK;
+}
+
+template <typename T, int MODE>
+static int launch_any(const GroupedParams &P, cudaStream_t st) {
+  const int64_t units = MODE == kDw ? (P.piece ? group_tiles_bound(P.n, P.experts, P.piece) : P.experts) : group_tiles_bound(P.n, P.experts, kATile);
+  const int64_t columns = MODE == kForward ? div_up(P.c_out, kATile) : MODE == kDx ? div_up(P.c_in, kATile) : any_tiles(P.c_in, P.c_out);
+  SB_CHECK_ARG(columns < 65536 && units < (int64_t(1) << 31), "grouped_linear: too many tiles");
+  SB_CHECK_CUDA(launch_dependent(grouped_any_kernel<T, MODE>, dim3(static_cast<unsigned>(units < 1 ? 1 : units), static_cast<unsigned>(columns)),
+                                 dim3(kAThreads), 0, st, P));
+  return SPIRA_B200_OK;
+}
+
+}  // namespace sb
+
+using namespace sb;
+
+#define SB_DISPATCH_HALF(dtype, T, ...)                              \
+  [&]() -> int {                                                     \
+    if ((dtype) == SPIRA_B200_F16) { using T = __half; __VA_ARGS__ } \
+    using T = __nv_bfloat16; __VA_ARGS__                             \
+  }()
+
+extern "C" int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, int32_t *status, void *stream) {
+  int rc = grouped_check("grouped_linear", desc);
+  if (rc != SPIRA_B200_OK || desc->n == 0) return rc;
+  const spira_b200_grouped_desc &D = *desc;
+  SB_CHECK_ARG(D.x && D.weight && D.y, "grouped_linear: null pointer");
+  GroupedParams P{D.x, D.weight, D.bias, D.offsets, D.y, nullptr, D.x_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, D.relu, 0};
+  return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kForward>(P, as_stream(stream))););
+}
+
+extern "C" int spira_b200_grouped_linear_dx(const spira_b200_grouped_desc *desc, int32_t *status, void *stream) {
+  int rc = grouped_check("grouped_linear_dx", desc);
+  if (rc != SPIRA_B200_OK || desc->n == 0) return rc;
+  const spira_b200_grouped_desc &D = *desc;
+  SB_CHECK_ARG(D.dy && D.weight && D.dx, "grouped_linear_dx: null pointer");
+  GroupedParams P{D.dy, D.weight, nullptr, D.offsets, D.dx, nullptr, D.dy_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, 0, 0};
+  return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kDx>(P, as_stream(stream))););
+}
+
+extern "C" int spira_b200_grouped_linear_dw_workspace(const spira_b200_grouped_desc *desc, size_t *bytes) {
+  int rc = grouped_check("grouped_linear_dw", desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(bytes, "grouped_linear_dw: null pointer");
+  const int piece = dw_piece(desc->n, desc->experts, any_tiles(desc->c_in, desc->c_out));
+  *bytes = piece ? static_cast<size_t>(group_tiles_bound(desc->n, desc->experts, piece)) * desc->c_in * desc->c_out * 4 : 0;
+  return SPIRA_B200_OK;
+}
+
+extern "C" int spira_b200_grouped_linear_dw(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
+  int rc = grouped_check("grouped_linear_dw", desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  const spira_b200_grouped_desc &D = *desc;
+  SB_CHECK_ARG(D.dweight, "grouped_linear_dw: null pointer");
+  cudaStream_t st = as_stream(stream);
+  const int64_t size = static_cast<int64_t>(D.c_in) * D.c_out;
+  if (D.n == 0) {
+    SB_CHECK_CUDA(cudaMemsetAsync(D.dweight, 0, static_cast<size_t>(D.experts) * size * 2, st));
+    return SPIRA_B200_OK;
+  }
+  SB_CHECK_ARG(D.x && D.dy, "grouped_linear_dw: null pointer");
+  size_t need = 0;
+  rc = spira_b200_grouped_linear_dw_workspace(desc, &need);
+  if (rc != SPIRA_B200_OK) return rc;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SPIRA_B200_ERR_WORKSPACE, "grouped_linear_dw: workspace of %zu bytes is smaller than %zu", workspace_bytes, need);
+  const int piece = dw_piece(D.n, D.experts, any_tiles(D.c_in, D.c_out));
+  GroupedParams P{D.x, D.dy, nullptr, D.offsets, D.dweight, static_cast<float *>(workspace), D.x_stride, D.dy_stride, static_cast<int>(D.n), D.experts,
+                  D.c_in, D.c_out, 0, piece};
+  return SB_DISPATCH_HALF(D.dtype, T, {
+    rc = launch_any<T, kDw>(P, st);
+    if (rc != SPIRA_B200_OK || piece == 0) return rc;
+    const unsigned blocks = static_cast<unsigned>(div_up(size, 256) < 1024 ? div_up(size, 256) : 1024);
+    SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(blocks, D.experts), dim3(256), 0, st, static_cast<const float *>(workspace), D.offsets,
+                                   static_cast<int>(D.n), D.experts, piece, size, static_cast<T *>(D.dweight)));
+    return SPIRA_B200_OK;
+  });
+}
+
+extern "C" int spira_b200_grouped_linear_dz_workspace(const spira_b200_grouped_desc *desc, size_t *bytes) {
+  int rc = grouped_check("grouped_linear_dz", desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(bytes, "grouped_linear_dz: null pointer");
+  *bytes = desc->dbias ? static_cast<size_t>(group_tiles_bound(desc->n, desc->experts, kDzPiece)) * desc->c_out * 4 : 0;
+  return SPIRA_B200_OK;
+}
+
+extern "C" int spira_b200_grouped_linear_dz(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, void *stream) {
+  int rc = grouped_check("grouped_linear_dz", desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  const spira_b200_grouped_desc &D = *desc;
+  SB_CHECK_ARG(D.dz || D.dbias, "grouped_linear_dz: null pointer");
+  cudaStream_t st = as_stream(stream);
+  if (D.n == 0) {
+    if (D.dbias) SB_CHECK_CUDA(cudaMemsetAsync(D.dbias, 0, static_cast<size_t>(D.experts) * D.c_out * 2, st));
+    return SPIRA_B200_OK;
+  }
+  SB_CHECK_ARG(D.dy && (!D.dz || D.y), "grouped_linear_dz: null pointer");
+  size_t need = 0;
+  rc = spira_b200_grouped_linear_dz_workspace(desc, &need);
+  if (rc != SPIRA_B200_OK) return rc;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SPIRA_B200_ERR_WORKSPACE, "grouped_linear_dz: workspace of %zu bytes is smaller than %zu", workspace_bytes, need);
+  float *partial = D.dbias ? static_cast<float *>(workspace) : nullptr;
+  const int n = static_cast<int>(D.n);
+  const unsigned units = static_cast<unsigned>(group_tiles_bound(n, D.experts, kDzPiece));
+  const bool wide = D.c_out % 8 == 0 && aligned16(D.dy) && D.dy_stride % 8 == 0 && aligned16(D.y) && aligned16(D.dz);
+  return SB_DISPATCH_HALF(D.dtype, T, {
+    const T *dy = static_cast<const T *>(D.dy);
+    const T *y = static_cast<const T *>(D.y);
+    T *dz = static_cast<T *>(D.dz);
+    if (wide) {
+      SB_CHECK_CUDA(launch_dependent(grouped_dz_kernel<T, 8>, dim3(units, static_cast<unsigned>(div_up(D.c_out / 8, 256))), dim3(256), 0, st, dy, D.dy_stride,
+                                     y, dz, partial, D.offsets, n, D.experts, D.c_out, kDzPiece));
+    } else {
+      SB_CHECK_CUDA(launch_dependent(grouped_dz_kernel<T, 1>, dim3(units, static_cast<unsigned>(div_up(D.c_out, 256))), dim3(256), 0, st, dy, D.dy_stride, y,
+                                     dz, partial, D.offsets, n, D.experts, D.c_out, kDzPiece));
+    }
+    if (!D.dbias) return SPIRA_B200_OK;
+    SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 256)), D.experts), dim3(256), 0, st,
+                                   static_cast<const float *>(partial), D.offsets, n, D.experts, kDzPiece, static_cast<int64_t>(D.c_out),
+                                   static_cast<T *>(D.dbias)));
+    return SPIRA_B200_OK;
+  });
+}

@@ -1,4 +1,5 @@
 from .conv import *
 from .activations import *
 from .normalizations import *
+from .experts import *
 from . import functional

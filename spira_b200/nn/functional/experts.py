@@ -1,0 +1,355 @@
+"""Expert feed-forward blocks over voxel rows: routing, row exchange and ragged products, with their gradients.
+
+    routing = expert_route(logits, top_k)                      # logits [N, E]
+    rows = expert_dispatch(feats, routing)                     # [N * top_k, C], in expert order
+    rows = grouped_linear(rows, weights, routing.offsets)      # weights [E, C, C_out]
+    feats = expert_combine(rows, routing)                      # [N, C_out]
+
+No reference counterpart (the reference stops at convolutions, BatchNorm and ReLU).  All calls run on the current stream
+of their tensors' device, never synchronise, and may be captured into a CUDA graph.  Results do not depend on scheduling:
+the same inputs give the same bits.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from spira_b200 import _lib
+from spira_b200.nn.functional import _C
+from spira_b200._lib import GroupedDesc
+
+__all__ = ["ExpertRouting", "expert_route", "expert_dispatch", "expert_combine", "grouped_linear"]
+
+MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 512, 32, 1024
+_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _launch(index: int, name: str, *args) -> None:
+    """One library call whose last argument is the current stream of device ``index``."""
+    if index == _current_device():
+        _lib.call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _raw_stream(index))
+
+
+def _fail(message: str):
+    raise RuntimeError("[spira_b200] " + message)
+
+
+def _device_of(*tensors) -> int:
+    """The device index all given tensors share; refuses CPU tensors and mixtures."""
+    index = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise NotImplementedError("spira_b200 runs on CUDA tensors only")
+        if index is None:
+            index = t.device.index
+        elif t.device.index != index:
+            _fail("tensors on different devices")
+    return index
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself if its columns are neighbours (rows may lie any distance apart), else a dense copy."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class ExpertRouting(NamedTuple):
+    """Result of :func:`expert_route` for ``N`` rows, ``k`` experts per row and ``E`` experts."""
+    weights: torch.Tensor    # [N, k] fp32, differentiable
+    experts: torch.Tensor    # [N, k] int32, -1: none
+    slots: torch.Tensor      # [N, k] int32: place of the pair in expert order, -1: none
+    order: torch.Tensor      # [N * k] int32: row * k + j of every place, -1 behind the last
+    offsets: torch.Tensor    # [E + 1] int32: first place of every expert
+
+
+# ------------------------------------------------------------------------------------------------ routing
+def _route(logits: torch.Tensor, top_k: int, renormalize: bool) -> ExpertRouting:
+    n, experts = logits.shape
+    dev = logits.device
+    weights = torch.empty((n, top_k), dtype=torch.float32, device=dev)
+    chosen = torch.empty((n, top_k), dtype=torch.int32, device=dev)
+    slots = torch.empty((n, top_k), dtype=torch.int32, device=dev)
+    order = torch.empty(n * top_k, dtype=torch.int32, device=dev)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
+    index = dev.index
+    need, workspace = C.c_size_t(), None
+    if n * top_k > 4096:          # (a few rows need no scratch: one CTA routes them)
+        with torch.cuda.device(index):
+            _lib.call("spira_b200_expert_route_workspace", n, experts, top_k, C.byref(need))
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    _launch(index, "spira_b200_expert_route", logits.data_ptr(), _DTYPES[logits.dtype], n, logits.stride(0), experts, top_k,
+            1 if renormalize else 0, weights.data_ptr(), chosen.data_ptr(), slots.data_ptr(), order.data_ptr(), offsets.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), need.value)
+    return ExpertRouting(weights, chosen, slots, order, offsets)
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, renormalize):
+        r = _route(logits, top_k, renormalize)
+        ctx.renormalize = renormalize
+        ctx.save_for_backward(logits, r.weights, r.experts)
+        ctx.mark_non_differentiable(r.experts, r.slots, r.order, r.offsets)
+        ctx.set_materialize_grads(False)
+        return tuple(r)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, *_):
+        if dweights is None:
+            return None, None, None
+        logits, weights, chosen = ctx.saved_tensors
+        n, experts = logits.shape
+        dweights = dweights.float()
+        dlogits = torch.empty((n, experts), dtype=logits.dtype, device=logits.device)
+        _launch(logits.device.index, "spira_b200_expert_route_backward", logits.data_ptr(), _DTYPES[logits.dtype], n, logits.stride(0),
+                experts, weights.shape[1], 1 if ctx.renormalize else 0, weights.data_ptr(), chosen.data_ptr(), dweights.data_ptr(),
+                dweights.stride(0), dweights.stride(1), dlogits.data_ptr())
+        return dlogits, None, None
+
+
+def expert_route(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> ExpertRouting:
+    """The ``top_k`` experts of every row of ``logits [N, E]`` (fp16, bf16 or fp32).
+
+    The largest logits win, equal ones by the lower index; an expert whose logit is ``-inf`` is never chosen, so a row may
+    get fewer than ``top_k`` experts or none (``experts`` and ``slots`` are -1 there, the weight 0).  ``weights`` is the
+    softmax over the chosen experts, or over all of them with ``renormalize=False``.  A NaN counts as the largest logit
+    and makes the weights of its row NaN."""
+    index = _device_of(logits)
+    if logits.dim() != 2 or logits.dtype not in _DTYPES:
+        _fail(f"Tensor logits is expected to be a float16, bfloat16 or float32 matrix [N, E], got {logits.dtype} {tuple(logits.shape)}")
+    top_k = int(top_k)
+    n, experts = logits.shape
+    if not 1 <= experts <= MAX_EXPERTS:
+        _fail(f"expert_route takes 1 to {MAX_EXPERTS} experts, got {experts}")
+    if not 1 <= top_k <= min(experts, MAX_TOP_K):
+        _fail(f"top_k must be 1 to min(experts, {MAX_TOP_K}), got {top_k}")
+    if n * top_k >= 1 << 31:
+        _fail(f"{n} rows x {top_k} experts are out of range")
+    logits = _rows(logits) if n and logits.stride(0) >= experts else logits.contiguous()
+    if _needs_grad(logits):
+        return ExpertRouting(*_Route.apply(logits, top_k, bool(renormalize)))
+    return _route(logits, top_k, renormalize)
+
+
+# ------------------------------------------------------------------------------------------------ rows to experts and back
+def _check_routing(routing: ExpertRouting):
+    slots, offsets = routing.slots, routing.offsets
+    if slots.dim() != 2 or slots.dtype != torch.int32 or offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.shape[0] < 2:
+        _fail("routing.slots is expected to be int32 [N, k] and routing.offsets int32 [E + 1]")
+    if not 1 <= slots.shape[1] <= MAX_TOP_K:
+        _fail(f"a routing holds 1 to {MAX_TOP_K} experts per row, got {slots.shape[1]}")
+    return slots if slots.is_contiguous() else slots.contiguous(), offsets if offsets.is_contiguous() else offsets.contiguous()
+
+
+def _check_rows(t: torch.Tensor, name: str, rows: int) -> torch.Tensor:
+    if t.dim() != 2 or t.dtype not in _DTYPES or t.shape[1] < 1:
+        _fail(f"Tensor {name} is expected to be a float16, bfloat16 or float32 matrix, got {t.dtype} {tuple(t.shape)}")
+    if t.shape[0] != rows:
+        _fail(f"The dimension 0 of Tensor {name} is expected to be {rows} but found {t.shape[0]}")
+    return _rows(t)
+
+
+def _dispatch(feats, slots, offsets):
+    n, k = slots.shape
+    channels = feats.shape[1]
+    rows = torch.empty((n * k, channels), dtype=feats.dtype, device=feats.device)
+    _launch(feats.device.index, "spira_b200_expert_dispatch", feats.data_ptr(), _DTYPES[feats.dtype], n, feats.stride(0), channels,
+            slots.data_ptr(), k, offsets.data_ptr(), offsets.shape[0] - 1, rows.data_ptr())
+    return rows
+
+
+def _combine(rows, weights, slots):
+    n, k = slots.shape
+    channels = rows.shape[1]
+    out = torch.empty((n, channels), dtype=rows.dtype, device=rows.device)
+    _launch(rows.device.index, "spira_b200_expert_combine", rows.data_ptr(), _DTYPES[rows.dtype], n, rows.stride(0), channels,
+            None if weights is None else weights.data_ptr(), 0 if weights is None else weights.stride(0),
+            0 if weights is None else weights.stride(1), slots.data_ptr(), k, out.data_ptr())
+    return out
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, feats, slots, offsets):
+        ctx.save_for_backward(slots)
+        return _dispatch(feats, slots, offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, drows):
+        return _combine(_rows(drows), None, ctx.saved_tensors[0]), None, None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, slots, offsets):
+        ctx.save_for_backward(rows, weights, slots, offsets)
+        return _combine(rows, weights, slots)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        rows, weights, slots, offsets = ctx.saved_tensors
+        dout = _rows(dout)
+        (n, k), channels = slots.shape, rows.shape[1]
+        drows = torch.empty((n * k, channels), dtype=rows.dtype, device=rows.device) if ctx.needs_input_grad[0] else None
+        dweights = torch.empty((n, k), dtype=torch.float32, device=rows.device) if ctx.needs_input_grad[1] else None
+        _launch(rows.device.index, "spira_b200_expert_combine_backward", rows.data_ptr(), dout.data_ptr(), _DTYPES[rows.dtype], n,
+                rows.stride(0), dout.stride(0), channels, weights.data_ptr(), weights.stride(0), weights.stride(1), slots.data_ptr(), k,
+                offsets.data_ptr(), offsets.shape[0] - 1, None if drows is None else drows.data_ptr(),
+                None if dweights is None else dweights.data_ptr())
+        return drows, dweights, None, None
+
+
+def expert_dispatch(feats: torch.Tensor, routing: ExpertRouting) -> torch.Tensor:
+    """``feats [N, C]`` -> ``[N * k, C]`` in the expert order of ``routing`` (a row appears once per expert it goes to); rows
+    behind ``routing.offsets[E]`` are zero."""
+    slots, offsets = _check_routing(routing)
+    _device_of(feats, slots, offsets)
+    feats = _check_rows(feats, "feats", slots.shape[0])
+    if _needs_grad(feats):
+        return _Dispatch.apply(feats, slots, offsets)
+    return _dispatch(feats, slots, offsets)
+
+
+def expert_combine(rows: torch.Tensor, routing: ExpertRouting) -> torch.Tensor:
+    """``rows [N * k, C]`` in expert order -> ``[N, C]``: every voxel's rows, weighted with ``routing.weights`` and added in
+    the order of its experts (fp32, one rounding).  Voxels without an expert are zero."""
+    slots, offsets = _check_routing(routing)
+    weights = routing.weights
+    _device_of(rows, slots, offsets, weights)
+    if weights.dtype != torch.float32 or weights.shape != slots.shape:
+        _fail(f"routing.weights is expected to be float32 {tuple(slots.shape)}, got {weights.dtype} {tuple(weights.shape)}")
+    rows = _check_rows(rows, "rows", slots.shape[0] * slots.shape[1])
+    if _needs_grad(rows, weights):
+        return _Combine.apply(rows, weights, slots, offsets)
+    return _combine(rows, weights, slots)
+
+
+# ------------------------------------------------------------------------------------------------ ragged products
+def _status(index: int) -> int:
+    """Address of the status word the tensor-core kernels raise; it must exist before a capture (it outlives the graph)."""
+    t = _C._status.get(index)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            _fail("make one grouped_linear call before capturing a graph (the device's status word does not exist yet)")
+        t = _C.status_word(torch.device("cuda", index))
+    return t.data_ptr()
+
+
+def _grouped_desc(x, weights, offsets, dy=None) -> GroupedDesc:
+    experts, c_in, c_out = weights.shape
+    d = GroupedDesc(dtype=_DTYPES[weights.dtype], experts=experts, c_in=c_in, c_out=c_out, n=x.shape[0] if x is not None else dy.shape[0],
+                    offsets=offsets.data_ptr(), weight=weights.data_ptr())
+    if x is not None:
+        d.x, d.x_stride = x.data_ptr(), x.stride(0)
+    if dy is not None:
+        d.dy, d.dy_stride = dy.data_ptr(), dy.stride(0)
+    return d
+
+
+def _grouped(x, weights, offsets, bias, relu):
+    index = x.device.index
+    y = torch.empty((x.shape[0], weights.shape[2]), dtype=x.dtype, device=x.device)
+    d = _grouped_desc(x, weights, offsets)
+    d.y, d.relu = y.data_ptr(), 1 if relu else 0
+    if bias is not None:
+        d.bias = bias.data_ptr()
+    _launch(index, "spira_b200_grouped_linear", C.byref(d), _status(index))
+    return y
+
+
+def _with_workspace(index, device, name, desc, *rest):
+    need = C.c_size_t()
+    if index == _current_device():
+        _lib.call(name + "_workspace", C.byref(desc), C.byref(need))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name + "_workspace", C.byref(desc), C.byref(need))
+    workspace = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    _launch(index, name, C.byref(desc), None if workspace is None else workspace.data_ptr(), need.value, *rest)
+
+
+class _Grouped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weights, offsets, bias, relu):
+        y = _grouped(x, weights, offsets, bias, relu)
+        ctx.relu, ctx.has_bias = relu, bias is not None
+        ctx.save_for_backward(x, weights, offsets, y if relu else None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weights, offsets, y = ctx.saved_tensors
+        dy = _rows(dy)
+        index, dev = x.device.index, x.device
+        status = _status(index)
+        want_dx, want_dw, want_db = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.has_bias and ctx.needs_input_grad[3]
+        dx = dw = db = None
+        if ctx.relu or want_db:
+            d = _grouped_desc(None, weights, offsets, dy)
+            if ctx.relu:
+                dz = torch.empty((dy.shape[0], weights.shape[2]), dtype=dy.dtype, device=dev)
+                d.y, d.dz = y.data_ptr(), dz.data_ptr()
+            if want_db:
+                db = torch.empty((weights.shape[0], weights.shape[2]), dtype=weights.dtype, device=dev)
+                d.dbias = db.data_ptr()
+            _with_workspace(index, dev, "spira_b200_grouped_linear_dz", d)
+            if ctx.relu:
+                dy = dz
+        if want_dx:
+            dx = torch.empty((dy.shape[0], weights.shape[1]), dtype=dy.dtype, device=dev)
+            d = _grouped_desc(None, weights, offsets, dy)
+            d.dx = dx.data_ptr()
+            _launch(index, "spira_b200_grouped_linear_dx", C.byref(d), status)
+        if want_dw:
+            dw = torch.empty_like(weights, memory_format=torch.contiguous_format)
+            d = _grouped_desc(x, weights, offsets, dy)
+            d.dweight = dw.data_ptr()
+            _with_workspace(index, dev, "spira_b200_grouped_linear_dw", d, status)
+        return dx, dw, None, db, None
+
+
+def grouped_linear(feats: torch.Tensor, weights: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   relu: bool = False) -> torch.Tensor:
+    """``relu?(feats[r] @ weights[e] + bias[e])`` for the rows ``offsets[e] <= r < offsets[e + 1]`` of every expert ``e``.
+
+    ``feats [N, C_in]`` and ``weights [E, C_in, C_out]`` are fp16 or bf16 (sums in fp32, one rounding), ``offsets [E + 1]``
+    is int32 on the device and is never read by the host; ``bias`` is ``[E, C_out]``.  Groups may be empty; rows outside
+    every group are zero in the result and have no gradient."""
+    index = _device_of(feats, weights, offsets, bias)
+    if feats.dim() != 2 or weights.dim() != 3:
+        _fail(f"feats is expected to be [N, C_in] and weights [E, C_in, C_out], got {tuple(feats.shape)} and {tuple(weights.shape)}")
+    if feats.dtype != weights.dtype or feats.dtype not in (torch.float16, torch.bfloat16):
+        _fail(f"feats and weights must both be float16 or both bfloat16 (fp32 accumulation), got {feats.dtype} and {weights.dtype}")
+    experts, c_in, c_out = weights.shape
+    if feats.shape[1] != c_in:
+        _fail(f"The dimension 1 of Tensor feats is expected to be {c_in} but found {feats.shape[1]}")
+    if not 1 <= experts <= MAX_GROUPS or c_in < 1 or c_out < 1:
+        _fail(f"grouped_linear takes 1 to {MAX_GROUPS} experts with at least one channel, got weights {tuple(weights.shape)}")
+    if offsets.dim() != 1 or offsets.shape[0] != experts + 1 or offsets.dtype != torch.int32:
+        _fail(f"offsets is expected to be int32 [{experts + 1}], got {offsets.dtype} {tuple(offsets.shape)}")
+    if bias is not None and (bias.dtype != feats.dtype or bias.shape != (experts, c_out)):
+        _fail(f"bias is expected to be {feats.dtype} [{experts}, {c_out}], got {bias.dtype} {tuple(bias.shape)}")
+    feats = _rows(feats)
+    weights, offsets = weights.contiguous(), offsets.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    if _needs_grad(feats, weights, bias):
+        return _Grouped.apply(feats, weights, offsets, bias, bool(relu))
+    return _grouped(feats, weights, offsets, bias, relu)

@@ -1,0 +1,177 @@
+"""Norms around a block, fused with the block's gate and the residual, with their gradients.
+
+    stream, normed = residual_norm(feats, block, weight=w, ...)
+
+No reference counterpart: the reference normalises with BatchNorm as a pass of its own (spira/nn/normalizations.py:8-10)
+and adds residuals as another (spira/tensors.py:47-53).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from spira_b200._lib import NormDesc
+from spira_b200.nn.functional.experts import _DTYPES, _device_of, _fail, _launch, _needs_grad, _rows, _with_workspace
+
+__all__ = ["residual_norm"]
+
+MAX_CHANNELS = 8192
+GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
+
+
+class _Spec:
+    """What stays the same between the forward and the backward call."""
+    __slots__ = ("layer", "pre", "post", "gate_kind", "residual_scale", "block_scale", "eps")
+
+
+def _desc(spec, x, block, gate, weight, bias, post_weight, post_bias) -> NormDesc:
+    params_f32 = 0
+    for p in (weight, bias, post_weight, post_bias, gate if spec.gate_kind == GATE_CHANNEL else None):
+        if p is not None:
+            params_f32 = 1 if p.dtype == torch.float32 else 0
+    d = NormDesc(dtype=_DTYPES[x.dtype], params_f32=params_f32, channels=x.shape[1], layer=spec.layer, pre=spec.pre, post=spec.post,
+                 gate_kind=spec.gate_kind, residual_scale=spec.residual_scale, block_scale=spec.block_scale, eps=spec.eps, n=x.shape[0],
+                 x=x.data_ptr(), x_stride=x.stride(0))
+    if block is not None:
+        d.block, d.block_stride = block.data_ptr(), block.stride(0)
+    if gate is not None:
+        d.gate, d.gate_stride = gate.data_ptr(), gate.stride(0)
+    if weight is not None:
+        d.weight = weight.data_ptr()
+    if bias is not None:
+        d.bias = bias.data_ptr()
+    if post_weight is not None:
+        d.post_weight = post_weight.data_ptr()
+    if post_bias is not None:
+        d.post_bias = post_bias.data_ptr()
+    return d
+
+
+def _forward(spec, x, block, gate, weight, bias, post_weight, post_bias, stats):
+    d = _desc(spec, x, block, gate, weight, bias, post_weight, post_bias)
+    stream = torch.empty(x.shape, dtype=x.dtype, device=x.device) if block is not None else None
+    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device) if spec.pre else None
+    if stream is not None:
+        d.stream = stream.data_ptr()
+    if normed is not None:
+        d.normed = normed.data_ptr()
+    if stats is not None:
+        d.stats = stats.data_ptr()
+    _launch(x.device.index, "spira_b200_residual_norm", C.byref(d))
+    return stream, normed
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, spec, x, block, gate, weight, bias, post_weight, post_bias):
+        stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device)
+        stream, normed = _forward(spec, x, block, gate, weight, bias, post_weight, post_bias, stats)
+        ctx.spec = spec
+        ctx.save_for_backward(x, block, gate, weight, bias, post_weight, post_bias, stats)
+        ctx.set_materialize_grads(False)
+        return stream, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dstream, dnormed):
+        x, block, gate, weight, bias, post_weight, post_bias, stats = ctx.saved_tensors
+        spec, need = ctx.spec, ctx.needs_input_grad
+        if dstream is None and dnormed is None:
+            return (None,) * 8
+        if spec.pre and dnormed is None:
+            dnormed = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+        d = _desc(spec, x, block, gate, weight, bias, post_weight, post_bias)
+        d.stats = stats.data_ptr()
+        if dstream is not None:
+            dstream = _rows(dstream)
+            d.dstream, d.dstream_stride = dstream.data_ptr(), dstream.stride(0)
+        if dnormed is not None:
+            dnormed = _rows(dnormed)
+            d.dnormed, d.dnormed_stride = dnormed.data_ptr(), dnormed.stride(0)
+        grads = [None]
+        for name, t, wanted in zip(("dx", "dblock", "dgate", "dweight", "dbias", "dpost_weight", "dpost_bias"),
+                                   (x, block, gate, weight, bias, post_weight, post_bias), need[1:]):
+            g = torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and wanted else None
+            if g is not None:
+                setattr(d, name, g.data_ptr())
+            grads.append(g)
+        if any(g is not None for g in grads[4:]) or (grads[3] is not None and spec.gate_kind == GATE_CHANNEL):
+            _with_workspace(x.device.index, x.device, "spira_b200_residual_norm_backward", d)
+        else:
+            _launch(x.device.index, "spira_b200_residual_norm_backward", C.byref(d), None, 0)
+        return tuple(grads)
+
+
+def residual_norm(feats: torch.Tensor, block: Optional[torch.Tensor] = None, *, weight: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, pre: bool = True, post: bool = False, post_weight: Optional[torch.Tensor] = None,
+                  post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, kind: str = "rms",
+                  residual_scale: float = 1.0, block_scale: float = 1.0, eps: float = 1e-6
+                  ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``(stream, normed)`` with
+
+    ``stream = residual_scale * feats + block_scale * gate * p``, ``p = norm(block) * post_weight + post_bias`` if ``post``
+    else ``block`` (without a block the stream is ``feats`` itself), and ``normed = norm(stream) * weight + bias`` (``None``
+    with ``pre=False``).
+
+    ``norm`` is ``v / sqrt(mean(v^2) + eps)`` for ``kind="rms"``, ``(v - mean) / sqrt(var + eps)`` for ``kind="layer"``, in
+    fp32 on the unrounded stream.  ``feats`` and ``block`` are ``[N, C]`` in fp16, bf16 or fp32, ``C <= 8192``; ``gate`` is a
+    parameter ``[C]``, or ``[N, 1]`` or ``[N, C]`` in the type of ``feats``.  Parameters are all fp32 or all of the type of
+    ``feats``; a missing one counts as ones (weights) or zeros (biases).  The two scales are constants."""
+    _device_of(feats, block, weight, bias, post_weight, post_bias, gate)
+    if feats.dim() != 2 or feats.dtype not in _DTYPES:
+        _fail(f"Tensor feats is expected to be a float16, bfloat16 or float32 matrix [N, C], got {feats.dtype} {tuple(feats.shape)}")
+    n, channels = feats.shape
+    if not 1 <= channels <= MAX_CHANNELS:
+        _fail(f"residual_norm takes 1 to {MAX_CHANNELS} channels, got {channels}")
+    if kind not in ("rms", "layer"):
+        _fail(f"kind must be 'rms' or 'layer', got {kind!r}")
+    if not eps > 0:
+        _fail(f"eps must be positive, got {eps}")
+    if block is None:
+        if post or gate is not None or post_weight is not None or post_bias is not None or residual_scale != 1.0 or block_scale != 1.0:
+            _fail("a gate, a scale or a norm after the block needs a block")
+        if not pre:
+            _fail("neither a block nor a norm: nothing to compute")
+    elif block.shape != feats.shape or block.dtype != feats.dtype:
+        _fail(f"block is expected to be {feats.dtype} {tuple(feats.shape)}, got {block.dtype} {tuple(block.shape)}")
+    if not pre and (weight is not None or bias is not None):
+        _fail("weight and bias belong to the norm that pre=False leaves out")
+    if not post and (post_weight is not None or post_bias is not None):
+        _fail("post_weight and post_bias need post=True")
+    spec = _Spec()
+    spec.layer, spec.pre, spec.post = int(kind == "layer"), int(bool(pre)), int(bool(post))
+    spec.residual_scale, spec.block_scale, spec.eps = float(residual_scale), float(block_scale), float(eps)
+    spec.gate_kind = GATE_NONE
+    if gate is not None:
+        if gate.dim() == 1:
+            spec.gate_kind = GATE_CHANNEL
+        elif gate.shape == (n, 1):
+            spec.gate_kind = GATE_ROW
+        elif gate.shape == (n, channels):
+            spec.gate_kind = GATE_FULL
+        else:
+            _fail(f"gate is expected to be [{channels}], [{n}, 1] or [{n}, {channels}], got {tuple(gate.shape)}")
+        if gate.dim() == 2 and gate.dtype != feats.dtype:
+            _fail(f"a gate per row or element has the type of feats, {feats.dtype}, got {gate.dtype}")
+        gate = _rows(gate) if gate.dim() == 2 else gate.contiguous()
+    dtype = None
+    for name, p in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias),
+                    ("gate", gate if spec.gate_kind == GATE_CHANNEL else None)):
+        if p is None:
+            continue
+        if p.shape != (channels,) or p.dtype not in (feats.dtype, torch.float32):
+            _fail(f"{name} is expected to be {feats.dtype} or float32 [{channels}], got {p.dtype} {tuple(p.shape)}")
+        if dtype is not None and p.dtype != dtype:
+            _fail("parameters of one call must have one type")
+        dtype = p.dtype
+    params = [p if p is None or p.is_contiguous() else p.contiguous() for p in (weight, bias, post_weight, post_bias)]
+    feats_rows = _rows(feats)
+    block = None if block is None else _rows(block)
+    if _needs_grad(feats, block, gate, *params):
+        stream, normed = _ResidualNorm.apply(spec, feats_rows, block, gate, *params)
+    else:
+        stream, normed = _forward(spec, feats_rows, block, gate, *params, None)
+    return feats if block is None else stream, normed

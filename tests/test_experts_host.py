@@ -1,0 +1,70 @@
+"""CPU: what the expert and norm operators refuse, and the layouts of their descriptors (no CUDA call is made)."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_descriptor_layouts_match_the_header():
+    from spira_b200 import _lib
+    assert ctypes.sizeof(_lib.GroupedDesc) == 6 * 4 + 3 * 8 + 10 * 8          # the library static_asserts the same sizes
+    assert ctypes.sizeof(_lib.NormDesc) == 8 * 4 + 4 * 4 + 6 * 8 + 19 * 8
+
+
+def test_cpu_tensors_are_refused():
+    from spira_b200.nn import functional as F
+    x = torch.zeros(4, 8)
+    offsets = torch.zeros(3, dtype=torch.int32)
+    routing = F.ExpertRouting(torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32),
+                              torch.zeros(8, dtype=torch.int32), offsets)
+    for call in (lambda: F.expert_route(x, 2), lambda: F.expert_dispatch(x, routing), lambda: F.expert_combine(torch.zeros(8, 8), routing),
+                 lambda: F.grouped_linear(x.half(), torch.zeros(2, 8, 8).half(), offsets), lambda: F.residual_norm(x, x)):
+        with pytest.raises(NotImplementedError, match="CUDA"):
+            call()
+
+
+def test_library_refuses_bad_arguments(lib):
+    from spira_b200 import _lib
+    n = ctypes.c_size_t()
+    err = lib.spira_b200_last_error
+    assert lib.spira_b200_expert_route_workspace(100000, 513, 2, ctypes.byref(n)) != 0 and b"experts=513" in err()
+    assert lib.spira_b200_expert_route_workspace(100000, 8, 9, ctypes.byref(n)) != 0 and b"top_k=9" in err()
+    assert lib.spira_b200_expert_route_workspace(-1, 8, 2, ctypes.byref(n)) != 0
+    assert lib.spira_b200_expert_route_workspace((1 << 31) // 2, 8, 2, ctypes.byref(n)) != 0 and b"out of range" in err()
+    assert lib.spira_b200_expert_route_workspace(100, 8, 2, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.spira_b200_expert_route(None, 7, 1, 8, 8, 2, 1, None, None, None, None, None, None, 0, None) != 0 and b"element type" in err()
+    assert lib.spira_b200_expert_route(None, 0, 1, 8, 8, 2, 1, None, None, None, None, None, None, 0, None) != 0 and b"null" in err()
+    assert lib.spira_b200_expert_dispatch(None, 0, 4, 8, 8, None, 33, None, 2, None, None) != 0 and b"top_k=33" in err()
+    assert lib.spira_b200_expert_combine(None, 0, 4, 8, 8, None, 0, 0, None, 2, None, None) != 0 and b"null" in err()
+    assert lib.spira_b200_expert_combine_backward(None, None, 0, 0, 8, 8, 8, None, 0, 0, None, 2, None, 2, None, None, None) == 0   # no rows
+    g = _lib.GroupedDesc(dtype=_lib.F32, experts=2, c_in=8, c_out=8, n=4)
+    for name in ("spira_b200_grouped_linear", "spira_b200_grouped_linear_dx"):
+        assert getattr(lib, name)(ctypes.byref(g), None, None) != 0 and b"neither fp16 nor bf16" in err()
+        assert getattr(lib, name)(None, None, None) != 0
+    g.dtype = _lib.F16
+    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"null pointer" in err()
+    g.experts = 1025
+    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"experts=1025" in err()
+    g.experts, g.c_in = 2, 0
+    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"channels" in err()
+    d = _lib.NormDesc(dtype=_lib.F16, channels=8193, pre=1, eps=1e-6, n=3)
+    assert lib.spira_b200_residual_norm(ctypes.byref(d), None) != 0 and b"channels=8193" in err()
+    d.channels = 64
+    assert lib.spira_b200_residual_norm(ctypes.byref(d), None) != 0 and b"null pointer" in err()
+    d.eps = 0.0
+    assert lib.spira_b200_residual_norm(ctypes.byref(d), None) != 0 and b"eps" in err()
+    d.eps, d.post = 1e-6, 1
+    assert lib.spira_b200_residual_norm(ctypes.byref(d), None) != 0 and b"needs a block" in err()
+    d.post, d.gate_kind = 0, 4
+    assert lib.spira_b200_residual_norm(ctypes.byref(d), None) != 0 and b"gate" in err()
+
+
+def test_modules_check_their_arguments():
+    from spira_b200 import nn as spnn
+    with pytest.raises(ValueError, match="top_k"):
+        spnn.SparseExperts(16, 32, 4, top_k=5)
+    with pytest.raises(ValueError, match="kind"):
+        spnn.ResidualNorm(16, kind="batch")
+    m = spnn.ResidualNorm(16, kind="layer", post=True, gate=True, gate_init=0.5)
+    assert sorted(n for n, _ in m.named_parameters()) == ["bias", "gate", "post_bias", "post_weight", "weight"]
+    assert sorted(n for n, _ in spnn.ResidualNorm(16).named_parameters()) == ["weight"]
