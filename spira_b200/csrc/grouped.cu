@@ -7,6 +7,7 @@
 // Rows outside every group are zero in y and dx.  Group boundaries are read on the device; the host only knows upper
 // bounds of the tile counts.  Sums over a group's rows are split into pieces that are added in a fixed order.
 //
+// Channel counts in whole 16-byte units and aligned tensors run on the tensor-core kernel (grouped_tc.cu).
 // `grouped_any_kernel` takes every channel count, stride and alignment: 64 x 64 tiles, element-wise loads into shared
 // memory, warp-level MMAs with fp32 accumulation.
 #include "common.cuh"
@@ -17,7 +18,6 @@ namespace sb {
 
 constexpr int kATile = 64, kAK = 32, kALd = kAK + 8;     // (row stride of 80 bytes: conflict-free fragment loads)
 constexpr int kAThreads = 128;
-constexpr int kForward = 0, kDx = 1, kDw = 2;
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -244,16 +244,32 @@ constexpr int kDzPiece = 256;
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Rows of a group that one CTA of the weight gradient adds up (0: all of them).  Splitting fills the SMs when the weight
-// matrices have few tiles, at the price of fp32 partial sums: about two CTAs per SM, at least 256 rows each.
-static int dw_piece(int64_t n, int experts, int64_t tiles) {
+// matrices have few tiles, at the price of fp32 partial sums: `ctas` per SM, at least 256 rows each.
+static int dw_piece(int64_t n, int experts, int64_t tiles, int ctas) {
   if (tiles * experts >= sm_count() || n <= 256) return 0;
-  const int64_t pieces = div_up(2 * static_cast<int64_t>(sm_count()), tiles);
+  const int64_t pieces = div_up(ctas * static_cast<int64_t>(sm_count()), tiles);
   int64_t piece = div_up(div_up(n, pieces), 64) * 64;
   if (piece < 256) piece = 256;
   return piece >= n ? 0 : static_cast<int>(piece);
 }
 
+// Which kernel a product runs on; one answer for a call and for its workspace.
+static bool tc_forward(const spira_b200_grouped_desc &D) {
+  return grouped_tc_available() && D.c_out % 8 == 0 && grouped_tc_rows_ok(D.x, D.x_stride, D.c_in, D.n) && aligned16(D.weight) && aligned16(D.bias) && aligned16(D.y);
+}
+static bool tc_dx(const spira_b200_grouped_desc &D) {
+  return grouped_tc_available() && D.c_in % 8 == 0 && grouped_tc_rows_ok(D.dy, D.dy_stride, D.c_out, D.n) && aligned16(D.weight) && aligned16(D.dx);
+}
+static bool tc_dw(const spira_b200_grouped_desc &D) {
+  return grouped_tc_available() && grouped_tc_rows_ok(D.x, D.x_stride, D.c_in, D.n) && grouped_tc_rows_ok(D.dy, D.dy_stride, D.c_out, D.n) && aligned16(D.dweight);
+}
+static unsigned long long wait_ns() { return static_cast<unsigned long long>(spira_b200_get_option("wait_limit_us")) * 1000ull; }
+
 static int64_t any_tiles(int c_in, int c_out) { return div_up(c_in, kATile) * div_up(c_out, kATile); }
+
+static int dw_rows(const spira_b200_grouped_desc &D) {
+  return tc_dw(D) ? dw_piece(D.n, D.experts, grouped_tc_dw_tiles(D.c_in, D.c_out), 1) : dw_piece(D.n, D.experts, any_tiles(D.c_in, D.c_out), 2);
+}
 
 static int grouped_check(const char *what, const spira_b200_grouped_desc *D) {
   SB_CHECK_ARG(D, "%s: null descriptor", what);
@@ -291,6 +307,7 @@ extern "C" int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, in
   if (rc != SPIRA_B200_OK || desc->n == 0) return rc;
   const spira_b200_grouped_desc &D = *desc;
   SB_CHECK_ARG(D.x && D.weight && D.y, "grouped_linear: null pointer");
+  if (tc_forward(D)) return grouped_tc_run(kForward, D, 0, nullptr, status, wait_ns(), as_stream(stream));
   GroupedParams P{D.x, D.weight, D.bias, D.offsets, D.y, nullptr, D.x_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, D.relu, 0};
   return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kForward>(P, as_stream(stream))););
 }
@@ -300,6 +317,7 @@ extern "C" int spira_b200_grouped_linear_dx(const spira_b200_grouped_desc *desc,
   if (rc != SPIRA_B200_OK || desc->n == 0) return rc;
   const spira_b200_grouped_desc &D = *desc;
   SB_CHECK_ARG(D.dy && D.weight && D.dx, "grouped_linear_dx: null pointer");
+  if (tc_dx(D)) return grouped_tc_run(kDx, D, 0, nullptr, status, wait_ns(), as_stream(stream));
   GroupedParams P{D.dy, D.weight, nullptr, D.offsets, D.dx, nullptr, D.dy_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, 0, 0};
   return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kDx>(P, as_stream(stream))););
 }
@@ -308,7 +326,7 @@ extern "C" int spira_b200_grouped_linear_dw_workspace(const spira_b200_grouped_d
   int rc = grouped_check("grouped_linear_dw", desc);
   if (rc != SPIRA_B200_OK) return rc;
   SB_CHECK_ARG(bytes, "grouped_linear_dw: null pointer");
-  const int piece = dw_piece(desc->n, desc->experts, any_tiles(desc->c_in, desc->c_out));
+  const int piece = dw_rows(*desc);
   *bytes = piece ? static_cast<size_t>(group_tiles_bound(desc->n, desc->experts, piece)) * desc->c_in * desc->c_out * 4 : 0;
   return SPIRA_B200_OK;
 }
@@ -330,11 +348,13 @@ extern "C" int spira_b200_grouped_linear_dw(const spira_b200_grouped_desc *desc,
   if (rc != SPIRA_B200_OK) return rc;
   if (need && (!workspace || workspace_bytes < need))
     return fail(SPIRA_B200_ERR_WORKSPACE, "grouped_linear_dw: workspace of %zu bytes is smaller than %zu", workspace_bytes, need);
-  const int piece = dw_piece(D.n, D.experts, any_tiles(D.c_in, D.c_out));
+  SB_CHECK_ARG(aligned16(workspace), "grouped_linear_dw: the workspace must be 16-byte aligned");
+  const int piece = dw_rows(D);
+  const bool tc = tc_dw(D);
   GroupedParams P{D.x, D.dy, nullptr, D.offsets, D.dweight, static_cast<float *>(workspace), D.x_stride, D.dy_stride, static_cast<int>(D.n), D.experts,
                   D.c_in, D.c_out, 0, piece};
   return SB_DISPATCH_HALF(D.dtype, T, {
-    rc = launch_any<T, kDw>(P, st);
+    rc = tc ? grouped_tc_run(kDw, D, piece, static_cast<float *>(workspace), status, wait_ns(), st) : launch_any<T, kDw>(P, st);
     if (rc != SPIRA_B200_OK || piece == 0) return rc;
     const unsigned blocks = static_cast<unsigned>(div_up(size, 256) < 1024 ? div_up(size, 256) : 1024);
     SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(blocks, D.experts), dim3(256), 0, st, static_cast<const float *>(workspace), D.offsets,

@@ -79,4 +79,11 @@ __device__ __forceinline__ void group_span(const int32_t *offsets, int experts, 
 // upper bound of the number of tiles of `rows` rows, for a host that does not know the offsets
 inline int64_t group_tiles_bound(int64_t n, int experts, int64_t rows) { return n / rows + (experts < n ? experts : n); }
 
+// The tensor-core path (grouped_tc.cu).  It takes channel counts in whole 16-byte units and 16-byte aligned tensors and rows.
+enum { kForward = 0, kDx = 1, kDw = 2 };
+bool grouped_tc_available();
+bool grouped_tc_rows_ok(const void *p, int64_t stride, int channels, int64_t n);
+int grouped_tc_dw_tiles(int c_in, int c_out);
+int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float *partial, int32_t *status, unsigned long long wait_ns, cudaStream_t st);
+
 }  // namespace sb

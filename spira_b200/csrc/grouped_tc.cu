@@ -1,0 +1,487 @@
+// Ragged products on the fifth-generation tensor cores: tcgen05.mma with operands moved by TMA, accumulators in tensor memory.
+//
+//   forward   y[rows of e]  = x W[e]       M = rows,  N = c_out, K = c_in    A = x  (K-major),  B = W[e]  (N-major)
+//   dx        dx[rows of e] = dz W[e]^T    M = rows,  N = c_in,  K = c_out   A = dz (K-major),  B = W[e]  (K-major)
+//   dW        dW[e] = x_e^T dz_e           M = c_in,  N = c_out, K = rows    A = x  (M-major),  B = dz    (N-major)
+//
+// No operand is transposed or copied: the three products read the same tensors and differ in the majors of the instruction
+// descriptor and in the boxes TMA fetches (128-byte swizzle everywhere).  A tile has 128 rows of M; rows past the end of a
+// group belong to the next one, they are multiplied and not stored.  In dW the rows are the reduction: the last step of a
+// group overwrites foreign rows with zeros in BOTH operands in shared memory (0 * NaN of a neighbour would not be 0).
+//
+// One persistent CTA per SM, 12 warps: warp 0 issues TMA loads, warp 1 the MMAs, warps 4-11 (two per tensor-memory lane
+// quarter) convert and store while the next tile accumulates in the other half of tensor memory.  Every CTA reads the group
+// boundaries once into shared memory.  Every wait is bounded; an expired one raises the status word.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "elem.cuh"
+#include "grouped.cuh"
+#include "ptx.cuh"
+
+namespace sb {
+
+using namespace sb::ptx;
+
+constexpr int kGRows = 128;                    // M of a tile
+constexpr int kGK = 64;                        // reduction per stage: 128 bytes, one swizzle row
+constexpr int kGABytes = kGRows * kGK * 2;
+constexpr int kGBlock = kGK * 64 * 2;          // one 64 x 64 box
+constexpr int kGMaxN = 256;
+constexpr int kGMaxStages = 8;
+constexpr int kGEpilogueWarps = 8, kGFirstEpilogueWarp = 4;
+constexpr int kGThreads = (kGFirstEpilogueWarp + kGEpilogueWarps) * 32;
+constexpr int kGSmemBudget = 224 * 1024;
+
+struct GroupedTcParams {
+  const int32_t *offsets;
+  void *out;                 // y, dx or dW
+  float *partial;            // dW in pieces: [unit][c_in][c_out]
+  const void *bias;
+  int32_t *status;
+  int n, experts, m_channels, n_channels, k_channels;   // m_channels: c_in in dW; k_channels: 0 in dW (rows)
+  int relu, piece;           // piece: rows per unit of dW, 0 = whole groups
+  int bn, n_tiles, m_tiles;  // columns per tile, column tiles, row tiles of dW
+  int stages, b_bytes, acc_stride, tmem_cols, off_bar, off_groups;
+  uint32_t idesc;
+  unsigned long long wait_ns;
+};
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+
+// Operand whose M (or N) elements are contiguous, 128-byte swizzle: 64 x 64 boxes (64 reduction rows of 128 bytes); eight
+// reduction rows are 1024 bytes, the next 64 elements of M / N are the next box.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(kGBlock >> 4) << 16;      // leading byte offset: next 64 elements of M / N
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;         // stride byte offset: next 8 reduction rows
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;                 // 128-byte swizzle
+  return d;
+}
+
+// Where tile t lies.  Tiles are numbered (group, unit of the group, column tile): neighbouring CTAs share the same rows.
+struct TcTile {
+  int expert, unit, row0, row_end;     // unit: number of the (group, unit) pair; rows: M of forward / dx, reduction of dW
+  int m0, n0;                          // first channel of M (dW) and of N
+  int steps;                           // reduction steps of kGK
+};
+
+template <int MODE>
+struct TileWalk {
+  const int *rows, *first;             // shared memory: group boundaries, first unit of every group
+  int expert = 0;
+  __device__ __forceinline__ TcTile at(const GroupedTcParams &P, int t) {
+    TcTile r;
+    const int per_unit = MODE == kDw ? P.m_tiles * P.n_tiles : P.n_tiles;
+    const int unit = t / per_unit, in_unit = t - unit * per_unit;
+    while (unit >= first[expert + 1]) ++expert;        // (t only grows)
+    const int index = unit - first[expert];
+    r.expert = expert;
+    r.unit = unit;
+    r.n0 = in_unit % P.n_tiles * P.bn;
+    if (MODE == kDw) {
+      r.m0 = in_unit / P.n_tiles * kGRows;
+      r.row0 = rows[expert] + index * P.piece;
+      r.row_end = P.piece && r.row0 + P.piece < rows[expert + 1] ? r.row0 + P.piece : rows[expert + 1];
+      r.steps = (r.row_end - r.row0 + kGK - 1) / kGK;
+    } else {
+      r.m0 = 0;
+      r.row0 = rows[expert] + index * kGRows;
+      r.row_end = rows[expert + 1];
+      r.steps = (P.k_channels + kGK - 1) / kGK;
+    }
+    return r;
+  }
+};
+
+// Group boundaries (clamped, never falling) and the first unit of every group, by one warp.
+template <int MODE>
+__device__ __forceinline__ void read_groups(const GroupedTcParams &P, int *rows, int *first) {
+  const int lane = threadIdx.x & 31;
+  int highest = 0, units = 0;
+  for (int e0 = 0; e0 <= P.experts; e0 += 32) {
+    const int e = e0 + lane;
+    int v = e <= P.experts ? clamped_offset(P.offsets, e, P.n) : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d && o > v) v = o;
+    }
+    v = v > highest ? v : highest;
+    if (e <= P.experts) rows[e] = v;
+    highest = __shfl_sync(0xffffffffu, v, 31);
+  }
+  __syncwarp();
+  const int unit_rows = MODE == kDw ? P.piece : kGRows;
+  for (int e0 = 0; e0 < P.experts; e0 += 32) {
+    const int e = e0 + lane;
+    int mine = 0;
+    if (e < P.experts) mine = unit_rows == 0 ? 1 : (rows[e + 1] - rows[e] + unit_rows - 1) / unit_rows;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (e < P.experts) first[e] = units + sum - mine;
+    units += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane == 0) first[P.experts] = units;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&h);
+}
+
+// Up to 32 columns of one row of the accumulator: bias, ReLU, one rounding, whole 32-byte sectors where they are aligned.
+template <typename T, int MODE>
+__device__ __forceinline__ void store_columns(const GroupedTcParams &P, const TcTile &tile, int m, int c0, int c_stop, const uint32_t (&r)[32]) {
+  const int col = tile.n0 + c0;
+  if (MODE == kDw && P.piece) {
+    float *dst = P.partial + (static_cast<int64_t>(tile.unit) * P.m_channels + m) * P.n_channels + col;
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      if (c0 + i < c_stop) *reinterpret_cast<uint4 *>(dst + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+    return;
+  }
+  T *dst = static_cast<T *>(P.out) + (MODE == kDw ? static_cast<int64_t>(tile.expert) * P.m_channels + m : static_cast<int64_t>(m)) * P.n_channels + col;
+  const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 16) {
+    if (c0 + i >= c_stop) break;
+    uint4 pack[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[i + 8 * h + e]);
+      if (MODE == kForward) {
+        if (P.bias && c0 + i + 8 * h < c_stop) {
+          float bias[8];
+          load_f32<T, 8>(static_cast<const T *>(P.bias) + static_cast<int64_t>(tile.expert) * P.n_channels + col + i + 8 * h, bias);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] += bias[e];
+        }
+        if (P.relu)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = f[e] < 0.f ? 0.f : f[e];      // (a NaN stays)
+      }
+      pack[h] = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+    }
+    if (wide && c0 + i + 16 <= c_stop) {
+      st_global_v8(dst + i, pack[0], pack[1]);
+    } else {
+      *reinterpret_cast<uint4 *>(dst + i) = pack[0];
+      if (c0 + i + 8 < c_stop) *reinterpret_cast<uint4 *>(dst + i + 8) = pack[1];
+    }
+  }
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_constant__ GroupedTcParams P, const __grid_constant__ CUtensorMap map_a,
+                                                                   const __grid_constant__ CUtensorMap map_b) {
+  extern __shared__ unsigned char grouped_smem_raw[];
+  const uint32_t raw = smem_u32(grouped_smem_raw);
+  unsigned char *smem = grouped_smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + P.off_bar;
+  auto bar_full = [&](int s) { return bar0 + 8u * s; };
+  auto bar_empty = [&](int s) { return bar0 + 8u * (kGMaxStages + s); };
+  auto bar_acc_full = [&](int b) { return bar0 + 8u * (2 * kGMaxStages + b); };
+  auto bar_acc_empty = [&](int b) { return bar0 + 8u * (2 * kGMaxStages + 2 + b); };
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + P.off_bar + 8 * (2 * kGMaxStages + 4));
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + P.off_bar + 8 * (2 * kGMaxStages + 4) + 4);
+  int *rows = reinterpret_cast<int *>(smem + P.off_groups), *first = rows + P.experts + 1;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int stages = P.stages, stage_bytes = kGABytes + P.b_bytes;
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(bar_full(s), 1);
+      mbar_init(bar_empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_acc_full(b), 1);
+      mbar_init(bar_acc_empty(b), 32 * kGEpilogueWarps);
+    }
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), P.tmem_cols);
+    tmem_relinquish();
+  }
+  pdl_wait();            // before the first global read of any thread
+  if (warp == 2) read_groups<MODE>(P, rows, first);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();         // (behind the allocation: a CTA of the next kernel on this SM cannot take the tensor memory first)
+  const uint32_t tmem_base = *tmem_slot;
+  const int total = first[P.experts] * (MODE == kDw ? P.m_tiles * P.n_tiles : P.n_tiles), G = gridDim.x;
+  TileWalk<MODE> walk{rows, first};
+
+  if (warp == 0) {
+    // =========================== TMA loads ===========================
+    if (lane == 0) {
+      int stage = 0, phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < total; t += G) {
+        const TcTile tile = walk.at(P, t);
+        for (int j = 0; j < tile.steps; ++j) {
+          if (!mbar_wait(bar_empty(stage), phase ^ 1, abort_flag, P.wait_ns)) { ok = false; break; }
+          const uint32_t a = sbase + stage * stage_bytes, b = a + kGABytes, bar = bar_full(stage);
+          mbar_arrive_expect_tx(bar, stage_bytes);
+          const int k = j * kGK;
+          if (MODE == kDw) {
+            for (int h = 0; h < 2; ++h) tma_2d(a + h * kGBlock, &map_a, tile.m0 + h * 64, tile.row0 + k, bar);
+            for (int h = 0; h < P.b_bytes / kGBlock; ++h) tma_2d(b + h * kGBlock, &map_b, tile.n0 + h * 64, tile.row0 + k, bar);
+          } else {
+            tma_2d(a, &map_a, k, tile.row0, bar);
+            if (MODE == kForward) {
+              for (int h = 0; h < P.b_bytes / kGBlock; ++h) tma_3d(b + h * kGBlock, &map_b, tile.n0 + h * 64, k, tile.expert, bar);
+            } else {
+              tma_3d(b, &map_b, k, tile.n0, tile.expert, bar);
+            }
+          }
+          if (++stage == stages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // =========================== MMAs ===========================
+    int stage = 0, phase = 0, tile_i = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < total; t += G, ++tile_i) {
+      const TcTile tile = walk.at(P, t);
+      const int b = tile_i & 1;
+      // (the whole warp leaves together: lanes may see the abort flag at different times)
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_acc_empty(b), ((acc_phase >> b) & 1u) ^ 1u, abort_flag, P.wait_ns))) break;
+      acc_phase ^= 1u << b;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + b * P.acc_stride;
+      const int length = MODE == kDw ? tile.row_end - tile.row0 : P.k_channels;
+      for (int j = 0; j < tile.steps; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_full(stage), phase, abort_flag, P.wait_ns))) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t sa = sbase + stage * stage_bytes, sb = sa + kGABytes;
+        const int left = length - j * kGK, depth = left < kGK ? left : kGK, ks = (depth + 15) / 16;
+        if (MODE == kDw && depth < ks * 16) {
+          // rows [depth, 16 ks) belong to the next group: a reduction row is one 128-byte line of every box
+          const int lines = ks * 16 - depth, boxes = 2 + P.b_bytes / kGBlock;
+          for (int i = lane; i < boxes * lines * 8; i += 32) {
+            const int box = i / (lines * 8), q = i % (lines * 8);
+            *reinterpret_cast<uint4 *>(smem + stage * stage_bytes + box * kGBlock + (depth + q / 8) * 128 + (q % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          const uint64_t a_desc = MODE == kDw ? smem_desc_mn_sw128(sa) : smem_desc_k_sw128(sa);
+          const uint64_t b_desc = MODE == kDx ? smem_desc_k_sw128(sb) : smem_desc_mn_sw128(sb);
+          // 16 steps of the reduction: 32 bytes further in a K-major row, 16 lines further in the other layout
+          constexpr uint32_t kA = MODE == kDw ? 2048 >> 4 : 32 >> 4, kB = MODE == kDx ? 32 >> 4 : 2048 >> 4;
+          for (int s = 0; s < ks; ++s) mma_f16_ss(d_tmem, a_desc + s * kA, b_desc + s * kB, P.idesc, (j | s) != 0);
+          mma_commit(bar_empty(stage));
+        }
+        __syncwarp();
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+      if (!ok) break;
+      if (lane == 0) mma_commit(bar_acc_full(b));
+      __syncwarp();
+    }
+  } else if (warp >= kGFirstEpilogueWarp) {
+    // =========================== epilogue ===========================
+    const int q = warp & 3, half = (warp - kGFirstEpilogueWarp) >> 2;
+    const int c_split = ((P.bn >> 1) + 15) & ~15;
+    uint32_t acc_phase = 0;
+    int tile_i = 0;
+    for (int t = blockIdx.x; t < total; t += G, ++tile_i) {
+      const TcTile tile = walk.at(P, t);
+      const int b = tile_i & 1;
+      const int m = (MODE == kDw ? tile.m0 : tile.row0) + q * 32 + lane;
+      const bool live = m < (MODE == kDw ? P.m_channels : tile.row_end);
+      const int n_end = tile.n0 + P.bn < P.n_channels ? P.bn : P.n_channels - tile.n0;      // columns of this tile
+      const int c_begin = half ? c_split : 0, c_stop = half ? n_end : (n_end < c_split ? n_end : c_split);
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_acc_full(b), (acc_phase >> b) & 1u, abort_flag, P.wait_ns))) break;
+      acc_phase ^= 1u << b;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + b * P.acc_stride + (static_cast<uint32_t>(q * 32) << 16);
+      for (int c0 = c_begin; c0 < c_stop; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32(taddr + c0, r);       // (columns behind the accumulator are read and not used)
+        tmem_ld_wait();
+        if (MODE == kDw && tile.steps == 0) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+        }
+        if (live) store_columns<T, MODE>(P, tile, m, c0, c_stop, r);
+        __syncwarp();
+      }
+      tc_fence_before();
+      mbar_arrive(bar_acc_empty(b));
+    }
+  } else if (warp == 3 && MODE != kDw) {
+    // rows of no group are zero
+    T *out = static_cast<T *>(P.out);
+    const int64_t width = P.n_channels / 8, before = rows[0] * width, behind = static_cast<int64_t>(P.n - rows[P.experts]) * width;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + lane; i < before + behind; i += static_cast<int64_t>(G) * 32)
+      reinterpret_cast<uint4 *>(out)[i < before ? i : rows[P.experts] * width + i - before] = make_uint4(0, 0, 0, 0);
+  }
+
+  // =========================== teardown ===========================
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    // a bounded wait expired: report, give copies in flight time to land, then release the tensor memory
+    if (tid == 0 && P.status) atomicExch(P.status, 1);
+    const unsigned long long t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) { }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, P.tmem_cols);
+  }
+}
+
+typedef CUresult (*GroupedEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                    const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static GroupedEncodeFn grouped_encode_fn() {
+  static GroupedEncodeFn fn = nullptr;
+  if (fn == nullptr) {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<GroupedEncodeFn>(p);
+  }
+  return fn;
+}
+
+// [n][channels] rows (stride in elements) or [experts][c_in][c_out] weights; boxes of 64 channels x box_rows, zeros outside.
+static int encode_map(CUtensorMap *map, int dtype, const void *p, int rank, int64_t channels, int64_t rows, int64_t row_stride, int64_t outer, int box_rows) {
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(outer)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_stride) * 2, static_cast<cuuint64_t>(row_stride) * rows * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = grouped_encode_fn()(map, dtype == SPIRA_B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+                                         const_cast<void *>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SPIRA_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+  return SPIRA_B200_OK;
+}
+
+bool grouped_tc_rows_ok(const void *p, int64_t stride, int channels, int64_t n) {
+  return channels % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (n == 1 || (stride % 8 == 0 && stride >= channels));
+}
+bool grouped_tc_available() { return grouped_encode_fn() != nullptr; }
+
+// Columns per tile: as few tiles of at most 256 as the width needs, of equal size; when the tiles would not fill the SMs
+// (few rows), narrower ones down to 64.
+static int columns_per_tile(int channels, int64_t units) {
+  int64_t tiles = div_up(channels, kGMaxN);
+  while (tiles * units < sm_count() && div_up(channels, 2 * tiles) >= 64) tiles *= 2;
+  return static_cast<int>(div_up(div_up(channels, tiles), 16) * 16);
+}
+
+int grouped_tc_dw_tiles(int c_in, int c_out) {
+  return static_cast<int>(div_up(c_in, kGRows) * div_up(c_out, columns_per_tile(c_out, int64_t(1) << 30)));
+}
+
+int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float *partial, int32_t *status, unsigned long long wait_ns, cudaStream_t st) {
+  GroupedTcParams P{};
+  P.offsets = D.offsets;
+  P.partial = partial;
+  P.status = status;
+  P.n = static_cast<int>(D.n);
+  P.experts = D.experts;
+  P.piece = piece;
+  P.wait_ns = wait_ns;
+  int64_t units;
+  if (mode == kDw) {
+    P.out = D.dweight;
+    P.m_channels = D.c_in;
+    P.n_channels = D.c_out;
+    P.m_tiles = static_cast<int>(div_up(D.c_in, kGRows));
+    units = (piece ? group_tiles_bound(D.n, D.experts, piece) : D.experts) * P.m_tiles;
+    P.bn = columns_per_tile(D.c_out, int64_t(1) << 30);
+  } else {
+    P.out = mode == kForward ? D.y : D.dx;
+    P.bias = mode == kForward ? D.bias : nullptr;
+    P.relu = mode == kForward ? D.relu : 0;
+    P.n_channels = mode == kForward ? D.c_out : D.c_in;
+    P.k_channels = mode == kForward ? D.c_in : D.c_out;
+    P.m_tiles = 1;
+    units = group_tiles_bound(D.n, D.experts, kGRows);
+    P.bn = columns_per_tile(P.n_channels, units);
+  }
+  P.n_tiles = static_cast<int>(div_up(P.n_channels, P.bn));
+  const bool b_n_major = mode != kDx;
+  P.b_bytes = b_n_major ? static_cast<int>(div_up(P.bn, 64)) * kGBlock : P.bn * 128;
+  P.acc_stride = 32;
+  while (P.acc_stride < P.bn) P.acc_stride *= 2;
+  P.tmem_cols = 2 * P.acc_stride;
+  P.idesc = (1u << 4) | (D.dtype == SPIRA_B200_BF16 ? (1u << 7) | (1u << 10) : 0u) | (mode == kDw ? 1u << 15 : 0u) | (b_n_major ? 1u << 16 : 0u) |
+            (static_cast<uint32_t>(P.bn >> 3) << 17) | ((128u >> 4) << 24);
+  const int fixed = 8 * (2 * kGMaxStages + 5) + 16 + 8 * (D.experts + 2);
+  const int stage_bytes = kGABytes + P.b_bytes;      // (multiples of 1024: 8 KB boxes, or bn * 128 with bn a multiple of 16)
+  P.stages = (kGSmemBudget - fixed) / stage_bytes;
+  if (P.stages > kGMaxStages) P.stages = kGMaxStages;
+  P.off_bar = P.stages * stage_bytes;
+  P.off_groups = P.off_bar + 8 * (2 * kGMaxStages + 5) + 8;
+  const size_t smem = static_cast<size_t>(P.off_bar) + fixed + 1024;
+
+  alignas(64) CUtensorMap map_a, map_b;
+  int rc;
+  const int64_t x_stride = D.n == 1 ? D.c_in : D.x_stride, dy_stride = D.n == 1 ? D.c_out : D.dy_stride;
+  if (mode == kForward) {
+    rc = encode_map(&map_a, D.dtype, D.x, 2, D.c_in, D.n, x_stride, 1, kGRows);
+    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, D.c_out, D.experts, kGK);
+  } else if (mode == kDx) {
+    rc = encode_map(&map_a, D.dtype, D.dy, 2, D.c_out, D.n, dy_stride, 1, kGRows);
+    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, D.c_out, D.experts, P.bn);
+  } else {
+    rc = encode_map(&map_a, D.dtype, D.x, 2, D.c_in, D.n, x_stride, 1, kGK);
+    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.dy, 2, D.c_out, D.n, dy_stride, 1, kGK);
+  }
+  if (rc != SPIRA_B200_OK) return rc;
+  const int64_t tiles = units * P.n_tiles;
+  SB_CHECK_ARG(tiles < (int64_t(1) << 31) - 65536, "grouped_linear: too many tiles");
+  const unsigned grid = static_cast<unsigned>(tiles < sm_count() ? (tiles < 1 ? 1 : tiles) : sm_count());
+  auto go = [&](auto kernel) -> int {
+    SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kGThreads), smem, st, P, map_a, map_b));
+    return SPIRA_B200_OK;
+  };
+  if (D.dtype == SPIRA_B200_F16)
+    return mode == kForward ? go(grouped_tc_kernel<__half, kForward>) : mode == kDx ? go(grouped_tc_kernel<__half, kDx>) : go(grouped_tc_kernel<__half, kDw>);
+  return mode == kForward ? go(grouped_tc_kernel<__nv_bfloat16, kForward>)
+         : mode == kDx    ? go(grouped_tc_kernel<__nv_bfloat16, kDx>)
+                          : go(grouped_tc_kernel<__nv_bfloat16, kDw>);
+}
+
+}  // namespace sb
