@@ -535,8 +535,10 @@ int spira_b200_expert_combine_backward(const void *rows, const void *dout, int d
 
 /* Ragged products: group e holds the rows [offsets[e], offsets[e + 1]) of x[n][c_in] and has the matrix weight[e][c_in][c_out].
  *   spira_b200_grouped_linear      y[r] = relu?(x[r] W[e] + bias[e]); rows outside every group are zero
- *   spira_b200_grouped_linear_dz   dz = dy (y > 0) (dz may be NULL: no ReLU), dbias[e] = column sums of dz (may be NULL);
- *                                  dz is written for the rows of groups only
+ *                                  (mask != NULL: also a bit per element, set where the value before the ReLU is
+ *                                  positive; spira_b200_grouped_linear_mask_bytes gives its size, 0 = this shape has none)
+ *   spira_b200_grouped_linear_dz   dz = dy where the mask is set, or where y > 0 without a mask (dz may be NULL: no ReLU),
+ *                                  dbias[e] = column sums of dz (may be NULL); dz is written for the rows of groups only
  *   spira_b200_grouped_linear_dx   dx[r] = dy[r] W[e]^T (pass dz as dy); rows outside every group are zero
  *   spira_b200_grouped_linear_dw   dweight[e] = x_e^T dy_e (zero for an empty group)
  * fp16 or bf16 in and out, fp32 sums, one rounding.  Offsets are read on the device; an entry counts as the largest of
@@ -547,8 +549,9 @@ typedef struct spira_b200_grouped_desc {
   int64_t n, x_stride, dy_stride;
   const int32_t *offsets;
   const void *x, *weight, *bias, *dy;
-  void *y, *dz, *dx, *dweight, *dbias;
+  void *y, *mask, *dz, *dx, *dweight, *dbias;
 } spira_b200_grouped_desc;
+int spira_b200_grouped_linear_mask_bytes(const spira_b200_grouped_desc *desc, size_t *bytes);
 int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, int32_t *status, void *stream);
 int spira_b200_grouped_linear_dz_workspace(const spira_b200_grouped_desc *desc, size_t *bytes);
 int spira_b200_grouped_linear_dz(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, void *stream);

@@ -81,7 +81,7 @@ class GroupedDesc(C.Structure):
     _fields_ = [("dtype", c_int32), ("experts", c_int32), ("c_in", c_int32), ("c_out", c_int32), ("relu", c_int32), ("reserved", c_int32),
                 ("n", c_int64), ("x_stride", c_int64), ("dy_stride", c_int64), ("offsets", c_void_p),
                 ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("dy", c_void_p),
-                ("y", c_void_p), ("dz", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p)]
+                ("y", c_void_p), ("mask", c_void_p), ("dz", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p)]
 
 
 class NormDesc(C.Structure):
@@ -168,6 +168,7 @@ SIGNATURES = {
     "spira_b200_expert_combine": [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p],
     "spira_b200_expert_combine_backward": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
                                            c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
+    "spira_b200_grouped_linear_mask_bytes": [C.POINTER(GroupedDesc), C.POINTER(c_size_t)],
     "spira_b200_grouped_linear": [C.POINTER(GroupedDesc), c_void_p, c_void_p],
     "spira_b200_grouped_linear_dz_workspace": [C.POINTER(GroupedDesc), C.POINTER(c_size_t)],
     "spira_b200_grouped_linear_dz": [C.POINTER(GroupedDesc), c_void_p, c_size_t, c_void_p],

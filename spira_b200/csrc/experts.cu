@@ -35,84 +35,95 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// One row on G neighbouring lanes, EPL consecutive experts per lane (G * EPL >= experts).  Few lanes with many experts
-// each keep the number of shuffles small: at 64 experts and k = 4, 4 lanes x 16 experts execute a quarter of the
-// instructions of 32 lanes x 2.
-template <typename T, int G, int EPL>
-__device__ __forceinline__ void route_row(const T *logits, int64_t row_stride, bool vec_ok, int64_t row, bool live, int experts, int k,
-                                          int renormalize, float *weights, int32_t *chosen, int *hist) {
-  const int g = threadIdx.x & (G - 1);
-  uint32_t key[EPL];
-  float total = 0.f;
-  const T *src = logits + row * row_stride + g * EPL;
-  if constexpr (EPL * sizeof(T) >= 16) {
-    if (live && vec_ok && (g + 1) * EPL <= experts) {
-      constexpr int V = 16 / sizeof(T);
+// EPL consecutive elements of a row from column c0 on as fp32, `fill` outside the row.
+template <typename T, int EPL>
+__device__ __forceinline__ void load_logits(const T *row, int c0, int experts, bool live, bool vec_ok, float fill, float (&v)[EPL]) {
+  constexpr int V = EPL * sizeof(T) >= 16 ? 16 / sizeof(T) : EPL;
+  if (live && vec_ok && c0 + EPL <= experts) {
 #pragma unroll
-      for (int i = 0; i < EPL; i += V) {
-        float f[V];
-        load_f32<T, V>(src + i, f);
+    for (int i = 0; i < EPL; i += V) {
+      float f[V];
+      load_f32<T, V>(row + c0 + i, f);
 #pragma unroll
-        for (int j = 0; j < V; ++j) key[i + j] = logit_key(f[j]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) key[i] = live && g * EPL + i < experts ? logit_key(to_f32(src[i])) : kGone;
+      for (int j = 0; j < V; ++j) v[i + j] = f[j];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) key[i] = live && g * EPL + i < experts ? logit_key(to_f32(src[i])) : kGone;
-  }
-  float top = 0.f, sum = 0.f;
-  for (int j = 0; j < k; ++j) {
-    uint32_t best = kGone;
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (key[i] > best) { best = key[i]; at = i; }     // (strict: the lowest index of equal logits)
-    int e = g * EPL + at;
-#pragma unroll
-    for (int d = 1; d < G; d *= 2) {
-      const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, d, G);
-      const int oe = __shfl_xor_sync(0xffffffffu, e, d, G);
-      if (ob > best || (ob == best && oe < e)) { best = ob; e = oe; }
-    }
-    if (j == 0) {
-      top = best == kGone ? 0.f : key_logit(best);
-      if (!renormalize) {      // the softmax runs over all experts: while every logit is still there
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (key[i] != kGone) total += expf(key_logit(key[i]) - top);
-#pragma unroll
-        for (int d = 1; d < G; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d, G);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (g * EPL + i == e) key[i] = kGone;
-    const float score = best == kGone ? 0.f : expf(key_logit(best) - top);
-    sum += score;
-    if (live && g == 0) {
-      weights[row * k + j] = score;                    // divided below, once the sum is known
-      chosen[row * k + j] = best == kGone ? -1 : e;
-      if (best != kGone) atomicAdd(hist + e, 1);
-    }
-  }
-  if (live && g == 0) {
-    const float denom = renormalize ? sum : total;
-    for (int j = 0; j < k; ++j)
-      if (chosen[row * k + j] >= 0) weights[row * k + j] = weights[row * k + j] / denom;
+    for (int i = 0; i < EPL; ++i) v[i] = live && c0 + i < experts ? to_f32(row[c0 + i]) : fill;
   }
 }
 
+// The rows [r0, r1) of a CTA.  A row takes G neighbouring lanes with EPL consecutive experts each (G * EPL >= experts): few
+// lanes with many experts keep the number of shuffles small (at 64 experts and k = 4, 4 lanes x 16 experts execute a
+// quarter of the instructions of 32 lanes x 2).  Choices are collected in shared memory, so that results leave in whole
+// lines and nothing is read back.
 template <typename T, int G, int EPL>
 __device__ __forceinline__ void route_rows(const T *logits, int64_t row_stride, int64_t r0, int64_t r1, int experts, int k, int renormalize,
-                                           float *weights, int32_t *chosen, int *hist) {
-  const bool vec_ok = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && row_stride * sizeof(T) % 16 == 0;
-  constexpr int kRows = kRouteThreads / G;
+                                           float *weights, int32_t *chosen, int *hist, int *stash) {
+  constexpr int V = EPL * sizeof(T) >= 16 ? 16 / sizeof(T) : EPL;
+  const bool vec_ok = reinterpret_cast<uintptr_t>(logits) % (V * sizeof(T)) == 0 && row_stride % V == 0;
+  const int g = threadIdx.x & (G - 1), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kRows = kRouteThreads / G, kWarpRows = 32 / G;
+  int *warp_e = stash + warp * kWarpRows * k * 2;                       // [rows of the warp][k]
+  float *warp_w = reinterpret_cast<float *>(warp_e + kWarpRows * k);
+  int *my_e = warp_e + lane / G * k;
+  float *my_w = warp_w + lane / G * k;
   for (int64_t r = r0; r < r1; r += kRows) {
     const int64_t row = r + threadIdx.x / G;
-    route_row<T, G, EPL>(logits, row_stride, vec_ok, row, row < r1, experts, k, renormalize, weights, chosen, hist);
+    const bool live = row < r1;
+    uint32_t key[EPL];
+    {
+      float v[EPL];
+      load_logits<T, EPL>(logits + row * row_stride, g * EPL, experts, live, vec_ok, -INFINITY, v);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) key[i] = logit_key(v[i]);
+    }
+    float top = 0.f, sum = 0.f, total = 0.f;
+    for (int j = 0; j < k; ++j) {
+      uint32_t best = kGone;
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (key[i] > best) { best = key[i]; at = i; }     // (strict: the lowest index of equal logits)
+      int e = g * EPL + at;
+#pragma unroll
+      for (int d = 1; d < G; d *= 2) {
+        const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, d, G);
+        const int oe = __shfl_xor_sync(0xffffffffu, e, d, G);
+        if (ob > best || (ob == best && oe < e)) { best = ob; e = oe; }
+      }
+      if (j == 0) {
+        top = best == kGone ? 0.f : key_logit(best);
+        if (!renormalize) {      // the softmax runs over all experts: while every logit is still there
+#pragma unroll
+          for (int i = 0; i < EPL; ++i)
+            if (key[i] != kGone) total += expf(key_logit(key[i]) - top);
+#pragma unroll
+          for (int d = 1; d < G; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d, G);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (g * EPL + i == e) key[i] = kGone;
+      const float score = best == kGone ? 0.f : expf(key_logit(best) - top);
+      sum += score;
+      if (g == 0) {
+        my_w[j] = score;
+        my_e[j] = best == kGone ? -1 : e;
+        if (live && best != kGone) atomicAdd(hist + e, 1);
+      }
+    }
+    __syncwarp();
+    const float denom = renormalize ? sum : total;
+    for (int j = g; j < k; j += G) my_w[j] = my_e[j] >= 0 ? my_w[j] / denom : 0.f;
+    __syncwarp();
+    const int64_t first = r + warp * kWarpRows;
+    const int count = static_cast<int>(r1 - first < kWarpRows ? (r1 > first ? r1 - first : 0) : kWarpRows) * k;
+    for (int i = lane; i < count; i += 32) {
+      weights[first * k + i] = warp_w[i];
+      chosen[first * k + i] = warp_e[i];
+    }
+    __syncwarp();
   }
 }
 
@@ -126,9 +137,14 @@ __device__ __forceinline__ void place_entries(const int32_t *chosen, int64_t n0,
   int *mine = warp_base + warp * experts;
   for (int e = lane; e < experts; e += 32) mine[e] = 0;
   __syncwarp();
-  for (int64_t i = p0 + lane; i < p1; i += 32) {
-    const int e = chosen[i];
-    if (e >= 0) atomicAdd(mine + e, 1);
+  constexpr int kBatch = 8;      // loads in flight
+  for (int64_t i = p0; i < p1; i += 32 * kBatch) {
+    int e[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) e[q] = i + 32 * q + lane < p1 ? chosen[i + 32 * q + lane] : -1;
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      if (e[q] >= 0) atomicAdd(mine + e[q], 1);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < experts; e += kRouteThreads) {
@@ -140,19 +156,26 @@ __device__ __forceinline__ void place_entries(const int32_t *chosen, int64_t n0,
     }
   }
   __syncthreads();
-  for (int64_t i = p0; i < p1; i += 32) {
-    const bool in = i + lane < p1;
-    const int e = in ? chosen[i + lane] : -1;
-    const uint32_t peers = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(peers & ((1u << lane) - 1u));
-    int slot = -1;
-    if (e >= 0) slot = mine[e] + rank;
-    __syncwarp();
-    if (e >= 0 && rank == 0) mine[e] += __popc(peers);
-    __syncwarp();
-    if (in) {
-      slots[i + lane] = slot;
-      if (slot >= 0) order[slot] = static_cast<int32_t>(i + lane);
+  for (int64_t i0 = p0; i0 < p1; i0 += 32 * kBatch) {
+    int batch[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) batch[q] = i0 + 32 * q + lane < p1 ? chosen[i0 + 32 * q + lane] : -1;
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int64_t i = i0 + 32 * q;
+      if (i >= p1) break;
+      const int e = batch[q];
+      const uint32_t peers = __match_any_sync(0xffffffffu, e);
+      const int rank = __popc(peers & ((1u << lane) - 1u));
+      int slot = -1;
+      if (e >= 0) slot = mine[e] + rank;
+      __syncwarp();
+      if (e >= 0 && rank == 0) mine[e] += __popc(peers);
+      __syncwarp();
+      if (i + lane < p1) {
+        slots[i + lane] = slot;
+        if (slot >= 0) order[slot] = static_cast<int32_t>(i + lane);
+      }
     }
   }
 }
@@ -188,12 +211,12 @@ struct RouteParams {
 template <typename T, int G, int EPL>
 __global__ void __launch_bounds__(kRouteThreads) route_small_kernel(const RouteParams P) {
   extern __shared__ int route_smem[];
-  int *hist = route_smem, *first = hist + P.experts, *warp_base = first + P.experts + 1;
+  int *hist = route_smem, *first = hist + P.experts, *warp_base = first + P.experts + 1, *stash = warp_base + kRouteWarps * P.experts;
   pdl_trigger();
   for (int e = threadIdx.x; e < P.experts; e += kRouteThreads) hist[e] = 0;
   pdl_wait();
   __syncthreads();
-  route_rows<T, G, EPL>(static_cast<const T *>(P.logits), P.row_stride, 0, P.n, P.experts, P.k, P.renormalize, P.weights, P.chosen, hist);
+  route_rows<T, G, EPL>(static_cast<const T *>(P.logits), P.row_stride, 0, P.n, P.experts, P.k, P.renormalize, P.weights, P.chosen, hist, stash);
   __syncthreads();
   if (threadIdx.x < 32) scan_experts(hist, first, P.experts);
   __syncthreads();
@@ -210,7 +233,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
   pdl_wait();
   __syncthreads();
   const int64_t r0 = blockIdx.x * P.rows_per_cta, r1 = r0 + P.rows_per_cta < P.n ? r0 + P.rows_per_cta : P.n;
-  route_rows<T, G, EPL>(static_cast<const T *>(P.logits), P.row_stride, r0, r1, P.experts, P.k, P.renormalize, P.weights, P.chosen, route_smem);
+  route_rows<T, G, EPL>(static_cast<const T *>(P.logits), P.row_stride, r0, r1, P.experts, P.k, P.renormalize, P.weights, P.chosen, route_smem,
+                        route_smem + P.experts);
   __syncthreads();
   for (int e = threadIdx.x; e < P.experts; e += kRouteThreads) P.block_hist[static_cast<int64_t>(blockIdx.x) * P.experts + e] = route_smem[e];
 }
@@ -226,7 +250,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
   const int G = gridDim.x;
   // a thread keeps to one expert where it can: few shared-memory additions
   const int lanes = P.experts < kRouteThreads ? kRouteThreads / P.experts : 1;
-  for (int e = threadIdx.x % P.experts, part = threadIdx.x / P.experts; part < lanes && e < P.experts; part += lanes) {
+  const int e = threadIdx.x % P.experts, part = threadIdx.x / P.experts;
+  if (part < lanes) {
     int all = 0, mine = 0;
 #pragma unroll 8
     for (int b = part; b < G; b += lanes) {
@@ -255,54 +280,97 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
 // dlogits: with u_j = dweights of the chosen experts and dot = sum_j u_j w_j,
 //   softmax over the chosen:  d[e_j] = w_j (u_j - dot), 0 elsewhere
 //   softmax over all:         d[e] = p_e ([e chosen] u_e - dot),  p_e = exp(l_e - max) / sum
-template <typename T, int G>
+template <typename T, int G, int EPL>
 __global__ void __launch_bounds__(256) route_backward_kernel(const T *logits, int64_t n, int64_t row_stride, int experts, int k, int renormalize,
                                                              const float *weights, const int32_t *chosen, const float *dweights,
                                                              int64_t dw_row, int64_t dw_col, T *dlogits) {
   pdl_trigger();
   pdl_wait();
+  constexpr int V = EPL * sizeof(T) >= 16 ? 16 / sizeof(T) : EPL;
+  const bool vec_ok = reinterpret_cast<uintptr_t>(logits) % (V * sizeof(T)) == 0 && row_stride % V == 0;
+  const bool out_ok = reinterpret_cast<uintptr_t>(dlogits) % (V * sizeof(T)) == 0 && experts % V == 0;
   const int g = threadIdx.x & (G - 1);
   constexpr int kRows = 256 / G;
-  const int64_t groups = (n + kRows - 1) / kRows;
-  for (int64_t b = blockIdx.x; b < groups; b += gridDim.x) {
-    const int64_t row = b * kRows + threadIdx.x / G;
-    const bool live = row < n;
-    float dot = 0.f;
-    if (live)
-      for (int j = 0; j < k; ++j)
-        if (chosen[row * k + j] >= 0) dot += dweights[row * dw_row + j * dw_col] * weights[row * k + j];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / G;
+  const bool live = row < n;
+  float v[EPL], d[EPL];
+  if (!renormalize) load_logits<T, EPL>(logits + row * row_stride, g * EPL, experts, live, vec_ok, -INFINITY, v);
+  float dot = 0.f;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) d[i] = 0.f;
+  for (int j0 = 0; j0 < k; j0 += G) {           // lane g brings entry j0 + g, then everybody sees all of them
+    const int j = j0 + g;
+    const bool there = live && j < k;
+    const int e = there ? chosen[row * k + j] : -1;
+    const float u = e >= 0 ? dweights[row * dw_row + j * dw_col] : 0.f, w = e >= 0 ? weights[row * k + j] : 0.f;
+    float part = e >= 0 ? u * w : 0.f;
+#pragma unroll
+    for (int s = 1; s < G; s *= 2) part += __shfl_xor_sync(0xffffffffu, part, s, G);
+    dot += part;
+    const int stop = k - j0 < G ? k - j0 : G;
+    for (int q = 0; q < stop; ++q) {
+      const int eq = __shfl_sync(0xffffffffu, e, q, G);
+      const float uq = __shfl_sync(0xffffffffu, u, q, G);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (eq == g * EPL + i) d[i] = uq;
+    }
+  }
+  // (renormalize: the places of the chosen are found a second time, now that the dot product is known)
+  if (renormalize) {
+    float r[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) r[i] = 0.f;
+    for (int j0 = 0; j0 < k; j0 += G) {
+      const int j = j0 + g;
+      const int e = live && j < k ? chosen[row * k + j] : -1;
+      const float w = e >= 0 ? weights[row * k + j] : 0.f;
+      const int stop = k - j0 < G ? k - j0 : G;
+      for (int q = 0; q < stop; ++q) {
+        const int eq = __shfl_sync(0xffffffffu, e, q, G);
+        const float wq = __shfl_sync(0xffffffffu, w, q, G);
+#pragma unroll
+        for (int i = 0; i < EPL; ++i)
+          if (eq == g * EPL + i) r[i] = wq * (d[i] - dot);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) d[i] = r[i];
+  } else {
     float top = -INFINITY, total = 0.f;
     bool nan = false;
-    if (!renormalize) {
-      for (int e = g; live && e < experts; e += G) {
-        const float v = to_f32(logits[row * row_stride + e]);
-        nan |= v != v;
-        top = fmaxf(top, v);
-      }
 #pragma unroll
-      for (int d = 1; d < G; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d, G));
-      for (int e = g; live && e < experts; e += G) {
-        const float v = to_f32(logits[row * row_stride + e]);
-        if (v > -INFINITY) total += expf(v - top);
-      }
-      if (nan) total = NAN;
+    for (int i = 0; i < EPL; ++i) {
+      nan |= v[i] != v[i];
+      top = fmaxf(top, v[i]);
+    }
 #pragma unroll
-      for (int d = 1; d < G; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d, G);
+    for (int s = 1; s < G; s *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s, G));
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      v[i] = v[i] == -INFINITY ? 0.f : expf(v[i] - top);
+      total += v[i];
     }
-    for (int e = g; live && e < experts; e += G) {
-      float u = 0.f, w = 0.f;
-      for (int j = 0; j < k; ++j)
-        if (chosen[row * k + j] == e) { u = dweights[row * dw_row + j * dw_col]; w = weights[row * k + j]; }
-      float d;
-      if (renormalize) {
-        d = w == 0.f ? 0.f : w * (u - dot);
-      } else {
-        const float v = to_f32(logits[row * row_stride + e]);
-        const float p = v == -INFINITY ? 0.f : expf(v - top) / total;
-        d = v == -INFINITY ? 0.f : p * (u - dot);
-      }
-      dlogits[row * experts + e] = from_f32<T>(d);
+    if (nan) total = NAN;
+#pragma unroll
+    for (int s = 1; s < G; s *= 2) total += __shfl_xor_sync(0xffffffffu, total, s, G);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) d[i] = v[i] == 0.f ? 0.f : v[i] / total * (d[i] - dot);
+  }
+  if (!live) return;
+  T *out = dlogits + row * experts + g * EPL;
+  if (out_ok && (g + 1) * EPL <= experts) {
+#pragma unroll
+    for (int i = 0; i < EPL; i += V) {
+      float f[V];
+#pragma unroll
+      for (int q = 0; q < V; ++q) f[q] = d[i + q];
+      store_f32<T, V>(out + i, f);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (g * EPL + i < experts) out[i] = from_f32<T>(d[i]);
   }
 }
 
@@ -317,6 +385,9 @@ struct MoveParams {
   float *dweights;
   int64_t n, x_stride, y_stride, w_row, w_col;
   int channels, k, experts;
+  int64_t rows_per_launch_row;       // rows of one blockIdx.y: rows * pieces stays below 2^31
+  uint64_t div_mul;                  // i / pieces = (i * div_mul) >> div_shift for 0 <= i < 2^31
+  int div_shift;
 };
 
 template <typename T, int V>
@@ -324,64 +395,74 @@ __device__ __forceinline__ void zero_tail(const MoveParams &P, T *rows, int vecs
   const int64_t total = P.n * P.k;
   int64_t tail = P.offsets[P.experts];
   tail = tail < 0 ? 0 : tail > total ? total : tail;
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * blockDim.x, work = (total - tail) * vecs;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * gridDim.y * blockDim.x, work = (total - tail) * vecs;
   const float zero[V] = {};
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < work; i += threads)
+  for (int64_t i = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < work; i += threads)
     store_f32<T, V>(rows + (tail + i / vecs) * P.channels + (i % vecs) * V, zero);
 }
 
-template <typename T, int V>
+// The row and the first channel of a thread; false behind the last row.
+template <int V>
+__device__ __forceinline__ bool my_piece(const MoveParams &P, int64_t &row, int &c) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t r = static_cast<uint32_t>((i * P.div_mul) >> P.div_shift);
+  row = static_cast<int64_t>(blockIdx.y) * P.rows_per_launch_row + r;
+  c = static_cast<int>(i - r * static_cast<uint32_t>(P.channels / V)) * V;
+  return r < P.rows_per_launch_row && row < P.n;
+}
+
+// K: experts per row, 0 = P.k.  The places of a row are known before its first load, all K copies are in flight together.
+template <typename T, int V, int K>
 __global__ void __launch_bounds__(256) dispatch_kernel(const MoveParams P) {
   pdl_trigger();
   pdl_wait();
-  const int vecs = P.channels / V;
-  const int64_t work = P.n * vecs, total = P.n * P.k;
+  const int64_t total = P.n * P.k;
   T *rows = static_cast<T *>(P.out);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < work; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / vecs;
-    const int c = static_cast<int>(i - row * vecs) * V;
+  int64_t row;
+  int c;
+  if (my_piece<V>(P, row, c)) {
     const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.x) + row * P.x_stride + c);
-    for (int j = 0; j < P.k; ++j) {
-      const int64_t slot = P.slots[row * P.k + j];
+    const int k = K ? K : P.k;
+#pragma unroll
+    for (int j = 0; j < k; ++j) {
+      const int64_t slot = P.slots[row * k + j];
       if (slot >= 0 && slot < total) *reinterpret_cast<Vec<T, V> *>(rows + slot * P.channels + c) = v;
     }
   }
-  zero_tail<T, V>(P, rows, vecs);
+  zero_tail<T, V>(P, rows, P.channels / V);
 }
 
-template <typename T, int V>
+template <typename T, int V, int K>
 __global__ void __launch_bounds__(256) combine_kernel(const MoveParams P) {
   pdl_trigger();
   pdl_wait();
-  const int vecs = P.channels / V;
-  const int64_t work = P.n * vecs, total = P.n * P.k;
+  const int64_t total = P.n * P.k;
   const T *rows = static_cast<const T *>(P.y);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < work; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / vecs;
-    const int c = static_cast<int>(i - row * vecs) * V;
-    float acc[V] = {};
-    for (int j0 = 0; j0 < P.k; j0 += 4) {       // four rows on their way at a time
-      Vec<T, V> v[4];
-      float w[4];
+  int64_t row;
+  int c;
+  if (!my_piece<V>(P, row, c)) return;
+  constexpr int B = K && K < 4 ? K : 4;          // rows on their way at a time
+  const int k = K ? K : P.k;
+  float acc[V] = {};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j] = 0.f;
-        const int64_t slot = j0 + j < P.k ? P.slots[row * P.k + j0 + j] : -1;
-        const bool there = slot >= 0 && slot < total;
-        if (there) {
-          w[j] = P.weights ? P.weights[row * P.w_row + (j0 + j) * P.w_col] : 1.f;
-          v[j] = *reinterpret_cast<const Vec<T, V> *>(rows + slot * P.y_stride + c);
-        } else {
-          v[j] = Vec<T, V>{};
-        }
-      }
+  for (int j0 = 0; j0 < k; j0 += B) {
+    Vec<T, V> v[B];
+    float w[B];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = fmaf(w[j], to_f32(v[j].v[e]), acc[e]);
+    for (int j = 0; j < B; ++j) {
+      const int64_t slot = j0 + j < k ? P.slots[row * k + j0 + j] : -1;
+      w[j] = j0 + j < k && P.weights ? P.weights[row * P.w_row + (j0 + j) * P.w_col] : 1.f;
+      const bool there = slot >= 0 && slot < total;
+      if (!there) w[j] = 0.f;
+      if (there) v[j] = *reinterpret_cast<const Vec<T, V> *>(rows + slot * P.y_stride + c);
+      else v[j] = Vec<T, V>{};
     }
-    store_f32<T, V>(static_cast<T *>(P.out) + row * P.channels + c, acc);
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(w[j], to_f32(v[j].v[e]), acc[e]);
   }
+  store_f32<T, V>(static_cast<T *>(P.out) + row * P.channels + c, acc);
 }
 
 // drows[slot] = w dout[t], dweights[t][j] = <dout[t], rows[slot]>: G lanes per row of `dout`.
@@ -434,24 +515,24 @@ static unsigned capped_blocks(int64_t work, int per_cta, int ctas_per_sm) {
   return static_cast<unsigned>(want < 1 ? 1 : want < cap ? want : cap);
 }
 
+// Two CTAs per SM, whole groups of 64 rows.
 static int route_rows_per_cta(int64_t n, int64_t *rows_per_cta) {
-  const int64_t ctas = sm_count();
-  int64_t r = div_up(n, ctas);
-  r = div_up(r, 64) * 64;
-  *rows_per_cta = r;
-  return static_cast<int>(div_up(n, r));
+  *rows_per_cta = div_up(div_up(n, 2 * sm_count()), 64) * 64;
+  return static_cast<int>(div_up(n, *rows_per_cta));
 }
 
+static size_t stash_bytes(int lanes, int k) { return static_cast<size_t>(kRouteThreads / lanes) * k * 8; }
 static size_t place_smem(int experts) { return static_cast<size_t>(3 * experts + 1 + kRouteWarps * experts) * 4; }
 
 template <typename T, int G, int EPL>
 static int launch_route(RouteParams &P, cudaStream_t st) {
   if (P.n * P.k <= kSmallRouteEntries) {
-    SB_CHECK_CUDA(launch_dependent(route_small_kernel<T, G, EPL>, dim3(1), dim3(kRouteThreads), place_smem(P.experts), st, P));
+    SB_CHECK_CUDA(launch_dependent(route_small_kernel<T, G, EPL>, dim3(1), dim3(kRouteThreads), place_smem(P.experts) + stash_bytes(G, P.k), st, P));
     return SPIRA_B200_OK;
   }
   const int ctas = route_rows_per_cta(P.n, &P.rows_per_cta);
-  SB_CHECK_CUDA(launch_dependent(route_choose_kernel<T, G, EPL>, dim3(ctas), dim3(kRouteThreads), static_cast<size_t>(P.experts) * 4, st, P));
+  SB_CHECK_CUDA(launch_dependent(route_choose_kernel<T, G, EPL>, dim3(ctas), dim3(kRouteThreads), static_cast<size_t>(P.experts) * 4 + stash_bytes(G, P.k),
+                                 st, P));
   SB_CHECK_CUDA(launch_dependent(route_place_kernel, dim3(ctas), dim3(kRouteThreads), place_smem(P.experts), st, P));
   return SPIRA_B200_OK;
 }
@@ -488,6 +569,25 @@ static int check_move(const char *what, const MoveParams &P, int dtype, int64_t 
 // 16-byte accesses need every row of every tensor to start on a 16-byte boundary.
 static bool rows_aligned(const void *p, int64_t stride, int size) {
   return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0);
+}
+
+template <typename T, int V>
+static int launch_move(MoveParams &P, bool combine, cudaStream_t st) {
+  const int64_t pieces = P.channels / V;
+  P.rows_per_launch_row = ((int64_t(1) << 31) - 512) / pieces;
+  if (P.rows_per_launch_row > P.n) P.rows_per_launch_row = P.n;
+  int bits = 0;
+  while ((int64_t(1) << bits) < pieces) ++bits;
+  P.div_shift = 31 + bits;
+  P.div_mul = ((uint64_t(1) << P.div_shift) + pieces - 1) / pieces;
+  const dim3 grid(static_cast<unsigned>(div_up(P.rows_per_launch_row * pieces, 256)), static_cast<unsigned>(div_up(P.n, P.rows_per_launch_row)));
+  SB_CHECK_ARG(grid.y < 65536, "too many rows x channels");
+  auto go = [&](auto kernel) -> int {
+    SB_CHECK_CUDA(launch_dependent(kernel, grid, dim3(256), 0, st, P));
+    return SPIRA_B200_OK;
+  };
+  if (combine) return P.k == 1 ? go(combine_kernel<T, V, 1>) : P.k == 2 ? go(combine_kernel<T, V, 2>) : P.k == 4 ? go(combine_kernel<T, V, 4>) : go(combine_kernel<T, V, 0>);
+  return P.k == 1 ? go(dispatch_kernel<T, V, 1>) : P.k == 2 ? go(dispatch_kernel<T, V, 2>) : P.k == 4 ? go(dispatch_kernel<T, V, 4>) : go(dispatch_kernel<T, V, 0>);
 }
 
 template <typename T, int V>
@@ -540,14 +640,17 @@ extern "C" int spira_b200_expert_route_backward(const void *logits, int dtype, i
   return SB_DISPATCH_ELEM(dtype, T, {
     const T *l = static_cast<const T *>(logits);
     T *d = static_cast<T *>(dlogits);
-    if (experts <= 16) {
-      SB_CHECK_CUDA(launch_dependent(route_backward_kernel<T, 8>, dim3(capped_blocks(n * 8, 256, 16)), dim3(256), 0, st, l, n, row_stride, experts, k,
+    auto go = [&](auto kernel, int lanes) -> int {
+      SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(div_up(n * lanes, 256))), dim3(256), 0, st, l, n, row_stride, experts, k,
                                      renormalize != 0 ? 1 : 0, weights, chosen, dweights, dweights_row, dweights_col, d));
-    } else {
-      SB_CHECK_CUDA(launch_dependent(route_backward_kernel<T, 32>, dim3(capped_blocks(n * 32, 256, 16)), dim3(256), 0, st, l, n, row_stride, experts, k,
-                                     renormalize != 0 ? 1 : 0, weights, chosen, dweights, dweights_row, dweights_col, d));
-    }
-    return SPIRA_B200_OK;
+      return SPIRA_B200_OK;
+    };
+    if (experts <= 8) return go(route_backward_kernel<T, 2, 4>, 2);
+    if (experts <= 16) return go(route_backward_kernel<T, 4, 4>, 4);
+    if (experts <= 32) return go(route_backward_kernel<T, 8, 4>, 8);
+    if (experts <= 64) return go(route_backward_kernel<T, 16, 4>, 16);
+    if (experts <= 128) return go(route_backward_kernel<T, 32, 4>, 32);
+    return go(route_backward_kernel<T, 32, 16>, 32);
   });
 }
 
@@ -563,10 +666,8 @@ extern "C" int spira_b200_expert_dispatch(const void *x, int dtype, int64_t n, i
   const bool wide = channels * size % 16 == 0 && rows_aligned(x, x_stride, size) && rows_aligned(rows, channels, size);
   cudaStream_t st = as_stream(stream);
   return SB_DISPATCH_ELEM(dtype, T, {
-    constexpr int V = 16 / sizeof(T);
-    if (wide) SB_CHECK_CUDA(launch_dependent(dispatch_kernel<T, V>, dim3(capped_blocks(n * (channels / V), 256, 16)), dim3(256), 0, st, P));
-    else SB_CHECK_CUDA(launch_dependent(dispatch_kernel<T, 1>, dim3(capped_blocks(n * channels, 256, 16)), dim3(256), 0, st, P));
-    return SPIRA_B200_OK;
+    if (wide) return launch_move<T, 16 / static_cast<int>(sizeof(T))>(P, false, st);
+    return launch_move<T, 1>(P, false, st);
   });
 }
 
@@ -582,10 +683,8 @@ extern "C" int spira_b200_expert_combine(const void *rows, int dtype, int64_t n,
   const bool wide = channels * size % 16 == 0 && rows_aligned(rows, row_stride, size) && rows_aligned(out, channels, size);
   cudaStream_t st = as_stream(stream);
   return SB_DISPATCH_ELEM(dtype, T, {
-    constexpr int V = 16 / sizeof(T);
-    if (wide) SB_CHECK_CUDA(launch_dependent(combine_kernel<T, V>, dim3(capped_blocks(n * (channels / V), 256, 16)), dim3(256), 0, st, P));
-    else SB_CHECK_CUDA(launch_dependent(combine_kernel<T, 1>, dim3(capped_blocks(n * channels, 256, 16)), dim3(256), 0, st, P));
-    return SPIRA_B200_OK;
+    if (wide) return launch_move<T, 16 / static_cast<int>(sizeof(T))>(P, true, st);
+    return launch_move<T, 1>(P, true, st);
   });
 }
 

@@ -105,25 +105,42 @@ __global__ void __launch_bounds__(kAThreads) grouped_any_kernel(const __grid_con
   const int g = lane >> 2, t4 = lane & 3;
   const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
   float acc[2][4][4] = {};
-  for (int k0 = k_begin; k0 < k_end; k0 += kAK) {
-    // neighbouring threads follow the direction in which the source is contiguous
-    for (int i = tid; i < kATile * kAK; i += kAThreads) {
+  // neighbouring threads follow the direction in which the source is contiguous; the next step's elements are on their way
+  // while this step multiplies
+  constexpr int kEach = kATile * kAK / kAThreads;
+  T ra[kEach], rb[kEach];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const int i = tid + q * kAThreads;
       const int m = MODE == kDw ? i % kATile : i / kAK, k = MODE == kDw ? i / kATile : i % kAK;
-      T v = zero;
+      ra[q] = zero;
       if (m0 + m < m_end && k0 + k < k_end)
-        v = MODE == kDw ? A[static_cast<int64_t>(k0 + k) * P.a_stride + m0 + m] : A[static_cast<int64_t>(m0 + m) * P.a_stride + k0 + k];
-      sa[m * kALd + k] = v;
+        ra[q] = MODE == kDw ? A[static_cast<int64_t>(k0 + k) * P.a_stride + m0 + m] : A[static_cast<int64_t>(m0 + m) * P.a_stride + k0 + k];
     }
-    for (int i = tid; i < kATile * kAK; i += kAThreads) {
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const int i = tid + q * kAThreads;
       const int n = MODE == kDx ? i / kAK : i % kATile, k = MODE == kDx ? i % kAK : i / kATile;
-      T v = zero;
+      rb[q] = zero;
       if (n0 + n < n_end && k0 + k < k_end) {
-        if (MODE == kForward) v = B[static_cast<int64_t>(k0 + k) * P.c_out + n0 + n];
-        else if (MODE == kDx) v = B[static_cast<int64_t>(n0 + n) * P.c_out + k0 + k];
-        else v = B[static_cast<int64_t>(k0 + k) * P.b_stride + n0 + n];
+        if (MODE == kForward) rb[q] = B[static_cast<int64_t>(k0 + k) * P.c_out + n0 + n];
+        else if (MODE == kDx) rb[q] = B[static_cast<int64_t>(n0 + n) * P.c_out + k0 + k];
+        else rb[q] = B[static_cast<int64_t>(k0 + k) * P.b_stride + n0 + n];
       }
-      sb_[n * kALd + k] = v;
     }
+  };
+  fetch(k_begin);
+  for (int k0 = k_begin; k0 < k_end; k0 += kAK) {
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const int i = tid + q * kAThreads;
+      const int m = MODE == kDw ? i % kATile : i / kAK, ka = MODE == kDw ? i / kATile : i % kAK;
+      const int n = MODE == kDx ? i / kAK : i % kATile, kb = MODE == kDx ? i % kAK : i / kATile;
+      sa[m * kALd + ka] = ra[q];
+      sb_[n * kALd + kb] = rb[q];
+    }
+    fetch(k0 + kAK);
     __syncthreads();
     const uint32_t *a32 = reinterpret_cast<const uint32_t *>(sa), *b32 = reinterpret_cast<const uint32_t *>(sb_);
 #pragma unroll
@@ -171,27 +188,43 @@ __global__ void __launch_bounds__(kAThreads) grouped_any_kernel(const __grid_con
       }
 }
 
+// Number of the first piece of group e and how many it has, by every warp for itself.
+__device__ __forceinline__ void group_pieces(const int32_t *offsets, int n, int e, int piece, int64_t &first, int &count) {
+  const int lane = threadIdx.x & 31;
+  int before = 0, highest = 0, last = 0;
+  for (int i0 = 0; i0 <= e; i0 += 32) {
+    const int i = i0 + lane;
+    int lo = i <= e ? clamped_offset(offsets, i, n) : 0;
+    int hi = i <= e ? clamped_offset(offsets, i + 1, n) : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, lo, d);
+      if (lane >= d && o > lo) lo = o;
+    }
+    lo = lo > highest ? lo : highest;
+    hi = hi > lo ? hi : lo;
+    const int mine = i <= e ? (hi - lo + piece - 1) / piece : 0;
+    int sum = mine;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    before += sum;
+    const int src = e - i0 < 31 ? e - i0 : 31;
+    last = __shfl_sync(0xffffffffu, mine, src);
+    highest = __shfl_sync(0xffffffffu, hi, 31);
+  }
+  first = before - last;
+  count = last;
+}
+
 // out[e][i] = sum over the pieces of group e, in order, of partial[piece][i]
 template <typename T>
 __global__ void __launch_bounds__(256) grouped_sum_kernel(const float *partial, const int32_t *offsets, int n, int experts, int piece, int64_t size, T *out) {
-  __shared__ int span[2];
   pdl_trigger();
   pdl_wait();
   const int e = blockIdx.y;
-  if (threadIdx.x == 0) {
-    int hi = clamped_offset(offsets, 0, n), first = 0, mine = 0;
-    for (int i = 0; i <= e; ++i) {
-      const int lo = hi, v = clamped_offset(offsets, i + 1, n);
-      hi = v > hi ? v : hi;
-      first += mine;
-      mine = (hi - lo + piece - 1) / piece;
-    }
-    span[0] = first;
-    span[1] = mine;
-  }
-  __syncthreads();
-  const int64_t first = span[0];
-  const int count = span[1];
+  int64_t first;
+  int count;
+  group_pieces(offsets, n, e, piece, first, count);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < size; i += static_cast<int64_t>(gridDim.x) * 256) {
     float t = 0.f;
 #pragma unroll 4
@@ -200,10 +233,11 @@ __global__ void __launch_bounds__(256) grouped_sum_kernel(const float *partial, 
   }
 }
 
-// dz = dy (y > 0) where a ReLU followed (dz != NULL), and partial column sums over pieces of a group's rows.
+// dz = dy where the ReLU let the value through (dz != NULL), and column sums over pieces of a group's rows.  What the ReLU
+// let through is a bit per element that the forward pass wrote (mask), or y > 0 where there is none.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) grouped_dz_kernel(const T *dy, int64_t dy_stride, const T *y, T *dz, float *partial, const int32_t *offsets,
-                                                         int n, int experts, int c_out, int piece) {
+__global__ void __launch_bounds__(256) grouped_dz_kernel(const T *dy, int64_t dy_stride, const T *y, const unsigned char *mask, int mask_pitch, T *dz,
+                                                         float *partial, const int32_t *offsets, int n, int experts, int c_out, int piece) {
   __shared__ float sums[256 * V];
   pdl_trigger();
   pdl_wait();
@@ -213,20 +247,37 @@ __global__ void __launch_bounds__(256) grouped_dz_kernel(const T *dy, int64_t dy
   const int vecs = c_out / V, wide = vecs - static_cast<int>(blockIdx.y) * 256 < 256 ? vecs - static_cast<int>(blockIdx.y) * 256 : 256;
   const int lanes = 256 / wide;                 // rows in parallel
   const int lane = threadIdx.x / wide, c = (blockIdx.y * 256 + threadIdx.x % wide) * V;
+  constexpr int kBatch = 4;                     // rows of a thread in flight
   float sum[V] = {};
   if (lane < lanes)
-    for (int r = r0 + lane; r < r1; r += lanes) {
-      float d[V];
-      load_f32<T, V>(dy + r * dy_stride + c, d);
-      if (dz) {
-        float f[V];
-        load_f32<T, V>(y + static_cast<int64_t>(r) * c_out + c, f);
+    for (int r = r0 + lane; r < r1; r += kBatch * lanes) {
+      Vec<T, V> d[kBatch], f[kBatch];
+      unsigned bits[kBatch];
 #pragma unroll
-        for (int i = 0; i < V; ++i) d[i] = f[i] > 0.f ? d[i] : 0.f;
-        store_f32<T, V>(dz + static_cast<int64_t>(r) * c_out + c, d);
+      for (int q = 0; q < kBatch; ++q) {
+        const int64_t row = r + q * lanes;
+        d[q] = Vec<T, V>{};
+        f[q] = Vec<T, V>{};
+        bits[q] = 0;
+        if (row < r1) {
+          d[q] = *reinterpret_cast<const Vec<T, V> *>(dy + row * dy_stride + c);
+          if (mask) bits[q] = mask[row * mask_pitch + c / 8] >> (c & 7);
+          else if (y) f[q] = *reinterpret_cast<const Vec<T, V> *>(y + row * c_out + c);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] += d[i];
+      for (int q = 0; q < kBatch; ++q) {
+        const int64_t row = r + q * lanes;
+        if (row >= r1) break;
+        if (dz) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (mask ? !(bits[q] >> i & 1) : !(to_f32(f[q].v[i]) > 0.f)) d[q].v[i] = from_f32<T>(0.f);
+          *reinterpret_cast<Vec<T, V> *>(dz + row * c_out + c) = d[q];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += to_f32(d[q].v[i]);
+      }
     }
   if (partial == nullptr) return;
 #pragma unroll
@@ -239,17 +290,44 @@ __global__ void __launch_bounds__(256) grouped_dz_kernel(const T *dy, int64_t dy
   }
 }
 
-constexpr int kDzPiece = 256;
+// Column sums of many short pieces: 32 columns x 32 strides of pieces per block, then a fixed tree.
+template <typename T>
+__global__ void __launch_bounds__(1024) grouped_column_sum_kernel(const float *partial, const int32_t *offsets, int n, int experts, int piece, int size, T *out) {
+  __shared__ float part[32][33];
+  pdl_trigger();
+  pdl_wait();
+  const int e = blockIdx.y, lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  int64_t first;
+  int count;
+  group_pieces(offsets, n, e, piece, first, count);
+  float t = 0.f;
+  if (c < size)
+#pragma unroll 4
+    for (int p = w; p < count; p += 32) t += partial[(first + p) * size + c];
+  part[w][lane] = t;
+  __syncthreads();
+  t = part[lane][w];
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) t += __shfl_xor_sync(0xffffffffu, t, d);
+  const int co = blockIdx.x * 32 + w;
+  if (lane == 0 && co < size) out[static_cast<int64_t>(e) * size + co] = from_f32<T>(t);
+}
+
+// Rows per piece of the column sums: a CTA per piece, two rounds of CTAs on the SMs, 32 to 256 rows.
+static int dz_piece(int64_t n) {
+  const int64_t p = div_up(div_up(n, 16 * sm_count()), 32) * 32;
+  return static_cast<int>(p < 32 ? 32 : p > 256 ? 256 : p);
+}
 
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Rows of a group that one CTA of the weight gradient adds up (0: all of them).  Splitting fills the SMs when the weight
-// matrices have few tiles, at the price of fp32 partial sums: `ctas` per SM, at least 256 rows each.
+// matrices have few tiles, at the price of fp32 partial sums: `ctas` per SM, at least 128 rows each.
 static int dw_piece(int64_t n, int experts, int64_t tiles, int ctas) {
-  if (tiles * experts >= sm_count() || n <= 256) return 0;
+  if (tiles * experts >= sm_count() || n <= 128) return 0;
   const int64_t pieces = div_up(ctas * static_cast<int64_t>(sm_count()), tiles);
   int64_t piece = div_up(div_up(n, pieces), 64) * 64;
-  if (piece < 256) piece = 256;
+  if (piece < 128) piece = 128;
   return piece >= n ? 0 : static_cast<int>(piece);
 }
 
@@ -307,6 +385,7 @@ extern "C" int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, in
   if (rc != SPIRA_B200_OK || desc->n == 0) return rc;
   const spira_b200_grouped_desc &D = *desc;
   SB_CHECK_ARG(D.x && D.weight && D.y, "grouped_linear: null pointer");
+  SB_CHECK_ARG(!D.mask || (D.relu && tc_forward(D)), "grouped_linear: no mask is written for this call (spira_b200_grouped_linear_mask_bytes is 0)");
   if (tc_forward(D)) return grouped_tc_run(kForward, D, 0, nullptr, status, wait_ns(), as_stream(stream));
   GroupedParams P{D.x, D.weight, D.bias, D.offsets, D.y, nullptr, D.x_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, D.relu, 0};
   return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kForward>(P, as_stream(stream))););
@@ -367,7 +446,7 @@ extern "C" int spira_b200_grouped_linear_dz_workspace(const spira_b200_grouped_d
   int rc = grouped_check("grouped_linear_dz", desc);
   if (rc != SPIRA_B200_OK) return rc;
   SB_CHECK_ARG(bytes, "grouped_linear_dz: null pointer");
-  *bytes = desc->dbias ? static_cast<size_t>(group_tiles_bound(desc->n, desc->experts, kDzPiece)) * desc->c_out * 4 : 0;
+  *bytes = desc->dbias ? static_cast<size_t>(group_tiles_bound(desc->n, desc->experts, dz_piece(desc->n))) * desc->c_out * 4 : 0;
   return SPIRA_B200_OK;
 }
 
@@ -381,7 +460,7 @@ extern "C" int spira_b200_grouped_linear_dz(const spira_b200_grouped_desc *desc,
     if (D.dbias) SB_CHECK_CUDA(cudaMemsetAsync(D.dbias, 0, static_cast<size_t>(D.experts) * D.c_out * 2, st));
     return SPIRA_B200_OK;
   }
-  SB_CHECK_ARG(D.dy && (!D.dz || D.y), "grouped_linear_dz: null pointer");
+  SB_CHECK_ARG(D.dy && (!D.dz || D.y || D.mask), "grouped_linear_dz: null pointer");
   size_t need = 0;
   rc = spira_b200_grouped_linear_dz_workspace(desc, &need);
   if (rc != SPIRA_B200_OK) return rc;
@@ -389,23 +468,28 @@ extern "C" int spira_b200_grouped_linear_dz(const spira_b200_grouped_desc *desc,
     return fail(SPIRA_B200_ERR_WORKSPACE, "grouped_linear_dz: workspace of %zu bytes is smaller than %zu", workspace_bytes, need);
   float *partial = D.dbias ? static_cast<float *>(workspace) : nullptr;
   const int n = static_cast<int>(D.n);
-  const unsigned units = static_cast<unsigned>(group_tiles_bound(n, D.experts, kDzPiece));
+  const int piece = dz_piece(n);
+  const unsigned units = static_cast<unsigned>(group_tiles_bound(n, D.experts, piece));
   const bool wide = D.c_out % 8 == 0 && aligned16(D.dy) && D.dy_stride % 8 == 0 && aligned16(D.y) && aligned16(D.dz);
   return SB_DISPATCH_HALF(D.dtype, T, {
-    const T *dy = static_cast<const T *>(D.dy);
-    const T *y = static_cast<const T *>(D.y);
-    T *dz = static_cast<T *>(D.dz);
-    if (wide) {
-      SB_CHECK_CUDA(launch_dependent(grouped_dz_kernel<T, 8>, dim3(units, static_cast<unsigned>(div_up(D.c_out / 8, 256))), dim3(256), 0, st, dy, D.dy_stride,
-                                     y, dz, partial, D.offsets, n, D.experts, D.c_out, kDzPiece));
-    } else {
-      SB_CHECK_CUDA(launch_dependent(grouped_dz_kernel<T, 1>, dim3(units, static_cast<unsigned>(div_up(D.c_out, 256))), dim3(256), 0, st, dy, D.dy_stride, y,
-                                     dz, partial, D.offsets, n, D.experts, D.c_out, kDzPiece));
-    }
-    if (!D.dbias) return SPIRA_B200_OK;
-    SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 256)), D.experts), dim3(256), 0, st,
-                                   static_cast<const float *>(partial), D.offsets, n, D.experts, kDzPiece, static_cast<int64_t>(D.c_out),
-                                   static_cast<T *>(D.dbias)));
+    auto go = [&](auto kernel, int columns) -> int {
+      SB_CHECK_CUDA(launch_dependent(kernel, dim3(units, static_cast<unsigned>(div_up(columns, 256))), dim3(256), 0, st, static_cast<const T *>(D.dy),
+                                     D.dy_stride, static_cast<const T *>(D.y), static_cast<const unsigned char *>(D.mask), mask_pitch(D.c_out),
+                                     static_cast<T *>(D.dz), partial, D.offsets, n, D.experts, D.c_out, piece));
+      return SPIRA_B200_OK;
+    };
+    rc = wide ? go(grouped_dz_kernel<T, 8>, D.c_out / 8) : go(grouped_dz_kernel<T, 1>, D.c_out);
+    if (rc != SPIRA_B200_OK || !D.dbias) return rc;
+    SB_CHECK_CUDA(launch_dependent(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(1024), 0, st,
+                                   static_cast<const float *>(partial), D.offsets, n, D.experts, piece, D.c_out, static_cast<T *>(D.dbias)));
     return SPIRA_B200_OK;
   });
+}
+
+extern "C" int spira_b200_grouped_linear_mask_bytes(const spira_b200_grouped_desc *desc, size_t *bytes) {
+  int rc = grouped_check("grouped_linear_mask", desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(bytes, "grouped_linear_mask: null pointer");
+  *bytes = desc->n > 0 && desc->relu && tc_forward(*desc) ? static_cast<size_t>(desc->n) * mask_pitch(desc->c_out) : 0;
+  return SPIRA_B200_OK;
 }

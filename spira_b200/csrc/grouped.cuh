@@ -79,6 +79,9 @@ __device__ __forceinline__ void group_span(const int32_t *offsets, int experts, 
 // upper bound of the number of tiles of `rows` rows, for a host that does not know the offsets
 inline int64_t group_tiles_bound(int64_t n, int experts, int64_t rows) { return n / rows + (experts < n ? experts : n); }
 
+// Bytes per row of the ReLU mask: a bit per column, rows of whole 4-byte words.
+inline int mask_pitch(int c_out) { return (c_out + 31) / 32 * 4; }
+
 // The tensor-core path (grouped_tc.cu).  It takes channel counts in whole 16-byte units and 16-byte aligned tensors and rows.
 enum { kForward = 0, kDx = 1, kDw = 2 };
 bool grouped_tc_available();

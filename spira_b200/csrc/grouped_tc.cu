@@ -9,10 +9,14 @@
 // group belong to the next one, they are multiplied and not stored.  In dW the rows are the reduction: the last step of a
 // group overwrites foreign rows with zeros in BOTH operands in shared memory (0 * NaN of a neighbour would not be 0).
 //
-// One persistent CTA per SM, 12 warps: warp 0 issues TMA loads, warp 1 the MMAs, warps 4-11 (two per tensor-memory lane
-// quarter) convert and store while the next tile accumulates in the other half of tensor memory.  Every CTA reads the group
+// One persistent CTA per SM, 20 warps: warp 0 issues TMA loads, warp 1 the MMAs, warps 4-19 (four per tensor-memory lane
+// quarter, a quarter of the columns each) convert and store while the next tile accumulates in the other half of tensor
+// memory.  Narrow products (few reduction steps per tile) are bound by this conversion: it takes 2.5 instructions per
+// element with bias and ReLU, the mask of the ReLU two more.  Every CTA reads the group
 // boundaries once into shared memory.  Every wait is bounded; an expired one raises the status word.
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "elem.cuh"
@@ -29,9 +33,11 @@ constexpr int kGABytes = kGRows * kGK * 2;
 constexpr int kGBlock = kGK * 64 * 2;          // one 64 x 64 box
 constexpr int kGMaxN = 256;
 constexpr int kGMaxStages = 8;
-constexpr int kGEpilogueWarps = 8, kGFirstEpilogueWarp = 4;
+constexpr int kGEpilogueWarps = 16, kGFirstEpilogueWarp = 4;
 constexpr int kGThreads = (kGFirstEpilogueWarp + kGEpilogueWarps) * 32;
 constexpr int kGSmemBudget = 224 * 1024;
+constexpr int kGBiasBytes = kGEpilogueWarps * 64 * 4;   // a warp's columns of the bias as fp32
+constexpr int kGSorted = 64;                   // groups up to which dW takes the longest first
 
 struct GroupedTcParams {
   const int32_t *offsets;
@@ -42,7 +48,9 @@ struct GroupedTcParams {
   int n, experts, m_channels, n_channels, k_channels;   // m_channels: c_in in dW; k_channels: 0 in dW (rows)
   int relu, piece;           // piece: rows per unit of dW, 0 = whole groups
   int bn, n_tiles, m_tiles;  // columns per tile, column tiles, row tiles of dW
-  int stages, b_bytes, acc_stride, tmem_cols, off_bar, off_groups;
+  int stages, b_bytes, acc_stride, tmem_cols, off_bias, off_bar, off_groups;
+  unsigned char *mask;       // forward: a bit per element that the ReLU let through
+  int mask_pitch;
   uint32_t idesc;
   unsigned long long wait_ns;
 };
@@ -79,14 +87,15 @@ struct TcTile {
 
 template <int MODE>
 struct TileWalk {
-  const int *rows, *first;             // shared memory: group boundaries, first unit of every group
-  int expert = 0;
+  const int *rows, *first, *by_size;   // shared memory: group boundaries, first unit of every group, dW: groups by length
+  int place = 0;
   __device__ __forceinline__ TcTile at(const GroupedTcParams &P, int t) {
     TcTile r;
     const int per_unit = MODE == kDw ? P.m_tiles * P.n_tiles : P.n_tiles;
     const int unit = t / per_unit, in_unit = t - unit * per_unit;
-    while (unit >= first[expert + 1]) ++expert;        // (t only grows)
-    const int index = unit - first[expert];
+    while (unit >= first[place + 1]) ++place;          // (t only grows)
+    const int index = unit - first[place];
+    const int expert = MODE == kDw && P.piece == 0 && P.experts <= kGSorted ? by_size[place] : place;
     r.expert = expert;
     r.unit = unit;
     r.n0 = in_unit % P.n_tiles * P.bn;
@@ -107,7 +116,7 @@ struct TileWalk {
 
 // Group boundaries (clamped, never falling) and the first unit of every group, by one warp.
 template <int MODE>
-__device__ __forceinline__ void read_groups(const GroupedTcParams &P, int *rows, int *first) {
+__device__ __forceinline__ void read_groups(const GroupedTcParams &P, int *rows, int *first, int *by_size) {
   const int lane = threadIdx.x & 31;
   int highest = 0, units = 0;
   for (int e0 = 0; e0 <= P.experts; e0 += 32) {
@@ -138,63 +147,80 @@ __device__ __forceinline__ void read_groups(const GroupedTcParams &P, int *rows,
     units += __shfl_sync(0xffffffffu, sum, 31);
   }
   if (lane == 0) first[P.experts] = units;
+  // whole groups as units of dW: the longest first, so that the last round of CTAs has the short ones
+  if (MODE == kDw && P.piece == 0 && P.experts <= kGSorted)
+    for (int e = lane; e < P.experts; e += 32) {
+      const int mine = rows[e + 1] - rows[e];
+      int rank = 0;
+      for (int f = 0; f < P.experts; ++f) {
+        const int other = rows[f + 1] - rows[f];
+        rank += other > mine || (other == mine && f < e);
+      }
+      by_size[rank] = e;
+    }
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t *>(&h);
-}
+// The CTA's tile of round r: rounds run over the CTAs in alternating direction.
+__device__ __forceinline__ int round_tile(int r) { return r * static_cast<int>(gridDim.x) + (r & 1 ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x)); }
 
-// Up to 32 columns of one row of the accumulator: bias, ReLU, one rounding, whole 32-byte sectors where they are aligned.
-template <typename T, int MODE>
-__device__ __forceinline__ void store_columns(const GroupedTcParams &P, const TcTile &tile, int m, int c0, int c_stop, const uint32_t (&r)[32]) {
-  const int col = tile.n0 + c0;
-  if (MODE == kDw && P.piece) {
-    float *dst = P.partial + (static_cast<int64_t>(tile.unit) * P.m_channels + m) * P.n_channels + col;
-#pragma unroll
-    for (int i = 0; i < 32; i += 4)
-      if (c0 + i < c_stop) *reinterpret_cast<uint4 *>(dst + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
-    return;
+// Two values rounded into one word (a in the low half), negative ones to zero with kRelu (a NaN stays).
+template <typename T, bool kRelu>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) {
+    if (kRelu) asm("cvt.rn.relu.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  } else {
+    if (kRelu) asm("cvt.rn.relu.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   }
-  T *dst = static_cast<T *>(P.out) + (MODE == kDw ? static_cast<int64_t>(tile.expert) * P.m_channels + m : static_cast<int64_t>(m)) * P.n_channels + col;
+  return r;
+}
+
+// W (16 or 32) columns of one row of the accumulator, rounded and stored in whole 32-byte sectors where they are aligned.
+// `bits` gets a bit per column, set where the value is positive (the sign of 0 - v).
+template <typename T, int W, bool kRelu>
+__device__ __forceinline__ void store_columns(uint32_t (&r)[W], const float *bias, bool want_bits, T *dst, int valid, uint32_t &bits) {
+  if (bias) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const float4 b = *reinterpret_cast<const float4 *>(bias + i);
+      r[i] = __float_as_uint(__uint_as_float(r[i]) + b.x);
+      r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) + b.y);
+      r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) + b.z);
+      r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) + b.w);
+    }
+  }
+  if (kRelu && want_bits) {
+    bits = 0;
+#pragma unroll
+    for (int i = W - 1; i >= 0; --i) bits = __funnelshift_l(__float_as_uint(0.f - __uint_as_float(r[i])), bits, 1);
+  }
   const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
 #pragma unroll
-  for (int i = 0; i < 32; i += 16) {
-    if (c0 + i >= c_stop) break;
-    uint4 pack[2];
+  for (int i = 0; i < W; i += 16) {
+    uint4 v[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[i + 8 * h + e]);
-      if (MODE == kForward) {
-        if (P.bias && c0 + i + 8 * h < c_stop) {
-          float bias[8];
-          load_f32<T, 8>(static_cast<const T *>(P.bias) + static_cast<int64_t>(tile.expert) * P.n_channels + col + i + 8 * h, bias);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] += bias[e];
-        }
-        if (P.relu)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = f[e] < 0.f ? 0.f : f[e];      // (a NaN stays)
-      }
-      pack[h] = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+      const uint32_t *q = r + i + 8 * h;
+      v[h] = make_uint4(pack2<T, kRelu>(__uint_as_float(q[0]), __uint_as_float(q[1])), pack2<T, kRelu>(__uint_as_float(q[2]), __uint_as_float(q[3])),
+                        pack2<T, kRelu>(__uint_as_float(q[4]), __uint_as_float(q[5])), pack2<T, kRelu>(__uint_as_float(q[6]), __uint_as_float(q[7])));
     }
-    if (wide && c0 + i + 16 <= c_stop) {
-      st_global_v8(dst + i, pack[0], pack[1]);
+    if (wide && i + 16 <= valid) {
+      st_global_v8(dst + i, v[0], v[1]);
     } else {
-      *reinterpret_cast<uint4 *>(dst + i) = pack[0];
-      if (c0 + i + 8 < c_stop) *reinterpret_cast<uint4 *>(dst + i + 8) = pack[1];
+      if (i < valid) *reinterpret_cast<uint4 *>(dst + i) = v[0];
+      if (i + 8 < valid) *reinterpret_cast<uint4 *>(dst + i + 8) = v[1];
     }
   }
+}
+
+// fp32 partial sums of dW: W columns of one row.
+template <int W>
+__device__ __forceinline__ void store_partial(const uint32_t (&r)[W], float *dst, int valid) {
+#pragma unroll
+  for (int i = 0; i < W; i += 4)
+    if (i < valid) *reinterpret_cast<uint4 *>(dst + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
 }
 
 template <typename T, int MODE>
@@ -211,7 +237,7 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
   auto bar_acc_empty = [&](int b) { return bar0 + 8u * (2 * kGMaxStages + 2 + b); };
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + P.off_bar + 8 * (2 * kGMaxStages + 4));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + P.off_bar + 8 * (2 * kGMaxStages + 4) + 4);
-  int *rows = reinterpret_cast<int *>(smem + P.off_groups), *first = rows + P.experts + 1;
+  int *rows = reinterpret_cast<int *>(smem + P.off_groups), *first = rows + P.experts + 1, *by_size = first + P.experts + 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int stages = P.stages, stage_bytes = kGABytes + P.b_bytes;
@@ -232,21 +258,24 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
     tmem_relinquish();
   }
   pdl_wait();            // before the first global read of any thread
-  if (warp == 2) read_groups<MODE>(P, rows, first);
+  if (warp == 2) read_groups<MODE>(P, rows, first, by_size);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   pdl_trigger();         // (behind the allocation: a CTA of the next kernel on this SM cannot take the tensor memory first)
   const uint32_t tmem_base = *tmem_slot;
   const int total = first[P.experts] * (MODE == kDw ? P.m_tiles * P.n_tiles : P.n_tiles), G = gridDim.x;
-  TileWalk<MODE> walk{rows, first};
+  TileWalk<MODE> walk{rows, first, by_size};
+  const int rounds = (total + G - 1) / G;
 
   if (warp == 0) {
     // =========================== TMA loads ===========================
     if (lane == 0) {
       int stage = 0, phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < total; t += G) {
+      for (int round = 0; ok && round < rounds; ++round) {
+        const int t = round_tile(round);
+        if (t >= total) break;
         const TcTile tile = walk.at(P, t);
         for (int j = 0; j < tile.steps; ++j) {
           if (!mbar_wait(bar_empty(stage), phase ^ 1, abort_flag, P.wait_ns)) { ok = false; break; }
@@ -274,7 +303,9 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
     int stage = 0, phase = 0, tile_i = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < total; t += G, ++tile_i) {
+    for (; ok && tile_i < rounds; ++tile_i) {
+      const int t = round_tile(tile_i);
+      if (t >= total) break;
       const TcTile tile = walk.at(P, t);
       const int b = tile_i & 1;
       // (the whole warp leaves together: lanes may see the abort flag at different times)
@@ -315,34 +346,80 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
     }
   } else if (warp >= kGFirstEpilogueWarp) {
     // =========================== epilogue ===========================
-    const int q = warp & 3, half = (warp - kGFirstEpilogueWarp) >> 2;
-    const int c_split = ((P.bn >> 1) + 15) & ~15;
+    const int q = warp & 3, part = (warp - kGFirstEpilogueWarp) >> 2;
+    const int width = P.bn / 4;                      // columns of this warp: a multiple of 16, at most 64
+    float *bias_s = reinterpret_cast<float *>(smem + P.off_bias) + (warp - kGFirstEpilogueWarp) * 64;
+    const bool relu = MODE == kForward && P.relu;
+    int bias_at = -1;                                // what bias_s holds: expert * n_tiles + column tile
     uint32_t acc_phase = 0;
-    int tile_i = 0;
-    for (int t = blockIdx.x; t < total; t += G, ++tile_i) {
+    for (int tile_i = 0; tile_i < rounds; ++tile_i) {
+      const int t = round_tile(tile_i);
+      if (t >= total) break;
       const TcTile tile = walk.at(P, t);
       const int b = tile_i & 1;
-      const int m = (MODE == kDw ? tile.m0 : tile.row0) + q * 32 + lane;
-      const bool live = m < (MODE == kDw ? P.m_channels : tile.row_end);
-      const int n_end = tile.n0 + P.bn < P.n_channels ? P.bn : P.n_channels - tile.n0;      // columns of this tile
-      const int c_begin = half ? c_split : 0, c_stop = half ? n_end : (n_end < c_split ? n_end : c_split);
+      const int m = (MODE == kDw ? tile.m0 : tile.row0) + q * 32 + lane, m_end = MODE == kDw ? P.m_channels : tile.row_end;
+      const int col = tile.n0 + part * width;
+      const int valid = m < m_end ? P.n_channels - col : 0;      // columns of this row that exist (a multiple of 8)
+      const float *bias = nullptr;
+      if (MODE == kForward && P.bias) {
+        const int at = tile.expert * P.n_tiles + tile.n0 / P.bn;
+        if (at != bias_at) {
+          bias_at = at;
+          const T *src = static_cast<const T *>(P.bias) + static_cast<int64_t>(tile.expert) * P.n_channels + col;
+          __syncwarp();
+          for (int i = lane; i < width; i += 32) bias_s[i] = col + i < P.n_channels ? to_f32(src[i]) : 0.f;
+          __syncwarp();
+        }
+        bias = bias_s;
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(bar_acc_full(b), (acc_phase >> b) & 1u, abort_flag, P.wait_ns))) break;
       acc_phase ^= 1u << b;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + b * P.acc_stride + (static_cast<uint32_t>(q * 32) << 16);
-      for (int c0 = c_begin; c0 < c_stop; c0 += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32(taddr + c0, r);       // (columns behind the accumulator are read and not used)
-        tmem_ld_wait();
+      const uint32_t taddr = tmem_base + b * P.acc_stride + (static_cast<uint32_t>(q * 32) << 16) + part * width;
+      const int64_t out_row = MODE == kDw ? static_cast<int64_t>(tile.expert) * P.m_channels + m : m;
+      T *dst = static_cast<T *>(P.out) + out_row * P.n_channels + col;
+      float *dst_partial = MODE == kDw ? P.partial + (static_cast<int64_t>(tile.unit) * P.m_channels + m) * P.n_channels + col : nullptr;
+      uint32_t bits[2] = {0, 0};
+      auto emit = [&](auto &r, int c0, uint32_t &word) {
+        constexpr int W = sizeof(r) / 4;
         if (MODE == kDw && tile.steps == 0) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0;
+          for (int i = 0; i < W; ++i) r[i] = 0;
         }
-        if (live) store_columns<T, MODE>(P, tile, m, c0, c_stop, r);
+        if (c0 < valid) {
+          if (MODE == kDw && P.piece) store_partial<W>(r, dst_partial + c0, valid - c0);
+          else if (relu) store_columns<T, W, true>(r, bias ? bias + c0 : nullptr, P.mask != nullptr, dst + c0, valid - c0, word);
+          else store_columns<T, W, false>(r, bias ? bias + c0 : nullptr, false, dst + c0, valid - c0, word);
+        }
         __syncwarp();
+      };
+#pragma unroll
+      for (int piece = 0; piece < 2; ++piece) {
+        const int c0 = 32 * piece;
+        if (width - c0 >= 32) {
+          uint32_t r[32];
+          tmem_ld_32x32(taddr + c0, r);
+          tmem_ld_wait();
+          emit(r, c0, bits[piece]);
+        } else if (width - c0 == 16) {
+          uint32_t r[16];
+          tmem_ld_32x16(taddr + c0, r);
+          tmem_ld_wait();
+          emit(r, c0, bits[piece]);
+        }
       }
       tc_fence_before();
       mbar_arrive(bar_acc_empty(b));
+      if (MODE == kForward && P.mask && valid > 0) {
+        unsigned char *line = P.mask + static_cast<int64_t>(m) * P.mask_pitch + col / 8;
+        if (width == 64 && (reinterpret_cast<uintptr_t>(line) & 7) == 0 && valid > 32) {
+          *reinterpret_cast<uint2 *>(line) = make_uint2(bits[0], bits[1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * i < width && 16 * i < valid) *reinterpret_cast<uint16_t *>(line + 2 * i) = static_cast<uint16_t>(bits[i / 2] >> (16 * (i & 1)));
+        }
+      }
     }
   } else if (warp == 3 && MODE != kDw) {
     // rows of no group are zero
@@ -400,12 +477,12 @@ bool grouped_tc_rows_ok(const void *p, int64_t stride, int channels, int64_t n) 
 }
 bool grouped_tc_available() { return grouped_encode_fn() != nullptr; }
 
-// Columns per tile: as few tiles of at most 256 as the width needs, of equal size; when the tiles would not fill the SMs
-// (few rows), narrower ones down to 64.
+// Columns per tile: as few tiles of at most 256 as the width needs, of equal size in whole
+// units of 64; when the tiles would not fill the SMs (few rows), narrower ones.
 static int columns_per_tile(int channels, int64_t units) {
   int64_t tiles = div_up(channels, kGMaxN);
   while (tiles * units < sm_count() && div_up(channels, 2 * tiles) >= 64) tiles *= 2;
-  return static_cast<int>(div_up(div_up(channels, tiles), 16) * 16);
+  return static_cast<int>(div_up(div_up(channels, tiles), 64) * 64);
 }
 
 int grouped_tc_dw_tiles(int c_in, int c_out) {
@@ -433,6 +510,8 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
     P.out = mode == kForward ? D.y : D.dx;
     P.bias = mode == kForward ? D.bias : nullptr;
     P.relu = mode == kForward ? D.relu : 0;
+    P.mask = mode == kForward ? static_cast<unsigned char *>(D.mask) : nullptr;
+    P.mask_pitch = mask_pitch(D.c_out);
     P.n_channels = mode == kForward ? D.c_out : D.c_in;
     P.k_channels = mode == kForward ? D.c_in : D.c_out;
     P.m_tiles = 1;
@@ -447,13 +526,14 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
   P.tmem_cols = 2 * P.acc_stride;
   P.idesc = (1u << 4) | (D.dtype == SPIRA_B200_BF16 ? (1u << 7) | (1u << 10) : 0u) | (mode == kDw ? 1u << 15 : 0u) | (b_n_major ? 1u << 16 : 0u) |
             (static_cast<uint32_t>(P.bn >> 3) << 17) | ((128u >> 4) << 24);
-  const int fixed = 8 * (2 * kGMaxStages + 5) + 16 + 8 * (D.experts + 2);
+  const int fixed = kGBiasBytes + 8 * (2 * kGMaxStages + 5) + 16 + 12 * (D.experts + 2);
   const int stage_bytes = kGABytes + P.b_bytes;      // (multiples of 1024: 8 KB boxes, or bn * 128 with bn a multiple of 16)
   P.stages = (kGSmemBudget - fixed) / stage_bytes;
   if (P.stages > kGMaxStages) P.stages = kGMaxStages;
-  P.off_bar = P.stages * stage_bytes;
+  P.off_bias = P.stages * stage_bytes;
+  P.off_bar = P.off_bias + kGBiasBytes;
   P.off_groups = P.off_bar + 8 * (2 * kGMaxStages + 5) + 8;
-  const size_t smem = static_cast<size_t>(P.off_bar) + fixed + 1024;
+  const size_t smem = static_cast<size_t>(P.off_bias) + fixed + 1024;
 
   alignas(64) CUtensorMap map_a, map_b;
   int rc;

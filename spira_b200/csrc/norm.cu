@@ -19,6 +19,7 @@ namespace sb {
 
 constexpr int kNormMaxChannels = 8192;
 constexpr int kGateNone = 0, kGateChannel = 1, kGateRow = 2, kGateFull = 3;
+constexpr int kNormBackwardCtas = 3;     // per SM at most: every CTA writes one set of partial sums
 constexpr int kSums = 5;      // weight, bias, post_weight, post_bias, gate
 
 struct NormParams {
@@ -104,7 +105,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[ITEMS][V], const bool
 
 // L threads per row, each with ITEMS pieces of V neighbouring channels, L pieces apart.
 template <typename T, int V, int L, int ITEMS>
-__global__ void __launch_bounds__(L > 256 ? L : 256) norm_forward_kernel(const __grid_constant__ NormParams P) {
+__global__ void __launch_bounds__(L > 256 ? L : 256, ITEMS > 1 || L > 256 ? 1 : 3) norm_forward_kernel(const __grid_constant__ NormParams P) {
   constexpr int kThreads = L > 256 ? L : 256;
   __shared__ float scratch[32];
   pdl_trigger();
@@ -115,18 +116,39 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) norm_forward_kernel(const _
   bool in[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) in[i] = (i * L + g) * V < P.channels;
+  // the next row's values are on their way while this row is worked on
+  Vec<T, V> raw_x[ITEMS], raw_p[ITEMS], raw_g[ITEMS];
+  auto fetch = [&](int64_t b) {
+    const int64_t row = b * kRows + threadIdx.x / L;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      raw_x[i] = raw_p[i] = raw_g[i] = Vec<T, V>{};
+      if (b < rounds && row < P.n && in[i]) {
+        const int c = (i * L + g) * V;
+        raw_x[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.x) + row * P.x_stride + c);
+        if (P.block) raw_p[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.block) + row * P.block_stride + c);
+        if (P.gate_kind == kGateFull) raw_g[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.gate) + row * P.gate_stride + c);
+      }
+    }
+  };
+  constexpr bool kAhead = ITEMS <= 2;
+  if (kAhead) fetch(blockIdx.x);
   for (int64_t b = blockIdx.x; b < rounds; b += gridDim.x) {
     const int64_t row = b * kRows + threadIdx.x / L;
     const bool live = row < P.n;
-    float x[ITEMS][V] = {}, p[ITEMS][V] = {};
-    if (live) {
+    if (!kAhead) fetch(b);
+    float x[ITEMS][V], p[ITEMS][V];
+    Vec<T, V> gates[ITEMS];
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-        if (in[i]) {
-          load_f32<T, V>(static_cast<const T *>(P.x) + row * P.x_stride + (i * L + g) * V, x[i]);
-          if (P.block) load_f32<T, V>(static_cast<const T *>(P.block) + row * P.block_stride + (i * L + g) * V, p[i]);
-        }
+    for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        x[i][e] = to_f32(raw_x[i].v[e]);
+        p[i][e] = to_f32(raw_p[i].v[e]);
+      }
+      gates[i] = raw_g[i];
     }
+    if (kAhead) fetch(b + gridDim.x);
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
     if (P.block) {
       if (P.post) {
@@ -157,10 +179,9 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) norm_forward_kernel(const _
         const int c = (i * L + g) * V;
         float gate[V];
         if (P.gate_kind == kGateChannel) load_param<T, V>(P.gate, P.params_f32, c, gate);
-        else if (P.gate_kind == kGateFull && live) load_f32<T, V>(static_cast<const T *>(P.gate) + row * P.gate_stride + c, gate);
         else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) gate[e] = row_gate;
+          for (int e = 0; e < V; ++e) gate[e] = P.gate_kind == kGateFull ? to_f32(gates[i].v[e]) : row_gate;
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) x[i][e] = P.residual_scale * x[i][e] + P.block_scale * (gate[e] * p[i][e]);
@@ -194,7 +215,7 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) norm_forward_kernel(const _
 }
 
 template <typename T, int V, int L, int ITEMS>
-__global__ void __launch_bounds__(L > 256 ? L : 256) norm_backward_kernel(const __grid_constant__ NormParams P) {
+__global__ void __launch_bounds__(L > 256 ? L : 256, ITEMS > 1 || L > 256 ? 1 : 2) norm_backward_kernel(const __grid_constant__ NormParams P) {
   constexpr int kThreads = L > 256 ? L : 256;
   __shared__ float scratch[64];
   extern __shared__ float column_sums[];      // [kThreads / L][channels]
@@ -208,25 +229,46 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) norm_backward_kernel(const 
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) in[i] = (i * L + g) * V < P.channels;
   float sum[kSums][ITEMS][V] = {};
+  Vec<T, V> raw_x[ITEMS], raw_p[ITEMS], raw_g[ITEMS], raw_d[ITEMS], raw_h[ITEMS];
+  float4 raw_st = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto piece = [&](const void *base, int64_t at) { return *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(base) + at); };
+  auto fetch = [&](int64_t b) {
+    const int64_t row = b * kRows + threadIdx.x / L;
+    const bool there = b < rounds && row < P.n;
+    if (there) raw_st = reinterpret_cast<const float4 *>(P.stats)[row];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      raw_x[i] = raw_p[i] = raw_g[i] = raw_d[i] = raw_h[i] = Vec<T, V>{};
+      if (there && in[i]) {
+        const int c = (i * L + g) * V;
+        if (P.pre) raw_x[i] = piece(P.x, row * P.x_stride + c);
+        if (P.block) raw_p[i] = piece(P.block, row * P.block_stride + c);
+        if (P.dstream) raw_d[i] = piece(P.dstream, row * P.dstream_stride + c);
+        if (P.pre) raw_h[i] = piece(P.dnormed, row * P.dnormed_stride + c);
+        if (P.gate_kind == kGateFull) raw_g[i] = piece(P.gate, row * P.gate_stride + c);
+      }
+    }
+  };
+  constexpr bool kAhead = ITEMS == 1;      // (two pieces per thread leave no registers for a second row)
+  if (kAhead) fetch(blockIdx.x);
   for (int64_t b = blockIdx.x; b < rounds; b += gridDim.x) {
     const int64_t row = b * kRows + threadIdx.x / L;
     const bool live = row < P.n;
-    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-    float hat[ITEMS][V] = {}, p[ITEMS][V] = {}, gate[ITEMS][V] = {}, d[ITEMS][V] = {}, dh[ITEMS][V] = {};
+    if (!kAhead) fetch(b);
+    const float4 st = live ? raw_st : make_float4(0.f, 0.f, 0.f, 0.f);
+    float hat[ITEMS][V], p[ITEMS][V], gate[ITEMS][V], d[ITEMS][V], dh[ITEMS][V];
     const float row_gate = P.gate_kind == kGateRow && live ? to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]) : 1.f;
-    if (live) {
-      st = reinterpret_cast<const float4 *>(P.stats)[row];
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-        if (in[i]) {
-          const int c = (i * L + g) * V;
-          if (P.pre) load_f32<T, V>(static_cast<const T *>(P.x) + row * P.x_stride + c, hat[i]);
-          if (P.block) load_f32<T, V>(static_cast<const T *>(P.block) + row * P.block_stride + c, p[i]);
-          if (P.dstream) load_f32<T, V>(static_cast<const T *>(P.dstream) + row * P.dstream_stride + c, d[i]);
-          if (P.pre) load_f32<T, V>(static_cast<const T *>(P.dnormed) + row * P.dnormed_stride + c, dh[i]);
-          if (P.gate_kind == kGateFull) load_f32<T, V>(static_cast<const T *>(P.gate) + row * P.gate_stride + c, gate[i]);
-        }
-    }
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        hat[i][e] = to_f32(raw_x[i].v[e]);
+        p[i][e] = to_f32(raw_p[i].v[e]);
+        gate[i][e] = to_f32(raw_g[i].v[e]);
+        d[i][e] = to_f32(raw_d[i].v[e]);
+        dh[i][e] = to_f32(raw_h[i].v[e]);
+      }
+    if (kAhead) fetch(b + gridDim.x);
     // the block's normalised value, its affine form is rebuilt where it is needed
     float sums[2] = {0.f, 0.f};
 #pragma unroll
@@ -411,34 +453,39 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__
   }
 }
 
+// CTAs of a kernel that fit on an SM (asked once per kernel).
+template <typename K>
+static int resident_ctas(K kernel, int threads) {
+  int n = 0;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) == cudaSuccess && n > 0 ? n : 1;
+}
+
 template <typename T, int V, int L, int ITEMS>
 static int launch_norm(const NormParams &P, bool backward, int *ctas, cudaStream_t st) {
   constexpr int kThreads = L > 256 ? L : 256;
   constexpr int kRows = kThreads / L;
   const int64_t rounds = div_up(P.n, kRows);
   if (!backward) {
-    const int64_t cap = static_cast<int64_t>(sm_count()) * (2048 / kThreads);
+    static const int resident = resident_ctas(norm_forward_kernel<T, V, L, ITEMS>, kThreads);
+    const int64_t cap = static_cast<int64_t>(sm_count()) * resident;
     SB_CHECK_CUDA(launch_dependent(norm_forward_kernel<T, V, L, ITEMS>, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), 0, st, P));
     return SPIRA_B200_OK;
   }
-  const int64_t cap = static_cast<int64_t>(sm_count()) * (kThreads > 256 ? 1 : 2);
+  static const int resident = resident_ctas(norm_backward_kernel<T, V, L, ITEMS>, kThreads);
+  const int64_t cap = static_cast<int64_t>(sm_count()) * (resident < kNormBackwardCtas ? resident : kNormBackwardCtas);
   const int grid = static_cast<int>(rounds < cap ? rounds : cap);
-  if (P.n == 0) {                    // (only the size of the grid is asked for)
-    *ctas = static_cast<int>(cap);
-    return SPIRA_B200_OK;
-  }
   *ctas = grid;
   const size_t smem = kRows > 1 ? static_cast<size_t>(kRows) * P.channels * 4 : 0;
   SB_CHECK_CUDA(launch_dependent(norm_backward_kernel<T, V, L, ITEMS>, dim3(grid), dim3(kThreads), smem, st, P));
   return SPIRA_B200_OK;
 }
 
-// Threads per row and pieces per thread: the fewest lanes that hold the row with little waste (12 pieces of a 96-channel
-// row: 4 lanes x 3), so that a row sum takes few shuffles; rows too long for a warp's registers take a whole CTA.
+// Threads per row and pieces per thread: the fewest lanes that hold the row, so that a row sum takes few shuffles; rows too
+// long for a warp's registers take a whole CTA.
 template <typename T, int V>
 static int launch_norm_shape(const NormParams &P, bool backward, int *ctas, cudaStream_t st) {
   const int pieces = P.channels / V;
-  if (V > 1) {
+  if constexpr (V > 1) {
     if (pieces <= 4) return launch_norm<T, V, 4, 1>(P, backward, ctas, st);
     if (pieces <= 8) return launch_norm<T, V, 8, 1>(P, backward, ctas, st);
     if (pieces <= 16) return launch_norm<T, V, 16, 1>(P, backward, ctas, st);
@@ -447,10 +494,16 @@ static int launch_norm_shape(const NormParams &P, bool backward, int *ctas, cuda
   if (pieces <= 64) return launch_norm<T, V, 32, 2>(P, backward, ctas, st);
   if (pieces <= 256) return launch_norm<T, V, 256, 1>(P, backward, ctas, st);
   if (pieces <= 512) return launch_norm<T, V, 256, 2>(P, backward, ctas, st);
-  if (pieces <= 1024) return launch_norm<T, V, 512, 2>(P, backward, ctas, st);
-  if (pieces <= 2048) return launch_norm<T, V, 1024, 2>(P, backward, ctas, st);
-  if (V == 1 && pieces <= 4096) return launch_norm<T, V, 1024, 4>(P, backward, ctas, st);
-  return launch_norm<T, V, 1024, V == 1 ? 8 : 2>(P, backward, ctas, st);
+  if constexpr (V == 8) {
+    return launch_norm<T, V, 512, 2>(P, backward, ctas, st);       // (8192 channels are 1024 pieces)
+  } else {
+    if (pieces <= 1024) return launch_norm<T, V, 512, 2>(P, backward, ctas, st);
+    if constexpr (V == 1) {
+      if (pieces > 4096) return launch_norm<T, V, 1024, 8>(P, backward, ctas, st);
+      if (pieces > 2048) return launch_norm<T, V, 1024, 4>(P, backward, ctas, st);
+    }
+    return launch_norm<T, V, 1024, 2>(P, backward, ctas, st);
+  }
 }
 
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -515,7 +568,7 @@ extern "C" int spira_b200_residual_norm_backward_workspace(const spira_b200_norm
   int rc = norm_check("residual_norm_backward", desc);
   if (rc != SPIRA_B200_OK) return rc;
   SB_CHECK_ARG(bytes, "residual_norm_backward: null pointer");
-  *bytes = static_cast<size_t>(sm_count()) * 2 * kSums * desc->channels * 4;      // (at most two CTAs per SM)
+  *bytes = static_cast<size_t>(sm_count()) * kNormBackwardCtas * kSums * desc->channels * 4;
   return SPIRA_B200_OK;
 }
 

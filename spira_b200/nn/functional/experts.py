@@ -262,15 +262,24 @@ def _grouped_desc(x, weights, offsets, dy=None) -> GroupedDesc:
     return d
 
 
-def _grouped(x, weights, offsets, bias, relu):
+def _grouped(x, weights, offsets, bias, relu, want_mask=False):
+    """The product and, for a backward pass, what its ReLU let through: the bit mask the kernel writes, or None where the
+    shape has none (then the sign of the result says it)."""
     index = x.device.index
-    y = torch.empty((x.shape[0], weights.shape[2]), dtype=x.dtype, device=x.device)
+    y = x.new_empty((x.shape[0], weights.shape[2]))
     d = _grouped_desc(x, weights, offsets)
     d.y, d.relu = y.data_ptr(), 1 if relu else 0
     if bias is not None:
         d.bias = bias.data_ptr()
+    mask = None
+    if want_mask and relu:
+        need = C.c_size_t()
+        _lib.call("spira_b200_grouped_linear_mask_bytes", C.byref(d), C.byref(need))
+        if need.value:
+            mask = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+            d.mask = mask.data_ptr()
     _launch(index, "spira_b200_grouped_linear", C.byref(d), _status(index))
-    return y
+    return (y, mask) if want_mask else y
 
 
 def _with_workspace(index, device, name, desc, *rest):
@@ -287,15 +296,15 @@ def _with_workspace(index, device, name, desc, *rest):
 class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weights, offsets, bias, relu):
-        y = _grouped(x, weights, offsets, bias, relu)
+        y, mask = _grouped(x, weights, offsets, bias, relu, want_mask=True)
         ctx.relu, ctx.has_bias = relu, bias is not None
-        ctx.save_for_backward(x, weights, offsets, y if relu else None)
+        ctx.save_for_backward(x, weights, offsets, y if relu and mask is None else None, mask)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weights, offsets, y = ctx.saved_tensors
+        x, weights, offsets, y, mask = ctx.saved_tensors
         dy = _rows(dy)
         index, dev = x.device.index, x.device
         status = _status(index)
@@ -305,7 +314,11 @@ class _Grouped(torch.autograd.Function):
             d = _grouped_desc(None, weights, offsets, dy)
             if ctx.relu:
                 dz = torch.empty((dy.shape[0], weights.shape[2]), dtype=dy.dtype, device=dev)
-                d.y, d.dz = y.data_ptr(), dz.data_ptr()
+                d.dz = dz.data_ptr()
+                if mask is not None:
+                    d.mask = mask.data_ptr()
+                else:
+                    d.y = y.data_ptr()
             if want_db:
                 db = torch.empty((weights.shape[0], weights.shape[2]), dtype=weights.dtype, device=dev)
                 d.dbias = db.data_ptr()

@@ -7,7 +7,7 @@ import torch
 
 def test_descriptor_layouts_match_the_header():
     from spira_b200 import _lib
-    assert ctypes.sizeof(_lib.GroupedDesc) == 6 * 4 + 3 * 8 + 10 * 8          # the library static_asserts the same sizes
+    assert ctypes.sizeof(_lib.GroupedDesc) == 6 * 4 + 3 * 8 + 11 * 8          # the library static_asserts the same sizes
     assert ctypes.sizeof(_lib.NormDesc) == 8 * 4 + 4 * 4 + 6 * 8 + 19 * 8
 
 
