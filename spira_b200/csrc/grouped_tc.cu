@@ -9,6 +9,10 @@
 // group belong to the next one, they are multiplied and not stored.  In dW the rows are the reduction: the last step of a
 // group overwrites foreign rows with zeros in BOTH operands in shared memory (0 * NaN of a neighbour would not be 0).
 //
+// With many rows per group two CTAs of a cluster share a tile of 256 rows (cta_group::2): each holds its 128 rows of A and
+// half of the columns of B, the leader issues the MMAs for both, and every byte of B crosses from L2 to one SM instead of
+// two (32 instead of 48 KB per stage, six stages instead of four).
+//
 // One persistent CTA per SM, 20 warps: warp 0 issues TMA loads, warp 1 the MMAs, warps 4-19 (four per tensor-memory lane
 // quarter, a quarter of the columns each) convert and store while the next tile accumulates in the other half of tensor
 // memory.  Narrow products (few reduction steps per tile) are bound by this conversion: it takes 2.5 instructions per
@@ -47,6 +51,7 @@ struct GroupedTcParams {
   int32_t *status;
   int n, experts, m_channels, n_channels, k_channels;   // m_channels: c_in in dW; k_channels: 0 in dW (rows)
   int relu, piece;           // piece: rows per unit of dW, 0 = whole groups
+  int tile_rows;             // M of a tile: 128, or 256 for a pair of CTAs
   int bn, n_tiles, m_tiles;  // columns per tile, column tiles, row tiles of dW
   int stages, b_bytes, acc_stride, tmem_cols, off_bias, off_bar, off_groups;
   unsigned char *mask;       // forward: a bit per element that the ReLU let through
@@ -55,15 +60,110 @@ struct GroupedTcParams {
   unsigned long long wait_ns;
 };
 
+template <bool PAIR>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-               : "memory");
+  if constexpr (PAIR)      // (the barrier may lie in the other CTA of the pair)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
-               : "memory");
+  if constexpr (PAIR)
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+
+// ---- the two CTAs of a pair
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Bounded like mbar_wait, for arrivals of the other CTA.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned long long limit_ns) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+  int spins = 0;
+  while (true) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if ((++spins & 63) == 0) {
+      if (*abort_flag != 0) return false;
+      if (global_timer_ns() - t0 > limit_ns) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void group_tmem_alloc(uint32_t dst, uint32_t cols) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(dst, cols);
+    tmem_relinquish();
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void group_tmem_dealloc(uint32_t addr, uint32_t cols) {
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+  else tmem_dealloc(addr, cols);
+}
+template <bool PAIR>
+__device__ __forceinline__ void group_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    mma_f16_ss(d, a, b, idesc, accumulate);
+}
+// Arrives once the MMAs issued so far are done: on this CTA's barrier, or on the same barrier of both CTAs.
+template <bool PAIR>
+__device__ __forceinline__ void group_commit(uint32_t bar) {
+  if constexpr (PAIR) {
+    const uint16_t both = 3;
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(both) : "memory");
+  } else {
+    mma_commit(bar);
+  }
 }
 
 // Operand whose M (or N) elements are contiguous, 128-byte swizzle: 64 x 64 boxes (64 reduction rows of 128 bytes); eight
@@ -100,13 +200,13 @@ struct TileWalk {
     r.unit = unit;
     r.n0 = in_unit % P.n_tiles * P.bn;
     if (MODE == kDw) {
-      r.m0 = in_unit / P.n_tiles * kGRows;
+      r.m0 = in_unit / P.n_tiles * P.tile_rows;
       r.row0 = rows[expert] + index * P.piece;
       r.row_end = P.piece && r.row0 + P.piece < rows[expert + 1] ? r.row0 + P.piece : rows[expert + 1];
       r.steps = (r.row_end - r.row0 + kGK - 1) / kGK;
     } else {
       r.m0 = 0;
-      r.row0 = rows[expert] + index * kGRows;
+      r.row0 = rows[expert] + index * P.tile_rows;
       r.row_end = rows[expert + 1];
       r.steps = (P.k_channels + kGK - 1) / kGK;
     }
@@ -132,7 +232,7 @@ __device__ __forceinline__ void read_groups(const GroupedTcParams &P, int *rows,
     highest = __shfl_sync(0xffffffffu, v, 31);
   }
   __syncwarp();
-  const int unit_rows = MODE == kDw ? P.piece : kGRows;
+  const int unit_rows = MODE == kDw ? P.piece : P.tile_rows;
   for (int e0 = 0; e0 < P.experts; e0 += 32) {
     const int e = e0 + lane;
     int mine = 0;
@@ -160,8 +260,8 @@ __device__ __forceinline__ void read_groups(const GroupedTcParams &P, int *rows,
     }
 }
 
-// The CTA's tile of round r: rounds run over the CTAs in alternating direction.
-__device__ __forceinline__ int round_tile(int r) { return r * static_cast<int>(gridDim.x) + (r & 1 ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x)); }
+// The tile of worker `me` of G in round r: rounds run over the workers in alternating direction.
+__device__ __forceinline__ int round_tile(int r, int me, int G) { return r * G + (r & 1 ? G - 1 - me : me); }
 
 // Two values rounded into one word (a in the low half), negative ones to zero with kRelu (a NaN stays).
 template <typename T, bool kRelu>
@@ -223,7 +323,7 @@ __device__ __forceinline__ void store_partial(const uint32_t (&r)[W], float *dst
     if (i < valid) *reinterpret_cast<uint4 *>(dst + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
 }
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool PAIR>
 __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_constant__ GroupedTcParams P, const __grid_constant__ CUtensorMap map_a,
                                                                    const __grid_constant__ CUtensorMap map_b) {
   extern __shared__ unsigned char grouped_smem_raw[];
@@ -235,38 +335,46 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
   auto bar_empty = [&](int s) { return bar0 + 8u * (kGMaxStages + s); };
   auto bar_acc_full = [&](int b) { return bar0 + 8u * (2 * kGMaxStages + b); };
   auto bar_acc_empty = [&](int b) { return bar0 + 8u * (2 * kGMaxStages + 2 + b); };
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + P.off_bar + 8 * (2 * kGMaxStages + 4));
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + P.off_bar + 8 * (2 * kGMaxStages + 4) + 4);
+  // dW of a pair, last step of a group: the follower's rows have landed (its own barrier) / are cleaned (the leader's)
+  auto bar_tail = [&](int s) { return bar0 + 8u * (2 * kGMaxStages + 4 + s); };
+  auto bar_clean = [&](int s) { return bar0 + 8u * (3 * kGMaxStages + 4 + s); };
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + P.off_bar + 8 * (4 * kGMaxStages + 4));
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + P.off_bar + 8 * (4 * kGMaxStages + 4) + 4);
   int *rows = reinterpret_cast<int *>(smem + P.off_groups), *first = rows + P.experts + 1, *by_size = first + P.experts + 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
+  const int me = PAIR ? blockIdx.x / 2 : blockIdx.x, G = PAIR ? gridDim.x / 2 : gridDim.x;
   const int stages = P.stages, stage_bytes = kGABytes + P.b_bytes;
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(bar_full(s), 1);
       mbar_init(bar_empty(s), 1);
+      if (PAIR && MODE == kDw) {
+        mbar_init(bar_tail(s), 1);
+        mbar_init(bar_clean(s), 1);
+      }
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_acc_full(b), 1);
-      mbar_init(bar_acc_empty(b), 32 * kGEpilogueWarps);
+      mbar_init(bar_acc_empty(b), kGEpilogueWarps * (PAIR ? 2 : 1));
     }
     *abort_flag = 0;
     mbar_init_fence();
   }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), P.tmem_cols);
-    tmem_relinquish();
-  }
+  if (warp == 1) group_tmem_alloc<PAIR>(smem_u32(tmem_slot), P.tmem_cols);
   pdl_wait();            // before the first global read of any thread
   if (warp == 2) read_groups<MODE>(P, rows, first, by_size);
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();      // the other CTA's barriers are ready too
   tc_fence_after();
   pdl_trigger();         // (behind the allocation: a CTA of the next kernel on this SM cannot take the tensor memory first)
   const uint32_t tmem_base = *tmem_slot;
-  const int total = first[P.experts] * (MODE == kDw ? P.m_tiles * P.n_tiles : P.n_tiles), G = gridDim.x;
+  const int total = first[P.experts] * (MODE == kDw ? P.m_tiles * P.n_tiles : P.n_tiles);
   TileWalk<MODE> walk{rows, first, by_size};
   const int rounds = (total + G - 1) / G;
+  const int b_columns = PAIR ? P.bn / 2 : P.bn;
 
   if (warp == 0) {
     // =========================== TMA loads ===========================
@@ -274,23 +382,36 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
       int stage = 0, phase = 0;
       bool ok = true;
       for (int round = 0; ok && round < rounds; ++round) {
-        const int t = round_tile(round);
+        const int t = round_tile(round, me, G);
         if (t >= total) break;
         const TcTile tile = walk.at(P, t);
+        const bool tail = MODE == kDw && (tile.row_end - tile.row0) % 16 != 0;
         for (int j = 0; j < tile.steps; ++j) {
           if (!mbar_wait(bar_empty(stage), phase ^ 1, abort_flag, P.wait_ns)) { ok = false; break; }
-          const uint32_t a = sbase + stage * stage_bytes, b = a + kGABytes, bar = bar_full(stage);
-          mbar_arrive_expect_tx(bar, stage_bytes);
-          const int k = j * kGK;
-          if (MODE == kDw) {
-            for (int h = 0; h < 2; ++h) tma_2d(a + h * kGBlock, &map_a, tile.m0 + h * 64, tile.row0 + k, bar);
-            for (int h = 0; h < P.b_bytes / kGBlock; ++h) tma_2d(b + h * kGBlock, &map_b, tile.n0 + h * 64, tile.row0 + k, bar);
-          } else {
-            tma_2d(a, &map_a, k, tile.row0, bar);
-            if (MODE == kForward) {
-              for (int h = 0; h < P.b_bytes / kGBlock; ++h) tma_3d(b + h * kGBlock, &map_b, tile.n0 + h * 64, k, tile.expert, bar);
+          const uint32_t a = sbase + stage * stage_bytes, b = a + kGABytes;
+          uint32_t bar = bar_full(stage);
+          if constexpr (PAIR) {
+            // one barrier of the leader counts the bytes of both CTAs; a step that is cleaned first is counted by each CTA
+            if (tail && j == tile.steps - 1) {
+              if (rank != 0) bar = bar_tail(stage);
+              mbar_arrive_expect_tx(bar, stage_bytes);
             } else {
-              tma_3d(b, &map_b, k, tile.n0, tile.expert, bar);
+              if (rank == 0) mbar_arrive_expect_tx(bar, 2 * stage_bytes);
+              else bar = map_to_rank(bar, 0);
+            }
+          } else {
+            mbar_arrive_expect_tx(bar, stage_bytes);
+          }
+          const int k = j * kGK, n0 = tile.n0 + rank * b_columns;
+          if (MODE == kDw) {
+            for (int h = 0; h < 2; ++h) tma_2d<PAIR>(a + h * kGBlock, &map_a, tile.m0 + rank * kGRows + h * 64, tile.row0 + k, bar);
+            for (int h = 0; h < P.b_bytes / kGBlock; ++h) tma_2d<PAIR>(b + h * kGBlock, &map_b, n0 + h * 64, tile.row0 + k, bar);
+          } else {
+            tma_2d<PAIR>(a, &map_a, k, tile.row0 + rank * kGRows, bar);
+            if (MODE == kForward) {
+              for (int h = 0; h < P.b_bytes / kGBlock; ++h) tma_3d<PAIR>(b + h * kGBlock, &map_b, n0 + h * 64, k, tile.expert, bar);
+            } else {
+              tma_3d<PAIR>(b, &map_b, k, n0, tile.expert, bar);
             }
           }
           if (++stage == stages) { stage = 0; phase ^= 1; }
@@ -299,50 +420,79 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
     }
     __syncwarp();
   } else if (warp == 1) {
-    // =========================== MMAs ===========================
-    int stage = 0, phase = 0, tile_i = 0;
-    uint32_t acc_phase = 0;
-    bool ok = true;
-    for (; ok && tile_i < rounds; ++tile_i) {
-      const int t = round_tile(tile_i);
-      if (t >= total) break;
-      const TcTile tile = walk.at(P, t);
-      const int b = tile_i & 1;
-      // (the whole warp leaves together: lanes may see the abort flag at different times)
-      if (!__all_sync(0xffffffffu, mbar_wait(bar_acc_empty(b), ((acc_phase >> b) & 1u) ^ 1u, abort_flag, P.wait_ns))) break;
-      acc_phase ^= 1u << b;
-      tc_fence_after();
-      const uint32_t d_tmem = tmem_base + b * P.acc_stride;
-      const int length = MODE == kDw ? tile.row_end - tile.row0 : P.k_channels;
-      for (int j = 0; j < tile.steps; ++j) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar_full(stage), phase, abort_flag, P.wait_ns))) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t sa = sbase + stage * stage_bytes, sb = sa + kGABytes;
-        const int left = length - j * kGK, depth = left < kGK ? left : kGK, ks = (depth + 15) / 16;
-        if (MODE == kDw && depth < ks * 16) {
-          // rows [depth, 16 ks) belong to the next group: a reduction row is one 128-byte line of every box
-          const int lines = ks * 16 - depth, boxes = 2 + P.b_bytes / kGBlock;
-          for (int i = lane; i < boxes * lines * 8; i += 32) {
-            const int box = i / (lines * 8), q = i % (lines * 8);
-            *reinterpret_cast<uint4 *>(smem + stage * stage_bytes + box * kGBlock + (depth + q / 8) * 128 + (q % 8) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async();
-        }
-        __syncwarp();
-        if (lane == 0) {
-          const uint64_t a_desc = MODE == kDw ? smem_desc_mn_sw128(sa) : smem_desc_k_sw128(sa);
-          const uint64_t b_desc = MODE == kDx ? smem_desc_k_sw128(sb) : smem_desc_mn_sw128(sb);
-          // 16 steps of the reduction: 32 bytes further in a K-major row, 16 lines further in the other layout
-          constexpr uint32_t kA = MODE == kDw ? 2048 >> 4 : 32 >> 4, kB = MODE == kDx ? 32 >> 4 : 2048 >> 4;
-          for (int s = 0; s < ks; ++s) mma_f16_ss(d_tmem, a_desc + s * kA, b_desc + s * kB, P.idesc, (j | s) != 0);
-          mma_commit(bar_empty(stage));
-        }
-        __syncwarp();
-        if (++stage == stages) { stage = 0; phase ^= 1; }
+    // =========================== MMAs (a pair: by the leader) ===========================
+    // rows [depth, 16 ks) of a last step belong to the next group: a reduction row is one 128-byte line of every box
+    auto clean = [&](int stage, int depth, int ks) {
+      const int lines = ks * 16 - depth, boxes = 2 + P.b_bytes / kGBlock;
+      for (int i = lane; i < boxes * lines * 8; i += 32) {
+        const int box = i / (lines * 8), q = i % (lines * 8);
+        *reinterpret_cast<uint4 *>(smem + stage * stage_bytes + box * kGBlock + (depth + q / 8) * 128 + (q % 8) * 16) = make_uint4(0, 0, 0, 0);
       }
-      if (!ok) break;
-      if (lane == 0) mma_commit(bar_acc_full(b));
+      asm volatile("fence.proxy.async;" ::: "memory");
       __syncwarp();
+    };
+    int stage = 0, phase = 0, tile_i = 0;
+    uint32_t acc_phase = 0, tail_phase = 0;      // tail_phase: parity of every stage's tail / clean barrier
+    bool ok = true;
+    if (rank == 0) {
+      for (; ok && tile_i < rounds; ++tile_i) {
+        const int t = round_tile(tile_i, me, G);
+        if (t >= total) break;
+        const TcTile tile = walk.at(P, t);
+        const int b = tile_i & 1;
+        // (the whole warp leaves together: lanes may see the abort flag at different times)
+        const bool free_acc = PAIR ? mbar_wait_cluster(bar_acc_empty(b), ((acc_phase >> b) & 1u) ^ 1u, abort_flag, P.wait_ns)
+                                   : mbar_wait(bar_acc_empty(b), ((acc_phase >> b) & 1u) ^ 1u, abort_flag, P.wait_ns);
+        if (!__all_sync(0xffffffffu, free_acc)) break;
+        acc_phase ^= 1u << b;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + b * P.acc_stride;
+        const int length = MODE == kDw ? tile.row_end - tile.row0 : P.k_channels;
+        for (int j = 0; j < tile.steps; ++j) {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_full(stage), phase, abort_flag, P.wait_ns))) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = sbase + stage * stage_bytes, sb = sa + kGABytes;
+          const int left = length - j * kGK, depth = left < kGK ? left : kGK, ks = (depth + 15) / 16;
+          if (MODE == kDw && depth < ks * 16) {
+            clean(stage, depth, ks);
+            if (PAIR) {
+              if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar_clean(stage), (tail_phase >> stage) & 1u, abort_flag, P.wait_ns))) { ok = false; break; }
+              tail_phase ^= 1u << stage;
+              tc_fence_after();
+            }
+          }
+          __syncwarp();
+          if (lane == 0) {
+            const uint64_t a_desc = MODE == kDw ? smem_desc_mn_sw128(sa) : smem_desc_k_sw128(sa);
+            const uint64_t b_desc = MODE == kDx ? smem_desc_k_sw128(sb) : smem_desc_mn_sw128(sb);
+            // 16 steps of the reduction: 32 bytes further in a K-major row, 16 lines further in the other layout
+            constexpr uint32_t kA = MODE == kDw ? 2048 >> 4 : 32 >> 4, kB = MODE == kDx ? 32 >> 4 : 2048 >> 4;
+            for (int s = 0; s < ks; ++s) group_mma<PAIR>(d_tmem, a_desc + s * kA, b_desc + s * kB, P.idesc, (j | s) != 0);
+            group_commit<PAIR>(bar_empty(stage));
+          }
+          __syncwarp();
+          if (++stage == stages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        if (lane == 0) group_commit<PAIR>(bar_acc_full(b));
+        __syncwarp();
+      }
+    } else if (MODE == kDw) {
+      // follower: cleans its rows of every last step and tells the leader
+      for (; ok && tile_i < rounds; ++tile_i) {
+        const int t = round_tile(tile_i, me, G);
+        if (t >= total) break;
+        const TcTile tile = walk.at(P, t);
+        const int length = tile.row_end - tile.row0, depth = length - (tile.steps - 1) * kGK, ks = (depth + 15) / 16;
+        if (length % 16 != 0) {
+          const int s = (stage + tile.steps - 1) % stages;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_tail(s), (tail_phase >> s) & 1u, abort_flag, P.wait_ns))) break;
+          tail_phase ^= 1u << s;
+          clean(s, depth, ks);
+          if (lane == 0) mbar_arrive_cluster(map_to_rank(bar_clean(s), 0));
+        }
+        stage = (stage + tile.steps) % stages;
+      }
     }
   } else if (warp >= kGFirstEpilogueWarp) {
     // =========================== epilogue ===========================
@@ -353,11 +503,11 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
     int bias_at = -1;                                // what bias_s holds: expert * n_tiles + column tile
     uint32_t acc_phase = 0;
     for (int tile_i = 0; tile_i < rounds; ++tile_i) {
-      const int t = round_tile(tile_i);
+      const int t = round_tile(tile_i, me, G);
       if (t >= total) break;
       const TcTile tile = walk.at(P, t);
       const int b = tile_i & 1;
-      const int m = (MODE == kDw ? tile.m0 : tile.row0) + q * 32 + lane, m_end = MODE == kDw ? P.m_channels : tile.row_end;
+      const int m = (MODE == kDw ? tile.m0 : tile.row0) + rank * kGRows + q * 32 + lane, m_end = MODE == kDw ? P.m_channels : tile.row_end;
       const int col = tile.n0 + part * width;
       const int valid = m < m_end ? P.n_channels - col : 0;      // columns of this row that exist (a multiple of 8)
       const float *bias = nullptr;
@@ -409,7 +559,11 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
         }
       }
       tc_fence_before();
-      mbar_arrive(bar_acc_empty(b));
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster(map_to_rank(bar_acc_empty(b), 0));
+        else mbar_arrive(bar_acc_empty(b));
+      }
       if (MODE == kForward && P.mask && valid > 0) {
         unsigned char *line = P.mask + static_cast<int64_t>(m) * P.mask_pitch + col / 8;
         if (width == 64 && (reinterpret_cast<uintptr_t>(line) & 7) == 0 && valid > 32) {
@@ -425,7 +579,7 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
     // rows of no group are zero
     T *out = static_cast<T *>(P.out);
     const int64_t width = P.n_channels / 8, before = rows[0] * width, behind = static_cast<int64_t>(P.n - rows[P.experts]) * width;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + lane; i < before + behind; i += static_cast<int64_t>(G) * 32)
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + lane; i < before + behind; i += static_cast<int64_t>(gridDim.x) * 32)
       reinterpret_cast<uint4 *>(out)[i < before ? i : rows[P.experts] * width + i - before] = make_uint4(0, 0, 0, 0);
   }
 
@@ -439,9 +593,10 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
     while (global_timer_ns() - t0 < 200000ull) { }
     __syncthreads();
   }
+  if (PAIR) cluster_sync();      // nobody leaves while the other CTA still signals its barriers or uses its memory
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, P.tmem_cols);
+    group_tmem_dealloc<PAIR>(tmem_base, P.tmem_cols);
   }
 }
 
@@ -489,6 +644,14 @@ int grouped_tc_dw_tiles(int c_in, int c_out) {
   return static_cast<int>(div_up(c_in, kGRows) * div_up(c_out, columns_per_tile(c_out, int64_t(1) << 30)));
 }
 
+// Two CTAs per tile where it has the rows and columns for both and enough work to fill the SMs in pairs.  Measured:
+// 80 026 rows in 16 groups, 512 -> 2048: PAIRFIGURES.
+static bool use_pair(int mode, const spira_b200_grouped_desc &D, int piece) {
+  if (mode == kDw) return D.c_in > kGRows && D.c_out >= 128 && D.n / D.experts >= 256;
+  const int n = mode == kForward ? D.c_out : D.c_in, k = mode == kForward ? D.c_in : D.c_out;
+  return n >= 128 && k >= 192 && D.n / D.experts >= 512 && D.n / 256 * div_up(n, kGMaxN) >= sm_count() / 2;
+}
+
 int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float *partial, int32_t *status, unsigned long long wait_ns, cudaStream_t st) {
   GroupedTcParams P{};
   P.offsets = D.offsets;
@@ -498,12 +661,14 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
   P.experts = D.experts;
   P.piece = piece;
   P.wait_ns = wait_ns;
+  const bool pair = use_pair(mode, D, piece);
+  P.tile_rows = pair ? 2 * kGRows : kGRows;
   int64_t units;
   if (mode == kDw) {
     P.out = D.dweight;
     P.m_channels = D.c_in;
     P.n_channels = D.c_out;
-    P.m_tiles = static_cast<int>(div_up(D.c_in, kGRows));
+    P.m_tiles = static_cast<int>(div_up(D.c_in, P.tile_rows));
     units = (piece ? group_tiles_bound(D.n, D.experts, piece) : D.experts) * P.m_tiles;
     P.bn = columns_per_tile(D.c_out, int64_t(1) << 30);
   } else {
@@ -515,24 +680,27 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
     P.n_channels = mode == kForward ? D.c_out : D.c_in;
     P.k_channels = mode == kForward ? D.c_in : D.c_out;
     P.m_tiles = 1;
-    units = group_tiles_bound(D.n, D.experts, kGRows);
-    P.bn = columns_per_tile(P.n_channels, units);
+    units = group_tiles_bound(D.n, D.experts, P.tile_rows);
+    P.bn = columns_per_tile(P.n_channels, pair ? int64_t(1) << 30 : units);
   }
+  if (pair) P.bn = static_cast<int>(div_up(P.bn, 128) * 128);      // (each CTA holds half of the columns in 64-wide boxes)
   P.n_tiles = static_cast<int>(div_up(P.n_channels, P.bn));
   const bool b_n_major = mode != kDx;
-  P.b_bytes = b_n_major ? static_cast<int>(div_up(P.bn, 64)) * kGBlock : P.bn * 128;
+  const int b_columns = pair ? P.bn / 2 : P.bn;
+  P.b_bytes = b_columns * 128;             // (a multiple of 8 KB: whole boxes)
   P.acc_stride = 32;
   while (P.acc_stride < P.bn) P.acc_stride *= 2;
   P.tmem_cols = 2 * P.acc_stride;
   P.idesc = (1u << 4) | (D.dtype == SPIRA_B200_BF16 ? (1u << 7) | (1u << 10) : 0u) | (mode == kDw ? 1u << 15 : 0u) | (b_n_major ? 1u << 16 : 0u) |
-            (static_cast<uint32_t>(P.bn >> 3) << 17) | ((128u >> 4) << 24);
-  const int fixed = kGBiasBytes + 8 * (2 * kGMaxStages + 5) + 16 + 12 * (D.experts + 2);
-  const int stage_bytes = kGABytes + P.b_bytes;      // (multiples of 1024: 8 KB boxes, or bn * 128 with bn a multiple of 16)
+            (static_cast<uint32_t>(P.bn >> 3) << 17) | (static_cast<uint32_t>(P.tile_rows >> 4) << 24);
+  const int bars = 8 * (4 * kGMaxStages + 5);
+  const int fixed = kGBiasBytes + bars + 16 + 12 * (D.experts + 2);
+  const int stage_bytes = kGABytes + P.b_bytes;
   P.stages = (kGSmemBudget - fixed) / stage_bytes;
   if (P.stages > kGMaxStages) P.stages = kGMaxStages;
   P.off_bias = P.stages * stage_bytes;
   P.off_bar = P.off_bias + kGBiasBytes;
-  P.off_groups = P.off_bar + 8 * (2 * kGMaxStages + 5) + 8;
+  P.off_groups = P.off_bar + bars + 8;
   const size_t smem = static_cast<size_t>(P.off_bias) + fixed + 1024;
 
   alignas(64) CUtensorMap map_a, map_b;
@@ -543,7 +711,7 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
     if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, D.c_out, D.experts, kGK);
   } else if (mode == kDx) {
     rc = encode_map(&map_a, D.dtype, D.dy, 2, D.c_out, D.n, dy_stride, 1, kGRows);
-    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, D.c_out, D.experts, P.bn);
+    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, D.c_out, D.experts, b_columns);
   } else {
     rc = encode_map(&map_a, D.dtype, D.x, 2, D.c_in, D.n, x_stride, 1, kGK);
     if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.dy, 2, D.c_out, D.n, dy_stride, 1, kGK);
@@ -551,17 +719,37 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
   if (rc != SPIRA_B200_OK) return rc;
   const int64_t tiles = units * P.n_tiles;
   SB_CHECK_ARG(tiles < (int64_t(1) << 31) - 65536, "grouped_linear: too many tiles");
-  const unsigned grid = static_cast<unsigned>(tiles < sm_count() ? (tiles < 1 ? 1 : tiles) : sm_count());
+  const int64_t workers = pair ? sm_count() / 2 : sm_count();
+  const unsigned grid = static_cast<unsigned>(tiles < workers ? (tiles < 1 ? 1 : tiles) : workers) * (pair ? 2 : 1);
   auto go = [&](auto kernel) -> int {
     SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kGThreads), smem, st, P, map_a, map_b));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kGThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    if (pair) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+      attr[cfg.numAttrs].val.clusterDim.x = 2;
+      attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+      ++cfg.numAttrs;
+    }
+    if (pdl_enabled()) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+      ++cfg.numAttrs;
+    }
+    cfg.attrs = attr;
+    SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, map_a, map_b));
     return SPIRA_B200_OK;
   };
-  if (D.dtype == SPIRA_B200_F16)
-    return mode == kForward ? go(grouped_tc_kernel<__half, kForward>) : mode == kDx ? go(grouped_tc_kernel<__half, kDx>) : go(grouped_tc_kernel<__half, kDw>);
-  return mode == kForward ? go(grouped_tc_kernel<__nv_bfloat16, kForward>)
-         : mode == kDx    ? go(grouped_tc_kernel<__nv_bfloat16, kDx>)
-                          : go(grouped_tc_kernel<__nv_bfloat16, kDw>);
+  auto pick = [&](auto type) -> int {
+    using T = decltype(type);
+    if (pair) return mode == kForward ? go(grouped_tc_kernel<T, kForward, true>) : mode == kDx ? go(grouped_tc_kernel<T, kDx, true>) : go(grouped_tc_kernel<T, kDw, true>);
+    return mode == kForward ? go(grouped_tc_kernel<T, kForward, false>) : mode == kDx ? go(grouped_tc_kernel<T, kDx, false>) : go(grouped_tc_kernel<T, kDw, false>);
+  };
+  return D.dtype == SPIRA_B200_F16 ? pick(__half{}) : pick(__nv_bfloat16{});
 }
 
 }  // namespace sb

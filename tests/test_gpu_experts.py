@@ -267,7 +267,8 @@ def plain_products(x, w, offsets, b, relu, dy, y_own):
 
 
 SHAPES = [(1, 1, 1, 1), (2, 8, 256, 1024), (5, 3, 19, 100), (130, 4, 16, 16), (129, 1, 64, 64), (300, 7, 20, 33), (257, 5, 40, 24), (1000, 3, 96, 384),
-          (777, 6, 72, 264), (512, 2, 136, 520), (2000, 2, 512, 48), (640, 9, 8, 8), (4100, 4, 32, 32), (33, 40, 48, 80), (1500, 3, 17, 64), (1500, 3, 64, 17)]
+          (777, 6, 72, 264), (512, 2, 136, 520), (2000, 2, 512, 48), (640, 9, 8, 8), (4100, 4, 32, 32), (33, 40, 48, 80), (1500, 3, 17, 64), (1500, 3, 64, 17),
+          (20000, 3, 256, 512), (19001, 7, 264, 392), (30000, 2, 200, 136), (9000, 5, 384, 192)]
 
 
 @pytest.mark.parametrize("dtype", HALF)
