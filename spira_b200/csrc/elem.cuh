@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -28,16 +29,36 @@ struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
 template <typename T, int N>
-__device__ __forceinline__ void load_f32(const T *p, float (&f)[N]) {
-  const Vec<T, N> r = *reinterpret_cast<const Vec<T, N> *>(p);
+__device__ __forceinline__ void vec_to_f32(const Vec<T, N> &r, float (&f)[N]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value && N % 2 == 0) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&r);      // a bf16 is the upper half of its fp32
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = to_f32(r.v[i]);
+    for (int i = 0; i < N; i += 2) {
+      f[i] = __uint_as_float(w[i / 2] << 16);
+      f[i + 1] = __uint_as_float(w[i / 2] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_f32(r.v[i]);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(const T *p, float (&f)[N]) {
+  vec_to_f32<T, N>(*reinterpret_cast<const Vec<T, N> *>(p), f);
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_f32(T *p, const float (&f)[N]) {
   Vec<T, N> r;
+  if constexpr (std::is_same<T, __half>::value && N % 2 == 0) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(f[i]);
+    for (int i = 0; i < N; i += 2) *reinterpret_cast<__half2 *>(&r.v[i]) = __floats2half2_rn(f[i], f[i + 1]);
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value && N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *reinterpret_cast<__nv_bfloat162 *>(&r.v[i]) = __floats2bfloat162_rn(f[i], f[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(f[i]);
+  }
   *reinterpret_cast<Vec<T, N> *>(p) = r;
 }
 

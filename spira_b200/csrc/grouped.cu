@@ -313,10 +313,10 @@ __global__ void __launch_bounds__(1024) grouped_column_sum_kernel(const float *p
   if (lane == 0 && co < size) out[static_cast<int64_t>(e) * size + co] = from_f32<T>(t);
 }
 
-// Rows per piece of the column sums: a CTA per piece, two rounds of CTAs on the SMs, 32 to 256 rows.
+// Rows per piece of the column sums: a CTA per piece, all of them resident at once (eight per SM), at least 32 rows.
 static int dz_piece(int64_t n) {
-  const int64_t p = div_up(div_up(n, 16 * sm_count()), 32) * 32;
-  return static_cast<int>(p < 32 ? 32 : p > 256 ? 256 : p);
+  const int64_t p = div_up(div_up(n, 15 * sm_count() / 2), 8) * 8;
+  return static_cast<int>(p < 32 ? 32 : p);
 }
 
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -53,7 +53,8 @@ struct GroupedTcParams {
   int relu, piece;           // piece: rows per unit of dW, 0 = whole groups
   int tile_rows;             // M of a tile: 128, or 256 for a pair of CTAs
   int bn, n_tiles, m_tiles;  // columns per tile, column tiles, row tiles of dW
-  int stages, b_bytes, acc_stride, tmem_cols, off_bias, off_bar, off_groups;
+  int stages, b_bytes, acc_stride, tmem_cols, off_bias, off_stage, off_bar, off_groups;
+  int box_cols;              // columns of a block that leaves through shared memory and TMA (32 or 48), 0: direct stores
   unsigned char *mask;       // forward: a bit per element that the ReLU let through
   int mask_pitch;
   uint32_t idesc;
@@ -182,6 +183,15 @@ __device__ __forceinline__ void group_commit(uint32_t bar) {
   }
 }
 
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y),
+               "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // Operand whose M (or N) elements are contiguous, 128-byte swizzle: 64 x 64 boxes (64 reduction rows of 128 bytes); eight
 // reduction rows are 1024 bytes, the next 64 elements of M / N are the next box.
 __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr) {
@@ -293,10 +303,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return r;
 }
 
-// W (16 or 32) columns of one row of the accumulator, rounded and stored in whole 32-byte sectors where they are aligned.
-// `bits` gets a bit per column, set where the value is positive (the sign of 0 - v).
+// W (16 or 32) columns of one row of the accumulator: bias, ReLU, one rounding.  `bits` gets a bit per column, set where the
+// value is positive (the sign of 0 - v).
 template <typename T, int W, bool kRelu>
-__device__ __forceinline__ void store_columns(uint32_t (&r)[W], const float *bias, bool want_bits, T *dst, int valid, uint32_t &bits) {
+__device__ __forceinline__ void convert_columns(uint32_t (&r)[W], const float *bias, bool want_bits, uint4 (&v)[W / 8], uint32_t &bits) {
   if (bias) {
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
@@ -312,21 +322,25 @@ __device__ __forceinline__ void store_columns(uint32_t (&r)[W], const float *bia
 #pragma unroll
     for (int i = W - 1; i >= 0; --i) bits = __funnelshift_l(__float_as_uint(0.f - __uint_as_float(r[i])), bits, 1);
   }
+#pragma unroll
+  for (int h = 0; h < W / 8; ++h) {
+    const uint32_t *q = r + 8 * h;
+    v[h] = make_uint4(pack2<T, kRelu>(__uint_as_float(q[0]), __uint_as_float(q[1])), pack2<T, kRelu>(__uint_as_float(q[2]), __uint_as_float(q[3])),
+                      pack2<T, kRelu>(__uint_as_float(q[4]), __uint_as_float(q[5])), pack2<T, kRelu>(__uint_as_float(q[6]), __uint_as_float(q[7])));
+  }
+}
+
+// The same row's 16-byte units to global memory, whole 32-byte sectors where they are aligned.
+template <typename T, int U>
+__device__ __forceinline__ void store_units(const uint4 (&v)[U], T *dst, int valid) {
   const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
 #pragma unroll
-  for (int i = 0; i < W; i += 16) {
-    uint4 v[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t *q = r + i + 8 * h;
-      v[h] = make_uint4(pack2<T, kRelu>(__uint_as_float(q[0]), __uint_as_float(q[1])), pack2<T, kRelu>(__uint_as_float(q[2]), __uint_as_float(q[3])),
-                        pack2<T, kRelu>(__uint_as_float(q[4]), __uint_as_float(q[5])), pack2<T, kRelu>(__uint_as_float(q[6]), __uint_as_float(q[7])));
-    }
-    if (wide && i + 16 <= valid) {
-      st_global_v8(dst + i, v[0], v[1]);
+  for (int h = 0; h < U; h += 2) {
+    if (wide && 8 * h + 16 <= valid) {
+      st_global_v8(dst + 8 * h, v[h], v[h + 1]);
     } else {
-      if (i < valid) *reinterpret_cast<uint4 *>(dst + i) = v[0];
-      if (i + 8 < valid) *reinterpret_cast<uint4 *>(dst + i + 8) = v[1];
+      if (8 * h < valid) *reinterpret_cast<uint4 *>(dst + 8 * h) = v[h];
+      if (8 * h + 8 < valid) *reinterpret_cast<uint4 *>(dst + 8 * h + 8) = v[h + 1];
     }
   }
 }
@@ -341,7 +355,7 @@ __device__ __forceinline__ void store_partial(const uint32_t (&r)[W], float *dst
 
 template <typename T, int MODE, bool PAIR>
 __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_constant__ GroupedTcParams P, const __grid_constant__ CUtensorMap map_a,
-                                                                   const __grid_constant__ CUtensorMap map_b) {
+                                                                   const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out) {
   extern __shared__ unsigned char grouped_smem_raw[];
   const uint32_t raw = smem_u32(grouped_smem_raw);
   unsigned char *smem = grouped_smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -519,6 +533,7 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
     const int width = P.bn / 4;                      // columns of this warp: a multiple of 16, at most 64
     float *bias_s = reinterpret_cast<float *>(smem + P.off_bias) + (warp - kGFirstEpilogueWarp) * 64;
     const bool relu = MODE == kForward && P.relu;
+    unsigned char *stage_ptr = smem + P.off_stage + (warp - kGFirstEpilogueWarp) * P.box_cols * 64;
     int bias_at = -1;                                // what bias_s holds: expert * n_tiles + column tile
     uint32_t acc_phase = 0;
     for (int tile_i = 0; tile_i < rounds; ++tile_i) {
@@ -549,18 +564,47 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
       T *dst = static_cast<T *>(P.out) + out_row * P.n_channels + col;
       float *dst_partial = MODE == kDw ? P.partial + (static_cast<int64_t>(tile.unit) * P.m_channels + m) * P.n_channels + col : nullptr;
       uint32_t bits[2] = {0, 0};
-      auto emit = [&](auto &r, int c0, uint32_t &word) {
+      const int m_warp = m - lane;
+      const bool by_tma = MODE != kDw && P.box_cols != 0 && m_warp + 32 <= m_end;     // (rows of the next group are not ours to write)
+      // columns [c0, c0 + W) of this warp; `last`: the block they belong to is complete
+      auto emit = [&](auto &r, int c0, uint32_t &word, bool last) {
         constexpr int W = sizeof(r) / 4;
         if (MODE == kDw && tile.steps == 0) {
 #pragma unroll
           for (int i = 0; i < W; ++i) r[i] = 0;
         }
-        if (c0 < valid) {
-          if (MODE == kDw && P.piece) store_partial<W>(r, dst_partial + c0, valid - c0);
-          else if (relu) store_columns<T, W, true>(r, bias ? bias + c0 : nullptr, P.mask != nullptr, dst + c0, valid - c0, word);
-          else store_columns<T, W, false>(r, bias ? bias + c0 : nullptr, false, dst + c0, valid - c0, word);
+        if (MODE == kDw && P.piece) {
+          if (c0 < valid) store_partial<W>(r, dst_partial + c0, valid - c0);
+          __syncwarp();
+          return;
         }
-        __syncwarp();
+        uint4 v[W / 8];
+        if (relu) convert_columns<T, W, true>(r, bias ? bias + c0 : nullptr, P.mask != nullptr, v, word);
+        else convert_columns<T, W, false>(r, bias ? bias + c0 : nullptr, false, v, word);
+        if (!by_tma) {
+          if (c0 < valid) store_units<T, W / 8>(v, dst + c0, valid - c0);
+          __syncwarp();
+          return;
+        }
+        if (P.box_cols == 32) {      // 64-byte swizzle: unit u of row r lies at unit u ^ (r / 2 % 4)
+          if (lane == 0) tma_store_wait_read();
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < W / 8; ++u) *reinterpret_cast<uint4 *>(stage_ptr + lane * 64 + 16 * (u ^ ((lane >> 1) & 3))) = v[u];
+        } else {                     // 96-byte rows as they are
+          if (c0 == 0) {
+            if (lane == 0) tma_store_wait_read();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int u = 0; u < W / 8; ++u) *reinterpret_cast<uint4 *>(stage_ptr + lane * 96 + 2 * c0 + 16 * u) = v[u];
+        }
+        if (last) {
+          fence_proxy_async();
+          __syncwarp();
+          const int x = P.box_cols == 32 ? col + c0 : col;
+          if (lane == 0 && x < P.n_channels) tma_store_2d(&map_out, smem_u32(stage_ptr), x, m_warp);
+        }
       };
 #pragma unroll
       for (int piece = 0; piece < 2; ++piece) {
@@ -569,12 +613,12 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
           uint32_t r[32];
           tmem_ld_32x32(taddr + c0, r);
           tmem_ld_wait();
-          emit(r, c0, bits[piece]);
+          emit(r, c0, bits[piece], P.box_cols == 32);
         } else if (width - c0 == 16) {
           uint32_t r[16];
           tmem_ld_32x16(taddr + c0, r);
           tmem_ld_wait();
-          emit(r, c0, bits[piece]);
+          emit(r, c0, bits[piece], true);
         }
       }
       tc_fence_before();
@@ -594,6 +638,7 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
         }
       }
     }
+    if (MODE != kDw && lane == 0) tma_store_wait_all();
   } else if (warp == 3 && MODE != kDw) {
     // rows of no group are zero
     T *out = static_cast<T *>(P.out);
@@ -633,14 +678,17 @@ static GroupedEncodeFn grouped_encode_fn() {
   return fn;
 }
 
-// [n][channels] rows (stride in elements) or [experts][c_in][c_out] weights; boxes of 64 channels x box_rows, zeros outside.
-static int encode_map(CUtensorMap *map, int dtype, const void *p, int rank, int64_t channels, int64_t rows, int64_t row_stride, int64_t outer, int box_rows) {
+// [n][channels] rows (stride in elements) or [experts][c_in][c_out] weights; boxes of 64 channels x box_rows, zeros outside
+// (for stores: 32 channels with the 64-byte swizzle, or 48 without one).
+static int encode_map(CUtensorMap *map, int dtype, const void *p, int rank, int64_t channels, int64_t rows, int64_t row_stride, int64_t outer, int box_rows,
+                      int box_cols = 64) {
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(outer)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_stride) * 2, static_cast<cuuint64_t>(row_stride) * rows * 2};
-  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = grouped_encode_fn()(map, dtype == SPIRA_B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
-                                         const_cast<void *>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                         const_cast<void *>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                         box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
                                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(SPIRA_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
   return SPIRA_B200_OK;
@@ -663,12 +711,13 @@ int grouped_tc_dw_tiles(int c_in, int c_out) {
   return static_cast<int>(div_up(c_in, kGRows) * div_up(c_out, columns_per_tile(c_out, int64_t(1) << 30)));
 }
 
-// Two CTAs per tile where it has the rows and columns for both and enough work to fill the SMs in pairs.  Measured:
-// 80 026 rows in 16 groups, 512 -> 2048: PAIRFIGURES.
-static bool use_pair(int mode, const spira_b200_grouped_desc &D, int piece) {
+// Two CTAs per tile where it has the rows and columns for both, enough work to fill the SMs in pairs and a reduction long
+// enough for the fuller pipeline to matter.  Measured pair / single: 80 026 rows in 16 groups, 512 -> 2048: forward 146 /
+// 155 us, dx 111 / 131 us, dW 127 / 147 us; 40 000 rows in 8 groups, 256 -> 1024: forward 62 / 44 us.
+static bool use_pair(int mode, const spira_b200_grouped_desc &D) {
   if (mode == kDw) return D.c_in > kGRows && D.c_out >= 128 && D.n / D.experts >= 256;
   const int n = mode == kForward ? D.c_out : D.c_in, k = mode == kForward ? D.c_in : D.c_out;
-  return n >= 128 && k >= 192 && D.n / D.experts >= 512 && D.n / 256 * div_up(n, kGMaxN) >= sm_count() / 2;
+  return n >= 128 && k >= 384 && D.n / D.experts >= 512 && D.n / 256 * div_up(n, kGMaxN) >= sm_count() / 2;
 }
 
 int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float *partial, int32_t *status, unsigned long long wait_ns, cudaStream_t st) {
@@ -680,7 +729,7 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
   P.experts = D.experts;
   P.piece = piece;
   P.wait_ns = wait_ns;
-  const bool pair = use_pair(mode, D, piece);
+  const bool pair = use_pair(mode, D);
   P.tile_rows = pair ? 2 * kGRows : kGRows;
   int64_t units;
   if (mode == kDw) {
@@ -713,16 +762,25 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
   P.idesc = (1u << 4) | (D.dtype == SPIRA_B200_BF16 ? (1u << 7) | (1u << 10) : 0u) | (mode == kDw ? 1u << 15 : 0u) | (b_n_major ? 1u << 16 : 0u) |
             (static_cast<uint32_t>(P.bn >> 3) << 17) | (static_cast<uint32_t>(P.tile_rows >> 4) << 24);
   const int bars = 8 * (4 * kGMaxStages + 5);
-  const int fixed = kGBiasBytes + bars + 16 + 12 * (D.experts + 2);
+  int fixed = kGBiasBytes + bars + 16 + 12 * (D.experts + 2);
   const int stage_bytes = kGABytes + P.b_bytes;
+  // Stores: a scattered 16-byte store of 32 rows takes 32 passes of the load/store unit (4096 per tile of 128 x 256, where a
+  // reduction step takes 512), so results of short reductions leave through shared memory and TMA.  Longer ones hide the
+  // stores, and the staging buffers would cost a pipeline stage (80 026 x 2048 -> 512: 111 us direct, 121 us staged;
+  // 254 726 x 96 -> 384: 75 us staged, 81 us direct).
+  const int width = P.bn / 4, steps = static_cast<int>(div_up(P.k_channels, kGK));
+  P.box_cols = mode == kDw || width == 16 || steps > 8 ? 0 : width == 48 ? 48 : 32;
+  const int staging = kGEpilogueWarps * P.box_cols * 64;
+  fixed += staging;
   P.stages = (kGSmemBudget - fixed) / stage_bytes;
   if (P.stages > kGMaxStages) P.stages = kGMaxStages;
-  P.off_bias = P.stages * stage_bytes;
+  P.off_stage = P.stages * stage_bytes;
+  P.off_bias = P.off_stage + staging;
   P.off_bar = P.off_bias + kGBiasBytes;
   P.off_groups = P.off_bar + bars + 8;
-  const size_t smem = static_cast<size_t>(P.off_bias) + fixed + 1024;
+  const size_t smem = static_cast<size_t>(P.off_stage) + fixed + 1024;
 
-  alignas(64) CUtensorMap map_a, map_b;
+  alignas(64) CUtensorMap map_a, map_b, map_out;
   int rc;
   const int64_t x_stride = D.n == 1 ? D.c_in : D.x_stride, dy_stride = D.n == 1 ? D.c_out : D.dy_stride;
   if (mode == kForward) {
@@ -735,6 +793,8 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
     rc = encode_map(&map_a, D.dtype, D.x, 2, D.c_in, D.n, x_stride, 1, kGK);
     if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.dy, 2, D.c_out, D.n, dy_stride, 1, kGK);
   }
+  if (rc == SPIRA_B200_OK && P.box_cols) rc = encode_map(&map_out, D.dtype, P.out, 2, P.n_channels, D.n, P.n_channels, 1, 32, P.box_cols);
+  else map_out = map_a;
   if (rc != SPIRA_B200_OK) return rc;
   const int64_t tiles = units * P.n_tiles;
   SB_CHECK_ARG(tiles < (int64_t(1) << 31) - 65536, "grouped_linear: too many tiles");
@@ -760,7 +820,7 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
       ++cfg.numAttrs;
     }
     cfg.attrs = attr;
-    SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, map_a, map_b));
+    SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, map_a, map_b, map_out));
     return SPIRA_B200_OK;
   };
   auto pick = [&](auto type) -> int {

@@ -78,135 +78,117 @@ __device__ __forceinline__ void row_sums(float (&v)[M], float *scratch) {
   }
 }
 
-// mean and 1/deviation of the row in v (entries outside the row are skipped)
-template <int L, int ITEMS, int V>
-__device__ __forceinline__ void row_stats(const float (&v)[ITEMS][V], const bool (&in)[ITEMS], const NormParams &P, float *scratch, float &mean, float &r) {
+// f = w * f + b with what there is of the two parameters
+template <typename T, int V>
+__device__ __forceinline__ void affine(const void *w, const void *b, int f32, int c, float (&f)[V]) {
+  float q[V];
+  if (w) {
+    load_param<T, V>(w, f32, c, q);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] *= q[e];
+  }
+  if (b) {
+    load_param<T, V>(b, f32, c, q);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] += q[e];
+  }
+}
+
+// v becomes (v - mean) / deviation; st gets the mean and 1 / deviation.  Pieces outside the row are skipped.
+template <int L, int ITEMS, int V, bool LAYER>
+__device__ __forceinline__ void normalise(float (&v)[ITEMS][V], const bool (&in)[ITEMS], const NormParams &P, float *scratch, float &mean, float &r) {
   float s[1] = {0.f};
-  mean = 0.f;
-  if (P.layer) {
+  if (LAYER) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
+      if (in[i])
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[0] += in[i] ? v[i][e] : 0.f;
+        for (int e = 0; e < V; ++e) s[0] += v[i][e];
     row_sums<L, 1>(s, scratch);
     mean = s[0] * P.inv_channels;
     s[0] = 0.f;
   }
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i)
+    if (in[i])
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float d = v[i][e] - mean;
-      s[0] += in[i] ? d * d : 0.f;
-    }
+      for (int e = 0; e < V; ++e) {
+        if (LAYER) v[i][e] -= mean;
+        s[0] = fmaf(v[i][e], v[i][e], s[0]);
+      }
   row_sums<L, 1>(s, scratch);
-  r = 1.f / sqrtf(s[0] * P.inv_channels + P.eps);
+  r = rsqrtf(fmaf(s[0], P.inv_channels, P.eps));
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[i][e] *= r;
 }
 
-// L threads per row, each with ITEMS pieces of V neighbouring channels, L pieces apart.
-template <typename T, int V, int L, int ITEMS>
-__global__ void __launch_bounds__(L > 256 ? L : 256, ITEMS > 1 || L > 256 ? 1 : 3) norm_forward_kernel(const __grid_constant__ NormParams P) {
-  constexpr int kThreads = L > 256 ? L : 256;
+// Threads of a CTA: 256, or the row's if it takes more.
+template <int L>
+constexpr int kNormThreads = L > 256 ? L : 256;
+
+// L threads per row, each with ITEMS pieces of V neighbouring channels, L pieces apart.  What limits these kernels is not
+// memory alone but instructions (20 to 40 per element against 8 to 14 bytes): options are tested per row and never per
+// element, conversions work on pairs.
+template <typename T, int V, int L, int ITEMS, bool LAYER>
+__global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 4) norm_forward_kernel(const __grid_constant__ NormParams P) {
   __shared__ float scratch[32];
   pdl_trigger();
   pdl_wait();
   const int g = threadIdx.x % L;
-  constexpr int kRows = kThreads / L;
+  constexpr int kRows = kNormThreads<L> / L;
   const int64_t rounds = (P.n + kRows - 1) / kRows;
   bool in[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) in[i] = (i * L + g) * V < P.channels;
-  // the next row's values are on their way while this row is worked on
-  Vec<T, V> raw_x[ITEMS], raw_p[ITEMS], raw_g[ITEMS];
-  auto fetch = [&](int64_t b) {
-    const int64_t row = b * kRows + threadIdx.x / L;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      raw_x[i] = raw_p[i] = raw_g[i] = Vec<T, V>{};
-      if (b < rounds && row < P.n && in[i]) {
-        const int c = (i * L + g) * V;
-        raw_x[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.x) + row * P.x_stride + c);
-        if (P.block) raw_p[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.block) + row * P.block_stride + c);
-        if (P.gate_kind == kGateFull) raw_g[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.gate) + row * P.gate_stride + c);
-      }
-    }
-  };
-  constexpr bool kAhead = ITEMS <= 2;
-  if (kAhead) fetch(blockIdx.x);
   for (int64_t b = blockIdx.x; b < rounds; b += gridDim.x) {
     const int64_t row = b * kRows + threadIdx.x / L;
     const bool live = row < P.n;
-    if (!kAhead) fetch(b);
-    float x[ITEMS][V], p[ITEMS][V];
+    float x[ITEMS][V] = {}, p[ITEMS][V] = {};
     Vec<T, V> gates[ITEMS];
+    float row_gate = P.block_scale;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        x[i][e] = to_f32(raw_x[i].v[e]);
-        p[i][e] = to_f32(raw_p[i].v[e]);
+    for (int i = 0; i < ITEMS; ++i)
+      if (live && in[i]) {
+        const int c = (i * L + g) * V;
+        load_f32<T, V>(static_cast<const T *>(P.x) + row * P.x_stride + c, x[i]);
+        if (P.block) load_f32<T, V>(static_cast<const T *>(P.block) + row * P.block_stride + c, p[i]);
+        if (P.gate_kind == kGateFull) gates[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.gate) + row * P.gate_stride + c);
       }
-      gates[i] = raw_g[i];
-    }
-    if (kAhead) fetch(b + gridDim.x);
+    if (P.gate_kind == kGateRow && live) row_gate *= to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]);
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
     if (P.block) {
       if (P.post) {
-        row_stats<L, ITEMS, V>(p, in, P, scratch, st.x, st.y);
+        normalise<L, ITEMS, V, LAYER>(p, in, P, scratch, st.x, st.y);
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-          if (!in[i]) continue;
-          float w[V];
-          const int c = (i * L + g) * V;
-#pragma unroll
-          for (int e = 0; e < V; ++e) p[i][e] = (p[i][e] - st.x) * st.y;
-          if (P.post_weight) {
-            load_param<T, V>(P.post_weight, P.params_f32, c, w);
-#pragma unroll
-            for (int e = 0; e < V; ++e) p[i][e] *= w[e];
-          }
-          if (P.post_bias) {
-            load_param<T, V>(P.post_bias, P.params_f32, c, w);
-#pragma unroll
-            for (int e = 0; e < V; ++e) p[i][e] += w[e];
-          }
-        }
+        for (int i = 0; i < ITEMS; ++i)
+          if (in[i]) affine<T, V>(P.post_weight, P.post_bias, P.params_f32, (i * L + g) * V, p[i]);
       }
-      const float row_gate = P.gate_kind == kGateRow && live ? to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]) : 1.f;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         if (!in[i]) continue;
         const int c = (i * L + g) * V;
-        float gate[V];
-        if (P.gate_kind == kGateChannel) load_param<T, V>(P.gate, P.params_f32, c, gate);
-        else {
+        if (P.gate_kind == kGateChannel) {
+          affine<T, V>(P.gate, nullptr, P.params_f32, c, p[i]);
+        } else if (P.gate_kind == kGateFull) {
+          float f[V];
+          vec_to_f32<T, V>(gates[i], f);
 #pragma unroll
-          for (int e = 0; e < V; ++e) gate[e] = P.gate_kind == kGateFull ? to_f32(gates[i].v[e]) : row_gate;
+          for (int e = 0; e < V; ++e) p[i][e] *= f[e];
         }
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[i][e] = P.residual_scale * x[i][e] + P.block_scale * (gate[e] * p[i][e]);
-        if (live && P.stream) store_f32<T, V>(static_cast<T *>(P.stream) + row * P.channels + c, x[i]);
+        for (int e = 0; e < V; ++e) x[i][e] = fmaf(row_gate, p[i][e], P.residual_scale * x[i][e]);
+        if (live) store_f32<T, V>(static_cast<T *>(P.stream) + row * P.channels + c, x[i]);
       }
     }
     if (P.pre) {
-      row_stats<L, ITEMS, V>(x, in, P, scratch, st.z, st.w);
+      normalise<L, ITEMS, V, LAYER>(x, in, P, scratch, st.z, st.w);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         if (!in[i]) continue;
         const int c = (i * L + g) * V;
-        float w[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[i][e] = (x[i][e] - st.z) * st.w;
-        if (P.weight) {
-          load_param<T, V>(P.weight, P.params_f32, c, w);
-#pragma unroll
-          for (int e = 0; e < V; ++e) x[i][e] *= w[e];
-        }
-        if (P.bias) {
-          load_param<T, V>(P.bias, P.params_f32, c, w);
-#pragma unroll
-          for (int e = 0; e < V; ++e) x[i][e] += w[e];
-        }
+        affine<T, V>(P.weight, P.bias, P.params_f32, c, x[i]);
         if (live) store_f32<T, V>(static_cast<T *>(P.normed) + row * P.channels + c, x[i]);
       }
     }
@@ -214,9 +196,9 @@ __global__ void __launch_bounds__(L > 256 ? L : 256, ITEMS > 1 || L > 256 ? 1 : 
   }
 }
 
-template <typename T, int V, int L, int ITEMS>
-__global__ void __launch_bounds__(L > 256 ? L : 256, ITEMS > 1 || L > 256 ? 1 : 2) norm_backward_kernel(const __grid_constant__ NormParams P) {
-  constexpr int kThreads = L > 256 ? L : 256;
+template <typename T, int V, int L, int ITEMS, bool LAYER>
+__global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) norm_backward_kernel(const __grid_constant__ NormParams P) {
+  constexpr int kThreads = kNormThreads<L>;
   __shared__ float scratch[64];
   extern __shared__ float column_sums[];      // [kThreads / L][channels]
   pdl_trigger();
@@ -225,105 +207,94 @@ __global__ void __launch_bounds__(L > 256 ? L : 256, ITEMS > 1 || L > 256 ? 1 : 
   constexpr int kRows = kThreads / L;
   const int64_t rounds = (P.n + kRows - 1) / kRows;
   const float a = P.residual_scale, s = P.block_scale;
+  const void *post_w = P.post ? P.post_weight : nullptr, *post_b = P.post ? P.post_bias : nullptr;
   bool in[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) in[i] = (i * L + g) * V < P.channels;
   float sum[kSums][ITEMS][V] = {};
-  Vec<T, V> raw_x[ITEMS], raw_p[ITEMS], raw_g[ITEMS], raw_d[ITEMS], raw_h[ITEMS];
-  float4 raw_st = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto piece = [&](const void *base, int64_t at) { return *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(base) + at); };
-  auto fetch = [&](int64_t b) {
-    const int64_t row = b * kRows + threadIdx.x / L;
-    const bool there = b < rounds && row < P.n;
-    if (there) raw_st = reinterpret_cast<const float4 *>(P.stats)[row];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      raw_x[i] = raw_p[i] = raw_g[i] = raw_d[i] = raw_h[i] = Vec<T, V>{};
-      if (there && in[i]) {
-        const int c = (i * L + g) * V;
-        if (P.pre) raw_x[i] = piece(P.x, row * P.x_stride + c);
-        if (P.block) raw_p[i] = piece(P.block, row * P.block_stride + c);
-        if (P.dstream) raw_d[i] = piece(P.dstream, row * P.dstream_stride + c);
-        if (P.pre) raw_h[i] = piece(P.dnormed, row * P.dnormed_stride + c);
-        if (P.gate_kind == kGateFull) raw_g[i] = piece(P.gate, row * P.gate_stride + c);
-      }
-    }
-  };
-  constexpr bool kAhead = ITEMS == 1;      // (two pieces per thread leave no registers for a second row)
-  if (kAhead) fetch(blockIdx.x);
   for (int64_t b = blockIdx.x; b < rounds; b += gridDim.x) {
     const int64_t row = b * kRows + threadIdx.x / L;
     const bool live = row < P.n;
-    if (!kAhead) fetch(b);
-    const float4 st = live ? raw_st : make_float4(0.f, 0.f, 0.f, 0.f);
-    float hat[ITEMS][V], p[ITEMS][V], gate[ITEMS][V], d[ITEMS][V], dh[ITEMS][V];
-    const float row_gate = P.gate_kind == kGateRow && live ? to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]) : 1.f;
+    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+    // hat: x, then the stream's normalised value; bh: the block's normalised value (or the block); d: gradient of the stream
+    float hat[ITEMS][V] = {}, bh[ITEMS][V] = {}, d[ITEMS][V] = {}, u[ITEMS][V] = {};
+    Vec<T, V> gates[ITEMS];
+    float row_gate = 1.f;
+    if (live) {
+      st = reinterpret_cast<const float4 *>(P.stats)[row];
+      if (P.gate_kind == kGateRow) row_gate = to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]);
+    }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        hat[i][e] = to_f32(raw_x[i].v[e]);
-        p[i][e] = to_f32(raw_p[i].v[e]);
-        gate[i][e] = to_f32(raw_g[i].v[e]);
-        d[i][e] = to_f32(raw_d[i].v[e]);
-        dh[i][e] = to_f32(raw_h[i].v[e]);
+      if (live && in[i]) {
+        const int c = (i * L + g) * V;
+        if (P.pre) {
+          load_f32<T, V>(static_cast<const T *>(P.x) + row * P.x_stride + c, hat[i]);
+          load_f32<T, V>(static_cast<const T *>(P.dnormed) + row * P.dnormed_stride + c, u[i]);
+        }
+        if (P.block) load_f32<T, V>(static_cast<const T *>(P.block) + row * P.block_stride + c, bh[i]);
+        if (P.dstream) load_f32<T, V>(static_cast<const T *>(P.dstream) + row * P.dstream_stride + c, d[i]);
+        if (P.gate_kind == kGateFull) gates[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.gate) + row * P.gate_stride + c);
       }
-    if (kAhead) fetch(b + gridDim.x);
-    // the block's normalised value, its affine form is rebuilt where it is needed
     float sums[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      if (!in[i]) continue;
-      const int c = (i * L + g) * V;
-      if (P.gate_kind == kGateChannel) load_param<T, V>(P.gate, P.params_f32, c, gate[i]);
-      else if (P.gate_kind != kGateFull) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) gate[i][e] = row_gate;
-      }
-      if (P.post)
-#pragma unroll
-        for (int e = 0; e < V; ++e) p[i][e] = (p[i][e] - st.x) * st.y;
-      if (P.pre) {
-        float w[V], q[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) { w[e] = 1.f; q[e] = p[i][e]; }
-        if (P.post && P.post_weight) {
-          load_param<T, V>(P.post_weight, P.params_f32, c, w);
-#pragma unroll
-          for (int e = 0; e < V; ++e) q[e] *= w[e];
-        }
-        if (P.post && P.post_bias) {
-          load_param<T, V>(P.post_bias, P.params_f32, c, w);
-#pragma unroll
-          for (int e = 0; e < V; ++e) q[e] += w[e];
-        }
-        if (P.block)
-#pragma unroll
-          for (int e = 0; e < V; ++e) hat[i][e] = a * hat[i][e] + s * (gate[i][e] * q[e]);
-#pragma unroll
-        for (int e = 0; e < V; ++e) hat[i][e] = (hat[i][e] - st.z) * st.w;
-        if (P.weight) load_param<T, V>(P.weight, P.params_f32, c, w);
-        else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) w[e] = 1.f;
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          sum[0][i][e] += dh[i][e] * hat[i][e];
-          sum[1][i][e] += dh[i][e];
-          dh[i][e] *= w[e];
-          sums[0] += dh[i][e] * hat[i][e];
-          sums[1] += dh[i][e];
-        }
-      }
-    }
-    if (P.pre) {
-      row_sums<L, 2>(sums, scratch);
-      const float m0 = sums[0] * P.inv_channels, m1 = P.layer ? sums[1] * P.inv_channels : 0.f;
+    if (P.post) {
+      const float shift = -st.x * st.y;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) d[i][e] += st.w * (dh[i][e] - hat[i][e] * m0 - m1);
+        for (int e = 0; e < V; ++e) bh[i][e] = LAYER ? fmaf(bh[i][e], st.y, shift) : bh[i][e] * st.y;
+    }
+    // the factor of the block's value in the stream without block_scale
+    auto load_gate = [&](int i, int c, float (&f)[V]) {
+      if (P.gate_kind == kGateChannel) load_param<T, V>(P.gate, P.params_f32, c, f);
+      else if (P.gate_kind == kGateFull && live) vec_to_f32<T, V>(gates[i], f);
+      else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = row_gate;
+      }
+    };
+    if (P.pre) {
+      const float shift = -st.z * st.w;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        if (!in[i]) continue;
+        const int c = (i * L + g) * V;
+        if (P.block) {
+          float q[V], f[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) q[e] = bh[i][e];
+          affine<T, V>(post_w, post_b, P.params_f32, c, q);
+          if (P.gate_kind != kGateNone) {
+            load_gate(i, c, f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) q[e] *= f[e];
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) hat[i][e] = fmaf(s, q[e], a * hat[i][e]);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          hat[i][e] = LAYER ? fmaf(hat[i][e], st.w, shift) : hat[i][e] * st.w;
+          sum[0][i][e] = fmaf(u[i][e], hat[i][e], sum[0][i][e]);
+          sum[1][i][e] += u[i][e];
+        }
+        affine<T, V>(P.weight, nullptr, P.params_f32, c, u[i]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          sums[0] = fmaf(u[i][e], hat[i][e], sums[0]);
+          if (LAYER) sums[1] += u[i][e];
+        }
+      }
+      row_sums<L, 2>(sums, scratch);
+      const float m0 = -sums[0] * P.inv_channels * st.w, m1 = LAYER ? -sums[1] * P.inv_channels * st.w : 0.f;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          d[i][e] = fmaf(u[i][e], st.w, d[i][e]);
+          d[i][e] = fmaf(hat[i][e], m0, d[i][e]);
+          if (LAYER) d[i][e] += m1;
+        }
     }
     if (live && P.dx)
 #pragma unroll
@@ -341,32 +312,42 @@ __global__ void __launch_bounds__(L > 256 ? L : 256, ITEMS > 1 || L > 256 ? 1 : 
       for (int i = 0; i < ITEMS; ++i) {
         if (!in[i]) continue;
         const int c = (i * L + g) * V;
-        float w[V], q[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) { w[e] = 1.f; q[e] = 0.f; }
-        if (P.post && P.post_weight) load_param<T, V>(P.post_weight, P.params_f32, c, w);
-        if (P.gate_kind != kGateNone && P.post && P.post_bias) load_param<T, V>(P.post_bias, P.params_f32, c, q);
-        float dg[V];
+        for (int e = 0; e < V; ++e) d[i][e] *= s;
+        if (P.gate_kind != kGateNone) {
+          float q[V], f[V];
+          load_gate(i, c, f);
+          if (P.dgate) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          dg[e] = s * d[i][e] * (p[i][e] * w[e] + q[e]);
-          const float v = s * gate[i][e] * d[i][e];
-          if (P.post) {
-            sum[2][i][e] += v * p[i][e];
-            sum[3][i][e] += v;
+            for (int e = 0; e < V; ++e) q[e] = bh[i][e];
+            affine<T, V>(post_w, post_b, P.params_f32, c, q);
+#pragma unroll
+            for (int e = 0; e < V; ++e) q[e] *= d[i][e];
+            if (P.gate_kind == kGateChannel) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) sum[4][i][e] += q[e];
+            } else if (P.gate_kind == kGateRow) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) gate_sum[0] += q[e];
+            } else if (live) {
+              store_f32<T, V>(static_cast<T *>(P.dgate) + row * P.channels + c, q);
+            }
           }
-          d[i][e] = v * w[e];
-          sums[0] += d[i][e] * p[i][e];
-          sums[1] += d[i][e];
+#pragma unroll
+          for (int e = 0; e < V; ++e) d[i][e] *= f[e];
         }
-        if (P.gate_kind == kGateChannel) {
+        if (P.post) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) sum[4][i][e] += dg[e];
-        } else if (P.gate_kind == kGateRow) {
+          for (int e = 0; e < V; ++e) {
+            sum[2][i][e] = fmaf(d[i][e], bh[i][e], sum[2][i][e]);
+            sum[3][i][e] += d[i][e];
+          }
+          affine<T, V>(post_w, nullptr, P.params_f32, c, d[i]);
 #pragma unroll
-          for (int e = 0; e < V; ++e) gate_sum[0] += dg[e];
-        } else if (P.gate_kind == kGateFull && live && P.dgate) {
-          store_f32<T, V>(static_cast<T *>(P.dgate) + row * P.channels + c, dg);
+          for (int e = 0; e < V; ++e) {
+            sums[0] = fmaf(d[i][e], bh[i][e], sums[0]);
+            if (LAYER) sums[1] += d[i][e];
+          }
         }
       }
       if (P.gate_kind == kGateRow && P.dgate) {
@@ -376,11 +357,11 @@ __global__ void __launch_bounds__(L > 256 ? L : 256, ITEMS > 1 || L > 256 ? 1 : 
       if (P.dblock) {
         if (P.post) {
           row_sums<L, 2>(sums, scratch);
-          const float m0 = sums[0] * P.inv_channels, m1 = P.layer ? sums[1] * P.inv_channels : 0.f;
+          const float m0 = -sums[0] * P.inv_channels, m1 = LAYER ? -sums[1] * P.inv_channels : 0.f;
 #pragma unroll
           for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[i][e] = st.y * (d[i][e] - p[i][e] * m0 - m1);
+            for (int e = 0; e < V; ++e) d[i][e] = st.y * fmaf(bh[i][e], m0, LAYER ? d[i][e] + m1 : d[i][e]);
         }
         if (live)
 #pragma unroll
@@ -460,24 +441,30 @@ static int resident_ctas(K kernel, int threads) {
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) == cudaSuccess && n > 0 ? n : 1;
 }
 
-template <typename T, int V, int L, int ITEMS>
-static int launch_norm(const NormParams &P, bool backward, int *ctas, cudaStream_t st) {
-  constexpr int kThreads = L > 256 ? L : 256;
+template <typename T, int V, int L, int ITEMS, bool LAYER>
+static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaStream_t st) {
+  constexpr int kThreads = kNormThreads<L>;
   constexpr int kRows = kThreads / L;
   const int64_t rounds = div_up(P.n, kRows);
   if (!backward) {
-    static const int resident = resident_ctas(norm_forward_kernel<T, V, L, ITEMS>, kThreads);
+    static const int resident = resident_ctas(norm_forward_kernel<T, V, L, ITEMS, LAYER>, kThreads);
     const int64_t cap = static_cast<int64_t>(sm_count()) * resident;
-    SB_CHECK_CUDA(launch_dependent(norm_forward_kernel<T, V, L, ITEMS>, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), 0, st, P));
+    SB_CHECK_CUDA(launch_dependent(norm_forward_kernel<T, V, L, ITEMS, LAYER>, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), 0,
+                                   st, P));
     return SPIRA_B200_OK;
   }
-  static const int resident = resident_ctas(norm_backward_kernel<T, V, L, ITEMS>, kThreads);
+  static const int resident = resident_ctas(norm_backward_kernel<T, V, L, ITEMS, LAYER>, kThreads);
   const int64_t cap = static_cast<int64_t>(sm_count()) * (resident < kNormBackwardCtas ? resident : kNormBackwardCtas);
   const int grid = static_cast<int>(rounds < cap ? rounds : cap);
   *ctas = grid;
   const size_t smem = kRows > 1 ? static_cast<size_t>(kRows) * P.channels * 4 : 0;
-  SB_CHECK_CUDA(launch_dependent(norm_backward_kernel<T, V, L, ITEMS>, dim3(grid), dim3(kThreads), smem, st, P));
+  SB_CHECK_CUDA(launch_dependent(norm_backward_kernel<T, V, L, ITEMS, LAYER>, dim3(grid), dim3(kThreads), smem, st, P));
   return SPIRA_B200_OK;
+}
+
+template <typename T, int V, int L, int ITEMS>
+static int launch_norm(const NormParams &P, bool backward, int *ctas, cudaStream_t st) {
+  return P.layer ? launch_norm_kind<T, V, L, ITEMS, true>(P, backward, ctas, st) : launch_norm_kind<T, V, L, ITEMS, false>(P, backward, ctas, st);
 }
 
 // Threads per row and pieces per thread: the fewest lanes that hold the row, so that a row sum takes few shuffles; rows too
