@@ -14,6 +14,7 @@
 // Bound by memory: forward 2 row reads + 2 row writes, backward 4 + 2 (one more of each with a gate per element).
 #include "common.cuh"
 #include "elem.cuh"
+#include "ptx.cuh"
 
 namespace sb {
 
@@ -28,9 +29,128 @@ struct NormParams {
   void *stream, *normed, *dx, *dblock, *dgate;
   float *stats;               // [n][4]: mean and 1/deviation of the block, mean and 1/deviation of the stream
   float *partial;             // [CTAs][kSums][channels]
-  int64_t n, x_stride, block_stride, gate_stride, dstream_stride, dnormed_stride;
+  int n, x_stride, block_stride, gate_stride, dstream_stride, dnormed_stride;      // (element strides below 2^31: one wide multiply per row)
   int channels, layer, pre, post, gate_kind, params_f32;
   float residual_scale, block_scale, eps, inv_channels;
+};
+
+// Arithmetic on V neighbouring channels, two at a time where V is even (packed fp32 instructions: half the issue slots).
+__device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2(float &d0, float &d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float &d0, float &d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+template <int V>
+struct Ops {
+  typedef float A[V];
+  // d = a * b + c
+  static __device__ __forceinline__ void fma(A &d, const A &a, const A &b, const A &c) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) fma2(d[e], d[e + 1], a[e], a[e + 1], b[e], b[e + 1], c[e], c[e + 1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = fmaf(a[e], b[e], c[e]);
+    }
+  }
+  // d = a * s + c
+  static __device__ __forceinline__ void fma(A &d, const A &a, float s, const A &c) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) fma2(d[e], d[e + 1], a[e], a[e + 1], s, s, c[e], c[e + 1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = fmaf(a[e], s, c[e]);
+    }
+  }
+  // d = a * s + t
+  static __device__ __forceinline__ void fma(A &d, const A &a, float s, float t) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) fma2(d[e], d[e + 1], a[e], a[e + 1], s, s, t, t);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = fmaf(a[e], s, t);
+    }
+  }
+  static __device__ __forceinline__ void mul(A &d, const A &a, const A &b) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) mul2(d[e], d[e + 1], a[e], a[e + 1], b[e], b[e + 1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = a[e] * b[e];
+    }
+  }
+  static __device__ __forceinline__ void mul(A &d, const A &a, float s) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) mul2(d[e], d[e + 1], a[e], a[e + 1], s, s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = a[e] * s;
+    }
+  }
+  static __device__ __forceinline__ void add(A &d, const A &a, const A &b) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) add2(d[e], d[e + 1], a[e], a[e + 1], b[e], b[e + 1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = a[e] + b[e];
+    }
+  }
+  static __device__ __forceinline__ void add(A &d, const A &a, float t) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) add2(d[e], d[e + 1], a[e], a[e + 1], t, t);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = a[e] + t;
+    }
+  }
+  static __device__ __forceinline__ float sum(const A &a) {
+    if constexpr (V == 8) {
+      float t[4];
+      add2(t[0], t[1], a[0], a[1], a[2], a[3]);
+      add2(t[2], t[3], a[4], a[5], a[6], a[7]);
+      add2(t[0], t[1], t[0], t[1], t[2], t[3]);
+      return t[0] + t[1];
+    } else if constexpr (V == 4) {
+      float t[2];
+      add2(t[0], t[1], a[0], a[1], a[2], a[3]);
+      return t[0] + t[1];
+    } else {
+      float t = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) t += a[e];
+      return t;
+    }
+  }
+  static __device__ __forceinline__ float dot(const A &a, const A &b) {
+    if constexpr (V == 8 || V == 4) {
+      float t[2];
+      mul2(t[0], t[1], a[0], a[1], b[0], b[1]);
+#pragma unroll
+      for (int e = 2; e < V; e += 2) fma2(t[0], t[1], a[e], a[e + 1], b[e], b[e + 1], t[0], t[1]);
+      return t[0] + t[1];
+    } else {
+      float t = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) t = fmaf(a[e], b[e], t);
+      return t;
+    }
+  }
 };
 
 // V parameters from element `c` on, as fp32 (parameters are stored in the rows' type or in fp32).
@@ -78,121 +198,188 @@ __device__ __forceinline__ void row_sums(float (&v)[M], float *scratch) {
   }
 }
 
-// f = w * f + b with what there is of the two parameters
-template <typename T, int V>
-__device__ __forceinline__ void affine(const void *w, const void *b, int f32, int c, float (&f)[V]) {
+// v[r] = w * v[r] + b with what there is of the two parameters, for R rows
+template <typename T, int V, int R>
+__device__ __forceinline__ void affine(const void *w, const void *b, int f32, int c, float (&v)[R][V]) {
   float q[V];
   if (w) {
     load_param<T, V>(w, f32, c, q);
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] *= q[e];
+    for (int r = 0; r < R; ++r) Ops<V>::mul(v[r], v[r], q);
   }
   if (b) {
     load_param<T, V>(b, f32, c, q);
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] += q[e];
+    for (int r = 0; r < R; ++r) Ops<V>::add(v[r], v[r], q);
   }
 }
 
-// v becomes (v - mean) / deviation; st gets the mean and 1 / deviation.  Pieces outside the row are skipped.
-template <int L, int ITEMS, int V, bool LAYER>
-__device__ __forceinline__ void normalise(float (&v)[ITEMS][V], const bool (&in)[ITEMS], const NormParams &P, float *scratch, float &mean, float &r) {
-  float s[1] = {0.f};
+// v becomes (v - mean) / deviation for R rows at once; mean and 1 / deviation are returned.  Pieces outside the row are skipped.
+template <int L, int ITEMS, int R, int V, bool LAYER>
+__device__ __forceinline__ void normalise(float (&v)[ITEMS][R][V], const bool (&in)[ITEMS], const NormParams &P, float *scratch, float (&mean)[R], float (&dev)[R]) {
+  float s[R];
   if (LAYER) {
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      if (in[i])
+    for (int r = 0; r < R; ++r) {
+      s[r] = 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[0] += v[i][e];
-    row_sums<L, 1>(s, scratch);
-    mean = s[0] * P.inv_channels;
-    s[0] = 0.f;
+      for (int i = 0; i < ITEMS; ++i)
+        if (in[i]) s[r] += Ops<V>::sum(v[i][r]);
+    }
+    row_sums<L, R>(s, scratch);
+#pragma unroll
+    for (int r = 0; r < R; ++r) mean[r] = s[r] * P.inv_channels;
   }
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i)
-    if (in[i])
+  for (int r = 0; r < R; ++r) {
+    s[r] = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (LAYER) v[i][e] -= mean;
-        s[0] = fmaf(v[i][e], v[i][e], s[0]);
-      }
-  row_sums<L, 1>(s, scratch);
-  r = rsqrtf(fmaf(s[0], P.inv_channels, P.eps));
+    for (int i = 0; i < ITEMS; ++i) {
+      if (LAYER) Ops<V>::add(v[i][r], v[i][r], -mean[r]);
+      const float t = Ops<V>::dot(v[i][r], v[i][r]);
+      if (in[i]) s[r] += t;
+    }
+  }
+  row_sums<L, R>(s, scratch);
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i)
+  for (int r = 0; r < R; ++r) {
+    dev[r] = rsqrtf(fmaf(s[r], P.inv_channels, P.eps));
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[i][e] *= r;
+    for (int i = 0; i < ITEMS; ++i) Ops<V>::mul(v[i][r], v[i][r], dev[r]);
+  }
 }
 
 // Threads of a CTA: 256, or the row's if it takes more.
 template <int L>
 constexpr int kNormThreads = L > 256 ? L : 256;
 
-// L threads per row, each with ITEMS pieces of V neighbouring channels, L pieces apart.  What limits these kernels is not
-// memory alone but instructions (20 to 40 per element against 8 to 14 bytes): options are tested per row and never per
-// element, conversions work on pairs.
-template <typename T, int V, int L, int ITEMS, bool LAYER>
-__global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 4) norm_forward_kernel(const __grid_constant__ NormParams P) {
-  __shared__ float scratch[32];
+// The rows on their way: every thread copies its own 16-byte pieces of the next rows into shared memory (cp.async, past the
+// L1, where the parameters stay) and reads them back itself, so no barrier is needed and no register waits for a load.
+// A ring of kDepth rounds of kPieces pieces per thread; 0 where the pieces are not 16 bytes or would take too much room.
+template <int THREADS, int PIECES, bool WIDE>
+struct Ring {
+  static constexpr int kStage = THREADS * PIECES * 16;
+  static constexpr int kDepth = !WIDE ? 0 : kStage <= 24 * 1024 ? 3 : kStage <= 80 * 1024 ? 2 : 0;
+  static constexpr int kBytes = kDepth * kStage;
+  unsigned char *base;      // this thread's first piece
+  __device__ __forceinline__ explicit Ring(unsigned char *smem) : base(smem + threadIdx.x * 16) {}
+  __device__ __forceinline__ unsigned char *piece(int stage, int i) const { return base + (stage * PIECES + i) * THREADS * 16; }
+  __device__ __forceinline__ void copy(int stage, int i, const void *src) const { ptx::cp_async_16(ptx::smem_u32(piece(stage, i)), src, 16); }
+  static __device__ __forceinline__ void commit() { ptx::cp_async_commit(); }
+  static __device__ __forceinline__ void wait() { ptx::cp_async_wait<kDepth == 0 ? 0 : kDepth - 1>(); }
+};
+
+// L threads per row, each with ITEMS pieces of V neighbouring channels, L pieces apart, and R rows at once.  What limits
+// these kernels is not memory alone but instructions and the latency of a row's chain (load, row sum, row sum, store):
+// loads run rounds ahead, options are tested per row and never per element, conversions and arithmetic work on pairs, two rows share the parameter
+// loads and overlap their sums.  Loads are clamped into the tensor instead of guarded; only stores and sums ask whether a
+// row or a piece exists.
+template <typename T, int V, int L, int ITEMS, int R, bool LAYER>
+__global__ void __launch_bounds__(kNormThreads<L>) norm_forward_kernel(const __grid_constant__ NormParams P) {
+  __shared__ float scratch[64];
   pdl_trigger();
   pdl_wait();
   const int g = threadIdx.x % L;
   constexpr int kRows = kNormThreads<L> / L;
-  const int64_t rounds = (P.n + kRows - 1) / kRows;
+  const int rounds = (P.n + kRows * R - 1) / (kRows * R);
   bool in[ITEMS];
+  int col[ITEMS];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) in[i] = (i * L + g) * V < P.channels;
-  for (int64_t b = blockIdx.x; b < rounds; b += gridDim.x) {
-    const int64_t row = b * kRows + threadIdx.x / L;
-    const bool live = row < P.n;
-    float x[ITEMS][V] = {}, p[ITEMS][V] = {};
-    Vec<T, V> gates[ITEMS];
-    float row_gate = P.block_scale;
+  for (int i = 0; i < ITEMS; ++i) {
+    in[i] = (i * L + g) * V < P.channels;
+    col[i] = in[i] ? (i * L + g) * V : 0;
+  }
+  extern __shared__ __align__(16) unsigned char norm_ring[];
+  typedef Ring<kNormThreads<L>, 3 * ITEMS * R, V * sizeof(T) == 16> Rows;
+  const Rows ring(norm_ring);
+  constexpr int kDepth = Rows::kDepth;
+  auto source = [&](int which, int64_t row, int c) -> const T * {
+    if (which == 0) return static_cast<const T *>(P.x) + row * P.x_stride + c;
+    if (which == 1) return static_cast<const T *>(P.block) + row * P.block_stride + c;
+    return static_cast<const T *>(P.gate) + row * P.gate_stride + c;
+  };
+  const bool used[3] = {true, P.block != nullptr, P.gate_kind == kGateFull};
+  auto row_of = [&](int b, int r) {
+    const int row = (b * kRows + static_cast<int>(threadIdx.x) / L) * R + r;
+    return row < P.n ? row : P.n - 1;
+  };
+  auto fetch = [&](int stage, int b) {
+    if (b < rounds)
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      if (live && in[i]) {
-        const int c = (i * L + g) * V;
-        load_f32<T, V>(static_cast<const T *>(P.x) + row * P.x_stride + c, x[i]);
-        if (P.block) load_f32<T, V>(static_cast<const T *>(P.block) + row * P.block_stride + c, p[i]);
-        if (P.gate_kind == kGateFull) gates[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.gate) + row * P.gate_stride + c);
+      for (int w = 0; w < 3; ++w)
+        if (used[w])
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) ring.copy(stage, (w * R + r) * ITEMS + i, source(w, row_of(b, r), col[i]));
+    Rows::commit();
+  };
+  auto take = [&](int stage, int w, int r, int i, int64_t row) -> Vec<T, V> {
+    if constexpr (kDepth > 0) return *reinterpret_cast<const Vec<T, V> *>(ring.piece(stage, (w * R + r) * ITEMS + i));
+    else return *reinterpret_cast<const Vec<T, V> *>(source(w, row, col[i]));
+  };
+  int stage = 0;
+  if constexpr (kDepth > 0)
+    for (int k = 0; k < kDepth - 1; ++k) fetch(k, blockIdx.x + k * gridDim.x);
+  for (int b = blockIdx.x; b < rounds; b += gridDim.x) {
+    if constexpr (kDepth > 0) {
+      fetch(stage == 0 ? kDepth - 1 : stage - 1, b + (kDepth - 1) * gridDim.x);
+      Rows::wait();
+    }
+    const int row0 = (b * kRows + static_cast<int>(threadIdx.x) / L) * R;
+    float x[ITEMS][R][V], p[ITEMS][R][V];
+    Vec<T, V> gates[ITEMS][R];
+    float row_gate[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row_of(b, r);
+      row_gate[r] = P.block_scale;
+      if (P.gate_kind == kGateRow) row_gate[r] *= to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        vec_to_f32<T, V>(take(stage, 0, r, i, row), x[i][r]);
+        if (P.block) vec_to_f32<T, V>(take(stage, 1, r, i, row), p[i][r]);
+        if (P.gate_kind == kGateFull) gates[i][r] = take(stage, 2, r, i, row);
       }
-    if (P.gate_kind == kGateRow && live) row_gate *= to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]);
-    float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+    }
+    if (++stage >= kDepth) stage = 0;
+    float block_mean[R] = {}, block_dev[R] = {}, mean[R] = {}, dev[R] = {};
     if (P.block) {
       if (P.post) {
-        normalise<L, ITEMS, V, LAYER>(p, in, P, scratch, st.x, st.y);
+        normalise<L, ITEMS, R, V, LAYER>(p, in, P, scratch, block_mean, block_dev);
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-          if (in[i]) affine<T, V>(P.post_weight, P.post_bias, P.params_f32, (i * L + g) * V, p[i]);
+        for (int i = 0; i < ITEMS; ++i) affine<T, V, R>(P.post_weight, P.post_bias, P.params_f32, col[i], p[i]);
       }
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        if (!in[i]) continue;
-        const int c = (i * L + g) * V;
-        if (P.gate_kind == kGateChannel) {
-          affine<T, V>(P.gate, nullptr, P.params_f32, c, p[i]);
-        } else if (P.gate_kind == kGateFull) {
-          float f[V];
-          vec_to_f32<T, V>(gates[i], f);
+        if (P.gate_kind == kGateChannel) affine<T, V, R>(P.gate, nullptr, P.params_f32, col[i], p[i]);
 #pragma unroll
-          for (int e = 0; e < V; ++e) p[i][e] *= f[e];
+        for (int r = 0; r < R; ++r) {
+          if (P.gate_kind == kGateFull) {
+            float f[V];
+            vec_to_f32<T, V>(gates[i][r], f);
+            Ops<V>::mul(p[i][r], p[i][r], f);
+          }
+          Ops<V>::mul(x[i][r], x[i][r], P.residual_scale);
+          Ops<V>::fma(x[i][r], p[i][r], row_gate[r], x[i][r]);
+          if (in[i] && row0 + r < P.n) store_f32<T, V>(static_cast<T *>(P.stream) + static_cast<int64_t>(row0 + r) * P.channels + col[i], x[i][r]);
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[i][e] = fmaf(row_gate, p[i][e], P.residual_scale * x[i][e]);
-        if (live) store_f32<T, V>(static_cast<T *>(P.stream) + row * P.channels + c, x[i]);
       }
     }
     if (P.pre) {
-      normalise<L, ITEMS, V, LAYER>(x, in, P, scratch, st.z, st.w);
+      normalise<L, ITEMS, R, V, LAYER>(x, in, P, scratch, mean, dev);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        if (!in[i]) continue;
-        const int c = (i * L + g) * V;
-        affine<T, V>(P.weight, P.bias, P.params_f32, c, x[i]);
-        if (live) store_f32<T, V>(static_cast<T *>(P.normed) + row * P.channels + c, x[i]);
+        affine<T, V, R>(P.weight, P.bias, P.params_f32, col[i], x[i]);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (in[i] && row0 + r < P.n) store_f32<T, V>(static_cast<T *>(P.normed) + static_cast<int64_t>(row0 + r) * P.channels + col[i], x[i][r]);
       }
     }
-    if (P.stats && live && g == 0) reinterpret_cast<float4 *>(P.stats)[row] = st;
+    if (P.stats && g == 0)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (row0 + r < P.n) reinterpret_cast<float4 *>(P.stats)[row0 + r] = make_float4(block_mean[r], block_dev[r], mean[r], dev[r]);
   }
 }
 
@@ -200,153 +387,176 @@ template <typename T, int V, int L, int ITEMS, bool LAYER>
 __global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) norm_backward_kernel(const __grid_constant__ NormParams P) {
   constexpr int kThreads = kNormThreads<L>;
   __shared__ float scratch[64];
-  extern __shared__ float column_sums[];      // [kThreads / L][channels]
+  extern __shared__ __align__(16) unsigned char norm_ring[];
+  float *column_sums = reinterpret_cast<float *>(norm_ring);      // [kThreads / L][channels], once the rows are through
   pdl_trigger();
   pdl_wait();
+  typedef Ops<V> O;
   const int g = threadIdx.x % L;
   constexpr int kRows = kThreads / L;
-  const int64_t rounds = (P.n + kRows - 1) / kRows;
-  const float a = P.residual_scale, s = P.block_scale;
+  const int rounds = (P.n + kRows - 1) / kRows;
+  const float a = P.block ? P.residual_scale : 1.f, s = P.block_scale;
   const void *post_w = P.post ? P.post_weight : nullptr, *post_b = P.post ? P.post_bias : nullptr;
   bool in[ITEMS];
+  int col[ITEMS];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) in[i] = (i * L + g) * V < P.channels;
+  for (int i = 0; i < ITEMS; ++i) {
+    in[i] = (i * L + g) * V < P.channels;
+    col[i] = in[i] ? (i * L + g) * V : 0;
+  }
+  typedef Ring<kThreads, 5 * ITEMS, V * sizeof(T) == 16> Rows;
+  const Rows ring(norm_ring);
+  constexpr int kDepth = Rows::kDepth;
+  // 0: x, 1: gradient of the normed rows, 2: block, 3: gradient of the stream, 4: gate
+  auto source = [&](int which, int64_t row, int c) -> const T * {
+    if (which == 0) return static_cast<const T *>(P.x) + row * P.x_stride + c;
+    if (which == 1) return static_cast<const T *>(P.dnormed) + row * P.dnormed_stride + c;
+    if (which == 2) return static_cast<const T *>(P.block) + row * P.block_stride + c;
+    if (which == 3) return static_cast<const T *>(P.dstream) + row * P.dstream_stride + c;
+    return static_cast<const T *>(P.gate) + row * P.gate_stride + c;
+  };
+  const bool used[5] = {P.pre != 0, P.pre != 0, P.block != nullptr, P.dstream != nullptr, P.gate_kind == kGateFull};
+  auto row_of = [&](int b) {
+    const int row = b * kRows + static_cast<int>(threadIdx.x) / L;
+    return row < P.n ? row : P.n - 1;
+  };
+  auto fetch = [&](int stage, int b) {
+    if (b < rounds)
+#pragma unroll
+      for (int w = 0; w < 5; ++w)
+        if (used[w])
+#pragma unroll
+          for (int i = 0; i < ITEMS; ++i) ring.copy(stage, w * ITEMS + i, source(w, row_of(b), col[i]));
+    Rows::commit();
+  };
+  auto take = [&](int stage, int w, int i, int64_t row) -> Vec<T, V> {
+    if constexpr (kDepth > 0) return *reinterpret_cast<const Vec<T, V> *>(ring.piece(stage, w * ITEMS + i));
+    else return *reinterpret_cast<const Vec<T, V> *>(source(w, row, col[i]));
+  };
+  int stage = 0;
+  if constexpr (kDepth > 0)
+    for (int k = 0; k < kDepth - 1; ++k) fetch(k, blockIdx.x + k * gridDim.x);
   float sum[kSums][ITEMS][V] = {};
-  for (int64_t b = blockIdx.x; b < rounds; b += gridDim.x) {
-    const int64_t row = b * kRows + threadIdx.x / L;
-    const bool live = row < P.n;
-    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-    // hat: x, then the stream's normalised value; bh: the block's normalised value (or the block); d: gradient of the stream
-    float hat[ITEMS][V] = {}, bh[ITEMS][V] = {}, d[ITEMS][V] = {}, u[ITEMS][V] = {};
+  for (int b = blockIdx.x; b < rounds; b += gridDim.x) {
+    if constexpr (kDepth > 0) {
+      fetch(stage == 0 ? kDepth - 1 : stage - 1, b + (kDepth - 1) * gridDim.x);
+      Rows::wait();
+    }
+    const bool live = b * kRows + static_cast<int>(threadIdx.x) / L < P.n;
+    const int64_t row = row_of(b);
+    const float4 st = reinterpret_cast<const float4 *>(P.stats)[row];
+    // hat: x, then the stream's normalised value; bh: the block's normalised value (or the block); q: its affine form times
+    // the gate; d: gradient of the stream
+    float hat[ITEMS][1][V], bh[ITEMS][V], d[ITEMS][V], u[ITEMS][1][V], q[ITEMS][1][V];
     Vec<T, V> gates[ITEMS];
-    float row_gate = 1.f;
-    if (live) {
-      st = reinterpret_cast<const float4 *>(P.stats)[row];
-      if (P.gate_kind == kGateRow) row_gate = to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]);
-    }
+    const float row_gate = P.gate_kind == kGateRow ? to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]) : 1.f;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      if (live && in[i]) {
-        const int c = (i * L + g) * V;
-        if (P.pre) {
-          load_f32<T, V>(static_cast<const T *>(P.x) + row * P.x_stride + c, hat[i]);
-          load_f32<T, V>(static_cast<const T *>(P.dnormed) + row * P.dnormed_stride + c, u[i]);
-        }
-        if (P.block) load_f32<T, V>(static_cast<const T *>(P.block) + row * P.block_stride + c, bh[i]);
-        if (P.dstream) load_f32<T, V>(static_cast<const T *>(P.dstream) + row * P.dstream_stride + c, d[i]);
-        if (P.gate_kind == kGateFull) gates[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(P.gate) + row * P.gate_stride + c);
+    for (int i = 0; i < ITEMS; ++i) {
+      if (P.pre) {
+        vec_to_f32<T, V>(take(stage, 0, i, row), hat[i][0]);
+        vec_to_f32<T, V>(take(stage, 1, i, row), u[i][0]);
       }
-    float sums[2] = {0.f, 0.f};
-    if (P.post) {
-      const float shift = -st.x * st.y;
+      if (P.block) vec_to_f32<T, V>(take(stage, 2, i, row), bh[i]);
+      if (P.dstream) {
+        vec_to_f32<T, V>(take(stage, 3, i, row), d[i]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) bh[i][e] = LAYER ? fmaf(bh[i][e], st.y, shift) : bh[i][e] * st.y;
-    }
-    // the factor of the block's value in the stream without block_scale
-    auto load_gate = [&](int i, int c, float (&f)[V]) {
-      if (P.gate_kind == kGateChannel) load_param<T, V>(P.gate, P.params_f32, c, f);
-      else if (P.gate_kind == kGateFull && live) vec_to_f32<T, V>(gates[i], f);
-      else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = row_gate;
+        for (int e = 0; e < V; ++e) d[i][e] = 0.f;
       }
+      if (P.gate_kind == kGateFull) gates[i] = take(stage, 4, i, row);
+    }
+    if (++stage >= kDepth) stage = 0;
+    auto load_gate = [&](int i, float (&f)[V]) {
+      if (P.gate_kind == kGateChannel) load_param<T, V>(P.gate, P.params_f32, col[i], f);
+      else vec_to_f32<T, V>(gates[i], f);
     };
-    if (P.pre) {
-      const float shift = -st.z * st.w;
+    float sums[2];
+    if (P.block) {
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        if (!in[i]) continue;
-        const int c = (i * L + g) * V;
+        if (P.post) O::fma(bh[i], bh[i], st.y, LAYER ? -st.x * st.y : 0.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) q[i][0][e] = bh[i][e];
+        affine<T, V, 1>(post_w, post_b, P.params_f32, col[i], q[i]);
+      }
+    }
+    if (P.pre) {
+      sums[0] = sums[1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
         if (P.block) {
-          float q[V], f[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) q[e] = bh[i][e];
-          affine<T, V>(post_w, post_b, P.params_f32, c, q);
-          if (P.gate_kind != kGateNone) {
-            load_gate(i, c, f);
-#pragma unroll
-            for (int e = 0; e < V; ++e) q[e] *= f[e];
+          O::mul(hat[i][0], hat[i][0], a);
+          if (P.gate_kind == kGateNone || P.gate_kind == kGateRow) {
+            O::fma(hat[i][0], q[i][0], s * row_gate, hat[i][0]);
+          } else {
+            float f[V];
+            load_gate(i, f);
+            O::mul(f, f, q[i][0]);
+            O::fma(hat[i][0], f, s, hat[i][0]);
           }
-#pragma unroll
-          for (int e = 0; e < V; ++e) hat[i][e] = fmaf(s, q[e], a * hat[i][e]);
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          hat[i][e] = LAYER ? fmaf(hat[i][e], st.w, shift) : hat[i][e] * st.w;
-          sum[0][i][e] = fmaf(u[i][e], hat[i][e], sum[0][i][e]);
-          sum[1][i][e] += u[i][e];
+        O::fma(hat[i][0], hat[i][0], st.w, LAYER ? -st.z * st.w : 0.f);
+        if (live) {                                          // (a row that does not exist adds nothing to the column sums)
+          O::fma(sum[0][i], u[i][0], hat[i][0], sum[0][i]);
+          O::add(sum[1][i], sum[1][i], u[i][0]);
         }
-        affine<T, V>(P.weight, nullptr, P.params_f32, c, u[i]);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          sums[0] = fmaf(u[i][e], hat[i][e], sums[0]);
-          if (LAYER) sums[1] += u[i][e];
+        affine<T, V, 1>(P.weight, nullptr, P.params_f32, col[i], u[i]);
+        const float t0 = O::dot(u[i][0], hat[i][0]), t1 = LAYER ? O::sum(u[i][0]) : 0.f;
+        if (in[i]) {
+          sums[0] += t0;
+          sums[1] += t1;
         }
       }
-      row_sums<L, 2>(sums, scratch);
+      row_sums<L, LAYER ? 2 : 1>(reinterpret_cast<float (&)[LAYER ? 2 : 1]>(sums), scratch);
       const float m0 = -sums[0] * P.inv_channels * st.w, m1 = LAYER ? -sums[1] * P.inv_channels * st.w : 0.f;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          d[i][e] = fmaf(u[i][e], st.w, d[i][e]);
-          d[i][e] = fmaf(hat[i][e], m0, d[i][e]);
-          if (LAYER) d[i][e] += m1;
-        }
+      for (int i = 0; i < ITEMS; ++i) {
+        if (LAYER) O::add(d[i], d[i], m1);
+        O::fma(d[i], u[i][0], st.w, d[i]);
+        O::fma(d[i], hat[i][0], m0, d[i]);
+      }
     }
-    if (live && P.dx)
+    if (P.dx)
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-        if (in[i]) {
-          float o[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) o[e] = P.block ? a * d[i][e] : d[i][e];
-          store_f32<T, V>(static_cast<T *>(P.dx) + row * P.channels + (i * L + g) * V, o);
-        }
+      for (int i = 0; i < ITEMS; ++i) {
+        float o[V];
+        O::mul(o, d[i], a);
+        if (live && in[i]) store_f32<T, V>(static_cast<T *>(P.dx) + row * P.channels + col[i], o);
+      }
     if (P.block) {
       sums[0] = sums[1] = 0.f;
       float gate_sum[1] = {0.f};
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        if (!in[i]) continue;
-        const int c = (i * L + g) * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) d[i][e] *= s;
+        O::mul(d[i], d[i], s);
         if (P.gate_kind != kGateNone) {
-          float q[V], f[V];
-          load_gate(i, c, f);
-          if (P.dgate) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) q[e] = bh[i][e];
-            affine<T, V>(post_w, post_b, P.params_f32, c, q);
-#pragma unroll
-            for (int e = 0; e < V; ++e) q[e] *= d[i][e];
-            if (P.gate_kind == kGateChannel) {
-#pragma unroll
-              for (int e = 0; e < V; ++e) sum[4][i][e] += q[e];
-            } else if (P.gate_kind == kGateRow) {
-#pragma unroll
-              for (int e = 0; e < V; ++e) gate_sum[0] += q[e];
-            } else if (live) {
-              store_f32<T, V>(static_cast<T *>(P.dgate) + row * P.channels + c, q);
-            }
+          O::mul(q[i][0], q[i][0], d[i]);                  // gradient of the gate
+          if (P.gate_kind == kGateRow) {
+            const float t = O::sum(q[i][0]);
+            if (in[i]) gate_sum[0] += t;
+            O::mul(d[i], d[i], row_gate);
+          } else {
+            if (P.gate_kind == kGateChannel && live) O::add(sum[4][i], sum[4][i], q[i][0]);
+            if (P.gate_kind == kGateFull && P.dgate && live && in[i]) store_f32<T, V>(static_cast<T *>(P.dgate) + row * P.channels + col[i], q[i][0]);
+            float f[V];
+            load_gate(i, f);
+            O::mul(d[i], d[i], f);
           }
-#pragma unroll
-          for (int e = 0; e < V; ++e) d[i][e] *= f[e];
         }
         if (P.post) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            sum[2][i][e] = fmaf(d[i][e], bh[i][e], sum[2][i][e]);
-            sum[3][i][e] += d[i][e];
+          if (live) {
+            O::fma(sum[2][i], d[i], bh[i], sum[2][i]);
+            O::add(sum[3][i], sum[3][i], d[i]);
           }
-          affine<T, V>(post_w, nullptr, P.params_f32, c, d[i]);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            sums[0] = fmaf(d[i][e], bh[i][e], sums[0]);
-            if (LAYER) sums[1] += d[i][e];
+          if (post_w) {
+            float f[V];
+            load_param<T, V>(post_w, P.params_f32, col[i], f);
+            O::mul(d[i], d[i], f);
+          }
+          const float t0 = O::dot(d[i], bh[i]), t1 = LAYER ? O::sum(d[i]) : 0.f;
+          if (in[i]) {
+            sums[0] += t0;
+            sums[1] += t1;
           }
         }
       }
@@ -356,21 +566,23 @@ __global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) 
       }
       if (P.dblock) {
         if (P.post) {
-          row_sums<L, 2>(sums, scratch);
+          row_sums<L, LAYER ? 2 : 1>(reinterpret_cast<float (&)[LAYER ? 2 : 1]>(sums), scratch);
           const float m0 = -sums[0] * P.inv_channels, m1 = LAYER ? -sums[1] * P.inv_channels : 0.f;
 #pragma unroll
-          for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-            for (int e = 0; e < V; ++e) d[i][e] = st.y * fmaf(bh[i][e], m0, LAYER ? d[i][e] + m1 : d[i][e]);
+          for (int i = 0; i < ITEMS; ++i) {
+            if (LAYER) O::add(d[i], d[i], m1);
+            O::fma(d[i], bh[i], m0, d[i]);
+            O::mul(d[i], d[i], st.y);
+          }
         }
-        if (live)
 #pragma unroll
-          for (int i = 0; i < ITEMS; ++i)
-            if (in[i]) store_f32<T, V>(static_cast<T *>(P.dblock) + row * P.channels + (i * L + g) * V, d[i]);
+        for (int i = 0; i < ITEMS; ++i)
+          if (live && in[i]) store_f32<T, V>(static_cast<T *>(P.dblock) + row * P.channels + col[i], d[i]);
       }
     }
   }
   if (P.partial == nullptr) return;
+  if constexpr (kDepth > 0) ptx::cp_async_wait<0>();
   // the CTA's column sums, rows of the CTA added in order
   const bool wanted[kSums] = {P.pre != 0 && P.weight, P.pre != 0 && P.bias, P.post != 0 && P.post_weight, P.post != 0 && P.post_bias,
                               P.gate_kind == kGateChannel};
@@ -434,31 +646,39 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__
   }
 }
 
-// CTAs of a kernel that fit on an SM (asked once per kernel).
+// CTAs of a kernel that fit on an SM with its shared memory (asked once per kernel).
 template <typename K>
-static int resident_ctas(K kernel, int threads) {
+static int resident_ctas(K kernel, int threads, int smem) {
   int n = 0;
-  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) == cudaSuccess && n > 0 ? n : 1;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 1;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0 ? n : 1;
 }
 
 template <typename T, int V, int L, int ITEMS, bool LAYER>
 static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaStream_t st) {
   constexpr int kThreads = kNormThreads<L>;
   constexpr int kRows = kThreads / L;
-  const int64_t rounds = div_up(P.n, kRows);
+  constexpr bool kWide = V * sizeof(T) == 16;
   if (!backward) {
-    static const int resident = resident_ctas(norm_forward_kernel<T, V, L, ITEMS, LAYER>, kThreads);
+    constexpr int R = L <= 32 && ITEMS == 1 ? 2 : 1;
+    constexpr int kSmem = Ring<kThreads, 3 * ITEMS * R, kWide>::kBytes;
+    const auto kernel = norm_forward_kernel<T, V, L, ITEMS, R, LAYER>;
+    const int64_t rounds = div_up(P.n, kRows * R);
+    static const int resident = resident_ctas(kernel, kThreads, kSmem);
     const int64_t cap = static_cast<int64_t>(sm_count()) * resident;
-    SB_CHECK_CUDA(launch_dependent(norm_forward_kernel<T, V, L, ITEMS, LAYER>, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), 0,
-                                   st, P));
+    SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), kSmem, st, P));
     return SPIRA_B200_OK;
   }
-  static const int resident = resident_ctas(norm_backward_kernel<T, V, L, ITEMS, LAYER>, kThreads);
+  // (columns sums of a CTA reuse the ring: 256 / L rows of L * ITEMS * V columns)
+  constexpr int kRing = Ring<kThreads, 5 * ITEMS, kWide>::kBytes, kColumns = kRows > 1 ? kThreads * ITEMS * V * 4 : 0;
+  constexpr int kSmem = kRing > kColumns ? kRing : kColumns;
+  const auto kernel = norm_backward_kernel<T, V, L, ITEMS, LAYER>;
+  const int64_t rounds = div_up(P.n, kRows);
+  static const int resident = resident_ctas(kernel, kThreads, kSmem);
   const int64_t cap = static_cast<int64_t>(sm_count()) * (resident < kNormBackwardCtas ? resident : kNormBackwardCtas);
   const int grid = static_cast<int>(rounds < cap ? rounds : cap);
   *ctas = grid;
-  const size_t smem = kRows > 1 ? static_cast<size_t>(kRows) * P.channels * 4 : 0;
-  SB_CHECK_CUDA(launch_dependent(norm_backward_kernel<T, V, L, ITEMS, LAYER>, dim3(grid), dim3(kThreads), smem, st, P));
+  SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kThreads), kSmem, st, P));
   return SPIRA_B200_OK;
 }
 
@@ -506,12 +726,14 @@ static bool norm_wide(const spira_b200_norm_desc &D, int size) {
 static int norm_check(const char *what, const spira_b200_norm_desc *D) {
   SB_CHECK_ARG(D, "%s: null descriptor", what);
   SB_CHECK_ARG(D->dtype >= SPIRA_B200_F16 && D->dtype <= SPIRA_B200_F32, "%s: unknown element type %d", what, D->dtype);
-  SB_CHECK_ARG(D->n >= 0 && D->n < (int64_t(1) << 31), "%s: n=%lld out of range", what, (long long)D->n);
+  SB_CHECK_ARG(D->n >= 0 && D->n < (int64_t(1) << 31) - 65536, "%s: n=%lld out of range", what, (long long)D->n);
   SB_CHECK_ARG(D->channels >= 1 && D->channels <= kNormMaxChannels, "%s: channels=%d must be 1 to %d", what, D->channels, kNormMaxChannels);
   SB_CHECK_ARG(D->gate_kind >= kGateNone && D->gate_kind <= kGateFull, "%s: unknown gate %d", what, D->gate_kind);
   SB_CHECK_ARG(D->eps > 0.f, "%s: eps must be positive", what);
   SB_CHECK_ARG(D->x_stride >= 0 && D->block_stride >= 0 && D->gate_stride >= 0 && D->dstream_stride >= 0 && D->dnormed_stride >= 0,
                "%s: negative row stride", what);
+  SB_CHECK_ARG((D->x_stride | D->block_stride | D->gate_stride | D->dstream_stride | D->dnormed_stride) < (int64_t(1) << 31),
+               "%s: rows more than 2^31 elements apart", what);
   if (D->n == 0) return SPIRA_B200_OK;      // (tensors without rows have no address)
   SB_CHECK_ARG(D->pre || D->block, "%s: neither a block nor a norm", what);
   SB_CHECK_ARG(D->block || (!D->post && D->gate_kind == kGateNone), "%s: a gate or a norm after the block needs a block", what);
@@ -525,8 +747,8 @@ static NormParams norm_params(const spira_b200_norm_desc &D) {
   P.weight = D.weight; P.bias = D.bias; P.post_weight = D.post_weight; P.post_bias = D.post_bias;
   P.stream = D.stream; P.normed = D.normed; P.dx = D.dx; P.dblock = D.dblock; P.dgate = D.dgate;
   P.stats = D.stats;
-  P.n = D.n; P.x_stride = D.x_stride; P.block_stride = D.block_stride; P.gate_stride = D.gate_stride;
-  P.dstream_stride = D.dstream_stride; P.dnormed_stride = D.dnormed_stride;
+  P.n = static_cast<int>(D.n); P.x_stride = static_cast<int>(D.x_stride); P.block_stride = static_cast<int>(D.block_stride); P.gate_stride = static_cast<int>(D.gate_stride);
+  P.dstream_stride = static_cast<int>(D.dstream_stride); P.dnormed_stride = static_cast<int>(D.dnormed_stride);
   P.channels = D.channels; P.layer = D.layer; P.pre = D.pre; P.post = D.post; P.gate_kind = D.gate_kind; P.params_f32 = D.params_f32;
   P.residual_scale = D.residual_scale; P.block_scale = D.block_scale; P.eps = D.eps; P.inv_channels = 1.f / static_cast<float>(D.channels);
   return P;
