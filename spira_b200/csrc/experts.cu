@@ -35,6 +35,17 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// A 16-bit logit has 19 significant bits as fp32, so logit and expert fit into 28 bits: one number per expert, equal
+// logits ordered by the lower index, and a maximum is one instruction per expert.
+constexpr uint32_t kKeyShift = 13;
+__device__ __forceinline__ uint32_t pack_key(uint32_t key, int expert) { return (key >> kKeyShift) << 9 | static_cast<uint32_t>(kMaxExperts - 1 - expert); }
+__device__ __forceinline__ uint32_t unpack_key(uint32_t packed) {
+  const uint32_t key = packed >> 9 << kKeyShift;
+  if (packed >> 9 == 0xffffffffu >> kKeyShift) return 0xffffffffu;                 // NaN
+  return key & 0x80000000u ? key : key | ((1u << kKeyShift) - 1);                  // (keys of negative numbers are inverted bits)
+}
+static_assert(kMaxExperts == 512, "the packed keys hold nine bits of expert");
+
 // EPL consecutive elements of a row from column c0 on as fp32, `fill` outside the row.
 template <typename T, int EPL>
 __device__ __forceinline__ void load_logits(const T *row, int c0, int experts, bool live, bool vec_ok, float fill, float (&v)[EPL]) {
@@ -64,6 +75,7 @@ __device__ __forceinline__ void route_rows(const T *logits, int64_t row_stride, 
   const bool vec_ok = reinterpret_cast<uintptr_t>(logits) % (V * sizeof(T)) == 0 && row_stride % V == 0;
   const int g = threadIdx.x & (G - 1), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kRows = kRouteThreads / G, kWarpRows = 32 / G;
+  constexpr bool kPacked = sizeof(T) == 2;
   int *warp_e = stash + warp * kWarpRows * k * 2;                       // [rows of the warp][k]
   float *warp_w = reinterpret_cast<float *>(warp_e + kWarpRows * k);
   int *my_e = warp_e + lane / G * k;
@@ -76,35 +88,54 @@ __device__ __forceinline__ void route_rows(const T *logits, int64_t row_stride, 
       float v[EPL];
       load_logits<T, EPL>(logits + row * row_stride, g * EPL, experts, live, vec_ok, -INFINITY, v);
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) key[i] = logit_key(v[i]);
+      for (int i = 0; i < EPL; ++i) {
+        key[i] = logit_key(v[i]);
+        if (kPacked) key[i] = key[i] == kGone ? kGone : pack_key(key[i], g * EPL + i);
+      }
     }
     float top = 0.f, sum = 0.f, total = 0.f;
+    uint32_t last = 0x80000000u;
     for (int j = 0; j < k; ++j) {
       uint32_t best = kGone;
-      int at = 0;
+      int e;
+      if constexpr (kPacked) {
+        // the largest key below the last one: differences wrap, what is not below it stays under 2^31
+        uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (key[i] > best) { best = key[i]; at = i; }     // (strict: the lowest index of equal logits)
-      int e = g * EPL + at;
+        for (int i = 0; i < EPL; ++i) m = max(m, key[i] - last);
 #pragma unroll
-      for (int d = 1; d < G; d *= 2) {
-        const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, d, G);
-        const int oe = __shfl_xor_sync(0xffffffffu, e, d, G);
-        if (ob > best || (ob == best && oe < e)) { best = ob; e = oe; }
+        for (int d = 1; d < G; d *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d, G));
+        last = m >= 0x80000000u ? m + last : kGone;
+        e = kMaxExperts - 1 - static_cast<int>(last & (kMaxExperts - 1));
+        best = last == kGone ? kGone : unpack_key(last);
+      } else {
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i)
+          if (key[i] > best) { best = key[i]; at = i; }     // (strict: the lowest index of equal logits)
+        e = g * EPL + at;
+#pragma unroll
+        for (int d = 1; d < G; d *= 2) {
+          const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, d, G);
+          const int oe = __shfl_xor_sync(0xffffffffu, e, d, G);
+          if (ob > best || (ob == best && oe < e)) { best = ob; e = oe; }
+        }
       }
       if (j == 0) {
         top = best == kGone ? 0.f : key_logit(best);
         if (!renormalize) {      // the softmax runs over all experts: while every logit is still there
 #pragma unroll
           for (int i = 0; i < EPL; ++i)
-            if (key[i] != kGone) total += expf(key_logit(key[i]) - top);
+            if (key[i] != kGone) total += expf(key_logit(kPacked ? unpack_key(key[i]) : key[i]) - top);
 #pragma unroll
           for (int d = 1; d < G; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d, G);
         }
       }
+      if constexpr (!kPacked) {
 #pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (g * EPL + i == e) key[i] = kGone;
+        for (int i = 0; i < EPL; ++i)
+          if (g * EPL + i == e) key[i] = kGone;
+      }
       const float score = best == kGone ? 0.f : expf(key_logit(best) - top);
       sum += score;
       if (g == 0) {

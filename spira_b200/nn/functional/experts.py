@@ -38,21 +38,31 @@ def _launch(index: int, name: str, *args) -> None:
             _lib.call(name, *args, _raw_stream(index))
 
 
+def _query(index: int, name: str, *args) -> None:
+    """A library call without a stream that depends on the device (scratch sizes)."""
+    if index == _current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args)
+
+
 def _fail(message: str):
     raise RuntimeError("[spira_b200] " + message)
 
 
 def _device_of(*tensors) -> int:
     """The device index all given tensors share; refuses CPU tensors and mixtures."""
-    index = None
+    index = -1
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device() if t.is_cuda else -1
+        if i < 0:
             raise NotImplementedError("spira_b200 runs on CUDA tensors only")
-        if index is None:
-            index = t.device.index
-        elif t.device.index != index:
+        if index < 0:
+            index = i
+        elif i != index:
             _fail("tensors on different devices")
     return index
 
@@ -78,18 +88,16 @@ class ExpertRouting(NamedTuple):
 # ------------------------------------------------------------------------------------------------ routing
 def _route(logits: torch.Tensor, top_k: int, renormalize: bool) -> ExpertRouting:
     n, experts = logits.shape
-    dev = logits.device
-    weights = torch.empty((n, top_k), dtype=torch.float32, device=dev)
-    chosen = torch.empty((n, top_k), dtype=torch.int32, device=dev)
-    slots = torch.empty((n, top_k), dtype=torch.int32, device=dev)
-    order = torch.empty(n * top_k, dtype=torch.int32, device=dev)
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
-    index = dev.index
+    weights = logits.new_empty((n, top_k), dtype=torch.float32)
+    chosen = logits.new_empty((n, top_k), dtype=torch.int32)
+    slots = torch.empty_like(chosen)
+    order = chosen.new_empty(n * top_k)
+    offsets = chosen.new_empty(experts + 1)
+    index = logits.get_device()
     need, workspace = C.c_size_t(), None
     if n * top_k > 4096:          # (a few rows need no scratch: one CTA routes them)
-        with torch.cuda.device(index):
-            _lib.call("spira_b200_expert_route_workspace", n, experts, top_k, C.byref(need))
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        _query(index, "spira_b200_expert_route_workspace", n, experts, top_k, C.byref(need))
+        workspace = chosen.new_empty((need.value + 3) // 4)
     _launch(index, "spira_b200_expert_route", logits.data_ptr(), _DTYPES[logits.dtype], n, logits.stride(0), experts, top_k,
             1 if renormalize else 0, weights.data_ptr(), chosen.data_ptr(), slots.data_ptr(), order.data_ptr(), offsets.data_ptr(),
             None if workspace is None else workspace.data_ptr(), need.value)
@@ -114,8 +122,8 @@ class _Route(torch.autograd.Function):
         logits, weights, chosen = ctx.saved_tensors
         n, experts = logits.shape
         dweights = dweights.float()
-        dlogits = torch.empty((n, experts), dtype=logits.dtype, device=logits.device)
-        _launch(logits.device.index, "spira_b200_expert_route_backward", logits.data_ptr(), _DTYPES[logits.dtype], n, logits.stride(0),
+        dlogits = logits.new_empty((n, experts))
+        _launch(logits.get_device(), "spira_b200_expert_route_backward", logits.data_ptr(), _DTYPES[logits.dtype], n, logits.stride(0),
                 experts, weights.shape[1], 1 if ctx.renormalize else 0, weights.data_ptr(), chosen.data_ptr(), dweights.data_ptr(),
                 dweights.stride(0), dweights.stride(1), dlogits.data_ptr())
         return dlogits, None, None
@@ -166,8 +174,8 @@ def _check_rows(t: torch.Tensor, name: str, rows: int) -> torch.Tensor:
 def _dispatch(feats, slots, offsets):
     n, k = slots.shape
     channels = feats.shape[1]
-    rows = torch.empty((n * k, channels), dtype=feats.dtype, device=feats.device)
-    _launch(feats.device.index, "spira_b200_expert_dispatch", feats.data_ptr(), _DTYPES[feats.dtype], n, feats.stride(0), channels,
+    rows = feats.new_empty((n * k, channels))
+    _launch(feats.get_device(), "spira_b200_expert_dispatch", feats.data_ptr(), _DTYPES[feats.dtype], n, feats.stride(0), channels,
             slots.data_ptr(), k, offsets.data_ptr(), offsets.shape[0] - 1, rows.data_ptr())
     return rows
 
@@ -175,8 +183,8 @@ def _dispatch(feats, slots, offsets):
 def _combine(rows, weights, slots):
     n, k = slots.shape
     channels = rows.shape[1]
-    out = torch.empty((n, channels), dtype=rows.dtype, device=rows.device)
-    _launch(rows.device.index, "spira_b200_expert_combine", rows.data_ptr(), _DTYPES[rows.dtype], n, rows.stride(0), channels,
+    out = rows.new_empty((n, channels))
+    _launch(rows.get_device(), "spira_b200_expert_combine", rows.data_ptr(), _DTYPES[rows.dtype], n, rows.stride(0), channels,
             None if weights is None else weights.data_ptr(), 0 if weights is None else weights.stride(0),
             0 if weights is None else weights.stride(1), slots.data_ptr(), k, out.data_ptr())
     return out
@@ -206,9 +214,9 @@ class _Combine(torch.autograd.Function):
         rows, weights, slots, offsets = ctx.saved_tensors
         dout = _rows(dout)
         (n, k), channels = slots.shape, rows.shape[1]
-        drows = torch.empty((n * k, channels), dtype=rows.dtype, device=rows.device) if ctx.needs_input_grad[0] else None
-        dweights = torch.empty((n, k), dtype=torch.float32, device=rows.device) if ctx.needs_input_grad[1] else None
-        _launch(rows.device.index, "spira_b200_expert_combine_backward", rows.data_ptr(), dout.data_ptr(), _DTYPES[rows.dtype], n,
+        drows = rows.new_empty((n * k, channels)) if ctx.needs_input_grad[0] else None
+        dweights = weights.new_empty((n, k)) if ctx.needs_input_grad[1] else None
+        _launch(rows.get_device(), "spira_b200_expert_combine_backward", rows.data_ptr(), dout.data_ptr(), _DTYPES[rows.dtype], n,
                 rows.stride(0), dout.stride(0), channels, weights.data_ptr(), weights.stride(0), weights.stride(1), slots.data_ptr(), k,
                 offsets.data_ptr(), offsets.shape[0] - 1, None if drows is None else drows.data_ptr(),
                 None if dweights is None else dweights.data_ptr())
@@ -265,7 +273,7 @@ def _grouped_desc(x, weights, offsets, dy=None) -> GroupedDesc:
 def _grouped(x, weights, offsets, bias, relu, want_mask=False):
     """The product and, for a backward pass, what its ReLU let through: the bit mask the kernel writes, or None where the
     shape has none (then the sign of the result says it)."""
-    index = x.device.index
+    index = x.get_device()
     y = x.new_empty((x.shape[0], weights.shape[2]))
     d = _grouped_desc(x, weights, offsets)
     d.y, d.relu = y.data_ptr(), 1 if relu else 0
@@ -276,20 +284,16 @@ def _grouped(x, weights, offsets, bias, relu, want_mask=False):
         need = C.c_size_t()
         _lib.call("spira_b200_grouped_linear_mask_bytes", C.byref(d), C.byref(need))
         if need.value:
-            mask = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+            mask = x.new_empty(need.value, dtype=torch.uint8)
             d.mask = mask.data_ptr()
     _launch(index, "spira_b200_grouped_linear", C.byref(d), _status(index))
     return (y, mask) if want_mask else y
 
 
-def _with_workspace(index, device, name, desc, *rest):
+def _with_workspace(index, like, name, desc, *rest):
     need = C.c_size_t()
-    if index == _current_device():
-        _lib.call(name + "_workspace", C.byref(desc), C.byref(need))
-    else:
-        with torch.cuda.device(index):
-            _lib.call(name + "_workspace", C.byref(desc), C.byref(need))
-    workspace = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    _query(index, name + "_workspace", C.byref(desc), C.byref(need))
+    workspace = like.new_empty(need.value, dtype=torch.uint8) if need.value else None
     _launch(index, name, C.byref(desc), None if workspace is None else workspace.data_ptr(), need.value, *rest)
 
 
@@ -306,35 +310,35 @@ class _Grouped(torch.autograd.Function):
     def backward(ctx, dy):
         x, weights, offsets, y, mask = ctx.saved_tensors
         dy = _rows(dy)
-        index, dev = x.device.index, x.device
+        index = x.get_device()
         status = _status(index)
         want_dx, want_dw, want_db = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.has_bias and ctx.needs_input_grad[3]
         dx = dw = db = None
         if ctx.relu or want_db:
             d = _grouped_desc(None, weights, offsets, dy)
             if ctx.relu:
-                dz = torch.empty((dy.shape[0], weights.shape[2]), dtype=dy.dtype, device=dev)
+                dz = dy.new_empty((dy.shape[0], weights.shape[2]))
                 d.dz = dz.data_ptr()
                 if mask is not None:
                     d.mask = mask.data_ptr()
                 else:
                     d.y = y.data_ptr()
             if want_db:
-                db = torch.empty((weights.shape[0], weights.shape[2]), dtype=weights.dtype, device=dev)
+                db = weights.new_empty((weights.shape[0], weights.shape[2]))
                 d.dbias = db.data_ptr()
-            _with_workspace(index, dev, "spira_b200_grouped_linear_dz", d)
+            _with_workspace(index, dy, "spira_b200_grouped_linear_dz", d)
             if ctx.relu:
                 dy = dz
         if want_dx:
-            dx = torch.empty((dy.shape[0], weights.shape[1]), dtype=dy.dtype, device=dev)
+            dx = dy.new_empty((dy.shape[0], weights.shape[1]))
             d = _grouped_desc(None, weights, offsets, dy)
             d.dx = dx.data_ptr()
             _launch(index, "spira_b200_grouped_linear_dx", C.byref(d), status)
         if want_dw:
-            dw = torch.empty_like(weights, memory_format=torch.contiguous_format)
+            dw = weights.new_empty(weights.shape)
             d = _grouped_desc(x, weights, offsets, dy)
             d.dweight = dw.data_ptr()
-            _with_workspace(index, dev, "spira_b200_grouped_linear_dw", d, status)
+            _with_workspace(index, dy, "spira_b200_grouped_linear_dw", d, status)
         return dx, dw, None, db, None
 
 

@@ -52,22 +52,22 @@ def _desc(spec, x, block, gate, weight, bias, post_weight, post_bias) -> NormDes
 
 def _forward(spec, x, block, gate, weight, bias, post_weight, post_bias, stats):
     d = _desc(spec, x, block, gate, weight, bias, post_weight, post_bias)
-    stream = torch.empty(x.shape, dtype=x.dtype, device=x.device) if block is not None else None
-    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device) if spec.pre else None
+    stream = x.new_empty(x.shape) if block is not None else None
+    normed = x.new_empty(x.shape) if spec.pre else None
     if stream is not None:
         d.stream = stream.data_ptr()
     if normed is not None:
         d.normed = normed.data_ptr()
     if stats is not None:
         d.stats = stats.data_ptr()
-    _launch(x.device.index, "spira_b200_residual_norm", C.byref(d))
+    _launch(x.get_device(), "spira_b200_residual_norm", C.byref(d))
     return stream, normed
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, spec, x, block, gate, weight, bias, post_weight, post_bias):
-        stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device)
+        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
         stream, normed = _forward(spec, x, block, gate, weight, bias, post_weight, post_bias, stats)
         ctx.spec = spec
         ctx.save_for_backward(x, block, gate, weight, bias, post_weight, post_bias, stats)
@@ -94,14 +94,14 @@ class _ResidualNorm(torch.autograd.Function):
         grads = [None]
         for name, t, wanted in zip(("dx", "dblock", "dgate", "dweight", "dbias", "dpost_weight", "dpost_bias"),
                                    (x, block, gate, weight, bias, post_weight, post_bias), need[1:]):
-            g = torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and wanted else None
+            g = t.new_empty(t.shape) if t is not None and wanted else None
             if g is not None:
                 setattr(d, name, g.data_ptr())
             grads.append(g)
         if any(g is not None for g in grads[4:]) or (grads[3] is not None and spec.gate_kind == GATE_CHANNEL):
-            _with_workspace(x.device.index, x.device, "spira_b200_residual_norm_backward", d)
+            _with_workspace(x.get_device(), x, "spira_b200_residual_norm_backward", d)
         else:
-            _launch(x.device.index, "spira_b200_residual_norm_backward", C.byref(d), None, 0)
+            _launch(x.get_device(), "spira_b200_residual_norm_backward", C.byref(d), None, 0)
         return tuple(grads)
 
 
