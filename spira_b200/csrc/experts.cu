@@ -35,16 +35,65 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// A 16-bit logit has 19 significant bits as fp32, so logit and expert fit into 28 bits: one number per expert, equal
-// logits ordered by the lower index, and a maximum is one instruction per expert.
-constexpr uint32_t kKeyShift = 13;
-__device__ __forceinline__ uint32_t pack_key(uint32_t key, int expert) { return (key >> kKeyShift) << 9 | static_cast<uint32_t>(kMaxExperts - 1 - expert); }
-__device__ __forceinline__ uint32_t unpack_key(uint32_t packed) {
-  const uint32_t key = packed >> 9 << kKeyShift;
-  if (packed >> 9 == 0xffffffffu >> kKeyShift) return 0xffffffffu;                 // NaN
-  return key & 0x80000000u ? key : key | ((1u << kKeyShift) - 1);                  // (keys of negative numbers are inverted bits)
+// 16-bit logits: order (16 bits) and expert (9 bits) make one number per expert, equal logits ordered by the lower index, so
+// that a maximum takes one instruction per expert.  Adding +0 makes -0 equal to +0 and every NaN the positive one, which
+// is then the largest; what is not above -inf counts as masked.
+__device__ __forceinline__ uint32_t canonical2(uint32_t w, __half) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0u));
+  return r;
+}
+__device__ __forceinline__ uint32_t canonical2(uint32_t w, __nv_bfloat16) {
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0u));
+  return r;
+}
+template <typename T>
+constexpr uint32_t kMinusInf16 = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+// the order of both halves of a word
+template <typename T>
+__device__ __forceinline__ uint32_t order2(uint32_t w) {
+  w = canonical2(w, T{});
+  const uint32_t negative = ((w >> 15) & 0x00010001u) * 0xffffu;
+  return w ^ (negative | 0x80008000u);
+}
+// a logit from its order
+template <typename T>
+__device__ __forceinline__ float order_logit(uint32_t o) {
+  const unsigned short h = static_cast<unsigned short>(o & 0x8000u ? o ^ 0x8000u : ~o);
+  T v;
+  *reinterpret_cast<unsigned short *>(&v) = h;
+  return to_f32(v);
 }
 static_assert(kMaxExperts == 512, "the packed keys hold nine bits of expert");
+
+// The packed keys of the experts [c0, c0 + EPL) of a row; experts that do not exist are masked.
+template <typename T, int EPL>
+__device__ __forceinline__ void load_packed(const T *row, int c0, int experts, bool live, bool vec_ok, uint32_t (&key)[EPL]) {
+  uint32_t w[EPL / 2];
+  if (live && vec_ok && c0 + EPL <= experts) {
+    constexpr int V = EPL >= 8 ? 4 : EPL / 2;      // words per access
+#pragma unroll
+    for (int i = 0; i < EPL / 2; i += V) {
+      const Vec<uint32_t, V> q = *reinterpret_cast<const Vec<uint32_t, V> *>(row + c0 + 2 * i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[i + j] = q.v[j];
+    }
+  } else {
+    const unsigned short *h = reinterpret_cast<const unsigned short *>(row + c0);
+#pragma unroll
+    for (int i = 0; i < EPL / 2; ++i) {
+      const uint32_t lo = live && c0 + 2 * i < experts ? h[2 * i] : kMinusInf16<T>, hi = live && c0 + 2 * i + 1 < experts ? h[2 * i + 1] : kMinusInf16<T>;
+      w[i] = lo | hi << 16;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EPL / 2; ++i) {
+    const uint32_t o = order2<T>(w[i]), tail = static_cast<uint32_t>(kMaxExperts - 1 - c0 - 2 * i);
+    key[2 * i] = (o & 0xffffu) * 512u + tail;
+    key[2 * i + 1] = (o >> 16) * 512u + tail - 1u;
+  }
+}
 
 // EPL consecutive elements of a row from column c0 on as fp32, `fill` outside the row.
 template <typename T, int EPL>
@@ -76,6 +125,7 @@ __device__ __forceinline__ void route_rows(const T *logits, int64_t row_stride, 
   const int g = threadIdx.x & (G - 1), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kRows = kRouteThreads / G, kWarpRows = 32 / G;
   constexpr bool kPacked = sizeof(T) == 2;
+  constexpr uint32_t kMaskedOrder = 0xffffu & ~kMinusInf16<T>;      // the order of -inf
   int *warp_e = stash + warp * kWarpRows * k * 2;                       // [rows of the warp][k]
   float *warp_w = reinterpret_cast<float *>(warp_e + kWarpRows * k);
   int *my_e = warp_e + lane / G * k;
@@ -84,30 +134,32 @@ __device__ __forceinline__ void route_rows(const T *logits, int64_t row_stride, 
     const int64_t row = r + threadIdx.x / G;
     const bool live = row < r1;
     uint32_t key[EPL];
-    {
+    if constexpr (kPacked) {
+      load_packed<T, EPL>(logits + row * row_stride, g * EPL, experts, live, vec_ok, key);
+    } else {
       float v[EPL];
       load_logits<T, EPL>(logits + row * row_stride, g * EPL, experts, live, vec_ok, -INFINITY, v);
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        key[i] = logit_key(v[i]);
-        if (kPacked) key[i] = key[i] == kGone ? kGone : pack_key(key[i], g * EPL + i);
-      }
+      for (int i = 0; i < EPL; ++i) key[i] = logit_key(v[i]);
     }
     float top = 0.f, sum = 0.f, total = 0.f;
     uint32_t last = 0x80000000u;
     for (int j = 0; j < k; ++j) {
       uint32_t best = kGone;
+      bool found;
+      float logit;
       int e;
       if constexpr (kPacked) {
         // the largest key below the last one: differences wrap, what is not below it stays under 2^31
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) m = max(m, key[i] - last);
+        for (int i = 0; i < EPL; ++i) m = __viaddmax_u32(key[i], 0u - last, m);
 #pragma unroll
         for (int d = 1; d < G; d *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d, G));
-        last = m >= 0x80000000u ? m + last : kGone;
+        last = m >= 0x80000000u ? m + last : 0;
         e = kMaxExperts - 1 - static_cast<int>(last & (kMaxExperts - 1));
-        best = last == kGone ? kGone : unpack_key(last);
+        found = last >> 9 > kMaskedOrder;
+        logit = order_logit<T>(last >> 9);
       } else {
         int at = 0;
 #pragma unroll
@@ -121,12 +173,18 @@ __device__ __forceinline__ void route_rows(const T *logits, int64_t row_stride, 
           if (ob > best || (ob == best && oe < e)) { best = ob; e = oe; }
         }
       }
+      if constexpr (!kPacked) {
+        found = best != kGone;
+        logit = key_logit(best);
+      }
       if (j == 0) {
-        top = best == kGone ? 0.f : key_logit(best);
+        top = found ? logit : 0.f;
         if (!renormalize) {      // the softmax runs over all experts: while every logit is still there
 #pragma unroll
-          for (int i = 0; i < EPL; ++i)
-            if (key[i] != kGone) total += expf(key_logit(kPacked ? unpack_key(key[i]) : key[i]) - top);
+          for (int i = 0; i < EPL; ++i) {
+            const bool there = kPacked ? key[i] >> 9 > kMaskedOrder : key[i] != kGone;
+            if (there) total += expf((kPacked ? order_logit<T>(key[i] >> 9) : key_logit(key[i])) - top);
+          }
 #pragma unroll
           for (int d = 1; d < G; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d, G);
         }
@@ -136,12 +194,12 @@ __device__ __forceinline__ void route_rows(const T *logits, int64_t row_stride, 
         for (int i = 0; i < EPL; ++i)
           if (g * EPL + i == e) key[i] = kGone;
       }
-      const float score = best == kGone ? 0.f : expf(key_logit(best) - top);
+      const float score = found ? expf(logit - top) : 0.f;
       sum += score;
       if (g == 0) {
         my_w[j] = score;
-        my_e[j] = best == kGone ? -1 : e;
-        if (live && best != kGone) atomicAdd(hist + e, 1);
+        my_e[j] = found ? e : -1;
+        if (live && found) atomicAdd(hist + e, 1);
       }
     }
     __syncwarp();
@@ -279,20 +337,31 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
   pdl_wait();
   __syncthreads();
   const int G = gridDim.x;
-  // a thread keeps to one expert where it can: few shared-memory additions
-  const int lanes = P.experts < kRouteThreads ? kRouteThreads / P.experts : 1;
-  const int e = threadIdx.x % P.experts, part = threadIdx.x / P.experts;
-  if (part < lanes) {
-    int all = 0, mine = 0;
+  // W neighbouring experts per thread (16-byte reads where the count allows), all CTAs spread over the threads
+  auto add_up = [&](auto width) {
+    constexpr int W = decltype(width)::value;
+    const int groups = P.experts / W, lanes = groups < kRouteThreads ? kRouteThreads / groups : 1;
+    for (int i = threadIdx.x; i < groups * lanes; i += kRouteThreads) {
+      const int e = i % groups * W;
+      int all[W] = {}, mine[W] = {};
 #pragma unroll 8
-    for (int b = part; b < G; b += lanes) {
-      const int c = P.block_hist[static_cast<int64_t>(b) * P.experts + e];
-      all += c;
-      if (b < static_cast<int>(blockIdx.x)) mine += c;
+      for (int b = i / groups; b < G; b += lanes) {
+        const Vec<int, W> c = *reinterpret_cast<const Vec<int, W> *>(P.block_hist + static_cast<int64_t>(b) * P.experts + e);
+#pragma unroll
+        for (int q = 0; q < W; ++q) {
+          all[q] += c.v[q];
+          if (b < static_cast<int>(blockIdx.x)) mine[q] += c.v[q];
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        atomicAdd(totals + e + q, all[q]);
+        if (mine[q]) atomicAdd(before + e + q, mine[q]);
+      }
     }
-    atomicAdd(totals + e, all);
-    atomicAdd(before + e, mine);
-  }
+  };
+  if (P.experts % 4 == 0) add_up(std::integral_constant<int, 4>{});
+  else add_up(std::integral_constant<int, 1>{});
   __syncthreads();
   if (threadIdx.x < 32) scan_experts(totals, first, P.experts);
   __syncthreads();

@@ -234,10 +234,11 @@ __global__ void __launch_bounds__(256) grouped_sum_kernel(const float *partial, 
 }
 
 // dz = dy where the ReLU let the value through (dz != NULL), and column sums over pieces of a group's rows.  What the ReLU
-// let through is a bit per element that the forward pass wrote (mask), or y > 0 where there is none.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) grouped_dz_kernel(const T *dy, int64_t dy_stride, const T *y, const unsigned char *mask, int mask_pitch, T *dz,
-                                                         float *partial, const int32_t *offsets, int n, int experts, int c_out, int piece) {
+// let through: MASK 1 a bit per element that the forward pass wrote, 2 y > 0, 0 everything (no ReLU).  A copy with four
+// rows of a thread in flight; four CTAs per SM.
+template <typename T, int V, int MASK>
+__global__ void __launch_bounds__(256, 4) grouped_dz_kernel(const T *dy, int64_t dy_stride, const T *y, const unsigned char *mask, int mask_pitch, T *dz,
+                                                            float *partial, const int32_t *offsets, int n, int experts, int c_out, int piece) {
   __shared__ float sums[256 * V];
   pdl_trigger();
   pdl_wait();
@@ -251,32 +252,33 @@ __global__ void __launch_bounds__(256) grouped_dz_kernel(const T *dy, int64_t dy
   float sum[V] = {};
   if (lane < lanes)
     for (int r = r0 + lane; r < r1; r += kBatch * lanes) {
-      Vec<T, V> d[kBatch], f[kBatch];
-      unsigned bits[kBatch];
+      Vec<T, V> d[kBatch], f[MASK == 2 ? kBatch : 1];
+      unsigned bits[MASK == 1 ? kBatch : 1];
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
-        const int64_t row = r + q * lanes;
-        d[q] = Vec<T, V>{};
-        f[q] = Vec<T, V>{};
-        bits[q] = 0;
-        if (row < r1) {
-          d[q] = *reinterpret_cast<const Vec<T, V> *>(dy + row * dy_stride + c);
-          if (mask) bits[q] = mask[row * mask_pitch + c / 8] >> (c & 7);
-          else if (y) f[q] = *reinterpret_cast<const Vec<T, V> *>(y + row * c_out + c);
-        }
+        const int row = r + q * lanes < r1 ? r + q * lanes : r;      // (past the end: the first row again, not used)
+        d[q] = *reinterpret_cast<const Vec<T, V> *>(dy + row * dy_stride + c);
+        if (MASK == 1) bits[q] = mask[static_cast<int64_t>(row) * mask_pitch + c / 8] >> (c & 7);
+        if (MASK == 2) f[q] = *reinterpret_cast<const Vec<T, V> *>(y + static_cast<int64_t>(row) * c_out + c);
       }
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
         const int64_t row = r + q * lanes;
         if (row >= r1) break;
-        if (dz) {
+        if (MASK == 1 && V == 8) {
+          uint32_t *w = reinterpret_cast<uint32_t *>(&d[q]);
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) w[i] &= (bits[q] >> 2 * i & 1u) * 0xffffu | (bits[q] >> (2 * i + 1) & 1u) * 0xffff0000u;
+        } else if (MASK != 0) {
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            if (mask ? !(bits[q] >> i & 1) : !(to_f32(f[q].v[i]) > 0.f)) d[q].v[i] = from_f32<T>(0.f);
-          *reinterpret_cast<Vec<T, V> *>(dz + row * c_out + c) = d[q];
+            if (MASK == 1 ? !(bits[q] >> i & 1) : !(to_f32(f[q].v[i]) > 0.f)) d[q].v[i] = from_f32<T>(0.f);
         }
+        if (dz) *reinterpret_cast<Vec<T, V> *>(dz + row * c_out + c) = d[q];
+        float v[V];
+        vec_to_f32<T, V>(d[q], v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += to_f32(d[q].v[i]);
+        for (int i = 0; i < V; ++i) sum[i] += v[i];
       }
     }
   if (partial == nullptr) return;
@@ -313,9 +315,9 @@ __global__ void __launch_bounds__(1024) grouped_column_sum_kernel(const float *p
   if (lane == 0 && co < size) out[static_cast<int64_t>(e) * size + co] = from_f32<T>(t);
 }
 
-// Rows per piece of the column sums: a CTA per piece, all of them resident at once (eight per SM), at least 32 rows.
+// Rows per piece of the column sums: a CTA per piece, all of them resident at once (four per SM), at least 32 rows.
 static int dz_piece(int64_t n) {
-  const int64_t p = div_up(div_up(n, 15 * sm_count() / 2), 8) * 8;
+  const int64_t p = div_up(div_up(n, 15 * sm_count() / 4), 8) * 8;
   return static_cast<int>(p < 32 ? 32 : p);
 }
 
@@ -478,7 +480,9 @@ extern "C" int spira_b200_grouped_linear_dz(const spira_b200_grouped_desc *desc,
                                      static_cast<T *>(D.dz), partial, D.offsets, n, D.experts, D.c_out, piece));
       return SPIRA_B200_OK;
     };
-    rc = wide ? go(grouped_dz_kernel<T, 8>, D.c_out / 8) : go(grouped_dz_kernel<T, 1>, D.c_out);
+    const int kind = !D.dz ? 0 : D.mask ? 1 : 2;
+    if (wide) rc = kind == 0 ? go(grouped_dz_kernel<T, 8, 0>, D.c_out / 8) : kind == 1 ? go(grouped_dz_kernel<T, 8, 1>, D.c_out / 8) : go(grouped_dz_kernel<T, 8, 2>, D.c_out / 8);
+    else rc = kind == 0 ? go(grouped_dz_kernel<T, 1, 0>, D.c_out) : kind == 1 ? go(grouped_dz_kernel<T, 1, 1>, D.c_out) : go(grouped_dz_kernel<T, 1, 2>, D.c_out);
     if (rc != SPIRA_B200_OK || !D.dbias) return rc;
     SB_CHECK_CUDA(launch_dependent(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(1024), 0, st,
                                    static_cast<const float *>(partial), D.offsets, n, D.experts, piece, D.c_out, static_cast<T *>(D.dbias)));
