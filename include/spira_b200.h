@@ -537,10 +537,10 @@ int spira_b200_expert_combine_backward(const void *rows, const void *dout, int d
  *   spira_b200_grouped_linear      y[r] = relu?(x[r] W[e] + bias[e]); rows outside every group are zero
  *                                  (mask != NULL: also a bit per element, set where the value before the ReLU is
  *                                  positive; spira_b200_grouped_linear_mask_bytes gives its size, 0 = this shape has none)
- *   spira_b200_grouped_linear_dz   dz = dy where the mask is set, or where y > 0 without a mask (dz may be NULL: no ReLU),
- *                                  dbias[e] = column sums of dz (may be NULL); dz is written for the rows of groups only
- *   spira_b200_grouped_linear_dx   dx[r] = dy[r] W[e]^T (pass dz as dy); rows outside every group are zero
- *   spira_b200_grouped_linear_dw   dweight[e] = x_e^T dy_e (zero for an empty group)
+ *   spira_b200_grouped_linear_backward   with dz = dy, with `relu` only where the mask is set (or y > 0 without a mask):
+ *                                  dx[r] = dz[r] W[e]^T (rows outside every group are zero), dweight[e] = x_e^T dz_e and
+ *                                  dbias[e] = column sums of dz_e (zero for an empty group); NULL outputs are left out.
+ *                                  The workspace is asked for with the same descriptor.
  * fp16 or bf16 in and out, fp32 sums, one rounding.  Offsets are read on the device; an entry counts as the largest of
  * those before it and as n at most, so a bad list cannot reach outside the tensors.  x and dy have unit column stride and
  * rows `x_stride` / `dy_stride` elements apart; everything else is dense. */
@@ -549,16 +549,13 @@ typedef struct spira_b200_grouped_desc {
   int64_t n, x_stride, dy_stride;
   const int32_t *offsets;
   const void *x, *weight, *bias, *dy;
-  void *y, *mask, *dz, *dx, *dweight, *dbias;
+  void *y, *mask, *dx, *dweight, *dbias;
 } spira_b200_grouped_desc;
 int spira_b200_grouped_linear_mask_bytes(const spira_b200_grouped_desc *desc, size_t *bytes);
 int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, int32_t *status, void *stream);
-int spira_b200_grouped_linear_dz_workspace(const spira_b200_grouped_desc *desc, size_t *bytes);
-int spira_b200_grouped_linear_dz(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
-int spira_b200_grouped_linear_dx(const spira_b200_grouped_desc *desc, int32_t *status, void *stream);
-int spira_b200_grouped_linear_dw_workspace(const spira_b200_grouped_desc *desc, size_t *bytes);
-int spira_b200_grouped_linear_dw(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status,
-                                 void *stream);
+int spira_b200_grouped_linear_backward_workspace(const spira_b200_grouped_desc *desc, size_t *bytes);
+int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status,
+                                       void *stream);
 
 /* Norms around a block, its gate and the residual, in one pass over the rows:
  *   p = post ? norm(block) * post_weight + post_bias : block

@@ -5,6 +5,7 @@ There is no fallback: if the library is missing or a call fails, an exception is
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -81,7 +82,7 @@ class GroupedDesc(C.Structure):
     _fields_ = [("dtype", c_int32), ("experts", c_int32), ("c_in", c_int32), ("c_out", c_int32), ("relu", c_int32), ("reserved", c_int32),
                 ("n", c_int64), ("x_stride", c_int64), ("dy_stride", c_int64), ("offsets", c_void_p),
                 ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("dy", c_void_p),
-                ("y", c_void_p), ("mask", c_void_p), ("dz", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p)]
+                ("y", c_void_p), ("mask", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p)]
 
 
 class NormDesc(C.Structure):
@@ -96,6 +97,11 @@ class NormDesc(C.Structure):
                 ("dstream", c_void_p), ("dnormed", c_void_p), ("dx", c_void_p), ("dblock", c_void_p), ("dgate", c_void_p),
                 ("dweight", c_void_p), ("dbias", c_void_p), ("dpost_weight", c_void_p), ("dpost_bias", c_void_p)]
 
+
+# The two descriptors above as packed bytes (an eager call fills one every time; a ctypes structure costs several times more)
+GROUPED_PACK = struct.Struct("<6i3q10Q")
+NORM_PACK = struct.Struct("<8i4f6q19Q")
+assert GROUPED_PACK.size == C.sizeof(GroupedDesc) and NORM_PACK.size == C.sizeof(NormDesc)
 
 F16, BF16, F32 = 0, 1, 2
 TAPE_CONV, TAPE_IDENTITY, TAPE_POINTWISE = 0, 1, 2
@@ -168,16 +174,13 @@ SIGNATURES = {
     "spira_b200_expert_combine": [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p],
     "spira_b200_expert_combine_backward": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
                                            c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
-    "spira_b200_grouped_linear_mask_bytes": [C.POINTER(GroupedDesc), C.POINTER(c_size_t)],
-    "spira_b200_grouped_linear": [C.POINTER(GroupedDesc), c_void_p, c_void_p],
-    "spira_b200_grouped_linear_dz_workspace": [C.POINTER(GroupedDesc), C.POINTER(c_size_t)],
-    "spira_b200_grouped_linear_dz": [C.POINTER(GroupedDesc), c_void_p, c_size_t, c_void_p],
-    "spira_b200_grouped_linear_dx": [C.POINTER(GroupedDesc), c_void_p, c_void_p],
-    "spira_b200_grouped_linear_dw_workspace": [C.POINTER(GroupedDesc), C.POINTER(c_size_t)],
-    "spira_b200_grouped_linear_dw": [C.POINTER(GroupedDesc), c_void_p, c_size_t, c_void_p, c_void_p],
-    "spira_b200_residual_norm": [C.POINTER(NormDesc), c_void_p],
-    "spira_b200_residual_norm_backward_workspace": [C.POINTER(NormDesc), C.POINTER(c_size_t)],
-    "spira_b200_residual_norm_backward": [C.POINTER(NormDesc), c_void_p, c_size_t, c_void_p],
+    "spira_b200_grouped_linear_mask_bytes": [c_void_p, C.POINTER(c_size_t)],
+    "spira_b200_grouped_linear": [c_void_p, c_void_p, c_void_p],
+    "spira_b200_grouped_linear_backward_workspace": [c_void_p, C.POINTER(c_size_t)],
+    "spira_b200_grouped_linear_backward": [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p],
+    "spira_b200_residual_norm": [c_void_p, c_void_p],
+    "spira_b200_residual_norm_backward_workspace": [c_void_p, C.POINTER(c_size_t)],
+    "spira_b200_residual_norm_backward": [c_void_p, c_void_p, c_size_t, c_void_p],
 }
 STATIC_SCRATCH_FLOATS = 4 * 1024 * 1024
 EXPORTS = sorted(list(SIGNATURES) + ["spira_b200_last_error"])
@@ -219,8 +222,8 @@ KERNELS_PER_CALL = {
     "spira_b200_pack_weights": 1, "spira_b200_conv_os": 1, "spira_b200_conv_os_grouped": 1, "spira_b200_conv_os_split": 1,
     "spira_b200_kmap_group": 2,
     "spira_b200_expert_route": 1, "spira_b200_expert_route_backward": 1, "spira_b200_expert_dispatch": 1, "spira_b200_expert_combine": 1,
-    "spira_b200_expert_combine_backward": 1, "spira_b200_grouped_linear": 1, "spira_b200_grouped_linear_dz": 1,
-    "spira_b200_grouped_linear_dx": 1, "spira_b200_grouped_linear_dw": 1, "spira_b200_residual_norm": 1, "spira_b200_residual_norm_backward": 1,
+    "spira_b200_expert_combine_backward": 1, "spira_b200_grouped_linear": 1, "spira_b200_grouped_linear_backward": 2,
+    "spira_b200_residual_norm": 1, "spira_b200_residual_norm_backward": 1,
     "spira_b200_conv_ws": 2, "spira_b200_conv_ws_fused": 1, "spira_b200_conv_ws_static": 2,
 }
 launch_count = 0          # kernels launched through `call` since import (or since it was last reset by the caller)

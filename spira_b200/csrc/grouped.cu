@@ -16,6 +16,8 @@
 
 namespace sb {
 
+static_assert(sizeof(spira_b200_grouped_desc) == 128, "spira_b200_grouped_desc layout");
+
 constexpr int kATile = 64, kAK = 32, kALd = kAK + 8;     // (row stride of 80 bytes: conflict-free fragment loads)
 constexpr int kAThreads = 128;
 
@@ -393,107 +395,118 @@ extern "C" int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, in
   return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kForward>(P, as_stream(stream))););
 }
 
-extern "C" int spira_b200_grouped_linear_dx(const spira_b200_grouped_desc *desc, int32_t *status, void *stream) {
-  int rc = grouped_check("grouped_linear_dx", desc);
-  if (rc != SPIRA_B200_OK || desc->n == 0) return rc;
-  const spira_b200_grouped_desc &D = *desc;
-  SB_CHECK_ARG(D.dy && D.weight && D.dx, "grouped_linear_dx: null pointer");
-  if (tc_dx(D)) return grouped_tc_run(kDx, D, 0, nullptr, status, wait_ns(), as_stream(stream));
-  GroupedParams P{D.dy, D.weight, nullptr, D.offsets, D.dx, nullptr, D.dy_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, 0, 0};
-  return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kDx>(P, as_stream(stream))););
-}
-
-extern "C" int spira_b200_grouped_linear_dw_workspace(const spira_b200_grouped_desc *desc, size_t *bytes) {
-  int rc = grouped_check("grouped_linear_dw", desc);
-  if (rc != SPIRA_B200_OK) return rc;
-  SB_CHECK_ARG(bytes, "grouped_linear_dw: null pointer");
-  const int piece = dw_rows(*desc);
-  *bytes = piece ? static_cast<size_t>(group_tiles_bound(desc->n, desc->experts, piece)) * desc->c_in * desc->c_out * 4 : 0;
-  return SPIRA_B200_OK;
-}
-
-extern "C" int spira_b200_grouped_linear_dw(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
-  int rc = grouped_check("grouped_linear_dw", desc);
-  if (rc != SPIRA_B200_OK) return rc;
-  const spira_b200_grouped_desc &D = *desc;
-  SB_CHECK_ARG(D.dweight, "grouped_linear_dw: null pointer");
-  cudaStream_t st = as_stream(stream);
-  const int64_t size = static_cast<int64_t>(D.c_in) * D.c_out;
-  if (D.n == 0) {
-    SB_CHECK_CUDA(cudaMemsetAsync(D.dweight, 0, static_cast<size_t>(D.experts) * size * 2, st));
-    return SPIRA_B200_OK;
-  }
-  SB_CHECK_ARG(D.x && D.dy, "grouped_linear_dw: null pointer");
-  size_t need = 0;
-  rc = spira_b200_grouped_linear_dw_workspace(desc, &need);
-  if (rc != SPIRA_B200_OK) return rc;
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(SPIRA_B200_ERR_WORKSPACE, "grouped_linear_dw: workspace of %zu bytes is smaller than %zu", workspace_bytes, need);
-  SB_CHECK_ARG(aligned16(workspace), "grouped_linear_dw: the workspace must be 16-byte aligned");
-  const int piece = dw_rows(D);
-  const bool tc = tc_dw(D);
-  GroupedParams P{D.x, D.dy, nullptr, D.offsets, D.dweight, static_cast<float *>(workspace), D.x_stride, D.dy_stride, static_cast<int>(D.n), D.experts,
-                  D.c_in, D.c_out, 0, piece};
-  return SB_DISPATCH_HALF(D.dtype, T, {
-    rc = tc ? grouped_tc_run(kDw, D, piece, static_cast<float *>(workspace), status, wait_ns(), st) : launch_any<T, kDw>(P, st);
-    if (rc != SPIRA_B200_OK || piece == 0) return rc;
-    const unsigned blocks = static_cast<unsigned>(div_up(size, 256) < 1024 ? div_up(size, 256) : 1024);
-    SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(blocks, D.experts), dim3(256), 0, st, static_cast<const float *>(workspace), D.offsets,
-                                   static_cast<int>(D.n), D.experts, piece, size, static_cast<T *>(D.dweight)));
-    return SPIRA_B200_OK;
-  });
-}
-
-extern "C" int spira_b200_grouped_linear_dz_workspace(const spira_b200_grouped_desc *desc, size_t *bytes) {
-  int rc = grouped_check("grouped_linear_dz", desc);
-  if (rc != SPIRA_B200_OK) return rc;
-  SB_CHECK_ARG(bytes, "grouped_linear_dz: null pointer");
-  *bytes = desc->dbias ? static_cast<size_t>(group_tiles_bound(desc->n, desc->experts, dz_piece(desc->n))) * desc->c_out * 4 : 0;
-  return SPIRA_B200_OK;
-}
-
-extern "C" int spira_b200_grouped_linear_dz(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, void *stream) {
-  int rc = grouped_check("grouped_linear_dz", desc);
-  if (rc != SPIRA_B200_OK) return rc;
-  const spira_b200_grouped_desc &D = *desc;
-  SB_CHECK_ARG(D.dz || D.dbias, "grouped_linear_dz: null pointer");
-  cudaStream_t st = as_stream(stream);
-  if (D.n == 0) {
-    if (D.dbias) SB_CHECK_CUDA(cudaMemsetAsync(D.dbias, 0, static_cast<size_t>(D.experts) * D.c_out * 2, st));
-    return SPIRA_B200_OK;
-  }
-  SB_CHECK_ARG(D.dy && (!D.dz || D.y || D.mask), "grouped_linear_dz: null pointer");
-  size_t need = 0;
-  rc = spira_b200_grouped_linear_dz_workspace(desc, &need);
-  if (rc != SPIRA_B200_OK) return rc;
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(SPIRA_B200_ERR_WORKSPACE, "grouped_linear_dz: workspace of %zu bytes is smaller than %zu", workspace_bytes, need);
-  float *partial = D.dbias ? static_cast<float *>(workspace) : nullptr;
-  const int n = static_cast<int>(D.n);
-  const int piece = dz_piece(n);
-  const unsigned units = static_cast<unsigned>(group_tiles_bound(n, D.experts, piece));
-  const bool wide = D.c_out % 8 == 0 && aligned16(D.dy) && D.dy_stride % 8 == 0 && aligned16(D.y) && aligned16(D.dz);
-  return SB_DISPATCH_HALF(D.dtype, T, {
-    auto go = [&](auto kernel, int columns) -> int {
-      SB_CHECK_CUDA(launch_dependent(kernel, dim3(units, static_cast<unsigned>(div_up(columns, 256))), dim3(256), 0, st, static_cast<const T *>(D.dy),
-                                     D.dy_stride, static_cast<const T *>(D.y), static_cast<const unsigned char *>(D.mask), mask_pitch(D.c_out),
-                                     static_cast<T *>(D.dz), partial, D.offsets, n, D.experts, D.c_out, piece));
-      return SPIRA_B200_OK;
-    };
-    const int kind = !D.dz ? 0 : D.mask ? 1 : 2;
-    if (wide) rc = kind == 0 ? go(grouped_dz_kernel<T, 8, 0>, D.c_out / 8) : kind == 1 ? go(grouped_dz_kernel<T, 8, 1>, D.c_out / 8) : go(grouped_dz_kernel<T, 8, 2>, D.c_out / 8);
-    else rc = kind == 0 ? go(grouped_dz_kernel<T, 1, 0>, D.c_out) : kind == 1 ? go(grouped_dz_kernel<T, 1, 1>, D.c_out) : go(grouped_dz_kernel<T, 1, 2>, D.c_out);
-    if (rc != SPIRA_B200_OK || !D.dbias) return rc;
-    SB_CHECK_CUDA(launch_dependent(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(1024), 0, st,
-                                   static_cast<const float *>(partial), D.offsets, n, D.experts, piece, D.c_out, static_cast<T *>(D.dbias)));
-    return SPIRA_B200_OK;
-  });
-}
-
 extern "C" int spira_b200_grouped_linear_mask_bytes(const spira_b200_grouped_desc *desc, size_t *bytes) {
   int rc = grouped_check("grouped_linear_mask", desc);
   if (rc != SPIRA_B200_OK) return rc;
   SB_CHECK_ARG(bytes, "grouped_linear_mask: null pointer");
   *bytes = desc->n > 0 && desc->relu && tc_forward(*desc) ? static_cast<size_t>(desc->n) * mask_pitch(desc->c_out) : 0;
   return SPIRA_B200_OK;
+}
+
+// Scratch of the backward pass: dz where a ReLU followed, then the partial sums (of dbias, later of dweight: one region).
+struct BackwardPlan {
+  bool need_dz;
+  int dz_rows, dw_rows;
+  size_t partial_at, bytes;
+};
+
+static BackwardPlan backward_plan(const spira_b200_grouped_desc &D, const spira_b200_grouped_desc &Z) {
+  BackwardPlan p{};
+  p.need_dz = D.relu && (D.dx || D.dweight);
+  p.dz_rows = dz_piece(D.n);
+  p.dw_rows = D.dweight ? dw_rows(Z) : 0;
+  p.partial_at = p.need_dz ? static_cast<size_t>(div_up(D.n * D.c_out * 2, 256) * 256) : 0;
+  const size_t db = D.dbias ? static_cast<size_t>(group_tiles_bound(D.n, D.experts, p.dz_rows)) * D.c_out * 4 : 0;
+  const size_t dw = p.dw_rows ? static_cast<size_t>(group_tiles_bound(D.n, D.experts, p.dw_rows)) * D.c_in * D.c_out * 4 : 0;
+  p.bytes = p.partial_at + (db > dw ? db : dw);
+  return p;
+}
+
+// The call with dz in the place of dy.
+static spira_b200_grouped_desc with_dz(const spira_b200_grouped_desc &D, const void *workspace) {
+  spira_b200_grouped_desc Z = D;
+  if (D.relu && (D.dx || D.dweight)) {
+    Z.dy = workspace;
+    Z.dy_stride = D.c_out;
+  }
+  return Z;
+}
+
+static int backward_check(const spira_b200_grouped_desc *D) {
+  int rc = grouped_check("grouped_linear_backward", D);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(D->dx || D->dweight || D->dbias || D->n == 0, "grouped_linear_backward: no gradient is asked for");
+  SB_CHECK_ARG(D->n == 0 || (D->dy && (!D->dx || D->weight) && (!D->dweight || D->x) && (!D->relu || D->mask || D->y)),
+               "grouped_linear_backward: null pointer");
+  return SPIRA_B200_OK;
+}
+
+extern "C" int spira_b200_grouped_linear_backward_workspace(const spira_b200_grouped_desc *desc, size_t *bytes) {
+  int rc = backward_check(desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(bytes, "grouped_linear_backward: null pointer");
+  *bytes = desc->n ? backward_plan(*desc, with_dz(*desc, nullptr)).bytes : 0;
+  return SPIRA_B200_OK;
+}
+
+extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status,
+                                                  void *stream) {
+  int rc = backward_check(desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  const spira_b200_grouped_desc &D = *desc;
+  cudaStream_t st = as_stream(stream);
+  const int64_t size = static_cast<int64_t>(D.c_in) * D.c_out;
+  if (D.n == 0) {
+    if (D.dweight) SB_CHECK_CUDA(cudaMemsetAsync(D.dweight, 0, static_cast<size_t>(D.experts) * size * 2, st));
+    if (D.dbias) SB_CHECK_CUDA(cudaMemsetAsync(D.dbias, 0, static_cast<size_t>(D.experts) * D.c_out * 2, st));
+    return SPIRA_B200_OK;
+  }
+  const spira_b200_grouped_desc Z = with_dz(D, workspace);
+  const BackwardPlan plan = backward_plan(D, with_dz(D, nullptr));      // (as the size was asked for: dz is aligned like a null pointer)
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
+    return fail(SPIRA_B200_ERR_WORKSPACE, "grouped_linear_backward: workspace of %zu bytes is smaller than %zu", workspace_bytes, plan.bytes);
+  SB_CHECK_ARG(aligned16(workspace), "grouped_linear_backward: the workspace must be 16-byte aligned");
+  float *partial = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + plan.partial_at);
+  const int n = static_cast<int>(D.n);
+  return SB_DISPATCH_HALF(D.dtype, T, {
+    if (plan.need_dz || D.dbias) {
+      T *dz = plan.need_dz ? static_cast<T *>(workspace) : nullptr;
+      const unsigned units = static_cast<unsigned>(group_tiles_bound(n, D.experts, plan.dz_rows));
+      const bool wide = D.c_out % 8 == 0 && aligned16(D.dy) && (D.dy_stride % 8 == 0 || n == 1) && (D.mask || aligned16(D.y));
+      auto go = [&](auto kernel, int columns) -> int {
+        SB_CHECK_CUDA(launch_dependent(kernel, dim3(units, static_cast<unsigned>(div_up(columns, 256))), dim3(256), 0, st, static_cast<const T *>(D.dy),
+                                       D.dy_stride, static_cast<const T *>(D.y), static_cast<const unsigned char *>(D.mask), mask_pitch(D.c_out), dz,
+                                       D.dbias ? partial : nullptr, D.offsets, n, D.experts, D.c_out, plan.dz_rows));
+        return SPIRA_B200_OK;
+      };
+      const int kind = !D.relu ? 0 : D.mask ? 1 : 2;
+      if (wide) rc = kind == 0 ? go(grouped_dz_kernel<T, 8, 0>, D.c_out / 8) : kind == 1 ? go(grouped_dz_kernel<T, 8, 1>, D.c_out / 8) : go(grouped_dz_kernel<T, 8, 2>, D.c_out / 8);
+      else rc = kind == 0 ? go(grouped_dz_kernel<T, 1, 0>, D.c_out) : kind == 1 ? go(grouped_dz_kernel<T, 1, 1>, D.c_out) : go(grouped_dz_kernel<T, 1, 2>, D.c_out);
+      if (rc != SPIRA_B200_OK) return rc;
+      if (D.dbias)
+        SB_CHECK_CUDA(launch_dependent(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(1024), 0, st,
+                                       static_cast<const float *>(partial), D.offsets, n, D.experts, plan.dz_rows, D.c_out, static_cast<T *>(D.dbias)));
+    }
+    if (D.dx) {
+      if (tc_dx(Z)) {
+        rc = grouped_tc_run(kDx, Z, 0, nullptr, status, wait_ns(), st);
+      } else {
+        GroupedParams P{Z.dy, Z.weight, nullptr, Z.offsets, Z.dx, nullptr, Z.dy_stride, 0, n, Z.experts, Z.c_in, Z.c_out, 0, 0};
+        rc = launch_any<T, kDx>(P, st);
+      }
+      if (rc != SPIRA_B200_OK) return rc;
+    }
+    if (!D.dweight) return SPIRA_B200_OK;
+    if (tc_dw(Z)) {
+      rc = grouped_tc_run(kDw, Z, plan.dw_rows, partial, status, wait_ns(), st);
+    } else {
+      GroupedParams P{Z.x, Z.dy, nullptr, Z.offsets, Z.dweight, partial, Z.x_stride, Z.dy_stride, n, Z.experts, Z.c_in, Z.c_out, 0, plan.dw_rows};
+      rc = launch_any<T, kDw>(P, st);
+    }
+    if (rc != SPIRA_B200_OK || plan.dw_rows == 0) return rc;
+    const unsigned blocks = static_cast<unsigned>(div_up(size, 256) < 1024 ? div_up(size, 256) : 1024);
+    SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(blocks, D.experts), dim3(256), 0, st, static_cast<const float *>(partial), D.offsets, n,
+                                   D.experts, plan.dw_rows, size, static_cast<T *>(D.dweight)));
+    return SPIRA_B200_OK;
+  });
 }

@@ -18,6 +18,8 @@
 
 namespace sb {
 
+static_assert(sizeof(spira_b200_norm_desc) == 248, "spira_b200_norm_desc layout");
+
 constexpr int kNormMaxChannels = 8192;
 constexpr int kGateNone = 0, kGateChannel = 1, kGateRow = 2, kGateFull = 3;
 constexpr int kNormBackwardCtas = 3;     // per SM at most: every CTA writes one set of partial sums
@@ -693,6 +695,11 @@ template <typename T, int V>
 static int launch_norm_shape(const NormParams &P, bool backward, int *ctas, cudaStream_t st) {
   const int pieces = P.channels / V;
   if constexpr (V > 1) {
+    if (!backward && pieces % 3 == 0 && pieces <= 96 && (pieces & (pieces - 1)) != 0) {      // 96, 192, 384 channels: three pieces leave no lane idle
+      if (pieces == 12) return launch_norm<T, V, 4, 3>(P, backward, ctas, st);
+      if (pieces == 24) return launch_norm<T, V, 8, 3>(P, backward, ctas, st);
+      if (pieces == 48) return launch_norm<T, V, 16, 3>(P, backward, ctas, st);
+    }
     if (pieces <= 4) return launch_norm<T, V, 4, 1>(P, backward, ctas, st);
     if (pieces <= 8) return launch_norm<T, V, 8, 1>(P, backward, ctas, st);
     if (pieces <= 16) return launch_norm<T, V, 16, 1>(P, backward, ctas, st);

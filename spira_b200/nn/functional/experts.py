@@ -15,11 +15,9 @@ import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from spira_b200 import _lib
 from spira_b200.nn.functional import _C
-from spira_b200._lib import GroupedDesc
 
 __all__ = ["ExpertRouting", "expert_route", "expert_dispatch", "expert_combine", "grouped_linear"]
 
@@ -72,6 +70,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _once() -> None:
+    """In a backward function: refuses to be recorded itself (``create_graph=True``)."""
+    if torch.is_grad_enabled():
+        _fail("the expert and norm operators can be differentiated once only (create_graph=True was asked for)")
+
+
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -115,8 +123,8 @@ class _Route(torch.autograd.Function):
         return tuple(r)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dweights, *_):
+        _once()
         if dweights is None:
             return None, None, None
         logits, weights, chosen = ctx.saved_tensors
@@ -197,8 +205,8 @@ class _Dispatch(torch.autograd.Function):
         return _dispatch(feats, slots, offsets)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, drows):
+        _once()
         return _combine(_rows(drows), None, ctx.saved_tensors[0]), None, None
 
 
@@ -209,8 +217,8 @@ class _Combine(torch.autograd.Function):
         return _combine(rows, weights, slots)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        _once()
         rows, weights, slots, offsets = ctx.saved_tensors
         dout = _rows(dout)
         (n, k), channels = slots.shape, rows.shape[1]
@@ -259,42 +267,34 @@ def _status(index: int) -> int:
     return t.data_ptr()
 
 
-def _grouped_desc(x, weights, offsets, dy=None) -> GroupedDesc:
+def _grouped_desc(n, weights, offsets, relu, x=None, bias=None, dy=None, y=None, mask=None, dx=None, dweight=None, dbias=None) -> bytes:
+    """``spira_b200_grouped_desc`` (fields as in ``_lib.GroupedDesc``)."""
     experts, c_in, c_out = weights.shape
-    d = GroupedDesc(dtype=_DTYPES[weights.dtype], experts=experts, c_in=c_in, c_out=c_out, n=x.shape[0] if x is not None else dy.shape[0],
-                    offsets=offsets.data_ptr(), weight=weights.data_ptr())
-    if x is not None:
-        d.x, d.x_stride = x.data_ptr(), x.stride(0)
-    if dy is not None:
-        d.dy, d.dy_stride = dy.data_ptr(), dy.stride(0)
-    return d
+    return _lib.GROUPED_PACK.pack(_DTYPES[weights.dtype], experts, c_in, c_out, relu, 0, n, 0 if x is None else x.stride(0),
+                                  0 if dy is None else dy.stride(0), offsets.data_ptr(), 0 if x is None else x.data_ptr(), weights.data_ptr(),
+                                  _addr(bias), _addr(dy), _addr(y), _addr(mask), _addr(dx), _addr(dweight), _addr(dbias))
 
 
 def _grouped(x, weights, offsets, bias, relu, want_mask=False):
     """The product and, for a backward pass, what its ReLU let through: the bit mask the kernel writes, or None where the
     shape has none (then the sign of the result says it)."""
-    index = x.get_device()
-    y = x.new_empty((x.shape[0], weights.shape[2]))
-    d = _grouped_desc(x, weights, offsets)
-    d.y, d.relu = y.data_ptr(), 1 if relu else 0
-    if bias is not None:
-        d.bias = bias.data_ptr()
+    index, n = x.get_device(), x.shape[0]
+    y = x.new_empty((n, weights.shape[2]))
     mask = None
     if want_mask and relu:
         need = C.c_size_t()
-        _lib.call("spira_b200_grouped_linear_mask_bytes", C.byref(d), C.byref(need))
+        _query(index, "spira_b200_grouped_linear_mask_bytes", _grouped_desc(n, weights, offsets, 1, x, bias, y=y), C.byref(need))
         if need.value:
             mask = x.new_empty(need.value, dtype=torch.uint8)
-            d.mask = mask.data_ptr()
-    _launch(index, "spira_b200_grouped_linear", C.byref(d), _status(index))
+    _launch(index, "spira_b200_grouped_linear", _grouped_desc(n, weights, offsets, 1 if relu else 0, x, bias, y=y, mask=mask), _status(index))
     return (y, mask) if want_mask else y
 
 
 def _with_workspace(index, like, name, desc, *rest):
     need = C.c_size_t()
-    _query(index, name + "_workspace", C.byref(desc), C.byref(need))
+    _query(index, name + "_workspace", desc, C.byref(need))
     workspace = like.new_empty(need.value, dtype=torch.uint8) if need.value else None
-    _launch(index, name, C.byref(desc), None if workspace is None else workspace.data_ptr(), need.value, *rest)
+    _launch(index, name, desc, None if workspace is None else workspace.data_ptr(), need.value, *rest)
 
 
 class _Grouped(torch.autograd.Function):
@@ -306,39 +306,17 @@ class _Grouped(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _once()
         x, weights, offsets, y, mask = ctx.saved_tensors
         dy = _rows(dy)
-        index = x.get_device()
-        status = _status(index)
-        want_dx, want_dw, want_db = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.has_bias and ctx.needs_input_grad[3]
-        dx = dw = db = None
-        if ctx.relu or want_db:
-            d = _grouped_desc(None, weights, offsets, dy)
-            if ctx.relu:
-                dz = dy.new_empty((dy.shape[0], weights.shape[2]))
-                d.dz = dz.data_ptr()
-                if mask is not None:
-                    d.mask = mask.data_ptr()
-                else:
-                    d.y = y.data_ptr()
-            if want_db:
-                db = weights.new_empty((weights.shape[0], weights.shape[2]))
-                d.dbias = db.data_ptr()
-            _with_workspace(index, dy, "spira_b200_grouped_linear_dz", d)
-            if ctx.relu:
-                dy = dz
-        if want_dx:
-            dx = dy.new_empty((dy.shape[0], weights.shape[1]))
-            d = _grouped_desc(None, weights, offsets, dy)
-            d.dx = dx.data_ptr()
-            _launch(index, "spira_b200_grouped_linear_dx", C.byref(d), status)
-        if want_dw:
-            dw = weights.new_empty(weights.shape)
-            d = _grouped_desc(x, weights, offsets, dy)
-            d.dweight = dw.data_ptr()
-            _with_workspace(index, dy, "spira_b200_grouped_linear_dw", d, status)
+        need = ctx.needs_input_grad
+        index, n = x.get_device(), x.shape[0]
+        dx = dy.new_empty(x.shape) if need[0] else None
+        dw = weights.new_empty(weights.shape) if need[1] else None
+        db = weights.new_empty((weights.shape[0], weights.shape[2])) if ctx.has_bias and need[3] else None
+        _with_workspace(index, dy, "spira_b200_grouped_linear_backward",
+                        _grouped_desc(n, weights, offsets, 1 if ctx.relu else 0, x, None, dy, y, mask, dx, dw, db), _status(index))
         return dx, dw, None, db, None
 
 

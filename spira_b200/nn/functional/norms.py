@@ -7,14 +7,12 @@ and adds residuals as another (spira/tensors.py:47-53).
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from spira_b200._lib import NormDesc
-from spira_b200.nn.functional.experts import _DTYPES, _device_of, _fail, _launch, _needs_grad, _rows, _with_workspace
+from spira_b200 import _lib
+from spira_b200.nn.functional.experts import _addr, _device_of, _DTYPES, _fail, _launch, _needs_grad, _once, _rows, _with_workspace
 
 __all__ = ["residual_norm"]
 
@@ -24,85 +22,60 @@ GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
 
 class _Spec:
     """What stays the same between the forward and the backward call."""
-    __slots__ = ("layer", "pre", "post", "gate_kind", "residual_scale", "block_scale", "eps")
+    __slots__ = ("params_f32", "layer", "pre", "post", "gate_kind", "residual_scale", "block_scale", "eps")
 
 
-def _desc(spec, x, block, gate, weight, bias, post_weight, post_bias) -> NormDesc:
-    params_f32 = 0
-    for p in (weight, bias, post_weight, post_bias, gate if spec.gate_kind == GATE_CHANNEL else None):
-        if p is not None:
-            params_f32 = 1 if p.dtype == torch.float32 else 0
-    d = NormDesc(dtype=_DTYPES[x.dtype], params_f32=params_f32, channels=x.shape[1], layer=spec.layer, pre=spec.pre, post=spec.post,
-                 gate_kind=spec.gate_kind, residual_scale=spec.residual_scale, block_scale=spec.block_scale, eps=spec.eps, n=x.shape[0],
-                 x=x.data_ptr(), x_stride=x.stride(0))
-    if block is not None:
-        d.block, d.block_stride = block.data_ptr(), block.stride(0)
-    if gate is not None:
-        d.gate, d.gate_stride = gate.data_ptr(), gate.stride(0)
-    if weight is not None:
-        d.weight = weight.data_ptr()
-    if bias is not None:
-        d.bias = bias.data_ptr()
-    if post_weight is not None:
-        d.post_weight = post_weight.data_ptr()
-    if post_bias is not None:
-        d.post_bias = post_bias.data_ptr()
-    return d
+def _desc(spec, x, params, stream=None, normed=None, stats=None, dstream=None, dnormed=None, grads=(None,) * 7) -> bytes:
+    """``spira_b200_norm_desc`` (fields as in ``_lib.NormDesc``); ``params`` = block, gate, weight, bias, post_weight, post_bias,
+    ``grads`` = the places for the gradients of x and of these."""
+    block, gate, weight, bias, post_weight, post_bias = params
+    dx, dblock, dgate, dweight, dbias, dpost_weight, dpost_bias = grads
+    return _lib.NORM_PACK.pack(
+        _DTYPES[x.dtype], spec.params_f32, x.shape[1], spec.layer, spec.pre, spec.post, spec.gate_kind, 0,
+        spec.residual_scale, spec.block_scale, spec.eps, 0.0,
+        x.shape[0], x.stride(0), 0 if block is None else block.stride(0), 0 if gate is None else gate.stride(0),
+        0 if dstream is None else dstream.stride(0), 0 if dnormed is None else dnormed.stride(0),
+        x.data_ptr(), _addr(block), _addr(gate), _addr(weight), _addr(bias), _addr(post_weight), _addr(post_bias), _addr(stream), _addr(normed),
+        _addr(stats), _addr(dstream), _addr(dnormed), _addr(dx), _addr(dblock), _addr(dgate), _addr(dweight), _addr(dbias), _addr(dpost_weight),
+        _addr(dpost_bias))
 
 
-def _forward(spec, x, block, gate, weight, bias, post_weight, post_bias, stats):
-    d = _desc(spec, x, block, gate, weight, bias, post_weight, post_bias)
-    stream = x.new_empty(x.shape) if block is not None else None
+def _forward(spec, x, params, stats):
+    stream = x.new_empty(x.shape) if params[0] is not None else None
     normed = x.new_empty(x.shape) if spec.pre else None
-    if stream is not None:
-        d.stream = stream.data_ptr()
-    if normed is not None:
-        d.normed = normed.data_ptr()
-    if stats is not None:
-        d.stats = stats.data_ptr()
-    _launch(x.get_device(), "spira_b200_residual_norm", C.byref(d))
+    _launch(x.get_device(), "spira_b200_residual_norm", _desc(spec, x, params, stream, normed, stats))
     return stream, normed
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, spec, x, block, gate, weight, bias, post_weight, post_bias):
+    def forward(ctx, spec, x, *params):
         stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
-        stream, normed = _forward(spec, x, block, gate, weight, bias, post_weight, post_bias, stats)
+        stream, normed = _forward(spec, x, params, stats)
         ctx.spec = spec
-        ctx.save_for_backward(x, block, gate, weight, bias, post_weight, post_bias, stats)
+        ctx.save_for_backward(x, *params, stats)
         ctx.set_materialize_grads(False)
         return stream, normed
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dstream, dnormed):
-        x, block, gate, weight, bias, post_weight, post_bias, stats = ctx.saved_tensors
-        spec, need = ctx.spec, ctx.needs_input_grad
+        _once()
+        x, *params, stats = ctx.saved_tensors
+        spec = ctx.spec
         if dstream is None and dnormed is None:
             return (None,) * 8
         if spec.pre and dnormed is None:
             dnormed = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
-        d = _desc(spec, x, block, gate, weight, bias, post_weight, post_bias)
-        d.stats = stats.data_ptr()
-        if dstream is not None:
-            dstream = _rows(dstream)
-            d.dstream, d.dstream_stride = dstream.data_ptr(), dstream.stride(0)
-        if dnormed is not None:
-            dnormed = _rows(dnormed)
-            d.dnormed, d.dnormed_stride = dnormed.data_ptr(), dnormed.stride(0)
-        grads = [None]
-        for name, t, wanted in zip(("dx", "dblock", "dgate", "dweight", "dbias", "dpost_weight", "dpost_bias"),
-                                   (x, block, gate, weight, bias, post_weight, post_bias), need[1:]):
-            g = t.new_empty(t.shape) if t is not None and wanted else None
-            if g is not None:
-                setattr(d, name, g.data_ptr())
-            grads.append(g)
-        if any(g is not None for g in grads[4:]) or (grads[3] is not None and spec.gate_kind == GATE_CHANNEL):
-            _with_workspace(x.get_device(), x, "spira_b200_residual_norm_backward", d)
+        dstream = None if dstream is None else _rows(dstream)
+        dnormed = None if dnormed is None else _rows(dnormed)
+        grads = [t.new_empty(t.shape) if t is not None and wanted else None for t, wanted in zip((x, *params), ctx.needs_input_grad[1:])]
+        desc = _desc(spec, x, params, None, None, stats, dstream, dnormed, grads)
+        if grads[3] is not None or grads[4] is not None or grads[5] is not None or grads[6] is not None \
+                or (grads[2] is not None and spec.gate_kind == GATE_CHANNEL):
+            _with_workspace(x.get_device(), x, "spira_b200_residual_norm_backward", desc)
         else:
-            _launch(x.get_device(), "spira_b200_residual_norm_backward", C.byref(d), None, 0)
-        return tuple(grads)
+            _launch(x.get_device(), "spira_b200_residual_norm_backward", desc, None, 0)
+        return (None, *grads)
 
 
 def residual_norm(feats: torch.Tensor, block: Optional[torch.Tensor] = None, *, weight: Optional[torch.Tensor] = None,
@@ -170,8 +143,9 @@ def residual_norm(feats: torch.Tensor, block: Optional[torch.Tensor] = None, *, 
     params = [p if p is None or p.is_contiguous() else p.contiguous() for p in (weight, bias, post_weight, post_bias)]
     feats_rows = _rows(feats)
     block = None if block is None else _rows(block)
+    spec.params_f32 = 1 if dtype is torch.float32 else 0
     if _needs_grad(feats, block, gate, *params):
         stream, normed = _ResidualNorm.apply(spec, feats_rows, block, gate, *params)
     else:
-        stream, normed = _forward(spec, feats_rows, block, gate, *params, None)
+        stream, normed = _forward(spec, feats_rows, (block, gate, *params), None)
     return feats if block is None else stream, normed

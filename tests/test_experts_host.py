@@ -7,7 +7,7 @@ import torch
 
 def test_descriptor_layouts_match_the_header():
     from spira_b200 import _lib
-    assert ctypes.sizeof(_lib.GroupedDesc) == 6 * 4 + 3 * 8 + 11 * 8          # the library static_asserts the same sizes
+    assert ctypes.sizeof(_lib.GroupedDesc) == 6 * 4 + 3 * 8 + 10 * 8          # the library static_asserts the same sizes
     assert ctypes.sizeof(_lib.NormDesc) == 8 * 4 + 4 * 4 + 6 * 8 + 19 * 8
 
 
@@ -38,15 +38,20 @@ def test_library_refuses_bad_arguments(lib):
     assert lib.spira_b200_expert_combine(None, 0, 4, 8, 8, None, 0, 0, None, 2, None, None) != 0 and b"null" in err()
     assert lib.spira_b200_expert_combine_backward(None, None, 0, 0, 8, 8, 8, None, 0, 0, None, 2, None, 2, None, None, None) == 0   # no rows
     g = _lib.GroupedDesc(dtype=_lib.F32, experts=2, c_in=8, c_out=8, n=4)
-    for name in ("spira_b200_grouped_linear", "spira_b200_grouped_linear_dx"):
-        assert getattr(lib, name)(ctypes.byref(g), None, None) != 0 and b"neither fp16 nor bf16" in err()
-        assert getattr(lib, name)(None, None, None) != 0
+    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"neither fp16 nor bf16" in err()
+    assert lib.spira_b200_grouped_linear(None, None, None) != 0
+    assert lib.spira_b200_grouped_linear_backward(ctypes.byref(g), None, 0, None, None) != 0 and b"neither fp16 nor bf16" in err()
+    assert lib.spira_b200_grouped_linear_backward_workspace(None, ctypes.byref(n)) != 0
     g.dtype = _lib.F16
     assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"null pointer" in err()
     g.experts = 1025
     assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"experts=1025" in err()
     g.experts, g.c_in = 2, 0
     assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"channels" in err()
+    g.c_in, g.offsets = 8, 4096
+    assert lib.spira_b200_grouped_linear_backward(ctypes.byref(g), None, 0, None, None) != 0 and b"no gradient" in err()
+    g.dweight = 4096
+    assert lib.spira_b200_grouped_linear_backward(ctypes.byref(g), None, 0, None, None) != 0 and b"null pointer" in err()
     d = _lib.NormDesc(dtype=_lib.F16, channels=8193, pre=1, eps=1e-6, n=3)
     assert lib.spira_b200_residual_norm(ctypes.byref(d), None) != 0 and b"channels=8193" in err()
     d.channels = 64

@@ -376,7 +376,7 @@ def plain_norm(x, block, weight, bias, post, post_weight, post_bias, gate, kind,
     return stream, norm(stream, weight, bias) if pre else None
 
 
-NORM_SHAPES = [(0, 16), (1, 1), (1, 256), (3, 7), (70, 8), (65, 96), (33, 100), (129, 256), (20, 257), (40, 512), (9, 1000), (7, 1030), (5, 2048), (5, 4096), (3, 5001), (3, 8192)]
+NORM_SHAPES = [(0, 16), (1, 1), (1, 256), (3, 7), (70, 8), (65, 96), (21, 192), (19, 384), (33, 100), (129, 256), (20, 257), (40, 512), (9, 1000), (7, 1030), (5, 2048), (5, 4096), (3, 5001), (3, 8192)]
 
 
 @pytest.mark.parametrize("dtype", ANY)
@@ -538,6 +538,16 @@ def test_refusals():
     for call, word in bad:
         with pytest.raises(RuntimeError, match=word):
             call()
+
+
+def test_second_derivatives_are_refused():
+    from spira_b200.nn import functional as F
+    x = rand(6, 8, dtype=torch.float16).requires_grad_(True)
+    w, o = rand(2, 8, 16, dtype=torch.float16), torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda")
+    r = some_routing(6, 4, 2, dead=0.0)
+    for y in (F.grouped_linear(x, w, o), F.residual_norm(x)[1], F.expert_dispatch(x, r), F.expert_combine(x.repeat(2, 1), r), F.expert_route(x, 2).weights):
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
 
 
 # ------------------------------------------------------------------------------------------------ together
