@@ -780,6 +780,10 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
   P.off_groups = P.off_bar + bars + 8;
   const size_t smem = static_cast<size_t>(P.off_stage) + fixed + 1024;
 
+  // A thread that has made no CUDA call yet (autograd's) has no current context, which the driver call below needs.
+  int device = 0;
+  SB_CHECK_CUDA(cudaGetDevice(&device));
+  SB_CHECK_CUDA(cudaSetDevice(device));
   alignas(64) CUtensorMap map_a, map_b, map_out;
   int rc;
   const int64_t x_stride = D.n == 1 ? D.c_in : D.x_stride, dy_stride = D.n == 1 ? D.c_out : D.dy_stride;

@@ -673,6 +673,49 @@ def test_same_bits_every_time_and_on_other_streams():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_threads_without_a_context():
+    """The first CUDA call of a thread may be the product's (autograd runs backward passes in a thread of its own)."""
+    import threading
+    from spira_b200.nn import functional as F
+    x, w, o = whole(300, 64, dtype=torch.float16), whole(2, 64, 64, dtype=torch.float16), torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
+    want = F.grouped_linear(x, w, o)
+    got, errors = [], []
+
+    def work():
+        try:
+            got.append(F.grouped_linear(x, w, o))
+        except Exception as e:
+            errors.append(e)
+    for _ in range(2):
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+    assert not errors and len(got) == 2 and all(torch.equal(g, want) for g in got)
+
+
+def test_capture_beside_a_living_eager_graph_raises():
+    """Autograd's own refusal (the leaves' accumulators belong to another stream) arrives as an exception, and the operators
+    work afterwards."""
+    from spira_b200.nn import functional as F
+    x, o = whole(300, 64, dtype=torch.float16), torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
+    w = whole(2, 64, 64, dtype=torch.float16).requires_grad_(True)
+    d = whole(300, 64, dtype=torch.float16, top=1, seed=3)
+    alive = F.grouped_linear(x, w, o)
+    want, = torch.autograd.grad(alive, w, d, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(F.grouped_linear(x, w, o), w, d)
+        graph.replay()
+        assert torch.equal(got, want)
+    except RuntimeError:
+        pass
+    torch.cuda.synchronize()
+    again, = torch.autograd.grad(F.grouped_linear(x, w, o), w, d)
+    assert torch.equal(again, want)
+
+
 def test_two_streams_at_once():
     sets = [pass_inputs(6000, seed=s) for s in (0, 100)]
     with torch.no_grad():
