@@ -693,27 +693,40 @@ def test_threads_without_a_context():
     assert not errors and len(got) == 2 and all(torch.equal(g, want) for g in got)
 
 
-def test_capture_beside_a_living_eager_graph_raises():
-    """Autograd's own refusal (the leaves' accumulators belong to another stream) arrives as an exception, and the operators
-    work afterwards."""
-    from spira_b200.nn import functional as F
-    x, o = whole(300, 64, dtype=torch.float16), torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
-    w = whole(2, 64, 64, dtype=torch.float16).requires_grad_(True)
-    d = whole(300, 64, dtype=torch.float16, top=1, seed=3)
-    alive = F.grouped_linear(x, w, o)
-    want, = torch.autograd.grad(alive, w, d, retain_graph=True)
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    try:
-        with torch.cuda.graph(graph):
-            got, = torch.autograd.grad(F.grouped_linear(x, w, o), w, d)
-        graph.replay()
-        assert torch.equal(got, want)
-    except RuntimeError:
-        pass
-    torch.cuda.synchronize()
-    again, = torch.autograd.grad(F.grouped_linear(x, w, o), w, d)
-    assert torch.equal(again, want)
+LIVING_GRAPH = """
+import torch
+from spira_b200.nn import functional as F
+x, o = torch.ones(300, 64, device="cuda", dtype=torch.float16), torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
+w = torch.ones(2, 64, 64, device="cuda", dtype=torch.float16, requires_grad=True)
+d = torch.ones(300, 64, device="cuda", dtype=torch.float16)
+alive = F.grouped_linear(x, w, o)
+want, = torch.autograd.grad(alive, w, d, retain_graph=True)
+before = torch.cuda.current_stream()
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(F.grouped_linear(x, w, o), w, d)
+    graph.replay()
+    assert torch.equal(got, want)
+except RuntimeError as e:
+    assert "capture" in str(e)
+torch.cuda.set_stream(before)
+torch.cuda.synchronize()
+again, = torch.autograd.grad(F.grouped_linear(x, w, o), w, d)
+assert torch.equal(again, want)
+print("alive")
+"""
+
+
+def test_capture_beside_a_living_eager_graph_ends_in_an_exception_at_most():
+    """Autograd refuses such a capture itself (the leaves' accumulators belong to another stream).  The refusal arrives as an
+    exception and the operators work afterwards; in a process of its own, because a failed capture leaves torch's
+    stream and allocator in the middle of it."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", LIVING_GRAPH], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0 and "alive" in r.stdout, (r.returncode, r.stderr[-2000:])
 
 
 def test_two_streams_at_once():
