@@ -536,11 +536,11 @@ int spira_b200_expert_combine_backward(const void *rows, const void *dout, int d
 /* Ragged products: group e holds the rows [offsets[e], offsets[e + 1]) of x[n][c_in] and has the matrix weight[e][c_in][c_out].
  *   spira_b200_grouped_linear      y[r] = relu?(x[r] W[e] + bias[e]); rows outside every group are zero
  *                                  (mask != NULL: also a bit per element, set where the value before the ReLU is
- *                                  positive; spira_b200_grouped_linear_mask_bytes gives its size, 0 = this shape has none)
+ *                                  positive; spira_b200_grouped_linear_workspace says how large it is, 0: this call has none)
  *   spira_b200_grouped_linear_backward   with dz = dy, with `relu` only where the mask is set (or y > 0 without a mask):
  *                                  dx[r] = dz[r] W[e]^T (rows outside every group are zero), dweight[e] = x_e^T dz_e and
  *                                  dbias[e] = column sums of dz_e (zero for an empty group); NULL outputs are left out.
- *                                  The workspace is asked for with the same descriptor.
+ * Workspaces are asked for with the descriptor of the call (they hold copies of what is not on 16-byte boundaries).
  * fp16 or bf16 in and out, fp32 sums, one rounding.  Offsets are read on the device; an entry counts as the largest of
  * those before it and as n at most, so a bad list cannot reach outside the tensors.  x and dy have unit column stride and
  * rows `x_stride` / `dy_stride` elements apart; everything else is dense. */
@@ -551,8 +551,8 @@ typedef struct spira_b200_grouped_desc {
   const void *x, *weight, *bias, *dy;
   void *y, *mask, *dx, *dweight, *dbias;
 } spira_b200_grouped_desc;
-int spira_b200_grouped_linear_mask_bytes(const spira_b200_grouped_desc *desc, size_t *bytes);
-int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, int32_t *status, void *stream);
+int spira_b200_grouped_linear_workspace(const spira_b200_grouped_desc *desc, size_t *workspace_bytes, size_t *mask_bytes);
+int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status, void *stream);
 int spira_b200_grouped_linear_backward_workspace(const spira_b200_grouped_desc *desc, size_t *bytes);
 int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status,
                                        void *stream);

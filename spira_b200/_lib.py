@@ -174,8 +174,8 @@ SIGNATURES = {
     "spira_b200_expert_combine": [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p],
     "spira_b200_expert_combine_backward": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
                                            c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
-    "spira_b200_grouped_linear_mask_bytes": [c_void_p, C.POINTER(c_size_t)],
-    "spira_b200_grouped_linear": [c_void_p, c_void_p, c_void_p],
+    "spira_b200_grouped_linear_workspace": [c_void_p, C.POINTER(c_size_t), C.POINTER(c_size_t)],
+    "spira_b200_grouped_linear": [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p],
     "spira_b200_grouped_linear_backward_workspace": [c_void_p, C.POINTER(c_size_t)],
     "spira_b200_grouped_linear_backward": [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p],
     "spira_b200_residual_norm": [c_void_p, c_void_p],

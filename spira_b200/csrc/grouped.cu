@@ -7,9 +7,10 @@
 // Rows outside every group are zero in y and dx.  Group boundaries are read on the device; the host only knows upper
 // bounds of the tile counts.  Sums over a group's rows are split into pieces that are added in a fixed order.
 //
-// Channel counts in whole 16-byte units and aligned tensors run on the tensor-core kernel (grouped_tc.cu).
-// `grouped_any_kernel` takes every channel count, stride and alignment: 64 x 64 tiles, element-wise loads into shared
-// memory, warp-level MMAs with fp32 accumulation.
+// Products run on the tensor-core kernel (grouped_tc.cu), which wants rows on 16-byte boundaries.  Channel counts, strides or
+// addresses that break them are met in two ways: large products copy what is off into rows of a pitch in whole units of 8
+// (and their result back), small ones run on `grouped_any_kernel`, which takes everything: 64 x 64 tiles, element-wise loads
+// into shared memory, warp-level MMAs with fp32 accumulation.
 #include "common.cuh"
 #include "elem.cuh"
 #include "grouped.cuh"
@@ -218,21 +219,58 @@ __device__ __forceinline__ void group_pieces(const int32_t *offsets, int n, int 
   count = last;
 }
 
-// out[e][i] = sum over the pieces of group e, in order, of partial[piece][i]
+// out[e][row][c] = sum over the pieces of group e, in order, of partial[piece][row][c]; rows of the partial sums are `pitch` long
 template <typename T>
-__global__ void __launch_bounds__(256) grouped_sum_kernel(const float *partial, const int32_t *offsets, int n, int experts, int piece, int64_t size, T *out) {
+__global__ void __launch_bounds__(256) grouped_sum_kernel(const float *partial, const int32_t *offsets, int n, int experts, int piece, int64_t rows, int columns,
+                                                          int pitch, T *out) {
   pdl_trigger();
   pdl_wait();
   const int e = blockIdx.y;
   int64_t first;
   int count;
   group_pieces(offsets, n, e, piece, first, count);
+  const int64_t size = rows * pitch;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < size; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / pitch;
+    const int c = static_cast<int>(i - row * pitch);
+    if (c >= columns) continue;
     float t = 0.f;
 #pragma unroll 4
     for (int p = 0; p < count; ++p) t += partial[(first + p) * size + i];
-    out[e * size + i] = from_f32<T>(t);
+    out[(e * rows + row) * columns + c] = from_f32<T>(t);
   }
+}
+
+// Rows of one pitch into rows of another (16-bit elements): neighbouring threads take neighbouring elements, four per thread
+// in flight.  Rows in groups of less than 2^31 elements (blockIdx.y), divided by multiplication.
+struct RepitchParams {
+  const unsigned short *src;
+  unsigned short *dst;
+  int64_t src_pitch, dst_pitch, rows, rows_per_group;
+  int columns, div_shift;
+  uint64_t div_mul;
+};
+
+__global__ void __launch_bounds__(256) grouped_repitch_kernel(const __grid_constant__ RepitchParams P) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t row0 = blockIdx.y * P.rows_per_group;
+  const int64_t here = P.rows - row0 < P.rows_per_group ? P.rows - row0 : P.rows_per_group;
+  const uint32_t count = static_cast<uint32_t>(here * P.columns), first = blockIdx.x * 1024u + threadIdx.x;
+  unsigned short v[4];
+  int64_t to[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t i = first + 256u * q;
+    if (i < count) {
+      const uint32_t r = static_cast<uint32_t>((i * P.div_mul) >> P.div_shift), c = i - r * static_cast<uint32_t>(P.columns);
+      v[q] = P.src[(row0 + r) * P.src_pitch + c];
+      to[q] = (row0 + r) * P.dst_pitch + c;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (first + 256u * q < count) P.dst[to[q]] = v[q];
 }
 
 // dz = dy where the ReLU let the value through (dz != NULL), and column sums over pieces of a group's rows.  What the ReLU
@@ -240,7 +278,7 @@ __global__ void __launch_bounds__(256) grouped_sum_kernel(const float *partial, 
 // rows of a thread in flight; four CTAs per SM.
 template <typename T, int V, int MASK>
 __global__ void __launch_bounds__(256, 4) grouped_dz_kernel(const T *dy, int64_t dy_stride, const T *y, const unsigned char *mask, int mask_pitch, T *dz,
-                                                            float *partial, const int32_t *offsets, int n, int experts, int c_out, int piece) {
+                                                            int64_t dz_pitch, float *partial, const int32_t *offsets, int n, int experts, int c_out, int piece) {
   __shared__ float sums[256 * V];
   pdl_trigger();
   pdl_wait();
@@ -276,7 +314,7 @@ __global__ void __launch_bounds__(256, 4) grouped_dz_kernel(const T *dy, int64_t
           for (int i = 0; i < V; ++i)
             if (MASK == 1 ? !(bits[q] >> i & 1) : !(to_f32(f[q].v[i]) > 0.f)) d[q].v[i] = from_f32<T>(0.f);
         }
-        if (dz) *reinterpret_cast<Vec<T, V> *>(dz + row * c_out + c) = d[q];
+        if (dz) *reinterpret_cast<Vec<T, V> *>(dz + row * dz_pitch + c) = d[q];
         float v[V];
         vec_to_f32<T, V>(d[q], v);
 #pragma unroll
@@ -335,23 +373,16 @@ static int dw_piece(int64_t n, int experts, int64_t tiles, int ctas) {
   return piece >= n ? 0 : static_cast<int>(piece);
 }
 
-// Which kernel a product runs on; one answer for a call and for its workspace.
-static bool tc_forward(const spira_b200_grouped_desc &D) {
-  return grouped_tc_available() && D.c_out % 8 == 0 && grouped_tc_rows_ok(D.x, D.x_stride, D.c_in, D.n) && aligned16(D.weight) && aligned16(D.bias) && aligned16(D.y);
+// Whether a product that needs copies for the tensor cores is worth them: 2^28 multiply-adds take the general kernel about
+// 11 us, the copies and their launches 5 to 10; measured 20 000 rows 501 -> 703: 217 us without, 67 us with copies.
+// With few rows per group the copy of the weights would outweigh the product.
+static bool worth_copies(const spira_b200_grouped_desc &D) {
+  return D.n * D.c_in >= (int64_t(1) << 28) / D.c_out && D.n >= 16 * static_cast<int64_t>(D.experts);
 }
-static bool tc_dx(const spira_b200_grouped_desc &D) {
-  return grouped_tc_available() && D.c_in % 8 == 0 && grouped_tc_rows_ok(D.dy, D.dy_stride, D.c_out, D.n) && aligned16(D.weight) && aligned16(D.dx);
-}
-static bool tc_dw(const spira_b200_grouped_desc &D) {
-  return grouped_tc_available() && grouped_tc_rows_ok(D.x, D.x_stride, D.c_in, D.n) && grouped_tc_rows_ok(D.dy, D.dy_stride, D.c_out, D.n) && aligned16(D.dweight);
-}
+
 static unsigned long long wait_ns() { return static_cast<unsigned long long>(spira_b200_get_option("wait_limit_us")) * 1000ull; }
 
 static int64_t any_tiles(int c_in, int c_out) { return div_up(c_in, kATile) * div_up(c_out, kATile); }
-
-static int dw_rows(const spira_b200_grouped_desc &D) {
-  return tc_dw(D) ? dw_piece(D.n, D.experts, grouped_tc_dw_tiles(D.c_in, D.c_out), 1) : dw_piece(D.n, D.experts, any_tiles(D.c_in, D.c_out), 2);
-}
 
 static int grouped_check(const char *what, const spira_b200_grouped_desc *D) {
   SB_CHECK_ARG(D, "%s: null descriptor", what);
@@ -384,52 +415,141 @@ using namespace sb;
     using T = __nv_bfloat16; __VA_ARGS__                             \
   }()
 
-extern "C" int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, int32_t *status, void *stream) {
+// A scratch plan hands out 256-byte aligned places.
+struct Scratch {
+  size_t bytes = 0;
+  size_t take(int64_t want) {
+    const size_t at = bytes;
+    bytes += (static_cast<size_t>(want) + 255) / 256 * 256;
+    return at;
+  }
+};
+constexpr size_t kNoCopy = ~size_t(0);
+
+struct ForwardPlan {
+  bool tc;
+  size_t x, w, y;        // where their copies lie, or kNoCopy
+  size_t bytes;
+};
+
+static ForwardPlan forward_plan(const spira_b200_grouped_desc &D) {
+  ForwardPlan p{false, kNoCopy, kNoCopy, kNoCopy, 0};
+  const bool x_ok = grouped_tc_rows_ok(D.x, D.x_stride, D.c_in, D.n), even = D.c_out % 8 == 0;
+  const bool w_ok = even && aligned16(D.weight), y_ok = even && aligned16(D.y);
+  p.tc = grouped_tc_available() && ((x_ok && w_ok && y_ok) || worth_copies(D));
+  if (!p.tc) return p;
+  Scratch s;
+  if (!x_ok) p.x = s.take(D.n * pitch8(D.c_in) * 2);
+  if (!w_ok) p.w = s.take(static_cast<int64_t>(D.experts) * D.c_in * pitch8(D.c_out) * 2);
+  if (!y_ok) p.y = s.take(D.n * pitch8(D.c_out) * 2);
+  p.bytes = s.bytes;
+  return p;
+}
+
+static int repitch(const void *src, int64_t src_pitch, void *dst, int64_t dst_pitch, int64_t rows, int columns, cudaStream_t st) {
+  RepitchParams P{static_cast<const unsigned short *>(src), static_cast<unsigned short *>(dst), src_pitch, dst_pitch, rows, 0, columns, 0, 0};
+  P.rows_per_group = ((int64_t(1) << 31) - 2048) / columns;
+  if (P.rows_per_group > rows) P.rows_per_group = rows;
+  int bits = 0;
+  while ((int64_t(1) << bits) < columns) ++bits;
+  P.div_shift = 31 + bits;
+  P.div_mul = ((uint64_t(1) << P.div_shift) + columns - 1) / columns;
+  const dim3 grid(static_cast<unsigned>(div_up(P.rows_per_group * columns, 1024)), static_cast<unsigned>(div_up(rows, P.rows_per_group)));
+  SB_CHECK_CUDA(launch_dependent(grouped_repitch_kernel, grid, dim3(256), 0, st, P));
+  return SPIRA_B200_OK;
+}
+
+static int check_workspace(const char *what, const void *workspace, size_t have, size_t need) {
+  if (need && (!workspace || have < need)) return fail(SPIRA_B200_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than %zu", what, have, need);
+  SB_CHECK_ARG(need == 0 || aligned16(workspace), "%s: the workspace must be 16-byte aligned", what);
+  return SPIRA_B200_OK;
+}
+
+extern "C" int spira_b200_grouped_linear_workspace(const spira_b200_grouped_desc *desc, size_t *workspace_bytes, size_t *mask_bytes) {
+  int rc = grouped_check("grouped_linear", desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(workspace_bytes && mask_bytes, "grouped_linear: null pointer");
+  *workspace_bytes = *mask_bytes = 0;
+  if (desc->n == 0) return SPIRA_B200_OK;
+  const ForwardPlan plan = forward_plan(*desc);
+  *workspace_bytes = plan.bytes;
+  *mask_bytes = desc->relu && plan.tc ? static_cast<size_t>(desc->n) * mask_pitch(desc->c_out) : 0;
+  return SPIRA_B200_OK;
+}
+
+extern "C" int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status, void *stream) {
   int rc = grouped_check("grouped_linear", desc);
   if (rc != SPIRA_B200_OK || desc->n == 0) return rc;
   const spira_b200_grouped_desc &D = *desc;
   SB_CHECK_ARG(D.x && D.weight && D.y, "grouped_linear: null pointer");
-  SB_CHECK_ARG(!D.mask || (D.relu && tc_forward(D)), "grouped_linear: no mask is written for this call (spira_b200_grouped_linear_mask_bytes is 0)");
-  if (tc_forward(D)) return grouped_tc_run(kForward, D, 0, nullptr, status, wait_ns(), as_stream(stream));
-  GroupedParams P{D.x, D.weight, D.bias, D.offsets, D.y, nullptr, D.x_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, D.relu, 0};
-  return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kForward>(P, as_stream(stream))););
-}
-
-extern "C" int spira_b200_grouped_linear_mask_bytes(const spira_b200_grouped_desc *desc, size_t *bytes) {
-  int rc = grouped_check("grouped_linear_mask", desc);
+  const ForwardPlan plan = forward_plan(D);
+  SB_CHECK_ARG(!D.mask || (D.relu && plan.tc), "grouped_linear: no mask is written for this call (spira_b200_grouped_linear_workspace says 0)");
+  cudaStream_t st = as_stream(stream);
+  if (!plan.tc) {
+    GroupedParams P{D.x, D.weight, D.bias, D.offsets, D.y, nullptr, D.x_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, D.relu, 0};
+    return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kForward>(P, st)););
+  }
+  rc = check_workspace("grouped_linear", workspace, workspace_bytes, plan.bytes);
   if (rc != SPIRA_B200_OK) return rc;
-  SB_CHECK_ARG(bytes, "grouped_linear_mask: null pointer");
-  *bytes = desc->n > 0 && desc->relu && tc_forward(*desc) ? static_cast<size_t>(desc->n) * mask_pitch(desc->c_out) : 0;
-  return SPIRA_B200_OK;
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  spira_b200_grouped_desc Z = D;
+  int w_pitch = D.c_out, y_pitch = D.c_out;
+  if (plan.x != kNoCopy) {
+    Z.x = ws + plan.x;
+    Z.x_stride = pitch8(D.c_in);
+    rc = repitch(D.x, D.x_stride, ws + plan.x, Z.x_stride, D.n, D.c_in, st);
+    if (rc != SPIRA_B200_OK) return rc;
+  }
+  if (plan.w != kNoCopy) {
+    Z.weight = ws + plan.w;
+    w_pitch = pitch8(D.c_out);
+    rc = repitch(D.weight, D.c_out, ws + plan.w, w_pitch, static_cast<int64_t>(D.experts) * D.c_in, D.c_out, st);
+    if (rc != SPIRA_B200_OK) return rc;
+  }
+  if (plan.y != kNoCopy) {
+    Z.y = ws + plan.y;
+    y_pitch = pitch8(D.c_out);
+  }
+  rc = grouped_tc_run(kForward, Z, w_pitch, y_pitch, 0, nullptr, status, wait_ns(), st);
+  if (rc != SPIRA_B200_OK || plan.y == kNoCopy) return rc;
+  return repitch(Z.y, y_pitch, D.y, D.c_out, D.n, D.c_out, st);
 }
 
-// Scratch of the backward pass: dz where a ReLU followed, then the partial sums (of dbias, later of dweight: one region).
+// The backward pass: dz (where a ReLU followed, or where dy itself is not fit for the tensor cores) and the column sums in
+// one copy of dy, then dx and dW from it.  Copies as in the forward pass; the partial sums of dbias and of dweight follow
+// one another in one place.
 struct BackwardPlan {
-  bool need_dz;
+  bool tc;
+  size_t dz, x, w, dx, dw, partial;
+  int64_t dz_pitch;
   int dz_rows, dw_rows;
-  size_t partial_at, bytes;
+  size_t bytes;
 };
 
-static BackwardPlan backward_plan(const spira_b200_grouped_desc &D, const spira_b200_grouped_desc &Z) {
+static BackwardPlan backward_plan(const spira_b200_grouped_desc &D) {
   BackwardPlan p{};
-  p.need_dz = D.relu && (D.dx || D.dweight);
+  const bool x_ok = !D.dweight || grouped_tc_rows_ok(D.x, D.x_stride, D.c_in, D.n), dy_ok = D.relu || grouped_tc_rows_ok(D.dy, D.dy_stride, D.c_out, D.n);
+  const bool w_ok = !D.dx || (D.c_out % 8 == 0 && aligned16(D.weight)), dx_ok = !D.dx || (D.c_in % 8 == 0 && aligned16(D.dx));
+  const bool dw_ok = !D.dweight || (D.c_out % 8 == 0 && aligned16(D.dweight));
+  p.tc = grouped_tc_available() && ((x_ok && dy_ok && w_ok && dx_ok && dw_ok) || worth_copies(D));
+  p.dz = p.x = p.w = p.dx = p.dw = kNoCopy;
   p.dz_rows = dz_piece(D.n);
-  p.dw_rows = D.dweight ? dw_rows(Z) : 0;
-  p.partial_at = p.need_dz ? static_cast<size_t>(div_up(D.n * D.c_out * 2, 256) * 256) : 0;
-  const size_t db = D.dbias ? static_cast<size_t>(group_tiles_bound(D.n, D.experts, p.dz_rows)) * D.c_out * 4 : 0;
-  const size_t dw = p.dw_rows ? static_cast<size_t>(group_tiles_bound(D.n, D.experts, p.dw_rows)) * D.c_in * D.c_out * 4 : 0;
-  p.bytes = p.partial_at + (db > dw ? db : dw);
-  return p;
-}
-
-// The call with dz in the place of dy.
-static spira_b200_grouped_desc with_dz(const spira_b200_grouped_desc &D, const void *workspace) {
-  spira_b200_grouped_desc Z = D;
-  if (D.relu && (D.dx || D.dweight)) {
-    Z.dy = workspace;
-    Z.dy_stride = D.c_out;
+  p.dz_pitch = pitch8(D.c_out);
+  Scratch s;
+  if ((D.dx || D.dweight) && (D.relu || (p.tc && !dy_ok))) p.dz = s.take(D.n * p.dz_pitch * 2);
+  if (D.dweight)
+    p.dw_rows = p.tc ? dw_piece(D.n, D.experts, grouped_tc_dw_tiles(D.c_in, D.c_out), 1) : dw_piece(D.n, D.experts, any_tiles(D.c_in, D.c_out), 2);
+  if (p.tc) {
+    if (!x_ok) p.x = s.take(D.n * pitch8(D.c_in) * 2);
+    if (!w_ok) p.w = s.take(static_cast<int64_t>(D.experts) * D.c_in * pitch8(D.c_out) * 2);
+    if (!dx_ok) p.dx = s.take(D.n * pitch8(D.c_in) * 2);
+    if (!dw_ok && p.dw_rows == 0) p.dw = s.take(static_cast<int64_t>(D.experts) * D.c_in * pitch8(D.c_out) * 2);
   }
-  return Z;
+  const int64_t db = D.dbias ? group_tiles_bound(D.n, D.experts, p.dz_rows) * D.c_out * 4 : 0;
+  const int64_t dw = p.dw_rows ? group_tiles_bound(D.n, D.experts, p.dw_rows) * D.c_in * (p.tc ? pitch8(D.c_out) : D.c_out) * 4 : 0;
+  p.partial = s.take(db > dw ? db : dw);
+  p.bytes = s.bytes;
+  return p;
 }
 
 static int backward_check(const spira_b200_grouped_desc *D) {
@@ -445,7 +565,7 @@ extern "C" int spira_b200_grouped_linear_backward_workspace(const spira_b200_gro
   int rc = backward_check(desc);
   if (rc != SPIRA_B200_OK) return rc;
   SB_CHECK_ARG(bytes, "grouped_linear_backward: null pointer");
-  *bytes = desc->n ? backward_plan(*desc, with_dz(*desc, nullptr)).bytes : 0;
+  *bytes = desc->n ? backward_plan(*desc).bytes : 0;
   return SPIRA_B200_OK;
 }
 
@@ -455,28 +575,27 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
   if (rc != SPIRA_B200_OK) return rc;
   const spira_b200_grouped_desc &D = *desc;
   cudaStream_t st = as_stream(stream);
-  const int64_t size = static_cast<int64_t>(D.c_in) * D.c_out;
   if (D.n == 0) {
-    if (D.dweight) SB_CHECK_CUDA(cudaMemsetAsync(D.dweight, 0, static_cast<size_t>(D.experts) * size * 2, st));
+    if (D.dweight) SB_CHECK_CUDA(cudaMemsetAsync(D.dweight, 0, static_cast<size_t>(D.experts) * D.c_in * D.c_out * 2, st));
     if (D.dbias) SB_CHECK_CUDA(cudaMemsetAsync(D.dbias, 0, static_cast<size_t>(D.experts) * D.c_out * 2, st));
     return SPIRA_B200_OK;
   }
-  const spira_b200_grouped_desc Z = with_dz(D, workspace);
-  const BackwardPlan plan = backward_plan(D, with_dz(D, nullptr));      // (as the size was asked for: dz is aligned like a null pointer)
-  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
-    return fail(SPIRA_B200_ERR_WORKSPACE, "grouped_linear_backward: workspace of %zu bytes is smaller than %zu", workspace_bytes, plan.bytes);
-  SB_CHECK_ARG(aligned16(workspace), "grouped_linear_backward: the workspace must be 16-byte aligned");
-  float *partial = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + plan.partial_at);
+  const BackwardPlan plan = backward_plan(D);
+  rc = check_workspace("grouped_linear_backward", workspace, workspace_bytes, plan.bytes);
+  if (rc != SPIRA_B200_OK) return rc;
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  float *partial = reinterpret_cast<float *>(ws + plan.partial);
   const int n = static_cast<int>(D.n);
+  spira_b200_grouped_desc Z = D;
   return SB_DISPATCH_HALF(D.dtype, T, {
-    if (plan.need_dz || D.dbias) {
-      T *dz = plan.need_dz ? static_cast<T *>(workspace) : nullptr;
+    if (plan.dz != kNoCopy || D.dbias) {
+      T *dz = plan.dz != kNoCopy ? reinterpret_cast<T *>(ws + plan.dz) : nullptr;
       const unsigned units = static_cast<unsigned>(group_tiles_bound(n, D.experts, plan.dz_rows));
       const bool wide = D.c_out % 8 == 0 && aligned16(D.dy) && (D.dy_stride % 8 == 0 || n == 1) && (D.mask || aligned16(D.y));
       auto go = [&](auto kernel, int columns) -> int {
         SB_CHECK_CUDA(launch_dependent(kernel, dim3(units, static_cast<unsigned>(div_up(columns, 256))), dim3(256), 0, st, static_cast<const T *>(D.dy),
                                        D.dy_stride, static_cast<const T *>(D.y), static_cast<const unsigned char *>(D.mask), mask_pitch(D.c_out), dz,
-                                       D.dbias ? partial : nullptr, D.offsets, n, D.experts, D.c_out, plan.dz_rows));
+                                       plan.dz_pitch, D.dbias ? partial : nullptr, D.offsets, n, D.experts, D.c_out, plan.dz_rows));
         return SPIRA_B200_OK;
       };
       const int kind = !D.relu ? 0 : D.mask ? 1 : 2;
@@ -486,10 +605,31 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
       if (D.dbias)
         SB_CHECK_CUDA(launch_dependent(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(1024), 0, st,
                                        static_cast<const float *>(partial), D.offsets, n, D.experts, plan.dz_rows, D.c_out, static_cast<T *>(D.dbias)));
+      if (dz) {
+        Z.dy = dz;
+        Z.dy_stride = plan.dz_pitch;
+      }
     }
+    int w_pitch = D.c_out;
+    const int dx_pitch = plan.dx != kNoCopy ? pitch8(D.c_in) : D.c_in, dw_pitch = plan.tc ? pitch8(D.c_out) : D.c_out;
+    if (plan.x != kNoCopy) {
+      Z.x = ws + plan.x;
+      Z.x_stride = pitch8(D.c_in);
+      rc = repitch(D.x, D.x_stride, ws + plan.x, Z.x_stride, D.n, D.c_in, st);
+      if (rc != SPIRA_B200_OK) return rc;
+    }
+    if (plan.w != kNoCopy) {
+      Z.weight = ws + plan.w;
+      w_pitch = pitch8(D.c_out);
+      rc = repitch(D.weight, D.c_out, ws + plan.w, w_pitch, static_cast<int64_t>(D.experts) * D.c_in, D.c_out, st);
+      if (rc != SPIRA_B200_OK) return rc;
+    }
+    if (plan.dx != kNoCopy) Z.dx = ws + plan.dx;
+    if (plan.dw != kNoCopy) Z.dweight = ws + plan.dw;
     if (D.dx) {
-      if (tc_dx(Z)) {
-        rc = grouped_tc_run(kDx, Z, 0, nullptr, status, wait_ns(), st);
+      if (plan.tc) {
+        rc = grouped_tc_run(kDx, Z, w_pitch, dx_pitch, 0, nullptr, status, wait_ns(), st);
+        if (rc == SPIRA_B200_OK && plan.dx != kNoCopy) rc = repitch(Z.dx, dx_pitch, D.dx, D.c_in, D.n, D.c_in, st);
       } else {
         GroupedParams P{Z.dy, Z.weight, nullptr, Z.offsets, Z.dx, nullptr, Z.dy_stride, 0, n, Z.experts, Z.c_in, Z.c_out, 0, 0};
         rc = launch_any<T, kDx>(P, st);
@@ -497,16 +637,18 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
       if (rc != SPIRA_B200_OK) return rc;
     }
     if (!D.dweight) return SPIRA_B200_OK;
-    if (tc_dw(Z)) {
-      rc = grouped_tc_run(kDw, Z, plan.dw_rows, partial, status, wait_ns(), st);
+    if (plan.tc) {
+      rc = grouped_tc_run(kDw, Z, w_pitch, dw_pitch, plan.dw_rows, partial, status, wait_ns(), st);
+      if (rc == SPIRA_B200_OK && plan.dw != kNoCopy) rc = repitch(Z.dweight, dw_pitch, D.dweight, D.c_out, static_cast<int64_t>(D.experts) * D.c_in, D.c_out, st);
     } else {
       GroupedParams P{Z.x, Z.dy, nullptr, Z.offsets, Z.dweight, partial, Z.x_stride, Z.dy_stride, n, Z.experts, Z.c_in, Z.c_out, 0, plan.dw_rows};
       rc = launch_any<T, kDw>(P, st);
     }
     if (rc != SPIRA_B200_OK || plan.dw_rows == 0) return rc;
-    const unsigned blocks = static_cast<unsigned>(div_up(size, 256) < 1024 ? div_up(size, 256) : 1024);
-    SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(blocks, D.experts), dim3(256), 0, st, static_cast<const float *>(partial), D.offsets, n,
-                                   D.experts, plan.dw_rows, size, static_cast<T *>(D.dweight)));
+    const int64_t want = div_up(static_cast<int64_t>(D.c_in) * dw_pitch, 256);
+    SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(static_cast<unsigned>(want < 1024 ? want : 1024), D.experts), dim3(256), 0, st,
+                                   static_cast<const float *>(partial), D.offsets, n, D.experts, plan.dw_rows, static_cast<int64_t>(D.c_in), D.c_out, dw_pitch,
+                                   static_cast<T *>(D.dweight)));
     return SPIRA_B200_OK;
   });
 }

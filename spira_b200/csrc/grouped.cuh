@@ -82,11 +82,15 @@ inline int64_t group_tiles_bound(int64_t n, int experts, int64_t rows) { return 
 // Bytes per row of the ReLU mask: a bit per column, rows of whole 4-byte words.
 inline int mask_pitch(int c_out) { return (c_out + 31) / 32 * 4; }
 
-// The tensor-core path (grouped_tc.cu).  It takes channel counts in whole 16-byte units and 16-byte aligned tensors and rows.
+inline int pitch8(int channels) { return (channels + 7) / 8 * 8; }
+
+// The tensor-core path (grouped_tc.cu).  Channel counts are free; tensors and rows start on 16-byte boundaries, so weights and
+// results have pitches (elements per row) in whole units of 8.
 enum { kForward = 0, kDx = 1, kDw = 2 };
 bool grouped_tc_available();
 bool grouped_tc_rows_ok(const void *p, int64_t stride, int channels, int64_t n);
 int grouped_tc_dw_tiles(int c_in, int c_out);
-int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float *partial, int32_t *status, unsigned long long wait_ns, cudaStream_t st);
+int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int w_pitch, int out_pitch, int piece, float *partial, int32_t *status,
+                   unsigned long long wait_ns, cudaStream_t st);
 
 }  // namespace sb

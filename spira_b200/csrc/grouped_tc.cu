@@ -50,6 +50,7 @@ struct GroupedTcParams {
   const void *bias;
   int32_t *status;
   int n, experts, m_channels, n_channels, k_channels;   // m_channels: c_in in dW; k_channels: 0 in dW (rows)
+  int out_pitch;             // elements per row of the result (and of the partial sums): n_channels in whole units of 8 at least
   int relu, piece;           // piece: rows per unit of dW, 0 = whole groups
   int tile_rows;             // M of a tile: 128, or 256 for a pair of CTAs
   int bn, n_tiles, m_tiles;  // columns per tile, column tiles, row tiles of dW
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
       const int b = tile_i & 1;
       const int m = (MODE == kDw ? tile.m0 : tile.row0) + rank * kGRows + q * 32 + lane, m_end = MODE == kDw ? P.m_channels : tile.row_end;
       const int col = tile.n0 + part * width;
-      const int valid = m < m_end ? P.n_channels - col : 0;      // columns of this row that exist (a multiple of 8)
+      const int valid = m < m_end ? P.n_channels - col : 0;      // columns of this row that exist (a unit of 8 may reach into the pitch)
       const float *bias = nullptr;
       if (MODE == kForward && P.bias) {
         const int at = tile.expert * P.n_tiles + tile.n0 / P.bn;
@@ -561,8 +562,8 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
       tc_fence_after();
       const uint32_t taddr = tmem_base + b * P.acc_stride + (static_cast<uint32_t>(q * 32) << 16) + part * width;
       const int64_t out_row = MODE == kDw ? static_cast<int64_t>(tile.expert) * P.m_channels + m : m;
-      T *dst = static_cast<T *>(P.out) + out_row * P.n_channels + col;
-      float *dst_partial = MODE == kDw ? P.partial + (static_cast<int64_t>(tile.unit) * P.m_channels + m) * P.n_channels + col : nullptr;
+      T *dst = static_cast<T *>(P.out) + out_row * P.out_pitch + col;
+      float *dst_partial = MODE == kDw ? P.partial + (static_cast<int64_t>(tile.unit) * P.m_channels + m) * P.out_pitch + col : nullptr;
       uint32_t bits[2] = {0, 0};
       const int m_warp = m - lane;
       const bool by_tma = MODE != kDw && P.box_cols != 0 && m_warp + 32 <= m_end;     // (rows of the next group are not ours to write)
@@ -642,7 +643,7 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
   } else if (warp == 3 && MODE != kDw) {
     // rows of no group are zero
     T *out = static_cast<T *>(P.out);
-    const int64_t width = P.n_channels / 8, before = rows[0] * width, behind = static_cast<int64_t>(P.n - rows[P.experts]) * width;
+    const int64_t width = P.out_pitch / 8, before = rows[0] * width, behind = static_cast<int64_t>(P.n - rows[P.experts]) * width;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + lane; i < before + behind; i += static_cast<int64_t>(gridDim.x) * 32)
       reinterpret_cast<uint4 *>(out)[i < before ? i : rows[P.experts] * width + i - before] = make_uint4(0, 0, 0, 0);
   }
@@ -695,7 +696,7 @@ static int encode_map(CUtensorMap *map, int dtype, const void *p, int rank, int6
 }
 
 bool grouped_tc_rows_ok(const void *p, int64_t stride, int channels, int64_t n) {
-  return channels % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (n == 1 || (stride % 8 == 0 && stride >= channels));
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (n == 1 || (stride % 8 == 0 && stride >= channels));
 }
 bool grouped_tc_available() { return grouped_encode_fn() != nullptr; }
 
@@ -720,7 +721,7 @@ static bool use_pair(int mode, const spira_b200_grouped_desc &D) {
   return n >= 128 && k >= 384 && D.n / D.experts >= 512 && D.n / 256 * div_up(n, kGMaxN) >= sm_count() / 2;
 }
 
-int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float *partial, int32_t *status, unsigned long long wait_ns, cudaStream_t st) {
+int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int w_pitch, int out_pitch, int piece, float *partial, int32_t *status, unsigned long long wait_ns, cudaStream_t st) {
   GroupedTcParams P{};
   P.offsets = D.offsets;
   P.partial = partial;
@@ -729,6 +730,7 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
   P.experts = D.experts;
   P.piece = piece;
   P.wait_ns = wait_ns;
+  P.out_pitch = out_pitch;
   const bool pair = use_pair(mode, D);
   P.tile_rows = pair ? 2 * kGRows : kGRows;
   int64_t units;
@@ -786,18 +788,18 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int piece, float 
   SB_CHECK_CUDA(cudaSetDevice(device));
   alignas(64) CUtensorMap map_a, map_b, map_out;
   int rc;
-  const int64_t x_stride = D.n == 1 ? D.c_in : D.x_stride, dy_stride = D.n == 1 ? D.c_out : D.dy_stride;
+  const int64_t x_stride = D.n == 1 ? pitch8(D.c_in) : D.x_stride, dy_stride = D.n == 1 ? pitch8(D.c_out) : D.dy_stride;
   if (mode == kForward) {
     rc = encode_map(&map_a, D.dtype, D.x, 2, D.c_in, D.n, x_stride, 1, kGRows);
-    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, D.c_out, D.experts, kGK);
+    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, w_pitch, D.experts, kGK);
   } else if (mode == kDx) {
     rc = encode_map(&map_a, D.dtype, D.dy, 2, D.c_out, D.n, dy_stride, 1, kGRows);
-    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, D.c_out, D.experts, b_columns);
+    if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.weight, 3, D.c_out, D.c_in, w_pitch, D.experts, b_columns);
   } else {
     rc = encode_map(&map_a, D.dtype, D.x, 2, D.c_in, D.n, x_stride, 1, kGK);
     if (rc == SPIRA_B200_OK) rc = encode_map(&map_b, D.dtype, D.dy, 2, D.c_out, D.n, dy_stride, 1, kGK);
   }
-  if (rc == SPIRA_B200_OK && P.box_cols) rc = encode_map(&map_out, D.dtype, P.out, 2, P.n_channels, D.n, P.n_channels, 1, 32, P.box_cols);
+  if (rc == SPIRA_B200_OK && P.box_cols) rc = encode_map(&map_out, D.dtype, P.out, 2, P.n_channels, D.n, P.out_pitch, 1, 32, P.box_cols);
   else map_out = map_a;
   if (rc != SPIRA_B200_OK) return rc;
   const int64_t tiles = units * P.n_tiles;

@@ -648,11 +648,17 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__
   }
 }
 
+// Allows a kernel its shared memory, on the current device (every device of the process is told on its own).
+template <typename K>
+static int allow_smem(K kernel, int smem) {
+  if (smem > 48 * 1024) SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  return SPIRA_B200_OK;
+}
+
 // CTAs of a kernel that fit on an SM with its shared memory (asked once per kernel).
 template <typename K>
 static int resident_ctas(K kernel, int threads, int smem) {
   int n = 0;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 1;
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0 ? n : 1;
 }
 
@@ -666,6 +672,8 @@ static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaS
     constexpr int kSmem = Ring<kThreads, 3 * ITEMS * R, kWide>::kBytes;
     const auto kernel = norm_forward_kernel<T, V, L, ITEMS, R, LAYER>;
     const int64_t rounds = div_up(P.n, kRows * R);
+    const int rc = allow_smem(kernel, kSmem);
+    if (rc != SPIRA_B200_OK) return rc;
     static const int resident = resident_ctas(kernel, kThreads, kSmem);
     const int64_t cap = static_cast<int64_t>(sm_count()) * resident;
     SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), kSmem, st, P));
@@ -676,6 +684,8 @@ static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaS
   constexpr int kSmem = kRing > kColumns ? kRing : kColumns;
   const auto kernel = norm_backward_kernel<T, V, L, ITEMS, LAYER>;
   const int64_t rounds = div_up(P.n, kRows);
+  const int rc = allow_smem(kernel, kSmem);
+  if (rc != SPIRA_B200_OK) return rc;
   static const int resident = resident_ctas(kernel, kThreads, kSmem);
   const int64_t cap = static_cast<int64_t>(sm_count()) * (resident < kNormBackwardCtas ? resident : kNormBackwardCtas);
   const int grid = static_cast<int>(rounds < cap ? rounds : cap);

@@ -277,17 +277,25 @@ def _grouped_desc(n, weights, offsets, relu, x=None, bias=None, dy=None, y=None,
 
 def _grouped(x, weights, offsets, bias, relu, want_mask=False):
     """The product and, for a backward pass, what its ReLU let through: the bit mask the kernel writes, or None where the
-    shape has none (then the sign of the result says it)."""
+    call has none (then the sign of the result says it)."""
     index, n = x.get_device(), x.shape[0]
     y = x.new_empty((n, weights.shape[2]))
-    mask = None
-    if want_mask and relu:
-        need = C.c_size_t()
-        _query(index, "spira_b200_grouped_linear_mask_bytes", _grouped_desc(n, weights, offsets, 1, x, bias, y=y), C.byref(need))
-        if need.value:
-            mask = x.new_empty(need.value, dtype=torch.uint8)
-    _launch(index, "spira_b200_grouped_linear", _grouped_desc(n, weights, offsets, 1 if relu else 0, x, bias, y=y, mask=mask), _status(index))
-    return (y, mask) if want_mask else y
+    mask, workspace, room = None, 0, 0
+    want_mask = want_mask and relu
+    relu = 1 if relu else 0
+    # channels, strides or addresses off the 16-byte boundaries may need scratch
+    off = ((x.shape[1] | y.shape[1] | x.stride(0)) & 7) | ((x.data_ptr() | weights.data_ptr()) & 15)
+    if want_mask or off:
+        need, mask_bytes = C.c_size_t(), C.c_size_t()
+        _query(index, "spira_b200_grouped_linear_workspace", _grouped_desc(n, weights, offsets, relu, x, bias, y=y), C.byref(need), C.byref(mask_bytes))
+        if want_mask and mask_bytes.value:
+            mask = x.new_empty(mask_bytes.value, dtype=torch.uint8)
+        room = need.value
+        if room:
+            scratch = x.new_empty(room, dtype=torch.uint8)
+            workspace = scratch.data_ptr()
+    _launch(index, "spira_b200_grouped_linear", _grouped_desc(n, weights, offsets, relu, x, bias, y=y, mask=mask), workspace, room, _status(index))
+    return y, mask
 
 
 def _with_workspace(index, like, name, desc, *rest):
@@ -347,4 +355,4 @@ def grouped_linear(feats: torch.Tensor, weights: torch.Tensor, offsets: torch.Te
         bias = bias.contiguous()
     if _needs_grad(feats, weights, bias):
         return _Grouped.apply(feats, weights, offsets, bias, bool(relu))
-    return _grouped(feats, weights, offsets, bias, relu)
+    return _grouped(feats, weights, offsets, bias, relu)[0]

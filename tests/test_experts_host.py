@@ -38,16 +38,16 @@ def test_library_refuses_bad_arguments(lib):
     assert lib.spira_b200_expert_combine(None, 0, 4, 8, 8, None, 0, 0, None, 2, None, None) != 0 and b"null" in err()
     assert lib.spira_b200_expert_combine_backward(None, None, 0, 0, 8, 8, 8, None, 0, 0, None, 2, None, 2, None, None, None) == 0   # no rows
     g = _lib.GroupedDesc(dtype=_lib.F32, experts=2, c_in=8, c_out=8, n=4)
-    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"neither fp16 nor bf16" in err()
-    assert lib.spira_b200_grouped_linear(None, None, None) != 0
+    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, 0, None, None) != 0 and b"neither fp16 nor bf16" in err()
+    assert lib.spira_b200_grouped_linear(None, None, 0, None, None) != 0
     assert lib.spira_b200_grouped_linear_backward(ctypes.byref(g), None, 0, None, None) != 0 and b"neither fp16 nor bf16" in err()
     assert lib.spira_b200_grouped_linear_backward_workspace(None, ctypes.byref(n)) != 0
     g.dtype = _lib.F16
-    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"null pointer" in err()
+    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, 0, None, None) != 0 and b"null pointer" in err()
     g.experts = 1025
-    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"experts=1025" in err()
+    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, 0, None, None) != 0 and b"experts=1025" in err()
     g.experts, g.c_in = 2, 0
-    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, None) != 0 and b"channels" in err()
+    assert lib.spira_b200_grouped_linear(ctypes.byref(g), None, 0, None, None) != 0 and b"channels" in err()
     g.c_in, g.offsets = 8, 4096
     assert lib.spira_b200_grouped_linear_backward(ctypes.byref(g), None, 0, None, None) != 0 and b"no gradient" in err()
     g.dweight = 4096

@@ -268,7 +268,8 @@ def plain_products(x, w, offsets, b, relu, dy, y_own):
 
 SHAPES = [(1, 1, 1, 1), (2, 8, 256, 1024), (5, 3, 19, 100), (130, 4, 16, 16), (129, 1, 64, 64), (300, 7, 20, 33), (257, 5, 40, 24), (1000, 3, 96, 384),
           (777, 6, 72, 264), (512, 2, 136, 520), (2000, 2, 512, 48), (640, 9, 8, 8), (4100, 4, 32, 32), (33, 40, 48, 80), (1500, 3, 17, 64), (1500, 3, 64, 17),
-          (20000, 3, 256, 512), (19001, 7, 264, 392), (30000, 2, 200, 136), (9000, 5, 384, 192)]
+          (20000, 3, 256, 512), (19001, 7, 264, 392), (30000, 2, 200, 136), (9000, 5, 384, 192),
+          (6000, 3, 201, 227), (9000, 2, 200, 151), (9000, 2, 151, 200), (20000, 1, 121, 129)]
 
 
 @pytest.mark.parametrize("dtype", HALF)
@@ -336,6 +337,31 @@ def test_products_strided_misaligned_and_foreign_rows():
     assert torch.equal(grads[0][0][o[big]:o[big + 1]], grads[1][0][o[big]:o[big + 1]])
     assert torch.equal(grads[0][1][big], grads[1][1][big])
     assert bool((grads[1][0][:4] == 0).all()) and bool((grads[1][0][n - 9:] == 0).all())
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_large_products_on_misaligned_rows(relu):
+    """Rows off the 16-byte boundaries of products large enough to be copied for the tensor cores, gradients included."""
+    from spira_b200.nn import functional as F
+    n, e, ci, co = 9000, 3, 200, 152
+    offsets = some_offsets(n, e, first=2, behind=7)
+    base, dbase = whole(n, ci + 3, dtype=torch.bfloat16), whole(n, co + 5, dtype=torch.bfloat16, top=1, seed=4)
+    w = whole(e, ci, co, dtype=torch.bfloat16, seed=2).requires_grad_(True)
+    out = []
+    for x, dy in ((base[:, 1:1 + ci], dbase[:, 3:3 + co]), (base[:, 1:1 + ci].contiguous(), dbase[:, 3:3 + co].contiguous())):
+        x = x.detach().requires_grad_(True)
+        y = F.grouped_linear(x, w, offsets, relu=relu)
+        out.append((y,) + torch.autograd.grad(y, [x, w], dy))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+def test_products_nan_passes_the_relu():
+    from spira_b200.nn import functional as F
+    for ci, co in ((64, 64), (20, 30)):
+        x, w = torch.ones(40, ci, dtype=torch.float16, device="cuda"), torch.ones(2, ci, co, dtype=torch.float16, device="cuda")
+        x[3, 5] = math.nan
+        y = F.grouped_linear(x, -w, torch.tensor([0, 10, 40], dtype=torch.int32, device="cuda"), relu=True)
+        assert bool(y[3].isnan().all()) and bool((y[torch.arange(40, device="cuda") != 3] == 0).all())
 
 
 def test_products_empty():
@@ -639,6 +665,36 @@ def test_block_behind_a_sparse_convolution_compiles():
         replayed = compiled(x)
         for a, b in zip(eager, replayed):
             assert torch.equal(a._features, b._features)
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last rows are what the same rows give on their own."""
+    from spira_b200.nn import functional as F
+    n, c = 1_060_000, 2048                                   # 2.17e9 elements, 4.3 GB
+    tail = 600
+    x = whole(1, c, dtype=torch.float16).expand(n, c).contiguous()
+    x[-tail:] = whole(tail, c, dtype=torch.float16, seed=1)
+    assert x.numel() > 1 << 31
+    stream, normed = F.residual_norm(x, x, gate=x)
+    want = F.residual_norm(x[-tail:].clone(), x[-tail:].clone(), gate=x[-tail:].clone())
+    assert torch.equal(stream[-tail:], want[0]) and torch.equal(normed[-tail:], want[1])
+    del stream, normed
+    logits = torch.zeros(n, 2, device="cuda")
+    logits[1::2, 1] = 1.0
+    r = F.expert_route(logits, 1)
+    rows = F.expert_dispatch(x, r)
+    back = F.expert_combine(rows, r)
+    assert torch.equal(back[-tail:], x[-tail:]) and torch.equal(back[:tail], x[:tail])
+    del back
+    w = whole(2, c, 24, dtype=torch.float16, top=1, seed=2)
+    y = F.grouped_linear(rows, w, r.offsets)
+    last = rows[-tail:].double() @ w[1].double()             # (sums below 2^24: exact in fp32)
+    assert torch.equal(y[-tail:], last.to(torch.float16))
+    del rows
+    wide = F.grouped_linear(y[:, :8].contiguous(), whole(2, 8, c, dtype=torch.float16, top=1, seed=3), r.offsets)
+    assert wide.numel() > 1 << 31
+    last = y[-tail:, :8].double() @ whole(2, 8, c, dtype=torch.float16, top=1, seed=3)[1].double()
+    assert torch.equal(wide[-tail:], last.to(torch.float16))
 
 
 # ------------------------------------------------------------------------------------------------ streams, graphs, repetition
