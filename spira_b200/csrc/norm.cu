@@ -257,19 +257,24 @@ constexpr int kNormThreads = L > 256 ? L : 256;
 
 // The rows on their way: every thread copies its own 16-byte pieces of the next rows into shared memory (cp.async, past the
 // L1, where the parameters stay) and reads them back itself, so no barrier is needed and no register waits for a load.
-// A ring of kDepth rounds of kPieces pieces per thread; 0 where the pieces are not 16 bytes or would take too much room.
-template <int THREADS, int PIECES, bool WIDE>
+// A ring of kDepth rounds of `tensors` x PER pieces per thread; no ring (kDepth 0) where pieces are not 16 bytes or MOST
+// tensors would take too much room.
+template <int THREADS, int PER, int MOST, bool WIDE>
 struct Ring {
-  static constexpr int kStage = THREADS * PIECES * 16;
-  static constexpr int kDepth = !WIDE ? 0 : kStage <= 24 * 1024 ? 3 : kStage <= 80 * 1024 ? 2 : 0;
-  static constexpr int kBytes = kDepth * kStage;
+  static constexpr int kMostStage = THREADS * PER * MOST * 16;
+  static constexpr int kDepth = !WIDE ? 0 : kMostStage <= 40 * 1024 ? 3 : kMostStage <= 80 * 1024 ? 2 : 0;
+  static constexpr int bytes(int tensors) { return kDepth * THREADS * PER * 16 * tensors; }
   unsigned char *base;      // this thread's first piece
-  __device__ __forceinline__ explicit Ring(unsigned char *smem) : base(smem + threadIdx.x * 16) {}
-  __device__ __forceinline__ unsigned char *piece(int stage, int i) const { return base + (stage * PIECES + i) * THREADS * 16; }
+  int stage_bytes;
+  __device__ __forceinline__ Ring(unsigned char *smem, int tensors) : base(smem + threadIdx.x * 16), stage_bytes(THREADS * PER * 16 * tensors) {}
+  __device__ __forceinline__ unsigned char *piece(int stage, int i) const { return base + stage * stage_bytes + i * (THREADS * 16); }
   __device__ __forceinline__ void copy(int stage, int i, const void *src) const { ptx::cp_async_16(ptx::smem_u32(piece(stage, i)), src, 16); }
   static __device__ __forceinline__ void commit() { ptx::cp_async_commit(); }
   static __device__ __forceinline__ void wait() { ptx::cp_async_wait<kDepth == 0 ? 0 : kDepth - 1>(); }
 };
+// Tensors whose rows go through the ring, in the kernels' order.
+__host__ __device__ __forceinline__ int forward_tensors(const NormParams &P) { return P.gate_kind == kGateFull ? 3 : P.block ? 2 : 1; }
+__host__ __device__ __forceinline__ int backward_tensors(const NormParams &P) { return P.gate_kind == kGateFull ? 5 : P.dstream ? 4 : P.block ? 3 : 2; }
 
 // L threads per row, each with ITEMS pieces of V neighbouring channels, L pieces apart, and R rows at once.  What limits
 // these kernels is not memory alone but instructions and the latency of a row's chain (load, row sum, row sum, store):
@@ -292,8 +297,8 @@ __global__ void __launch_bounds__(kNormThreads<L>) norm_forward_kernel(const __g
     col[i] = in[i] ? (i * L + g) * V : 0;
   }
   extern __shared__ __align__(16) unsigned char norm_ring[];
-  typedef Ring<kNormThreads<L>, 3 * ITEMS * R, V * sizeof(T) == 16> Rows;
-  const Rows ring(norm_ring);
+  typedef Ring<kNormThreads<L>, ITEMS * R, 3, V * sizeof(T) == 16> Rows;
+  const Rows ring(norm_ring, forward_tensors(P));
   constexpr int kDepth = Rows::kDepth;
   auto source = [&](int which, int64_t row, int c) -> const T * {
     if (which == 0) return static_cast<const T *>(P.x) + row * P.x_stride + c;
@@ -406,8 +411,8 @@ __global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) 
     in[i] = (i * L + g) * V < P.channels;
     col[i] = in[i] ? (i * L + g) * V : 0;
   }
-  typedef Ring<kThreads, 5 * ITEMS, V * sizeof(T) == 16> Rows;
-  const Rows ring(norm_ring);
+  typedef Ring<kThreads, ITEMS, 5, V * sizeof(T) == 16> Rows;
+  const Rows ring(norm_ring, backward_tensors(P));
   constexpr int kDepth = Rows::kDepth;
   // 0: x, 1: gradient of the normed rows, 2: block, 3: gradient of the stream, 4: gate
   auto source = [&](int which, int64_t row, int c) -> const T * {
@@ -648,14 +653,14 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__
   }
 }
 
-// Allows a kernel its shared memory, on the current device (every device of the process is told on its own).
+// Allows a kernel its shared memory (48 KB with its static part need no permission), on the current device (every device of the process is told on its own).
 template <typename K>
 static int allow_smem(K kernel, int smem) {
-  if (smem > 48 * 1024) SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 40 * 1024) SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   return SPIRA_B200_OK;
 }
 
-// CTAs of a kernel that fit on an SM with its shared memory (asked once per kernel).
+// CTAs of a kernel that fit on an SM with its shared memory (asked once per kernel and number of tensors; the answer is the same whoever writes it).
 template <typename K>
 static int resident_ctas(K kernel, int threads, int smem) {
   int n = 0;
@@ -669,28 +674,30 @@ static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaS
   constexpr bool kWide = V * sizeof(T) == 16;
   if (!backward) {
     constexpr int R = L <= 32 && ITEMS == 1 ? 2 : 1;
-    constexpr int kSmem = Ring<kThreads, 3 * ITEMS * R, kWide>::kBytes;
+    const int tensors = forward_tensors(P), smem = Ring<kThreads, ITEMS * R, 3, kWide>::bytes(tensors);
     const auto kernel = norm_forward_kernel<T, V, L, ITEMS, R, LAYER>;
     const int64_t rounds = div_up(P.n, kRows * R);
-    const int rc = allow_smem(kernel, kSmem);
+    const int rc = allow_smem(kernel, smem);
     if (rc != SPIRA_B200_OK) return rc;
-    static const int resident = resident_ctas(kernel, kThreads, kSmem);
-    const int64_t cap = static_cast<int64_t>(sm_count()) * resident;
-    SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), kSmem, st, P));
+    static int resident[4] = {0, 0, 0, 0};
+    if (resident[tensors] == 0) resident[tensors] = resident_ctas(kernel, kThreads, smem);
+    const int64_t cap = static_cast<int64_t>(sm_count()) * resident[tensors];
+    SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), smem, st, P));
     return SPIRA_B200_OK;
   }
-  // (columns sums of a CTA reuse the ring: 256 / L rows of L * ITEMS * V columns)
-  constexpr int kRing = Ring<kThreads, 5 * ITEMS, kWide>::kBytes, kColumns = kRows > 1 ? kThreads * ITEMS * V * 4 : 0;
-  constexpr int kSmem = kRing > kColumns ? kRing : kColumns;
+  // (column sums of a CTA reuse the ring: 256 / L rows of L * ITEMS * V columns)
+  constexpr int kColumns = kRows > 1 ? kThreads * ITEMS * V * 4 : 0;
+  const int tensors = backward_tensors(P), ring = Ring<kThreads, ITEMS, 5, kWide>::bytes(tensors), smem = ring > kColumns ? ring : kColumns;
   const auto kernel = norm_backward_kernel<T, V, L, ITEMS, LAYER>;
   const int64_t rounds = div_up(P.n, kRows);
-  const int rc = allow_smem(kernel, kSmem);
+  const int rc = allow_smem(kernel, smem);
   if (rc != SPIRA_B200_OK) return rc;
-  static const int resident = resident_ctas(kernel, kThreads, kSmem);
-  const int64_t cap = static_cast<int64_t>(sm_count()) * (resident < kNormBackwardCtas ? resident : kNormBackwardCtas);
+  static int resident[6] = {0, 0, 0, 0, 0, 0};
+  if (resident[tensors] == 0) resident[tensors] = resident_ctas(kernel, kThreads, smem);
+  const int64_t cap = static_cast<int64_t>(sm_count()) * (resident[tensors] < kNormBackwardCtas ? resident[tensors] : kNormBackwardCtas);
   const int grid = static_cast<int>(rounds < cap ? rounds : cap);
   *ctas = grid;
-  SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kThreads), kSmem, st, P));
+  SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kThreads), smem, st, P));
   return SPIRA_B200_OK;
 }
 
@@ -705,11 +712,6 @@ template <typename T, int V>
 static int launch_norm_shape(const NormParams &P, bool backward, int *ctas, cudaStream_t st) {
   const int pieces = P.channels / V;
   if constexpr (V > 1) {
-    if (!backward && pieces % 3 == 0 && pieces <= 96 && (pieces & (pieces - 1)) != 0) {      // 96, 192, 384 channels: three pieces leave no lane idle
-      if (pieces == 12) return launch_norm<T, V, 4, 3>(P, backward, ctas, st);
-      if (pieces == 24) return launch_norm<T, V, 8, 3>(P, backward, ctas, st);
-      if (pieces == 48) return launch_norm<T, V, 16, 3>(P, backward, ctas, st);
-    }
     if (pieces <= 4) return launch_norm<T, V, 4, 1>(P, backward, ctas, st);
     if (pieces <= 8) return launch_norm<T, V, 8, 1>(P, backward, ctas, st);
     if (pieces <= 16) return launch_norm<T, V, 16, 1>(P, backward, ctas, st);

@@ -65,6 +65,11 @@ def _device_of(*tensors) -> int:
     return index
 
 
+def _dense(like: torch.Tensor, rows: int, columns: int) -> torch.Tensor:
+    """An uninitialised dense matrix of the type and device of ``like`` (the cheapest of torch's allocating calls)."""
+    return like.new_empty_strided((rows, columns), (columns, 1))
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself if its columns are neighbours (rows may lie any distance apart), else a dense copy."""
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
@@ -96,8 +101,8 @@ class ExpertRouting(NamedTuple):
 # ------------------------------------------------------------------------------------------------ routing
 def _route(logits: torch.Tensor, top_k: int, renormalize: bool) -> ExpertRouting:
     n, experts = logits.shape
-    weights = logits.new_empty((n, top_k), dtype=torch.float32)
-    chosen = logits.new_empty((n, top_k), dtype=torch.int32)
+    weights = logits.new_empty_strided((n, top_k), (top_k, 1), dtype=torch.float32)
+    chosen = torch.empty_like(weights, dtype=torch.int32)
     slots = torch.empty_like(chosen)
     order = chosen.new_empty(n * top_k)
     offsets = chosen.new_empty(experts + 1)
@@ -130,7 +135,7 @@ class _Route(torch.autograd.Function):
         logits, weights, chosen = ctx.saved_tensors
         n, experts = logits.shape
         dweights = dweights.float()
-        dlogits = logits.new_empty((n, experts))
+        dlogits = _dense(logits, n, experts)
         _launch(logits.get_device(), "spira_b200_expert_route_backward", logits.data_ptr(), _DTYPES[logits.dtype], n, logits.stride(0),
                 experts, weights.shape[1], 1 if ctx.renormalize else 0, weights.data_ptr(), chosen.data_ptr(), dweights.data_ptr(),
                 dweights.stride(0), dweights.stride(1), dlogits.data_ptr())
@@ -182,7 +187,7 @@ def _check_rows(t: torch.Tensor, name: str, rows: int) -> torch.Tensor:
 def _dispatch(feats, slots, offsets):
     n, k = slots.shape
     channels = feats.shape[1]
-    rows = feats.new_empty((n * k, channels))
+    rows = _dense(feats, n * k, channels)
     _launch(feats.get_device(), "spira_b200_expert_dispatch", feats.data_ptr(), _DTYPES[feats.dtype], n, feats.stride(0), channels,
             slots.data_ptr(), k, offsets.data_ptr(), offsets.shape[0] - 1, rows.data_ptr())
     return rows
@@ -191,7 +196,7 @@ def _dispatch(feats, slots, offsets):
 def _combine(rows, weights, slots):
     n, k = slots.shape
     channels = rows.shape[1]
-    out = rows.new_empty((n, channels))
+    out = _dense(rows, n, channels)
     _launch(rows.get_device(), "spira_b200_expert_combine", rows.data_ptr(), _DTYPES[rows.dtype], n, rows.stride(0), channels,
             None if weights is None else weights.data_ptr(), 0 if weights is None else weights.stride(0),
             0 if weights is None else weights.stride(1), slots.data_ptr(), k, out.data_ptr())
@@ -222,8 +227,8 @@ class _Combine(torch.autograd.Function):
         rows, weights, slots, offsets = ctx.saved_tensors
         dout = _rows(dout)
         (n, k), channels = slots.shape, rows.shape[1]
-        drows = rows.new_empty((n * k, channels)) if ctx.needs_input_grad[0] else None
-        dweights = weights.new_empty((n, k)) if ctx.needs_input_grad[1] else None
+        drows = _dense(rows, n * k, channels) if ctx.needs_input_grad[0] else None
+        dweights = _dense(weights, n, k) if ctx.needs_input_grad[1] else None
         _launch(rows.get_device(), "spira_b200_expert_combine_backward", rows.data_ptr(), dout.data_ptr(), _DTYPES[rows.dtype], n,
                 rows.stride(0), dout.stride(0), channels, weights.data_ptr(), weights.stride(0), weights.stride(1), slots.data_ptr(), k,
                 offsets.data_ptr(), offsets.shape[0] - 1, None if drows is None else drows.data_ptr(),
@@ -279,7 +284,7 @@ def _grouped(x, weights, offsets, bias, relu, want_mask=False):
     """The product and, for a backward pass, what its ReLU let through: the bit mask the kernel writes, or None where the
     call has none (then the sign of the result says it)."""
     index, n = x.get_device(), x.shape[0]
-    y = x.new_empty((n, weights.shape[2]))
+    y = _dense(x, n, weights.shape[2])
     mask, workspace, room = None, 0, 0
     want_mask = want_mask and relu
     relu = 1 if relu else 0
@@ -320,9 +325,9 @@ class _Grouped(torch.autograd.Function):
         dy = _rows(dy)
         need = ctx.needs_input_grad
         index, n = x.get_device(), x.shape[0]
-        dx = dy.new_empty(x.shape) if need[0] else None
-        dw = weights.new_empty(weights.shape) if need[1] else None
-        db = weights.new_empty((weights.shape[0], weights.shape[2])) if ctx.has_bias and need[3] else None
+        dx = _dense(dy, n, x.shape[1]) if need[0] else None
+        dw = torch.empty_like(weights) if need[1] else None            # (dense: the call made it so)
+        db = _dense(weights, weights.shape[0], weights.shape[2]) if ctx.has_bias and need[3] else None
         _with_workspace(index, dy, "spira_b200_grouped_linear_backward",
                         _grouped_desc(n, weights, offsets, 1 if ctx.relu else 0, x, None, dy, y, mask, dx, dw, db), _status(index))
         return dx, dw, None, db, None

@@ -7,12 +7,12 @@ and adds residuals as another (spira/tensors.py:47-53).
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from spira_b200 import _lib
-from spira_b200.nn.functional.experts import _addr, _device_of, _DTYPES, _fail, _launch, _needs_grad, _once, _rows, _with_workspace
+from spira_b200.nn.functional.experts import _addr, _dense, _device_of, _DTYPES, _fail, _launch, _needs_grad, _once, _rows, _with_workspace
 
 __all__ = ["residual_norm"]
 
@@ -20,9 +20,16 @@ MAX_CHANNELS = 8192
 GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
 
 
-class _Spec:
+class _Spec(NamedTuple):
     """What stays the same between the forward and the backward call."""
-    __slots__ = ("params_f32", "layer", "pre", "post", "gate_kind", "residual_scale", "block_scale", "eps")
+    params_f32: bool
+    layer: bool
+    pre: bool
+    post: bool
+    gate_kind: int
+    residual_scale: float
+    block_scale: float
+    eps: float
 
 
 def _desc(spec, x, params, stream=None, normed=None, stats=None, dstream=None, dnormed=None, grads=(None,) * 7) -> bytes:
@@ -41,8 +48,9 @@ def _desc(spec, x, params, stream=None, normed=None, stats=None, dstream=None, d
 
 
 def _forward(spec, x, params, stats):
-    stream = x.new_empty(x.shape) if params[0] is not None else None
-    normed = x.new_empty(x.shape) if spec.pre else None
+    n, channels = x.shape
+    stream = _dense(x, n, channels) if params[0] is not None else None
+    normed = _dense(x, n, channels) if spec.pre else None
     _launch(x.get_device(), "spira_b200_residual_norm", _desc(spec, x, params, stream, normed, stats))
     return stream, normed
 
@@ -50,7 +58,7 @@ def _forward(spec, x, params, stats):
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, spec, x, *params):
-        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
+        stats = x.new_empty_strided((x.shape[0], 4), (4, 1), dtype=torch.float32)
         stream, normed = _forward(spec, x, params, stats)
         ctx.spec = spec
         ctx.save_for_backward(x, *params, stats)
@@ -68,7 +76,8 @@ class _ResidualNorm(torch.autograd.Function):
             dnormed = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
         dstream = None if dstream is None else _rows(dstream)
         dnormed = None if dnormed is None else _rows(dnormed)
-        grads = [t.new_empty(t.shape) if t is not None and wanted else None for t, wanted in zip((x, *params), ctx.needs_input_grad[1:])]
+        grads = [None if t is None or not wanted else torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+                 for t, wanted in zip((x, *params), ctx.needs_input_grad[1:])]
         desc = _desc(spec, x, params, None, None, stats, dstream, dnormed, grads)
         if grads[3] is not None or grads[4] is not None or grads[5] is not None or grads[6] is not None \
                 or (grads[2] is not None and spec.gate_kind == GATE_CHANNEL):
@@ -114,36 +123,31 @@ def residual_norm(feats: torch.Tensor, block: Optional[torch.Tensor] = None, *, 
         _fail("weight and bias belong to the norm that pre=False leaves out")
     if not post and (post_weight is not None or post_bias is not None):
         _fail("post_weight and post_bias need post=True")
-    spec = _Spec()
-    spec.layer, spec.pre, spec.post = int(kind == "layer"), int(bool(pre)), int(bool(post))
-    spec.residual_scale, spec.block_scale, spec.eps = float(residual_scale), float(block_scale), float(eps)
-    spec.gate_kind = GATE_NONE
+    gate_kind, channel_gate = GATE_NONE, None
     if gate is not None:
         if gate.dim() == 1:
-            spec.gate_kind = GATE_CHANNEL
-        elif gate.shape == (n, 1):
-            spec.gate_kind = GATE_ROW
-        elif gate.shape == (n, channels):
-            spec.gate_kind = GATE_FULL
+            gate_kind, channel_gate = GATE_CHANNEL, gate
+            gate = gate.contiguous()
+        elif gate.shape == (n, 1) or gate.shape == (n, channels):
+            gate_kind = GATE_ROW if gate.shape[1] == 1 else GATE_FULL
+            if gate.dtype != feats.dtype:
+                _fail(f"a gate per row or element has the type of feats, {feats.dtype}, got {gate.dtype}")
+            gate = _rows(gate)
         else:
             _fail(f"gate is expected to be [{channels}], [{n}, 1] or [{n}, {channels}], got {tuple(gate.shape)}")
-        if gate.dim() == 2 and gate.dtype != feats.dtype:
-            _fail(f"a gate per row or element has the type of feats, {feats.dtype}, got {gate.dtype}")
-        gate = _rows(gate) if gate.dim() == 2 else gate.contiguous()
-    dtype = None
-    for name, p in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias),
-                    ("gate", gate if spec.gate_kind == GATE_CHANNEL else None)):
-        if p is None:
-            continue
-        if p.shape != (channels,) or p.dtype not in (feats.dtype, torch.float32):
-            _fail(f"{name} is expected to be {feats.dtype} or float32 [{channels}], got {p.dtype} {tuple(p.shape)}")
-        if dtype is not None and p.dtype != dtype:
-            _fail("parameters of one call must have one type")
-        dtype = p.dtype
-    params = [p if p is None or p.is_contiguous() else p.contiguous() for p in (weight, bias, post_weight, post_bias)]
+    dtype, dense = None, True
+    for p in (weight, bias, post_weight, post_bias, channel_gate):
+        if p is not None:
+            if p.shape != (channels,) or (p.dtype != feats.dtype and p.dtype != torch.float32):
+                _fail(f"parameters (and a gate per channel) are expected to be {feats.dtype} or float32 [{channels}], got {p.dtype} {tuple(p.shape)}")
+            if dtype is not None and p.dtype != dtype:
+                _fail("parameters of one call must have one type")
+            dtype = p.dtype
+            dense = dense and p.is_contiguous()
+    params = (weight, bias, post_weight, post_bias) if dense else tuple(p if p is None else p.contiguous() for p in (weight, bias, post_weight, post_bias))
     feats_rows = _rows(feats)
     block = None if block is None else _rows(block)
-    spec.params_f32 = 1 if dtype is torch.float32 else 0
+    spec = _Spec(dtype is torch.float32, kind == "layer", bool(pre), bool(post), gate_kind, float(residual_scale), float(block_scale), float(eps))
     if _needs_grad(feats, block, gate, *params):
         stream, normed = _ResidualNorm.apply(spec, feats_rows, block, gate, *params)
     else:
