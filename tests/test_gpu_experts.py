@@ -83,7 +83,7 @@ def check_route(logits, k, renormalize):
 
 @pytest.mark.parametrize("dtype", ANY)
 @pytest.mark.parametrize("n,e,k", [(0, 4, 2), (1, 1, 1), (1, 8, 2), (3, 5, 5), (37, 16, 3), (255, 33, 4), (64, 64, 8), (129, 128, 2), (40, 200, 7),
-                                   (19, 512, 32), (1500, 7, 3), (2049, 9, 2), (2500, 65, 2)])
+                                   (19, 512, 32), (200, 40, 32), (1500, 7, 3), (2049, 9, 2), (2500, 65, 2)])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_route(dtype, n, e, k, renormalize):
     logits = rand(n, e, dtype=dtype, scale=2.0)
@@ -148,20 +148,27 @@ def test_route_gradient(dtype, renormalize, n, e, k):
     close(got, exact, size, 8 * (e + 20), "dlogits")
 
 
-def test_route_many_rows_against_torch():
+@pytest.mark.parametrize("e,k,dtype", [(64, 4, torch.float16), (20, 3, torch.bfloat16), (32, 32, torch.float16), (128, 2, torch.bfloat16), (250, 9, torch.float16),
+                                       (512, 8, torch.bfloat16), (64, 4, torch.float32), (9, 9, torch.float32)])
+def test_route_many_rows_against_torch(e, k, dtype):
     """A whole scene over many CTAs: places from a stable sort of the choices."""
     from spira_b200.nn import functional as F
-    logits = rand(127363, 64, dtype=torch.float16)
+    logits = rand(127363, e, dtype=dtype)
     logits[::50] = float("-inf")
-    r = F.expert_route(logits, 4)
+    logits[1::50, : e - 1] = float("-inf")
+    r = F.expert_route(logits, k)
     values, index = torch.sort(logits.float(), dim=1, descending=True, stable=True)
-    experts = torch.where(values[:, :4] > -math.inf, index[:, :4], -1)
+    experts = torch.where(values[:, :k] > -math.inf, index[:, :k], -1)
     assert torch.equal(r.experts, experts.int())
     flat = experts.reshape(-1)
-    order = torch.argsort(torch.where(flat < 0, 64, flat), stable=True)
+    order = torch.argsort(torch.where(flat < 0, e, flat), stable=True)
     total = int((flat >= 0).sum())
     assert torch.equal(r.order[:total], order[:total].int()) and bool((r.order[total:] == -1).all())
-    assert torch.equal(r.offsets.cpu(), torch.cat([torch.zeros(1, dtype=torch.long), torch.bincount(flat[flat >= 0], minlength=64).cumsum(0).cpu()]).int())
+    assert torch.equal(r.offsets.cpu(), torch.cat([torch.zeros(1, dtype=torch.long), torch.bincount(flat[flat >= 0], minlength=e).cumsum(0).cpu()]).int())
+    top = torch.where(values[:, :1] > -math.inf, values[:, :1], 0.0).double()
+    p = torch.where(experts >= 0, torch.exp(values[:, :k].double() - top), 0.0)
+    exact = p / p.sum(1, keepdim=True).clamp_min(1e-300)
+    assert bool(((r.weights.double() - exact).abs() <= (2 * (14 + 4) + k + 2) * U32 * exact + 1e-37).all())       # (differences of logits below 14)
     assert torch.equal(r.slots.view(-1)[order[:total]], torch.arange(total, device="cuda", dtype=torch.int32))
 
 
