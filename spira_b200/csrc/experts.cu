@@ -6,7 +6,9 @@
 //   combine   out[t] = sum_j weights[t][j] * rows[slots[t][j]]
 //
 // Every result is a function of the inputs alone: counts are integers, places follow from counts and ranks, sums run over
-// j in order.  All of it is bound by memory (or, for a few rows, by the launch).
+// j in order.  Dispatch and combine are bound by memory (127 363 x 96 fp16, k 2: 12 us = 6.0 TB/s there, 14 us = 5.3 TB/s
+// back), routing by the integer instructions of the selection (127 363 x 64 fp16, k 4: 19.6 us for 24 MB), all of it by
+// the launch for a few rows.
 #include <cfloat>
 #include <cmath>
 
@@ -570,7 +572,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const MoveParams P) {
   store_f32<T, V>(static_cast<T *>(P.out) + row * P.channels + c, acc);
 }
 
-// drows[slot] = w dout[t], dweights[t][j] = <dout[t], rows[slot]>: G lanes per row of `dout`.
+// drows[slot] = w dout[t], dweights[t][j] = <dout[t], rows[slot]> (40 013 x 256 bf16, k 2: 20 us = 5.0 TB/s): G lanes per row of `dout`, two of the row's experts at a
+// time, so that their gathers are in flight together and `dout` is read once for both.
 template <typename T, int V, int G>
 __global__ void __launch_bounds__(256) combine_backward_kernel(const MoveParams P) {
   pdl_trigger();
@@ -584,31 +587,43 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const MoveParams 
   for (int64_t b = blockIdx.x; b < groups; b += gridDim.x) {
     const int64_t row = b * kRows + threadIdx.x / G;
     const bool live = row < P.n;
-    for (int j = 0; j < P.k; ++j) {
-      const int64_t slot = live ? P.slots[row * P.k + j] : -1;
-      const bool there = slot >= 0 && slot < total;
-      float dot = 0.f;
-      if (there) {
-        const float w = P.weights ? P.weights[row * P.w_row + j * P.w_col] : 1.f;
+    for (int j0 = 0; j0 < P.k; j0 += 2) {
+      int64_t slot[2];
+      float w[2], dot[2] = {0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        slot[q] = live && j0 + q < P.k ? P.slots[row * P.k + j0 + q] : -1;
+        if (slot[q] >= total) slot[q] = -1;
+        w[q] = live && j0 + q < P.k && P.weights ? P.weights[row * P.w_row + (j0 + q) * P.w_col] : 1.f;
+      }
+      if (slot[0] >= 0 || slot[1] >= 0)
         for (int i = g; i < vecs; i += G) {
-          float d[V], y[V];
+          float d[V], y[2][V];
           load_f32<T, V>(dout + row * P.x_stride + i * V, d);
-          if (P.dweights) {
-            load_f32<T, V>(rows + slot * P.y_stride + i * V, y);
+          if (P.dweights)
 #pragma unroll
-            for (int e = 0; e < V; ++e) dot = fmaf(d[e], y[e], dot);
-          }
-          if (drows) {
+            for (int q = 0; q < 2; ++q)
+              if (slot[q] >= 0) load_f32<T, V>(rows + slot[q] * P.y_stride + i * V, y[q]);
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[e] *= w;
-            store_f32<T, V>(drows + slot * P.channels + i * V, d);
+          for (int q = 0; q < 2; ++q) {
+            if (slot[q] < 0) continue;
+            if (P.dweights)
+#pragma unroll
+              for (int e = 0; e < V; ++e) dot[q] = fmaf(d[e], y[q][e], dot[q]);
+            if (drows) {
+              float o[V];
+#pragma unroll
+              for (int e = 0; e < V; ++e) o[e] = d[e] * w[q];
+              store_f32<T, V>(drows + slot[q] * P.channels + i * V, o);
+            }
           }
         }
-      }
       if (P.dweights) {
 #pragma unroll
-        for (int d = 1; d < G; d *= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d, G);
-        if (live && g == 0) P.dweights[row * P.k + j] = dot;
+        for (int d = 1; d < G; d *= 2)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) dot[q] += __shfl_xor_sync(0xffffffffu, dot[q], d, G);
+        if (live && g < 2 && j0 + g < P.k) P.dweights[row * P.k + j0 + g] = g == 0 ? dot[0] : dot[1];
       }
     }
   }
@@ -710,8 +725,12 @@ static int launch_move(MoveParams &P, bool combine, cudaStream_t st) {
 template <typename T, int V>
 static int launch_combine_backward(const MoveParams &P, cudaStream_t st) {
   const int vecs = P.channels / V;
-  const int lanes = vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
-  const unsigned blocks = capped_blocks(P.n * lanes, 256, 16);
+  // as many lanes as the row has pieces, half of them where the rows fill the SMs all the same: two pieces per lane are in
+  // flight together (127 363 x 96, k 2: 28 instead of 33 us; 20 000 x 64, k 8: 13 with all lanes, 20 us with half).  No
+  // more CTAs than fit at once (39 us).
+  int lanes = vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
+  if (lanes > 4 && vecs <= 32 && P.n * (lanes / 2) >= 4 * 256 * static_cast<int64_t>(sm_count())) lanes /= 2;
+  const unsigned blocks = capped_blocks(P.n * lanes, 256, 8);
   if (lanes == 4) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 4>, dim3(blocks), dim3(256), 0, st, P));
   else if (lanes == 8) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 8>, dim3(blocks), dim3(256), 0, st, P));
   else if (lanes == 16) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 16>, dim3(blocks), dim3(256), 0, st, P));

@@ -15,9 +15,12 @@
 //
 // One persistent CTA per SM, 20 warps: warp 0 issues TMA loads, warp 1 the MMAs, warps 4-19 (four per tensor-memory lane
 // quarter, a quarter of the columns each) convert and store while the next tile accumulates in the other half of tensor
-// memory.  Narrow products (few reduction steps per tile) are bound by this conversion: it takes 2.5 instructions per
-// element with bias and ReLU, the mask of the ReLU two more.  Every CTA reads the group
-// boundaries once into shared memory.  Every wait is bounded; an expired one raises the status word.
+// memory.  Every CTA reads the group boundaries once into shared memory.  Every wait is bounded; an expired one raises the
+// status word.
+//
+// Measured: 254 726 rows in 8 groups 96 -> 384 fp16 with bias and ReLU 60 us: its 196 MB of results alone take 52 us at the
+// 3.8 TB/s at which this memory takes writes; 80 026 rows in 16 groups 512 -> 2048 bf16: forward with bias, ReLU and mask
+// 147 us, dx 106 us = 1590 TFLOP/s, dW 128 us (one dense library product of the size: 135, 109, 118 us).
 #include <cuda.h>
 
 #include <type_traits>

@@ -95,10 +95,12 @@ def test_route(dtype, n, e, k, renormalize):
     check_route(logits, k, renormalize)
 
 
-def test_route_ties_zeros_lowest_values_and_nan():
-    low = torch.finfo(torch.float32).min
+@pytest.mark.parametrize("dtype", ANY)
+def test_route_ties_zeros_lowest_values_and_nan(dtype):
+    low, tiny = torch.finfo(dtype).min, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps      # the smallest step above zero
     rows = torch.tensor([[0.0, -0.0, 0.0, -0.0, -1.0], [low, low, low, low, low], [low, 3.0, low, 3.0, low], [-math.inf] * 5,
-                         [1.0, math.nan, 2.0, math.nan, 0.0], [-math.inf, low, -math.inf, -math.inf, -math.inf], [5.0, 1e-40, -1e-40, 0.0, 5.0]])
+                         [1.0, math.nan, 2.0, math.nan, 0.0], [1.0, -math.nan, 2.0, 3.0, 0.0], [-math.inf, low, -math.inf, -math.inf, -math.inf],
+                         [5.0, tiny, -tiny, 0.0, 5.0], [-tiny, tiny, -0.0, 0.0, -2.0]], dtype=torch.float64).to(dtype)
     for k in (1, 2, 4, 5):
         for renormalize in (True, False):
             check_route(rows.cuda(), k, renormalize)
