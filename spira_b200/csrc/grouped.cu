@@ -332,10 +332,11 @@ __global__ void __launch_bounds__(256, 4) grouped_dz_kernel(const T *dy, int64_t
   }
 }
 
-// Column sums of many short pieces: 32 columns x 32 strides of pieces per block, then a fixed tree.
+// Column sums of many short pieces: 32 columns x 8 strides of pieces per block, then a fixed order.  Latency of the
+// loads: 64 x 16 blocks over 600 pieces 7.3 us; with 32 strides (1024 threads, two blocks per SM at a time) 12.1 us.
 template <typename T>
-__global__ void __launch_bounds__(1024) grouped_column_sum_kernel(const float *partial, const int32_t *offsets, int n, int experts, int piece, int size, T *out) {
-  __shared__ float part[32][33];
+__global__ void __launch_bounds__(256) grouped_column_sum_kernel(const float *partial, const int32_t *offsets, int n, int experts, int piece, int size, T *out) {
+  __shared__ float part[8][32];
   pdl_trigger();
   pdl_wait();
   const int e = blockIdx.y, lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
@@ -344,15 +345,16 @@ __global__ void __launch_bounds__(1024) grouped_column_sum_kernel(const float *p
   group_pieces(offsets, n, e, piece, first, count);
   float t = 0.f;
   if (c < size)
-#pragma unroll 4
-    for (int p = w; p < count; p += 32) t += partial[(first + p) * size + c];
+#pragma unroll 8
+    for (int p = w; p < count; p += 8) t += partial[(first + p) * size + c];
   part[w][lane] = t;
   __syncthreads();
-  t = part[lane][w];
+  if (w == 0 && c < size) {
+    t = 0.f;
 #pragma unroll
-  for (int d = 1; d < 32; d *= 2) t += __shfl_xor_sync(0xffffffffu, t, d);
-  const int co = blockIdx.x * 32 + w;
-  if (lane == 0 && co < size) out[static_cast<int64_t>(e) * size + co] = from_f32<T>(t);
+    for (int i = 0; i < 8; ++i) t += part[i][lane];
+    out[static_cast<int64_t>(e) * size + c] = from_f32<T>(t);
+  }
 }
 
 // Rows per piece of the column sums: a CTA per piece, all of them resident at once (four per SM), at least 32 rows.
@@ -603,7 +605,7 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
       else rc = kind == 0 ? go(grouped_dz_kernel<T, 1, 0>, D.c_out) : kind == 1 ? go(grouped_dz_kernel<T, 1, 1>, D.c_out) : go(grouped_dz_kernel<T, 1, 2>, D.c_out);
       if (rc != SPIRA_B200_OK) return rc;
       if (D.dbias)
-        SB_CHECK_CUDA(launch_dependent(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(1024), 0, st,
+        SB_CHECK_CUDA(launch_dependent(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(256), 0, st,
                                        static_cast<const float *>(partial), D.offsets, n, D.experts, plan.dz_rows, D.c_out, static_cast<T *>(D.dbias)));
       if (dz) {
         Z.dy = dz;
