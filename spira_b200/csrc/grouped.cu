@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kAThreads) grouped_any_kernel(const __grid_con
       expert = t.expert;
       unit = blockIdx.x;
       k_begin = t.begin + t.index * P.piece;
-      k_end = k_begin + P.piece < t.end ? k_begin + P.piece : t.end;
+      k_end = piece_end(k_begin, t.end, P.piece);
     }
     const int m_tiles = (P.c_in + kATile - 1) / kATile;
     m0 = static_cast<int>(blockIdx.y) % m_tiles * kATile;
@@ -206,7 +206,7 @@ __device__ __forceinline__ void group_pieces(const int32_t *offsets, int n, int 
     }
     lo = lo > highest ? lo : highest;
     hi = hi > lo ? hi : lo;
-    const int mine = i <= e ? (hi - lo + piece - 1) / piece : 0;
+    const int mine = i <= e ? pieces_of(hi - lo, piece) : 0;
     int sum = mine;
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(256, 4) grouped_dz_kernel(const T *dy, int64_t
   pdl_wait();
   const GroupTile t = find_group_tile(offsets, experts, n, piece, blockIdx.x);
   if (t.expert < 0) return;
-  const int r0 = t.begin + t.index * piece, r1 = r0 + piece < t.end ? r0 + piece : t.end;
+  const int r0 = t.begin + t.index * piece, r1 = piece_end(r0, t.end, piece);
   const int vecs = c_out / V, wide = vecs - static_cast<int>(blockIdx.y) * 256 < 256 ? vecs - static_cast<int>(blockIdx.y) * 256 : 256;
   const int lanes = 256 / wide;                 // rows in parallel
   const int lane = threadIdx.x / wide, c = (blockIdx.y * 256 + threadIdx.x % wide) * V;

@@ -24,6 +24,13 @@ __device__ __forceinline__ int clamped_offset(const int32_t *offsets, int e, int
   return v < 0 ? 0 : v > n ? n : v;
 }
 
+// Pieces of `rows` rows that `length` rows make, and where the piece from row `begin` on ends.  (Row numbers reach 2^31: the
+// sum of two of them does not fit their type.)
+__device__ __forceinline__ int pieces_of(int length, int rows) {
+  return static_cast<int>((static_cast<uint32_t>(length) + static_cast<uint32_t>(rows) - 1u) / static_cast<uint32_t>(rows));
+}
+__device__ __forceinline__ int piece_end(int begin, int end, int rows) { return end - begin > rows ? begin + rows : end; }
+
 // The t-th tile of `rows` rows over all groups, found by one whole warp (every lane gets the answer).
 __device__ __forceinline__ GroupTile find_group_tile(const int32_t *offsets, int experts, int n, int rows, int t) {
   const int lane = threadIdx.x & 31;
@@ -43,7 +50,7 @@ __device__ __forceinline__ GroupTile find_group_tile(const int32_t *offsets, int
     lo = run > highest ? run : highest;
     hi = hi > lo ? hi : lo;
     if (e >= experts) hi = lo;
-    const int mine = (hi - lo + rows - 1) / rows;
+    const int mine = pieces_of(hi - lo, rows);
     int sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {

@@ -232,8 +232,8 @@ struct TileWalk {
     if (MODE == kDw) {
       r.m0 = in_unit / P.n_tiles * P.tile_rows;
       r.row0 = rows[expert] + index * P.piece;
-      r.row_end = P.piece && r.row0 + P.piece < rows[expert + 1] ? r.row0 + P.piece : rows[expert + 1];
-      r.steps = (r.row_end - r.row0 + kGK - 1) / kGK;
+      r.row_end = P.piece ? piece_end(r.row0, rows[expert + 1], P.piece) : rows[expert + 1];
+      r.steps = pieces_of(r.row_end - r.row0, kGK);
     } else {
       r.m0 = 0;
       r.row0 = rows[expert] + index * P.tile_rows;
@@ -266,7 +266,7 @@ __device__ __forceinline__ void read_groups(const GroupedTcParams &P, int *rows,
   for (int e0 = 0; e0 < P.experts; e0 += 32) {
     const int e = e0 + lane;
     int mine = 0;
-    if (e < P.experts) mine = unit_rows == 0 ? 1 : (rows[e + 1] - rows[e] + unit_rows - 1) / unit_rows;
+    if (e < P.experts) mine = unit_rows == 0 ? 1 : pieces_of(rows[e + 1] - rows[e], unit_rows);
     int sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
