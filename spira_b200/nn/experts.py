@@ -19,7 +19,7 @@ from spira_b200.utils.apply import fapply
 class SparseExperts(Module):
     """``out = sum over the voxel's experts e of weight_e * (relu(x W1[e] + b1[e]) W2[e] + b2[e])``, experts and weights from
     ``expert_route(x @ router, top_k)``.  ``forward(inputs, mask)``: voxels where the boolean ``mask [N]`` is False go to no
-    expert and come out as zeros.  Weights are laid out like ``SparseConv.kernel``: ``[E, c_in, c_out]``."""
+    expert and come out as zeros; what they hold (also NaN) shows nowhere.  Weights are laid out like ``SparseConv.kernel``: ``[E, c_in, c_out]``."""
 
     def __init__(self, in_channels: int, hidden_channels: int, num_experts: int, top_k: int = 2, out_channels: Optional[int] = None,
                  bias: bool = True, renormalize: bool = True):
@@ -56,6 +56,8 @@ class SparseExperts(Module):
         return torch.mm(feats, self.router)
 
     def _run(self, feats: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if mask is not None and torch.is_grad_enabled():      # (0 * NaN would reach the router's gradient)
+            feats = feats.masked_fill(~mask[:, None], 0)
         logits = self.logits(feats)
         if mask is not None:
             logits = logits.masked_fill(~mask[:, None], float("-inf"))

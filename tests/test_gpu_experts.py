@@ -641,6 +641,29 @@ def test_block_forward_and_gradients():
             assert off(g, e) < 40 * 2.0 ** -11, (name, off(g, e))
 
 
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_masked_voxels_reach_nothing(renormalize):
+    """What masked voxels hold (NaN, infinities) shows in no result and no gradient: the same bits as with zeros there."""
+    import spira_b200 as sp
+    from spira_b200 import nn as spnn
+    torch.manual_seed(4)
+    moe = spnn.SparseExperts(32, 64, 5, top_k=2, renormalize=renormalize).cuda().half()
+    n = 300
+    mask = torch.rand(n, generator=torch.Generator().manual_seed(2)).cuda() > 0.3
+    clean = rand(n, 32, dtype=torch.float16).masked_fill(~mask[:, None], 0.0)
+    dirty = clean.clone()
+    dirty[~mask] = float("nan")
+    dirty[torch.nonzero(~mask)[0, 0]] = float("inf")
+    results = []
+    for feats in (clean, dirty):
+        feats.requires_grad_(True)
+        y = moe(sp.SparseTensor(torch.arange(n, dtype=torch.int32, device="cuda"), feats), mask)._features
+        results.append([y.detach(), *torch.autograd.grad(y, [feats, *moe.parameters()], rand(n, 32, dtype=torch.float16, seed=7))])
+    for a, b in zip(*results):
+        assert bool(torch.isfinite(b).all()) and torch.equal(a, b)
+    assert not bool(results[1][1][~mask].any())
+
+
 def test_block_behind_a_sparse_convolution_compiles():
     """The modules as layers of a network: eager, recorded and replayed on another scene, the same bits."""
     import spira_oracle as O  # noqa: F401
