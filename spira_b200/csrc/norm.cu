@@ -13,7 +13,7 @@
 // owns its columns for all rows its CTA visits, CTAs write partial sums, a second launch adds those in a fixed order.
 // Bound by memory and instructions together: forward 2 row reads + 2 row writes, backward 4 + 2 (one more of each with a
 // gate per element).  127 363 x 256 bf16, layer norms on both sides, a gate per element, fp32 parameters: forward 63 us =
-// 5.2 TB/s, backward 126 us = 4.1 TB/s; 127 363 x 96 fp16 with one rms norm: 22 us = 4.4 TB/s.
+// 5.2 TB/s, backward 111 us = 4.7 TB/s; 127 363 x 96 fp16 with one rms norm: 22 us = 4.4 TB/s.
 #include "common.cuh"
 #include "elem.cuh"
 #include "ptx.cuh"
@@ -256,6 +256,12 @@ __device__ __forceinline__ void normalise(float (&v)[ITEMS][R][V], const bool (&
 // Threads of a CTA: 256, or the row's if it takes more.
 template <int L>
 constexpr int kNormThreads = L > 256 ? L : 256;
+// The backward pass with two rows per thread: the parameters are read once for both and their sums overlap.  Registers decide:
+// 384 threads of 168 for pieces of 8 channels (127 363 x 256 bf16, layer, both sides, gate per element: 111 us; 256 threads
+// 136 us, 448 and spilling 149 us; one row at a time and twice 256 threads 125 us), 512 of 128 for pieces of 4
+// (127 363 x 128 fp32: 97 us, with 384 threads 103 us).
+template <int V, int L, int R>
+constexpr int kBackwardThreads = R == 1 ? kNormThreads<L> : V == 4 ? 512 : 384;
 
 // The rows on their way: every thread copies its own 16-byte pieces of the next rows into shared memory (cp.async, past the
 // L1, where the parameters stay) and reads them back itself, so no barrier is needed and no register waits for a load.
@@ -392,9 +398,9 @@ __global__ void __launch_bounds__(kNormThreads<L>) norm_forward_kernel(const __g
   }
 }
 
-template <typename T, int V, int L, int ITEMS, bool LAYER>
-__global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) norm_backward_kernel(const __grid_constant__ NormParams P) {
-  constexpr int kThreads = kNormThreads<L>;
+template <typename T, int V, int L, int ITEMS, int R, bool LAYER>
+__global__ void __launch_bounds__(kBackwardThreads<V, L, R>, L > 32 || ITEMS > 1 || R > 1 ? 1 : 2) norm_backward_kernel(const __grid_constant__ NormParams P) {
+  constexpr int kThreads = kBackwardThreads<V, L, R>;
   __shared__ float scratch[64];
   extern __shared__ __align__(16) unsigned char norm_ring[];
   float *column_sums = reinterpret_cast<float *>(norm_ring);      // [kThreads / L][channels], once the rows are through
@@ -402,8 +408,8 @@ __global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) 
   pdl_wait();
   typedef Ops<V> O;
   const int g = threadIdx.x % L;
-  constexpr int kRows = kThreads / L;
-  const int rounds = (P.n + kRows - 1) / kRows;
+  constexpr int kRows = kThreads / L, kBoth = LAYER ? 2 : 1;
+  const int rounds = (P.n + kRows * R - 1) / (kRows * R);
   const float a = P.block ? P.residual_scale : 1.f, s = P.block_scale;
   const void *post_w = P.post ? P.post_weight : nullptr, *post_b = P.post ? P.post_bias : nullptr;
   bool in[ITEMS];
@@ -413,7 +419,7 @@ __global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) 
     in[i] = (i * L + g) * V < P.channels;
     col[i] = in[i] ? (i * L + g) * V : 0;
   }
-  typedef Ring<kThreads, ITEMS, 5, V * sizeof(T) == 16> Rows;
+  typedef Ring<kThreads, ITEMS * R, 5, V * sizeof(T) == 16> Rows;
   const Rows ring(norm_ring, backward_tensors(P));
   constexpr int kDepth = Rows::kDepth;
   // 0: x, 1: gradient of the normed rows, 2: block, 3: gradient of the stream, 4: gate
@@ -425,8 +431,8 @@ __global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) 
     return static_cast<const T *>(P.gate) + row * P.gate_stride + c;
   };
   const bool used[5] = {P.pre != 0, P.pre != 0, P.block != nullptr, P.dstream != nullptr, P.gate_kind == kGateFull};
-  auto row_of = [&](int b) {
-    const int row = b * kRows + static_cast<int>(threadIdx.x) / L;
+  auto row_of = [&](int b, int r) {
+    const int row = (b * kRows + static_cast<int>(threadIdx.x) / L) * R + r;
     return row < P.n ? row : P.n - 1;
   };
   auto fetch = [&](int stage, int b) {
@@ -435,11 +441,13 @@ __global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) 
       for (int w = 0; w < 5; ++w)
         if (used[w])
 #pragma unroll
-          for (int i = 0; i < ITEMS; ++i) ring.copy(stage, w * ITEMS + i, source(w, row_of(b), col[i]));
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) ring.copy(stage, (w * R + r) * ITEMS + i, source(w, row_of(b, r), col[i]));
     Rows::commit();
   };
-  auto take = [&](int stage, int w, int i, int64_t row) -> Vec<T, V> {
-    if constexpr (kDepth > 0) return *reinterpret_cast<const Vec<T, V> *>(ring.piece(stage, w * ITEMS + i));
+  auto take = [&](int stage, int w, int r, int i, int64_t row) -> Vec<T, V> {
+    if constexpr (kDepth > 0) return *reinterpret_cast<const Vec<T, V> *>(ring.piece(stage, (w * R + r) * ITEMS + i));
     else return *reinterpret_cast<const Vec<T, V> *>(source(w, row, col[i]));
   };
   int stage = 0;
@@ -451,142 +459,178 @@ __global__ void __launch_bounds__(kNormThreads<L>, L > 32 || ITEMS > 1 ? 1 : 2) 
       fetch(stage == 0 ? kDepth - 1 : stage - 1, b + (kDepth - 1) * gridDim.x);
       Rows::wait();
     }
-    const bool live = b * kRows + static_cast<int>(threadIdx.x) / L < P.n;
-    const int64_t row = row_of(b);
-    const float4 st = reinterpret_cast<const float4 *>(P.stats)[row];
+    const int row0 = (b * kRows + static_cast<int>(threadIdx.x) / L) * R;
+    bool live[R];
+    int64_t row[R];
+    float4 st[R];
     // hat: x, then the stream's normalised value; bh: the block's normalised value (or the block); q: its affine form times
     // the gate; d: gradient of the stream
-    float hat[ITEMS][1][V], bh[ITEMS][V], d[ITEMS][V], u[ITEMS][1][V], q[ITEMS][1][V];
-    Vec<T, V> gates[ITEMS];
-    const float row_gate = P.gate_kind == kGateRow ? to_f32(static_cast<const T *>(P.gate)[row * P.gate_stride]) : 1.f;
+    float hat[ITEMS][R][V], bh[ITEMS][R][V], d[ITEMS][R][V], u[ITEMS][R][V], q[ITEMS][R][V];
+    Vec<T, V> gates[ITEMS][R];
+    float row_gate[R];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      if (P.pre) {
-        vec_to_f32<T, V>(take(stage, 0, i, row), hat[i][0]);
-        vec_to_f32<T, V>(take(stage, 1, i, row), u[i][0]);
-      }
-      if (P.block) vec_to_f32<T, V>(take(stage, 2, i, row), bh[i]);
-      if (P.dstream) {
-        vec_to_f32<T, V>(take(stage, 3, i, row), d[i]);
-      } else {
+    for (int r = 0; r < R; ++r) {
+      live[r] = row0 + r < P.n;
+      row[r] = row_of(b, r);
+      st[r] = reinterpret_cast<const float4 *>(P.stats)[row[r]];
+      row_gate[r] = P.gate_kind == kGateRow ? to_f32(static_cast<const T *>(P.gate)[row[r] * P.gate_stride]) : 1.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) d[i][e] = 0.f;
+      for (int i = 0; i < ITEMS; ++i) {
+        if (P.pre) {
+          vec_to_f32<T, V>(take(stage, 0, r, i, row[r]), hat[i][r]);
+          vec_to_f32<T, V>(take(stage, 1, r, i, row[r]), u[i][r]);
+        }
+        if (P.block) vec_to_f32<T, V>(take(stage, 2, r, i, row[r]), bh[i][r]);
+        if (P.dstream) {
+          vec_to_f32<T, V>(take(stage, 3, r, i, row[r]), d[i][r]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) d[i][r][e] = 0.f;
+        }
+        if (P.gate_kind == kGateFull) gates[i][r] = take(stage, 4, r, i, row[r]);
       }
-      if (P.gate_kind == kGateFull) gates[i] = take(stage, 4, i, row);
     }
     if (++stage >= kDepth) stage = 0;
-    auto load_gate = [&](int i, float (&f)[V]) {
+    auto load_gate = [&](int i, int r, float (&f)[V]) {
       if (P.gate_kind == kGateChannel) load_param<T, V>(P.gate, P.params_f32, col[i], f);
-      else vec_to_f32<T, V>(gates[i], f);
+      else vec_to_f32<T, V>(gates[i][r], f);
     };
-    float sums[2];
+    float sums[kBoth * R];      // [R], then [R] with kLayer
     if (P.block) {
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        if (P.post) O::fma(bh[i], bh[i], st.y, LAYER ? -st.x * st.y : 0.f);
 #pragma unroll
-        for (int e = 0; e < V; ++e) q[i][0][e] = bh[i][e];
-        affine<T, V, 1>(post_w, post_b, P.params_f32, col[i], q[i]);
+        for (int r = 0; r < R; ++r) {
+          if (P.post) O::fma(bh[i][r], bh[i][r], st[r].y, LAYER ? -st[r].x * st[r].y : 0.f);
+#pragma unroll
+          for (int e = 0; e < V; ++e) q[i][r][e] = bh[i][r][e];
+        }
+        affine<T, V, R>(post_w, post_b, P.params_f32, col[i], q[i]);
       }
     }
     if (P.pre) {
-      sums[0] = sums[1] = 0.f;
+#pragma unroll
+      for (int m = 0; m < kBoth * R; ++m) sums[m] = 0.f;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        if (P.block) {
-          O::mul(hat[i][0], hat[i][0], a);
-          if (P.gate_kind == kGateNone || P.gate_kind == kGateRow) {
-            O::fma(hat[i][0], q[i][0], s * row_gate, hat[i][0]);
-          } else {
-            float f[V];
-            load_gate(i, f);
-            O::mul(f, f, q[i][0]);
-            O::fma(hat[i][0], f, s, hat[i][0]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (P.block) {
+            O::mul(hat[i][r], hat[i][r], a);
+            if (P.gate_kind == kGateNone || P.gate_kind == kGateRow) {
+              O::fma(hat[i][r], q[i][r], s * row_gate[r], hat[i][r]);
+            } else {
+              float f[V];
+              load_gate(i, r, f);
+              O::mul(f, f, q[i][r]);
+              O::fma(hat[i][r], f, s, hat[i][r]);
+            }
+          }
+          O::fma(hat[i][r], hat[i][r], st[r].w, LAYER ? -st[r].z * st[r].w : 0.f);
+          if (live[r]) {                                          // (a row that does not exist adds nothing to the column sums)
+            O::fma(sum[0][i], u[i][r], hat[i][r], sum[0][i]);
+            O::add(sum[1][i], sum[1][i], u[i][r]);
           }
         }
-        O::fma(hat[i][0], hat[i][0], st.w, LAYER ? -st.z * st.w : 0.f);
-        if (live) {                                          // (a row that does not exist adds nothing to the column sums)
-          O::fma(sum[0][i], u[i][0], hat[i][0], sum[0][i]);
-          O::add(sum[1][i], sum[1][i], u[i][0]);
-        }
-        affine<T, V, 1>(P.weight, nullptr, P.params_f32, col[i], u[i]);
-        const float t0 = O::dot(u[i][0], hat[i][0]), t1 = LAYER ? O::sum(u[i][0]) : 0.f;
-        if (in[i]) {
-          sums[0] += t0;
-          sums[1] += t1;
+        affine<T, V, R>(P.weight, nullptr, P.params_f32, col[i], u[i]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float t0 = O::dot(u[i][r], hat[i][r]), t1 = LAYER ? O::sum(u[i][r]) : 0.f;
+          if (in[i]) {
+            sums[r] += t0;
+            if (LAYER) sums[(kBoth - 1) * R + r] += t1;
+          }
         }
       }
-      row_sums<L, LAYER ? 2 : 1>(reinterpret_cast<float (&)[LAYER ? 2 : 1]>(sums), scratch);
-      const float m0 = -sums[0] * P.inv_channels * st.w, m1 = LAYER ? -sums[1] * P.inv_channels * st.w : 0.f;
+      row_sums<L, kBoth * R>(sums, scratch);
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        if (LAYER) O::add(d[i], d[i], m1);
-        O::fma(d[i], u[i][0], st.w, d[i]);
-        O::fma(d[i], hat[i][0], m0, d[i]);
+      for (int r = 0; r < R; ++r) {
+        const float m0 = -sums[r] * P.inv_channels * st[r].w, m1 = LAYER ? -sums[(kBoth - 1) * R + r] * P.inv_channels * st[r].w : 0.f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+          if (LAYER) O::add(d[i][r], d[i][r], m1);
+          O::fma(d[i][r], u[i][r], st[r].w, d[i][r]);
+          O::fma(d[i][r], hat[i][r], m0, d[i][r]);
+        }
       }
     }
     if (P.dx)
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        float o[V];
-        O::mul(o, d[i], a);
-        if (live && in[i]) store_f32<T, V>(static_cast<T *>(P.dx) + row * P.channels + col[i], o);
-      }
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+          float o[V];
+          O::mul(o, d[i][r], a);
+          if (live[r] && in[i]) store_f32<T, V>(static_cast<T *>(P.dx) + row[r] * P.channels + col[i], o);
+        }
     if (P.block) {
-      sums[0] = sums[1] = 0.f;
-      float gate_sum[1] = {0.f};
+#pragma unroll
+      for (int m = 0; m < kBoth * R; ++m) sums[m] = 0.f;
+      float gate_sum[R] = {};
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        O::mul(d[i], d[i], s);
-        if (P.gate_kind != kGateNone) {
-          O::mul(q[i][0], q[i][0], d[i]);                  // gradient of the gate
-          if (P.gate_kind == kGateRow) {
-            const float t = O::sum(q[i][0]);
-            if (in[i]) gate_sum[0] += t;
-            O::mul(d[i], d[i], row_gate);
-          } else {
-            if (P.gate_kind == kGateChannel && live) O::add(sum[4][i], sum[4][i], q[i][0]);
-            if (P.gate_kind == kGateFull && P.dgate && live && in[i]) store_f32<T, V>(static_cast<T *>(P.dgate) + row * P.channels + col[i], q[i][0]);
-            float f[V];
-            load_gate(i, f);
-            O::mul(d[i], d[i], f);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          O::mul(d[i][r], d[i][r], s);
+          if (P.gate_kind != kGateNone) {
+            O::mul(q[i][r], q[i][r], d[i][r]);                  // gradient of the gate
+            if (P.gate_kind == kGateRow) {
+              const float t = O::sum(q[i][r]);
+              if (in[i]) gate_sum[r] += t;
+              O::mul(d[i][r], d[i][r], row_gate[r]);
+            } else {
+              if (P.gate_kind == kGateChannel && live[r]) O::add(sum[4][i], sum[4][i], q[i][r]);
+              if (P.gate_kind == kGateFull && P.dgate && live[r] && in[i])
+                store_f32<T, V>(static_cast<T *>(P.dgate) + row[r] * P.channels + col[i], q[i][r]);
+              float f[V];
+              load_gate(i, r, f);
+              O::mul(d[i][r], d[i][r], f);
+            }
           }
         }
         if (P.post) {
-          if (live) {
-            O::fma(sum[2][i], d[i], bh[i], sum[2][i]);
-            O::add(sum[3][i], sum[3][i], d[i]);
-          }
-          if (post_w) {
-            float f[V];
-            load_param<T, V>(post_w, P.params_f32, col[i], f);
-            O::mul(d[i], d[i], f);
-          }
-          const float t0 = O::dot(d[i], bh[i]), t1 = LAYER ? O::sum(d[i]) : 0.f;
-          if (in[i]) {
-            sums[0] += t0;
-            sums[1] += t1;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (live[r]) {
+              O::fma(sum[2][i], d[i][r], bh[i][r], sum[2][i]);
+              O::add(sum[3][i], sum[3][i], d[i][r]);
+            }
+          affine<T, V, R>(post_w, nullptr, P.params_f32, col[i], d[i]);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float t0 = O::dot(d[i][r], bh[i][r]), t1 = LAYER ? O::sum(d[i][r]) : 0.f;
+            if (in[i]) {
+              sums[r] += t0;
+              if (LAYER) sums[(kBoth - 1) * R + r] += t1;
+            }
           }
         }
       }
       if (P.gate_kind == kGateRow && P.dgate) {
-        row_sums<L, 1>(gate_sum, scratch);
-        if (live && g == 0) static_cast<T *>(P.dgate)[row] = from_f32<T>(gate_sum[0]);
+        row_sums<L, R>(gate_sum, scratch);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (live[r] && g == 0) static_cast<T *>(P.dgate)[row[r]] = from_f32<T>(gate_sum[r]);
       }
       if (P.dblock) {
         if (P.post) {
-          row_sums<L, LAYER ? 2 : 1>(reinterpret_cast<float (&)[LAYER ? 2 : 1]>(sums), scratch);
-          const float m0 = -sums[0] * P.inv_channels, m1 = LAYER ? -sums[1] * P.inv_channels : 0.f;
+          row_sums<L, kBoth * R>(sums, scratch);
 #pragma unroll
-          for (int i = 0; i < ITEMS; ++i) {
-            if (LAYER) O::add(d[i], d[i], m1);
-            O::fma(d[i], bh[i], m0, d[i]);
-            O::mul(d[i], d[i], st.y);
+          for (int r = 0; r < R; ++r) {
+            const float m0 = -sums[r] * P.inv_channels, m1 = LAYER ? -sums[(kBoth - 1) * R + r] * P.inv_channels : 0.f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+              if (LAYER) O::add(d[i][r], d[i][r], m1);
+              O::fma(d[i][r], bh[i][r], m0, d[i][r]);
+              O::mul(d[i][r], d[i][r], st[r].y);
+            }
           }
         }
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-          if (live && in[i]) store_f32<T, V>(static_cast<T *>(P.dblock) + row * P.channels + col[i], d[i]);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < ITEMS; ++i)
+            if (live[r] && in[i]) store_f32<T, V>(static_cast<T *>(P.dblock) + row[r] * P.channels + col[i], d[i][r]);
       }
     }
   }
@@ -687,19 +731,20 @@ static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaS
     SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), smem, st, P));
     return SPIRA_B200_OK;
   }
-  // (column sums of a CTA reuse the ring: 256 / L rows of L * ITEMS * V columns)
-  constexpr int kColumns = kRows > 1 ? kThreads * ITEMS * V * 4 : 0;
-  const int tensors = backward_tensors(P), ring = Ring<kThreads, ITEMS, 5, kWide>::bytes(tensors), smem = ring > kColumns ? ring : kColumns;
-  const auto kernel = norm_backward_kernel<T, V, L, ITEMS, LAYER>;
-  const int64_t rounds = div_up(P.n, kRows);
+  constexpr int RB = L <= 32 && ITEMS == 1 ? 2 : 1, kBackward = kBackwardThreads<V, L, RB>, kBackwardRows = kBackward / L;
+  // (column sums of a CTA reuse the ring: kBackward / L rows of L * ITEMS * V columns)
+  constexpr int kColumns = kBackwardRows > 1 ? kBackward * ITEMS * V * 4 : 0;
+  const int tensors = backward_tensors(P), ring = Ring<kBackward, ITEMS * RB, 5, kWide>::bytes(tensors), smem = ring > kColumns ? ring : kColumns;
+  const auto kernel = norm_backward_kernel<T, V, L, ITEMS, RB, LAYER>;
+  const int64_t rounds = div_up(P.n, kBackwardRows * RB);
   const int rc = allow_smem(kernel, smem);
   if (rc != SPIRA_B200_OK) return rc;
   static int resident[6] = {0, 0, 0, 0, 0, 0};
-  if (resident[tensors] == 0) resident[tensors] = resident_ctas(kernel, kThreads, smem);
+  if (resident[tensors] == 0) resident[tensors] = resident_ctas(kernel, kBackward, smem);
   const int64_t cap = static_cast<int64_t>(sm_count()) * (resident[tensors] < kNormBackwardCtas ? resident[tensors] : kNormBackwardCtas);
   const int grid = static_cast<int>(rounds < cap ? rounds : cap);
   *ctas = grid;
-  SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kThreads), smem, st, P));
+  SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kBackward), smem, st, P));
   return SPIRA_B200_OK;
 }
 
