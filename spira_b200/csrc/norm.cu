@@ -12,8 +12,8 @@
 // the saved row statistics, so it needs neither output of the forward pass.  Parameter gradients are column sums: a thread
 // owns its columns for all rows its CTA visits, CTAs write partial sums, a second launch adds those in a fixed order.
 // Bound by memory and instructions together: forward 2 row reads + 2 row writes, backward 4 + 2 (one more of each with a
-// gate per element).  127 363 x 256 bf16, layer norms on both sides, a gate per element, fp32 parameters: forward 63 us =
-// 5.2 TB/s, backward 111 us = 4.7 TB/s; 127 363 x 96 fp16 with one rms norm: 22 us = 4.4 TB/s.
+// gate per element).  127 363 x 256 bf16, layer norms on both sides, a gate per element, fp32 parameters: forward 62 us =
+// 5.3 TB/s, backward 107 us = 4.9 TB/s; 127 363 x 96 fp16 with one rms norm: 22 us = 4.4 TB/s.
 #include "common.cuh"
 #include "elem.cuh"
 #include "ptx.cuh"
@@ -202,19 +202,28 @@ __device__ __forceinline__ void row_sums(float (&v)[M], float *scratch) {
   }
 }
 
-// v[r] = w * v[r] + b with what there is of the two parameters, for R rows
-template <typename T, int V, int R>
+// v[r] = w * v[r] + b with what there is of the two parameters, for R rows.  BOTH: they usually come together (layer norms),
+// which is then one instruction per pair (127 363 x 256 bf16 forward 63 -> 62, backward 110 -> 107 us); asking for the pair
+// costs rms norms, which rarely have a bias, 20 registers (127 363 x 96 fp16 21.4 -> 23.4 us, held to three CTAs per SM 22.0).
+template <typename T, int V, int R, bool BOTH>
 __device__ __forceinline__ void affine(const void *w, const void *b, int f32, int c, float (&v)[R][V]) {
-  float q[V];
+  float q[V], t[V];
+  if (BOTH && w && b) {
+    load_param<T, V>(w, f32, c, q);
+    load_param<T, V>(b, f32, c, t);
+#pragma unroll
+    for (int r = 0; r < R; ++r) Ops<V>::fma(v[r], v[r], q, t);
+    return;
+  }
   if (w) {
     load_param<T, V>(w, f32, c, q);
 #pragma unroll
     for (int r = 0; r < R; ++r) Ops<V>::mul(v[r], v[r], q);
   }
   if (b) {
-    load_param<T, V>(b, f32, c, q);
+    load_param<T, V>(b, f32, c, t);
 #pragma unroll
-    for (int r = 0; r < R; ++r) Ops<V>::add(v[r], v[r], q);
+    for (int r = 0; r < R; ++r) Ops<V>::add(v[r], v[r], t);
   }
 }
 
@@ -288,9 +297,9 @@ __host__ __device__ __forceinline__ int backward_tensors(const NormParams &P) { 
 // these kernels is not memory alone but instructions and the latency of a row's chain (load, row sum, row sum, store):
 // loads run rounds ahead, options are tested per row and never per element, conversions and arithmetic work on pairs, two rows share the parameter
 // loads and overlap their sums.  Loads are clamped into the tensor instead of guarded; only stores and sums ask whether a
-// row or a piece exists.
+// row or a piece exists.  Pieces of 8 are held to 80 registers (no spills), so that three CTAs fit on an SM.
 template <typename T, int V, int L, int ITEMS, int R, bool LAYER>
-__global__ void __launch_bounds__(kNormThreads<L>) norm_forward_kernel(const __grid_constant__ NormParams P) {
+__global__ void __launch_bounds__(kNormThreads<L>, V == 8 && L <= 32 && ITEMS == 1 ? 3 : 1) norm_forward_kernel(const __grid_constant__ NormParams P) {
   __shared__ float scratch[64];
   pdl_trigger();
   pdl_wait();
@@ -363,11 +372,11 @@ __global__ void __launch_bounds__(kNormThreads<L>) norm_forward_kernel(const __g
       if (P.post) {
         normalise<L, ITEMS, R, V, LAYER>(p, in, P, scratch, block_mean, block_dev);
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) affine<T, V, R>(P.post_weight, P.post_bias, P.params_f32, col[i], p[i]);
+        for (int i = 0; i < ITEMS; ++i) affine<T, V, R, LAYER>(P.post_weight, P.post_bias, P.params_f32, col[i], p[i]);
       }
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        if (P.gate_kind == kGateChannel) affine<T, V, R>(P.gate, nullptr, P.params_f32, col[i], p[i]);
+        if (P.gate_kind == kGateChannel) affine<T, V, R, LAYER>(P.gate, nullptr, P.params_f32, col[i], p[i]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           if (P.gate_kind == kGateFull) {
@@ -385,7 +394,7 @@ __global__ void __launch_bounds__(kNormThreads<L>) norm_forward_kernel(const __g
       normalise<L, ITEMS, R, V, LAYER>(x, in, P, scratch, mean, dev);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        affine<T, V, R>(P.weight, P.bias, P.params_f32, col[i], x[i]);
+        affine<T, V, R, LAYER>(P.weight, P.bias, P.params_f32, col[i], x[i]);
 #pragma unroll
         for (int r = 0; r < R; ++r)
           if (in[i] && row0 + r < P.n) store_f32<T, V>(static_cast<T *>(P.normed) + static_cast<int64_t>(row0 + r) * P.channels + col[i], x[i][r]);
@@ -505,7 +514,7 @@ __global__ void __launch_bounds__(kBackwardThreads<V, L, R>, L > 32 || ITEMS > 1
 #pragma unroll
           for (int e = 0; e < V; ++e) q[i][r][e] = bh[i][r][e];
         }
-        affine<T, V, R>(post_w, post_b, P.params_f32, col[i], q[i]);
+        affine<T, V, R, LAYER>(post_w, post_b, P.params_f32, col[i], q[i]);
       }
     }
     if (P.pre) {
@@ -532,7 +541,7 @@ __global__ void __launch_bounds__(kBackwardThreads<V, L, R>, L > 32 || ITEMS > 1
             O::add(sum[1][i], sum[1][i], u[i][r]);
           }
         }
-        affine<T, V, R>(P.weight, nullptr, P.params_f32, col[i], u[i]);
+        affine<T, V, R, LAYER>(P.weight, nullptr, P.params_f32, col[i], u[i]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const float t0 = O::dot(u[i][r], hat[i][r]), t1 = LAYER ? O::sum(u[i][r]) : 0.f;
@@ -595,7 +604,7 @@ __global__ void __launch_bounds__(kBackwardThreads<V, L, R>, L > 32 || ITEMS > 1
               O::fma(sum[2][i], d[i][r], bh[i][r], sum[2][i]);
               O::add(sum[3][i], sum[3][i], d[i][r]);
             }
-          affine<T, V, R>(post_w, nullptr, P.params_f32, col[i], d[i]);
+          affine<T, V, R, LAYER>(post_w, nullptr, P.params_f32, col[i], d[i]);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const float t0 = O::dot(d[i][r], bh[i][r]), t1 = LAYER ? O::sum(d[i][r]) : 0.f;
