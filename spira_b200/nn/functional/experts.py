@@ -288,8 +288,9 @@ def _grouped(x, weights, offsets, bias, relu, want_mask=False):
     mask, workspace, room = None, 0, 0
     want_mask = want_mask and relu
     relu = 1 if relu else 0
-    # channels, strides or addresses off the 16-byte boundaries may need scratch
-    off = ((x.shape[1] | y.shape[1] | x.stride(0)) & 7) | ((x.data_ptr() | weights.data_ptr()) & 15)
+    # channels, strides or addresses off the 16-byte boundaries may need scratch, and so may rows that overlap
+    stride = x.stride(0)
+    off = ((x.shape[1] | y.shape[1] | stride) & 7) | ((x.data_ptr() | weights.data_ptr()) & 15) or stride < x.shape[1]
     if want_mask or off:
         need, mask_bytes = C.c_size_t(), C.c_size_t()
         _query(index, "spira_b200_grouped_linear_workspace", _grouped_desc(n, weights, offsets, relu, x, bias, y=y), C.byref(need), C.byref(mask_bytes))

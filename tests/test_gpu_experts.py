@@ -699,6 +699,35 @@ def test_block_behind_a_sparse_convolution_compiles():
             assert torch.equal(a._features, b._features)
 
 
+@pytest.mark.parametrize("n", [1, 300, 70_000])
+@pytest.mark.parametrize("step", [0, 8])
+def test_rows_that_overlap(n, step):
+    """Broadcast rows (all of them one row) and rows that start inside the one before: the same bits as of dense copies."""
+    from spira_b200.nn import functional as F
+    c = 64
+    base = whole(n * step + c, dtype=torch.float16, top=2)
+    lapped = base.as_strided((n, c), (step, 1))
+    dense = lapped.contiguous()
+    w = whole(3, c, c, dtype=torch.float16, top=1, seed=1)
+    o = torch.tensor([0, n // 3, n // 2, n], dtype=torch.int32, device="cuda")
+    r = F.expert_route(rand(n, 3), 2)
+    dy = whole(n, c, dtype=torch.float16, seed=2)
+    for relu in (False, True):
+        assert torch.equal(F.grouped_linear(lapped, w, o, relu=relu), F.grouped_linear(dense, w, o, relu=relu))
+    assert torch.equal(F.expert_dispatch(lapped, r), F.expert_dispatch(dense, r))
+    assert torch.equal(F.expert_route(lapped, 2).experts, F.expert_route(dense, 2).experts)
+    for a, b in zip(F.residual_norm(lapped, lapped, gate=lapped), F.residual_norm(dense, dense, gate=dense)):
+        assert torch.equal(a, b)
+    grads = []
+    for x, g in ((lapped, dy), (dense, dy), (dense, lapped)):
+        x, v = x.detach(), w.clone().requires_grad_(True)
+        x.requires_grad_(True)
+        grads.append(torch.autograd.grad(F.grouped_linear(x, v, o, relu=True), [x, v], g))
+    grads.append(torch.autograd.grad(F.grouped_linear(x, v, o, relu=True), [x, v], dense))
+    for a, b in (grads[0:2], grads[2:4]):
+        assert torch.equal(a[1], b[1]) and torch.equal(a[0], b[0])
+
+
 def test_offsets_past_32_bits():
     """Tensors of more than 2^31 elements: the last rows are what the same rows give on their own."""
     from spira_b200.nn import functional as F
