@@ -62,6 +62,15 @@ __device__ __forceinline__ void store_f32(T *p, const float (&f)[N]) {
   *reinterpret_cast<Vec<T, N> *>(p) = r;
 }
 
+// Allows a kernel `most` bytes of dynamic shared memory (48 KB with its static part need no permission).  The limit belongs to
+// the kernel on the current device and not to the call, so `most` is what the largest call of the kernel takes, whatever
+// this one needs: a call that set its own size could lower the limit between another thread's setting and its launch.
+template <typename K>
+inline int allow_smem(K kernel, size_t most) {
+  if (most > 40 * 1024) SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)));
+  return SPIRA_B200_OK;
+}
+
 inline int elem_size(int dtype) { return dtype == SPIRA_B200_F32 ? 4 : 2; }
 
 // Runs BODY with T = the element type of the code.

@@ -664,20 +664,24 @@ static int route_rows_per_cta(int64_t n, int64_t *rows_per_cta) {
 static size_t stash_bytes(int lanes, int k) { return static_cast<size_t>(kRouteThreads / lanes) * k * 8; }
 static size_t place_smem(int experts) { return static_cast<size_t>(3 * experts + 1 + kRouteWarps * (experts | 1)) * 4; }
 
-// (kernels may use 48 KB unasked; many experts or a large k take up to 200 KB)
+// `most`: what the largest call of this kernel takes (many experts or a large k: up to 200 KB)
 template <typename... KArgs>
-static int launch_route_kernel(void (*kernel)(KArgs...), int ctas, size_t smem, cudaStream_t st, const RouteParams &P) {
-  if (smem > 48 * 1024) SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+static int launch_route_kernel(void (*kernel)(KArgs...), int ctas, size_t smem, size_t most, cudaStream_t st, const RouteParams &P) {
+  const int rc = allow_smem(kernel, most);
+  if (rc != SPIRA_B200_OK) return rc;
   SB_CHECK_CUDA(launch_dependent(kernel, dim3(ctas), dim3(kRouteThreads), smem, st, P));
   return SPIRA_B200_OK;
 }
 
 template <typename T, int G, int EPL>
 static int launch_route(RouteParams &P, cudaStream_t st) {
-  if (P.n * P.k <= kSmallRouteEntries) return launch_route_kernel(route_small_kernel<T, G, EPL>, 1, place_smem(P.experts) + stash_bytes(G, P.k), st, P);
+  constexpr int kE = G * EPL, kK = kE < kMaxTopK ? kE : kMaxTopK;      // most experts and choices of this kernel
+  auto small = [](int experts, int k) { return place_smem(experts) + stash_bytes(G, k); };
+  auto choose = [](int experts, int k) { return static_cast<size_t>(experts) * 4 + stash_bytes(G, k); };
+  if (P.n * P.k <= kSmallRouteEntries) return launch_route_kernel(route_small_kernel<T, G, EPL>, 1, small(P.experts, P.k), small(kE, kK), st, P);
   const int ctas = route_rows_per_cta(P.n, &P.rows_per_cta);
-  const int rc = launch_route_kernel(route_choose_kernel<T, G, EPL>, ctas, static_cast<size_t>(P.experts) * 4 + stash_bytes(G, P.k), st, P);
-  return rc != SPIRA_B200_OK ? rc : launch_route_kernel(route_place_kernel, ctas, place_smem(P.experts), st, P);
+  const int rc = launch_route_kernel(route_choose_kernel<T, G, EPL>, ctas, choose(P.experts, P.k), choose(kE, kK), st, P);
+  return rc != SPIRA_B200_OK ? rc : launch_route_kernel(route_place_kernel, ctas, place_smem(P.experts), place_smem(kMaxExperts), st, P);
 }
 
 template <typename T>

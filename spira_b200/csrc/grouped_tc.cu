@@ -810,7 +810,8 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int w_pitch, int 
   const int64_t workers = pair ? sm_count() / 2 : sm_count();
   const unsigned grid = static_cast<unsigned>(tiles < workers ? (tiles < 1 ? 1 : tiles) : workers) * (pair ? 2 : 1);
   auto go = [&](auto kernel) -> int {
-    SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    const int allowed = allow_smem(kernel, kGSmemBudget + 1024);      // (what `stages` is cut to)
+    if (allowed != SPIRA_B200_OK) return allowed;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kGThreads);

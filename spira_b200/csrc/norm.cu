@@ -708,18 +708,16 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__
   }
 }
 
-// Allows a kernel its shared memory (48 KB with its static part need no permission), on the current device (every device of the process is told on its own).
+// CTAs of a kernel that fit on an SM with its shared memory, asked once per kernel and number of tensors (`known`; the answer is
+// the same whoever writes it, and a query that failed leaves none).
 template <typename K>
-static int allow_smem(K kernel, int smem) {
-  if (smem > 40 * 1024) SB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  return SPIRA_B200_OK;
-}
-
-// CTAs of a kernel that fit on an SM with its shared memory (asked once per kernel and number of tensors; the answer is the same whoever writes it).
-template <typename K>
-static int resident_ctas(K kernel, int threads, int smem) {
-  int n = 0;
-  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0 ? n : 1;
+static int resident_ctas(K kernel, int threads, int smem, int &known) {
+  int n = known;
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) return 1;
+    known = n;
+  }
+  return n;
 }
 
 template <typename T, int V, int L, int ITEMS, bool LAYER>
@@ -729,28 +727,30 @@ static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaS
   constexpr bool kWide = V * sizeof(T) == 16;
   if (!backward) {
     constexpr int R = L <= 32 && ITEMS == 1 ? 2 : 1;
-    const int tensors = forward_tensors(P), smem = Ring<kThreads, ITEMS * R, 3, kWide>::bytes(tensors);
+    typedef Ring<kThreads, ITEMS * R, 3, kWide> Rows;
+    const int tensors = forward_tensors(P), smem = Rows::bytes(tensors);
     const auto kernel = norm_forward_kernel<T, V, L, ITEMS, R, LAYER>;
     const int64_t rounds = div_up(P.n, kRows * R);
-    const int rc = allow_smem(kernel, smem);
+    const int rc = allow_smem(kernel, Rows::bytes(3));
     if (rc != SPIRA_B200_OK) return rc;
     static int resident[4] = {0, 0, 0, 0};
-    if (resident[tensors] == 0) resident[tensors] = resident_ctas(kernel, kThreads, smem);
-    const int64_t cap = static_cast<int64_t>(sm_count()) * resident[tensors];
+    const int64_t cap = static_cast<int64_t>(sm_count()) * resident_ctas(kernel, kThreads, smem, resident[tensors]);
     SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), smem, st, P));
     return SPIRA_B200_OK;
   }
   constexpr int RB = L <= 32 && ITEMS == 1 ? 2 : 1, kBackward = kBackwardThreads<V, L, RB>, kBackwardRows = kBackward / L;
   // (column sums of a CTA reuse the ring: kBackward / L rows of L * ITEMS * V columns)
   constexpr int kColumns = kBackwardRows > 1 ? kBackward * ITEMS * V * 4 : 0;
-  const int tensors = backward_tensors(P), ring = Ring<kBackward, ITEMS * RB, 5, kWide>::bytes(tensors), smem = ring > kColumns ? ring : kColumns;
+  typedef Ring<kBackward, ITEMS * RB, 5, kWide> Rows;
+  auto need = [](int tensors) { return Rows::bytes(tensors) > kColumns ? Rows::bytes(tensors) : kColumns; };
+  const int tensors = backward_tensors(P), smem = need(tensors);
   const auto kernel = norm_backward_kernel<T, V, L, ITEMS, RB, LAYER>;
   const int64_t rounds = div_up(P.n, kBackwardRows * RB);
-  const int rc = allow_smem(kernel, smem);
+  const int rc = allow_smem(kernel, need(5));
   if (rc != SPIRA_B200_OK) return rc;
   static int resident[6] = {0, 0, 0, 0, 0, 0};
-  if (resident[tensors] == 0) resident[tensors] = resident_ctas(kernel, kBackward, smem);
-  const int64_t cap = static_cast<int64_t>(sm_count()) * (resident[tensors] < kNormBackwardCtas ? resident[tensors] : kNormBackwardCtas);
+  const int fit = resident_ctas(kernel, kBackward, smem, resident[tensors]);
+  const int64_t cap = static_cast<int64_t>(sm_count()) * (fit < kNormBackwardCtas ? fit : kNormBackwardCtas);
   const int grid = static_cast<int>(rounds < cap ? rounds : cap);
   *ctas = grid;
   SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kBackward), smem, st, P));

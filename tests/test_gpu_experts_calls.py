@@ -1,0 +1,101 @@
+"""GPU: the expert and norm operators called in ways that a program may call them: from several threads at once, with a routing
+that the caller changed, under forward-mode differentiation, on every kernel that the sizes choose between."""
+import ctypes
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from test_gpu_experts import rand
+
+pytestmark = pytest.mark.gpu
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+# ------------------------------------------------------------------------------------------------ threads
+# Two threads call one function of the library as fast as they can, without Python between the calls.
+TWO_THREADS = r"""
+#include <atomic>
+#include <cstring>
+#include <thread>
+#include "spira_b200.h"
+struct Route { const void *logits; int64_t n; int32_t experts, k; float *weights; int32_t *chosen, *slots, *order, *offsets; };
+extern "C" int two_threads(const char *name, void *fn, const char *(*last_error)(void), const void *const *calls, void *const *streams, int32_t *status,
+                           int rounds, char *message) {
+  std::atomic<int> failed(0), ready(0);
+  auto one = [&](int i) -> int {
+    if (std::strcmp(name, "norm") == 0)
+      return reinterpret_cast<decltype(&spira_b200_residual_norm)>(fn)(static_cast<const spira_b200_norm_desc *>(calls[i]), streams[i]);
+    if (std::strcmp(name, "products") == 0)
+      return reinterpret_cast<decltype(&spira_b200_grouped_linear)>(fn)(static_cast<const spira_b200_grouped_desc *>(calls[i]), nullptr, 0, status, streams[i]);
+    const Route &q = *static_cast<const Route *>(calls[i]);
+    return reinterpret_cast<decltype(&spira_b200_expert_route)>(fn)(q.logits, SPIRA_B200_F32, q.n, q.experts, q.experts, q.k, 1, q.weights, q.chosen,
+                                                                     q.slots, q.order, q.offsets, nullptr, 0, streams[i]);
+  };
+  auto work = [&](int i) {
+    ++ready;
+    while (ready < 2) {}
+    for (int r = 0; r < rounds; ++r)
+      if (one(i) != 0 && failed++ == 0) std::strncpy(message, last_error(), 255);
+  };
+  std::thread a(work, 0), b(work, 1);
+  a.join();
+  b.join();
+  return failed;
+}
+"""
+
+
+class RouteCall(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("n", ctypes.c_int64), ("experts", ctypes.c_int32), ("k", ctypes.c_int32)] + \
+               [(q, ctypes.c_void_p) for q in ("weights", "chosen", "slots", "order", "offsets")]
+
+
+@pytest.mark.parametrize("kind", ["norm", "products", "routing"])
+def test_threads_that_launch_one_kernel_with_different_sizes(kind, tmp_path):
+    """Calls of one kernel that take different amounts of shared memory do not disturb each other, and each has its own result."""
+    from spira_b200 import _lib
+    from spira_b200.nn import functional as F
+    from spira_b200.nn.functional import _C, experts, norms
+    (tmp_path / "threads.cpp").write_text(TWO_THREADS)
+    subprocess.run(["g++", "-O2", "-shared", "-fPIC", "-pthread", "-I", str(ROOT / "include"), "-o", str(tmp_path / "threads.so"),
+                    str(tmp_path / "threads.cpp")], check=True)
+    run = ctypes.CDLL(str(tmp_path / "threads.so")).two_threads
+    lib, calls, keep, pairs = _lib.load(), [], [], []
+    if kind == "norm":                       # rows of three and of two tensors on their way
+        fn, x = lib.spira_b200_residual_norm, rand(64, 96, dtype=torch.float16)
+        for gate, gate_kind in ((x, norms.GATE_FULL), (None, norms.GATE_NONE)):
+            out = torch.empty_like(x), torch.empty_like(x)
+            spec = norms._Spec(False, False, True, False, gate_kind, 1.0, 1.0, 1e-6)
+            calls.append(ctypes.create_string_buffer(norms._desc(spec, x, (x, gate, None, None, None, None), *out)))
+            pairs.append((out, F.residual_norm(x, x, gate=gate)))
+    elif kind == "products":                 # few and many groups, narrow and wide tiles
+        fn = lib.spira_b200_grouped_linear
+        for e, c in ((2, 64), (900, 256)):
+            x, w, y = rand(64, 64, dtype=torch.float16), rand(e, 64, c, dtype=torch.float16), torch.empty(64, c, dtype=torch.float16, device="cuda")
+            o = torch.full((e + 1,), 64, dtype=torch.int32, device="cuda")
+            o[0] = 0
+            calls.append(ctypes.create_string_buffer(experts._grouped_desc(64, w, o, 0, x, None, y=y)))
+            pairs.append(((y,), (F.grouped_linear(x, w, o),)))
+            keep.append((x, w, o))
+    else:                                    # different numbers of experts and choices
+        fn = lib.spira_b200_expert_route
+        for e, k in ((512, 32), (400, 2)):
+            logits = rand(16, e)
+            want = F.expert_route(logits, k)
+            got = [torch.empty_like(t) for t in want]
+            calls.append(RouteCall(logits.data_ptr(), 16, e, k, *(t.data_ptr() for t in got)))
+            pairs.append((got, want))
+            keep.append(logits)
+    streams = [torch.cuda.Stream() for _ in calls]
+    status, message = _C.status_word(torch.device("cuda", torch.cuda.current_device())), ctypes.create_string_buffer(256)
+    torch.cuda.synchronize()
+    failed = run(kind.encode(), ctypes.cast(fn, ctypes.c_void_p), ctypes.cast(lib.spira_b200_last_error, ctypes.c_void_p),
+                 (ctypes.c_void_p * 2)(*(ctypes.addressof(c) for c in calls)), (ctypes.c_void_p * 2)(*(s.cuda_stream for s in streams)),
+                 ctypes.c_void_p(status.data_ptr()), 10000, message)
+    torch.cuda.synchronize()
+    assert failed == 0, (failed, message.value)
+    for got, want in pairs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
