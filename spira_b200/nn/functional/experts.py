@@ -7,7 +7,7 @@
 
 No reference counterpart (the reference stops at convolutions, BatchNorm and ReLU).  All calls run on the current stream
 of their tensors' device, never synchronise, and may be captured into a CUDA graph.  Results do not depend on scheduling:
-the same inputs give the same bits.
+the same inputs give the same bits.  Gradients once and in reverse mode only; anything else is refused.
 """
 from __future__ import annotations
 
@@ -15,6 +15,7 @@ import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from spira_b200 import _lib
 from spira_b200.nn.functional import _C
@@ -49,8 +50,15 @@ def _fail(message: str):
     raise RuntimeError("[spira_b200] " + message)
 
 
+def _no_tangents(*tensors) -> None:
+    """Refuses tensors with a forward-mode tangent: kernels read the values alone, a result would say that it is constant."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _fail("the expert and norm operators have no forward-mode derivatives (an input has a tangent)")
+
+
 def _device_of(*tensors) -> int:
     """The device index all given tensors share; refuses CPU tensors and mixtures."""
+    _no_tangents(*tensors)
     index = -1
     for t in tensors:
         if t is None:
@@ -79,8 +87,9 @@ def _addr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _once() -> None:
-    """In a backward function: refuses to be recorded itself (``create_graph=True``)."""
+def _once(*grads) -> None:
+    """In a backward function: refuses to be recorded itself (``create_graph=True``), and gradients with tangents."""
+    _no_tangents(*grads)
     if torch.is_grad_enabled():
         _fail("the expert and norm operators can be differentiated once only (create_graph=True was asked for)")
 
@@ -129,7 +138,7 @@ class _Route(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dweights, *_):
-        _once()
+        _once(dweights)
         if dweights is None:
             return None, None, None
         logits, weights, chosen = ctx.saved_tensors
@@ -211,7 +220,7 @@ class _Dispatch(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, drows):
-        _once()
+        _once(drows)
         return _combine(_rows(drows), None, ctx.saved_tensors[0]), None, None
 
 
@@ -223,7 +232,7 @@ class _Combine(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        _once()
+        _once(dout)
         rows, weights, slots, offsets = ctx.saved_tensors
         dout = _rows(dout)
         (n, k), channels = slots.shape, rows.shape[1]
@@ -321,7 +330,7 @@ class _Grouped(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _once()
+        _once(dy)
         x, weights, offsets, y, mask = ctx.saved_tensors
         dy = _rows(dy)
         need = ctx.needs_input_grad

@@ -67,7 +67,7 @@ class _ResidualNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dstream, dnormed):
-        _once()
+        _once(dstream, dnormed)
         x, *params, stats = ctx.saved_tensors
         spec = ctx.spec
         if dstream is None and dnormed is None:

@@ -73,3 +73,25 @@ def test_modules_check_their_arguments():
     m = spnn.ResidualNorm(16, kind="layer", post=True, gate=True, gate_init=0.5)
     assert sorted(n for n, _ in m.named_parameters()) == ["bias", "gate", "post_bias", "post_weight", "weight"]
     assert sorted(n for n, _ in spnn.ResidualNorm(16).named_parameters()) == ["weight"]
+
+
+def test_forward_mode_tangents_are_refused():
+    """Any tensor argument may carry one; the refusal comes before everything else, so it needs no device."""
+    import torch.autograd.forward_ad as fw
+    from spira_b200.nn import functional as F
+    x, w, o = torch.zeros(4, 8), torch.zeros(2, 8, 8), torch.zeros(3, dtype=torch.int32)
+    routing = F.ExpertRouting(torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), o)
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+        calls = [lambda: F.expert_route(dual(x), 2), lambda: F.expert_dispatch(dual(x), routing), lambda: F.expert_combine(dual(torch.zeros(8, 8)), routing),
+                 lambda: F.expert_combine(torch.zeros(8, 8), routing._replace(weights=dual(routing.weights))), lambda: F.grouped_linear(dual(x), w, o),
+                 lambda: F.grouped_linear(x, dual(w), o), lambda: F.grouped_linear(x, w, o, dual(torch.zeros(2, 8))), lambda: F.residual_norm(dual(x)),
+                 lambda: F.residual_norm(x, dual(x)), lambda: F.residual_norm(x, weight=dual(x[0])), lambda: F.residual_norm(x, bias=dual(x[0])),
+                 lambda: F.residual_norm(x, x, gate=dual(x)), lambda: F.residual_norm(x, x, post=True, post_weight=dual(x[0])),
+                 lambda: F.residual_norm(x, x, post=True, post_bias=dual(x[0]))]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(NotImplementedError, match="CUDA"):      # (a level without tangents changes nothing)
+            F.residual_norm(x)

@@ -99,3 +99,27 @@ def test_threads_that_launch_one_kernel_with_different_sizes(kind, tmp_path):
     assert failed == 0, (failed, message.value)
     for got, want in pairs:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------ forward mode
+def test_forward_mode_tangents_are_refused():
+    """Inputs with a tangent, and gradients with one on their way back, are refused; a level without tangents changes nothing."""
+    import torch.autograd.forward_ad as fw
+    from spira_b200.nn import functional as F
+    x, w = rand(6, 8, dtype=torch.float16).requires_grad_(True), rand(2, 8, 8, dtype=torch.float16)
+    o = torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda")
+    r = F.expert_route(rand(6, 4), 2)
+    calls = [lambda t: F.expert_route(t, 2).weights, lambda t: F.expert_dispatch(t, r), lambda t: F.expert_combine(t.repeat(2, 1), r),
+             lambda t: F.grouped_linear(t, w, o), lambda t: F.residual_norm(t)[1], lambda t: F.residual_norm(t, t, pre=False)[0]]
+    for call in calls:
+        y = call(x)
+        want, = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+        with fw.dual_level():
+            for t in (fw.make_dual(x.detach(), torch.ones_like(x)), fw.make_dual(x, torch.ones_like(x))):
+                with pytest.raises(RuntimeError):
+                    call(t)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, x, fw.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
+            assert torch.equal(call(x.detach()), y)
+            got, = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+        assert torch.equal(got, want)
