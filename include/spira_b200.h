@@ -520,18 +520,28 @@ int spira_b200_expert_route_backward(const void *logits, int dtype, int64_t n, i
                                      int64_t dweights_row, int64_t dweights_col, void *dlogits, void *stream);
 
 /* rows[slots[t][j]] = x[t]; rows behind offsets[experts] are zero.  rows is [n * k][channels].  Places outside
- * [0, n * k) are skipped, here and below. */
+ * [0, n * k) are skipped, here and below.  The slots have to name every place below offsets[experts] and none behind it: rows of
+ * places that none names are left as they were, a place that two name holds one of the two rows. */
 int spira_b200_expert_dispatch(const void *x, int dtype, int64_t n, int64_t x_stride, int channels, const int32_t *slots, int k,
                                const int32_t *offsets, int experts, void *rows, void *stream);
+/* The same for any slots: rows of places that no slot names are zero, wherever they lie.  `order` is a hint, the row * k + j
+ * that a place belongs to: a place costs nothing if that slot names it, so an order that is older than the slots
+ * is right too; NULL: every row is cleared first. */
+int spira_b200_expert_dispatch_cleared(const void *x, int dtype, int64_t n, int64_t x_stride, int channels, const int32_t *slots,
+                                       const int32_t *order, int k, void *rows, void *stream);
 /* out[t] = sum over j of weights[t][j] * rows[slots[t][j]] (fp32 sum in the order of j; weights == NULL: ones). */
 int spira_b200_expert_combine(const void *rows, int dtype, int64_t n, int64_t row_stride, int channels, const float *weights,
                               int64_t weights_row, int64_t weights_col, const int32_t *slots, int k, void *out, void *stream);
 /* drows[slots[t][j]] = weights[t][j] * dout[t] (zero behind offsets[experts]), dweights[t][j] = <dout[t], rows[slots[t][j]]>;
- * either may be NULL. */
+ * either may be NULL.  Slots as in expert_dispatch, or any with the second form. */
 int spira_b200_expert_combine_backward(const void *rows, const void *dout, int dtype, int64_t n, int64_t row_stride,
                                        int64_t dout_stride, int channels, const float *weights, int64_t weights_row,
                                        int64_t weights_col, const int32_t *slots, int k, const int32_t *offsets, int experts,
                                        void *drows, float *dweights, void *stream);
+int spira_b200_expert_combine_backward_cleared(const void *rows, const void *dout, int dtype, int64_t n, int64_t row_stride,
+                                               int64_t dout_stride, int channels, const float *weights, int64_t weights_row,
+                                               int64_t weights_col, const int32_t *slots, const int32_t *order, int k, void *drows,
+                                               float *dweights, void *stream);
 
 /* Ragged products: group e holds the rows [offsets[e], offsets[e + 1]) of x[n][c_in] and has the matrix weight[e][c_in][c_out].
  *   spira_b200_grouped_linear      y[r] = relu?(x[r] W[e] + bias[e]); rows outside every group are zero

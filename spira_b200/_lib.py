@@ -170,6 +170,9 @@ SIGNATURES = {
                                 c_void_p, c_size_t, c_void_p],
     "spira_b200_expert_route_backward": [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64,
                                          c_int64, c_void_p, c_void_p],
+    "spira_b200_expert_dispatch_cleared": [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
+    "spira_b200_expert_combine_backward_cleared": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64,
+                                                   c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
     "spira_b200_expert_dispatch": [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p],
     "spira_b200_expert_combine": [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p],
     "spira_b200_expert_combine_backward": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
@@ -221,7 +224,7 @@ KERNELS_PER_CALL = {
     "spira_b200_kmap_masks": 1, "spira_b200_kmap_masks_half": 1, "spira_b200_kmap_lists_from_masks": 3, "spira_b200_convert_transposed_os": 1, "spira_b200_transpose_map": 1,
     "spira_b200_pack_weights": 1, "spira_b200_conv_os": 1, "spira_b200_conv_os_grouped": 1, "spira_b200_conv_os_split": 1,
     "spira_b200_kmap_group": 2,
-    "spira_b200_expert_route": 1, "spira_b200_expert_route_backward": 1, "spira_b200_expert_dispatch": 1, "spira_b200_expert_combine": 1,
+    "spira_b200_expert_route": 1, "spira_b200_expert_route_backward": 1, "spira_b200_expert_dispatch_cleared": 2, "spira_b200_expert_combine_backward_cleared": 2, "spira_b200_expert_dispatch": 1, "spira_b200_expert_combine": 1,
     "spira_b200_expert_combine_backward": 1, "spira_b200_grouped_linear": 1, "spira_b200_grouped_linear_backward": 2,
     "spira_b200_residual_norm": 1, "spira_b200_residual_norm_backward": 1,
     "spira_b200_conv_ws": 2, "spira_b200_conv_ws_fused": 1, "spira_b200_conv_ws_static": 2,

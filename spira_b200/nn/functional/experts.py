@@ -193,12 +193,22 @@ def _check_rows(t: torch.Tensor, name: str, rows: int) -> torch.Tensor:
     return _rows(t)
 
 
-def _dispatch(feats, slots, offsets):
+def _order_hint(routing: ExpertRouting, slots: torch.Tensor) -> Optional[torch.Tensor]:
+    """``routing.order`` where it can tell the kernels which places are taken.  They check what it says: places that no slot names
+    are cleared whatever it holds (a caller may have taken slots out of a routing), a right one only spares them the rest."""
+    o = routing.order
+    if isinstance(o, torch.Tensor) and o.dtype is torch.int32 and o.shape == (slots.numel(),) and o.is_contiguous() \
+            and o.get_device() == slots.get_device():
+        return o
+    return None
+
+
+def _dispatch(feats, slots, order):
     n, k = slots.shape
     channels = feats.shape[1]
     rows = _dense(feats, n * k, channels)
-    _launch(feats.get_device(), "spira_b200_expert_dispatch", feats.data_ptr(), _DTYPES[feats.dtype], n, feats.stride(0), channels,
-            slots.data_ptr(), k, offsets.data_ptr(), offsets.shape[0] - 1, rows.data_ptr())
+    _launch(feats.get_device(), "spira_b200_expert_dispatch_cleared", feats.data_ptr(), _DTYPES[feats.dtype], n, feats.stride(0), channels,
+            slots.data_ptr(), _addr(order), k, rows.data_ptr())
     return rows
 
 
@@ -214,9 +224,9 @@ def _combine(rows, weights, slots):
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, feats, slots, offsets):
+    def forward(ctx, feats, slots, order):
         ctx.save_for_backward(slots)
-        return _dispatch(feats, slots, offsets)
+        return _dispatch(feats, slots, order)
 
     @staticmethod
     def backward(ctx, drows):
@@ -226,39 +236,41 @@ class _Dispatch(torch.autograd.Function):
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, weights, slots, offsets):
-        ctx.save_for_backward(rows, weights, slots, offsets)
+    def forward(ctx, rows, weights, slots, order):
+        ctx.save_for_backward(rows, weights, slots, order)
         return _combine(rows, weights, slots)
 
     @staticmethod
     def backward(ctx, dout):
         _once(dout)
-        rows, weights, slots, offsets = ctx.saved_tensors
+        rows, weights, slots, order = ctx.saved_tensors
         dout = _rows(dout)
         (n, k), channels = slots.shape, rows.shape[1]
         drows = _dense(rows, n * k, channels) if ctx.needs_input_grad[0] else None
         dweights = _dense(weights, n, k) if ctx.needs_input_grad[1] else None
-        _launch(rows.get_device(), "spira_b200_expert_combine_backward", rows.data_ptr(), dout.data_ptr(), _DTYPES[rows.dtype], n,
-                rows.stride(0), dout.stride(0), channels, weights.data_ptr(), weights.stride(0), weights.stride(1), slots.data_ptr(), k,
-                offsets.data_ptr(), offsets.shape[0] - 1, None if drows is None else drows.data_ptr(),
-                None if dweights is None else dweights.data_ptr())
+        _launch(rows.get_device(), "spira_b200_expert_combine_backward_cleared", rows.data_ptr(), dout.data_ptr(), _DTYPES[rows.dtype], n,
+                rows.stride(0), dout.stride(0), channels, weights.data_ptr(), weights.stride(0), weights.stride(1), slots.data_ptr(),
+                _addr(order), k, None if drows is None else drows.data_ptr(), None if dweights is None else dweights.data_ptr())
         return drows, dweights, None, None
 
 
 def expert_dispatch(feats: torch.Tensor, routing: ExpertRouting) -> torch.Tensor:
-    """``feats [N, C]`` -> ``[N * k, C]`` in the expert order of ``routing`` (a row appears once per expert it goes to); rows
-    behind ``routing.offsets[E]`` are zero."""
+    """``feats [N, C]`` -> ``[N * k, C]`` in the expert order of ``routing`` (a row appears once per expert it goes to); rows of
+    places that no slot names are zero (those behind ``routing.offsets[E]``, and those of pairs that were taken out of the
+    routing by setting their slot to -1).  Slots are distinct; a place that two of them name holds one of the two rows."""
     slots, offsets = _check_routing(routing)
     _device_of(feats, slots, offsets)
     feats = _check_rows(feats, "feats", slots.shape[0])
+    order = _order_hint(routing, slots)
     if _needs_grad(feats):
-        return _Dispatch.apply(feats, slots, offsets)
-    return _dispatch(feats, slots, offsets)
+        return _Dispatch.apply(feats, slots, order)
+    return _dispatch(feats, slots, order)
 
 
 def expert_combine(rows: torch.Tensor, routing: ExpertRouting) -> torch.Tensor:
     """``rows [N * k, C]`` in expert order -> ``[N, C]``: every voxel's rows, weighted with ``routing.weights`` and added in
-    the order of its experts (fp32, one rounding).  Voxels without an expert are zero."""
+    the order of its experts (fp32, one rounding).  Voxels without an expert are zero, and so is the gradient of rows that no
+    slot names."""
     slots, offsets = _check_routing(routing)
     weights = routing.weights
     _device_of(rows, slots, offsets, weights)
@@ -266,7 +278,7 @@ def expert_combine(rows: torch.Tensor, routing: ExpertRouting) -> torch.Tensor:
         _fail(f"routing.weights is expected to be float32 {tuple(slots.shape)}, got {weights.dtype} {tuple(weights.shape)}")
     rows = _check_rows(rows, "rows", slots.shape[0] * slots.shape[1])
     if _needs_grad(rows, weights):
-        return _Combine.apply(rows, weights, slots, offsets)
+        return _Combine.apply(rows, weights, slots, _order_hint(routing, slots))
     return _combine(rows, weights, slots)
 
 

@@ -95,3 +95,18 @@ def test_forward_mode_tangents_are_refused():
                 call()
         with pytest.raises(NotImplementedError, match="CUDA"):      # (a level without tangents changes nothing)
             F.residual_norm(x)
+
+
+def test_library_refuses_bad_arguments_of_the_cleared_forms(lib):
+    err = lib.spira_b200_last_error
+    dispatch, backward = lib.spira_b200_expert_dispatch_cleared, lib.spira_b200_expert_combine_backward_cleared
+    assert dispatch(None, 0, 0, 8, 8, None, None, 2, None, None) == 0                      # no rows
+    assert dispatch(None, 0, 4, 8, 8, None, None, 2, None, None) != 0 and b"null pointer" in err()
+    assert dispatch(None, 0, 4, 8, 8, None, None, 33, None, None) != 0 and b"top_k=33" in err()
+    assert dispatch(None, 3, 4, 8, 8, None, None, 2, None, None) != 0 and b"element type" in err()
+    assert dispatch(None, 0, 1 << 30, 8, 8, None, None, 2, None, None) != 0 and b"out of range" in err()
+    assert dispatch(None, 0, 4, 8, 0, None, None, 2, None, None) != 0 and b"channels" in err()
+    assert dispatch(None, 0, 4, -8, 8, None, None, 2, None, None) != 0 and b"stride" in err()
+    assert backward(None, None, 0, 0, 8, 8, 8, None, 0, 0, None, None, 2, None, None, None) == 0
+    assert backward(None, None, 0, 4, 8, 8, 8, None, 0, 0, None, None, 2, None, None, None) != 0 and b"null pointer" in err()
+    assert backward(None, None, 0, 4, 8, 8, 8, None, 0, 0, None, None, 0, None, None, None) != 0 and b"top_k=0" in err()

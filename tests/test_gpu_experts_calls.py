@@ -7,7 +7,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from test_gpu_experts import rand
+from test_gpu_experts import ANY, rand, whole
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,97 @@ def test_forward_mode_tangents_are_refused():
             assert torch.equal(call(x.detach()), y)
             got, = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------ a routing that the caller changed
+def stale_memory(n, c, dtype):
+    """Leaves NaN in the memory that the next tensors of this size get."""
+    t = [torch.full((n, c), float("nan"), dtype=dtype, device="cuda") for _ in range(6)]
+    torch.cuda.synchronize()
+    del t
+
+
+@pytest.mark.parametrize("dtype", ANY)
+@pytest.mark.parametrize("n,c,e,k", [(1, 8, 4, 2), (17, 33, 5, 3), (700, 96, 8, 2), (90, 1028, 9, 4), (3000, 7, 16, 2)])
+def test_rows_that_no_slot_names_are_zero(dtype, n, c, e, k):
+    """Pairs taken out of a routing, places exchanged, an order that is older than the slots, senseless or absent: rows and
+    gradients are those of the slots, and zero where there is none."""
+    from spira_b200.nn import functional as F
+    logits = rand(n, e)
+    if n > 1:
+        logits[n // 2:n // 2 + n // 8] = float("-inf")
+    r = F.expert_route(logits, k)
+    g = torch.Generator().manual_seed(n + c)
+    dropped = r.slots.masked_fill((torch.rand(n, k, generator=g) < 0.2).cuda(), -1)
+    none = torch.full_like(r.slots, -1)
+    shuffle = torch.randperm(n * k, generator=g).int().cuda()
+    moved = torch.where(r.slots >= 0, shuffle[r.slots.clamp_min(0).long()], -1)           # (places that the order does not know)
+    odd = torch.randint(-5, 2 * n * k, (n * k,), generator=g).int().cuda()
+    x, y = whole(n, c, dtype=dtype, seed=1).requires_grad_(True), whole(n * k, c, dtype=dtype, top=8, seed=2).requires_grad_(True)
+    w = (2.0 ** -torch.randint(0, 4, (n, k), device="cuda").float()).requires_grad_(True)
+    drows, dout = whole(n * k, c, dtype=dtype, seed=3), whole(n, c, dtype=dtype, seed=4)
+    for slots in (r.slots, dropped, none, moved, moved.masked_fill(dropped < 0, -1)):
+        for order in (r.order, odd, torch.full_like(r.order, -1), None, r.order[:-1], r.order.long()):
+            q = r._replace(slots=slots, weights=w, order=order)
+            stale_memory(n * k, c, dtype)
+            rows, out = F.expert_dispatch(x, q), F.expert_combine(y, q)
+            stale_memory(n * k, c, dtype)
+            dx, dy, dw = torch.autograd.grad([rows, out], [x, y, w], [drows, dout])
+            want_rows, want_out = torch.zeros(n * k, c, dtype=torch.float64, device="cuda"), torch.zeros(n, c, dtype=torch.float64, device="cuda")
+            want_dx, want_dy, want_dw = torch.zeros_like(want_out), torch.zeros_like(want_rows), torch.zeros(n, k, dtype=torch.float64, device="cuda")
+            for j in range(k):
+                t = (slots[:, j] >= 0).nonzero()[:, 0]
+                s = slots[t, j].long()
+                want_rows[s] = x.detach()[t].double()
+                want_out[t] += w.detach()[t, j, None].double() * y.detach()[s].double()
+                want_dx[t] += drows[s].double()
+                want_dy[s] = w.detach()[t, j, None].double() * dout[t].double()
+                want_dw[t, j] = (y.detach()[s].double() * dout[t].double()).sum(1)
+            # whole numbers and powers of two: every fp32 sum is exact
+            for got, want in ((rows, want_rows), (out, want_out), (dx, want_dx), (dy, want_dy), (dw, want_dw)):
+                assert torch.equal(got, want.to(got.dtype))
+
+
+def test_capacity_limit_reaches_the_products():
+    """An expert's pairs behind its capacity taken out by their slots: the products and their gradients are those of the kept rows."""
+    from spira_b200.nn import functional as F
+    n, c, e, k, room = 900, 64, 4, 2, 300
+    r = F.expert_route(rand(n, e), k)
+    x, w = whole(n, c, dtype=torch.float16).requires_grad_(True), whole(e, c, c, dtype=torch.float16, top=1, seed=1).requires_grad_(True)
+    first = r.offsets[:-1].long()[r.experts.long()]
+    slots = r.slots.masked_fill(r.slots - first >= room, -1)
+    assert int((slots < 0).sum()) > 100
+    stale_memory(n * k, c, torch.float16)
+    rows = F.expert_dispatch(x, r._replace(slots=slots))
+    stale_memory(n * k, c, torch.float16)
+    y = F.expert_combine(F.grouped_linear(rows, w, r.offsets), r._replace(slots=slots, weights=torch.ones_like(r.weights)))
+    d = whole(n, c, dtype=torch.float16, top=1, seed=2)
+    dx, dw = torch.autograd.grad(y, [x, w], d)
+    want, q, v = torch.zeros(n, c, dtype=torch.float64, device="cuda"), x.detach().double(), w.detach().double()
+    want_dx, want_dw = torch.zeros_like(q), torch.zeros_like(v)
+    for t, j in (slots >= 0).nonzero().tolist():
+        i = int(r.experts[t, j])
+        want[t] += (q[t] @ v[i]).half().double()
+        want_dx[t] += (v[i] @ d[t].double()).half().double()
+        want_dw[i] += q[t, :, None] * d[t].double()
+    assert torch.equal(y, want.half()) and torch.equal(dx, want_dx.half()) and torch.equal(dw, want_dw.half())
+
+
+@pytest.mark.parametrize("c", [96, 33])
+def test_library_forms_for_complete_routings(c):
+    """The calls without a clear: for slots as the routing made them, rows behind the last place are cleared by the call itself."""
+    from spira_b200 import _lib
+    from spira_b200.nn import functional as F
+    n, k = 700, 2
+    logits = rand(n, 8)
+    logits[100:180] = float("-inf")
+    r = F.expert_route(logits, k)
+    x, y, dout = rand(n, c, dtype=torch.float16), rand(n * k, c, dtype=torch.float16, seed=1).requires_grad_(True), rand(n, c, dtype=torch.float16, seed=2)
+    w = r.weights.clone().requires_grad_(True)
+    dy, dw = torch.autograd.grad(F.expert_combine(y, r._replace(weights=w)), [y, w], dout)
+    rows, drows, dweights = torch.full((n * k, c), float("nan"), dtype=torch.float16, device="cuda"), torch.full_like(y, float("nan")), torch.empty_like(w)
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.call("spira_b200_expert_dispatch", x.data_ptr(), _lib.F16, n, c, c, r.slots.data_ptr(), k, r.offsets.data_ptr(), 8, rows.data_ptr(), stream)
+    _lib.call("spira_b200_expert_combine_backward", y.data_ptr(), dout.data_ptr(), _lib.F16, n, c, c, c, w.data_ptr(), k, 1, r.slots.data_ptr(), k,
+              r.offsets.data_ptr(), 8, drows.data_ptr(), dweights.data_ptr(), stream)
+    assert torch.equal(rows, F.expert_dispatch(x, r)) and torch.equal(drows, dy) and torch.equal(dweights, dw)
