@@ -149,6 +149,9 @@ __device__ __forceinline__ bool group_wait(uint32_t bar, uint32_t parity, volati
   }
   return true;
 }
+// The limit of a wait for something that comes at the end of a tile: it spans all reduction steps of the tile (dW: of a whole
+// group, 10^6 rows take 5 ms), so each thousand of them has the limit of one wait to itself.
+__device__ __forceinline__ unsigned long long tile_limit(unsigned long long limit_ns, int steps) { return limit_ns * (1 + static_cast<unsigned>(steps) / 1024); }
 template <bool PAIR>
 __device__ __forceinline__ void group_tmem_alloc(uint32_t dst, uint32_t cols) {
   if constexpr (PAIR) {
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
         const int length = tile.row_end - tile.row0, depth = length - (tile.steps - 1) * kGK, ks = (depth + 15) / 16;
         if (length % 16 != 0) {
           const int s = (stage + tile.steps - 1) % stages;
-          if (!__all_sync(0xffffffffu, group_wait<false>(bar_tail(s), (tail_phase >> s) & 1u, abort_flag, P.wait_ns))) break;
+          if (!__all_sync(0xffffffffu, group_wait<false>(bar_tail(s), (tail_phase >> s) & 1u, abort_flag, tile_limit(P.wait_ns, tile.steps)))) break;
           tail_phase ^= 1u << s;
           clean(s, depth, ks);
           if (lane == 0) mbar_arrive_cluster(map_to_rank(bar_clean(s), 0));
@@ -560,7 +563,7 @@ __global__ void __launch_bounds__(kGThreads, 1) grouped_tc_kernel(const __grid_c
         }
         bias = bias_s;
       }
-      if (!__all_sync(0xffffffffu, group_wait<false>(bar_acc_full(b), (acc_phase >> b) & 1u, abort_flag, P.wait_ns))) break;
+      if (!__all_sync(0xffffffffu, group_wait<false>(bar_acc_full(b), (acc_phase >> b) & 1u, abort_flag, tile_limit(P.wait_ns, tile.steps)))) break;
       acc_phase ^= 1u << b;
       tc_fence_after();
       const uint32_t taddr = tmem_base + b * P.acc_stride + (static_cast<uint32_t>(q * 32) << 16) + part * width;

@@ -217,3 +217,32 @@ def test_library_forms_for_complete_routings(c):
     _lib.call("spira_b200_expert_combine_backward", y.data_ptr(), dout.data_ptr(), _lib.F16, n, c, c, c, w.data_ptr(), k, 1, r.slots.data_ptr(), k,
               r.offsets.data_ptr(), 8, drows.data_ptr(), dweights.data_ptr(), stream)
     assert torch.equal(rows, F.expert_dispatch(x, r)) and torch.equal(drows, dy) and torch.equal(dweights, dw)
+
+
+# ------------------------------------------------------------------------------------------------ bounded waits
+@pytest.mark.parametrize("c_in,c_out", [(256, 512), (64, 512)])
+def test_a_long_group_does_not_run_out_of_a_bounded_wait(c_in, c_out):
+    """All rows in one of many groups: the weight gradient is one sum over 10^6 rows, which takes several times the limit set here.
+    (256 channels run on pairs of CTAs.)"""
+    from spira_b200.nn import functional as F
+    from spira_b200.nn.functional import _C
+    n, e = 1_000_000, 160
+    x, dy = whole(n, c_in, dtype=torch.bfloat16, top=1), whole(n, c_out, dtype=torch.bfloat16, top=1, seed=1)
+    w = whole(e, c_in, c_out, dtype=torch.bfloat16, top=1, seed=2).requires_grad_(True)
+    offsets = torch.full((e + 1,), n, dtype=torch.int32, device="cuda")
+    offsets[:3] = 0
+    y = F.grouped_linear(x, w, offsets)
+    _C.check_status()
+    default = _C.get_option("wait_limit_us")
+    _C.set_option("wait_limit_us", 1000)
+    try:
+        dw, = torch.autograd.grad(y, w, dy)
+        torch.cuda.synchronize()
+    finally:
+        _C.set_option("wait_limit_us", default)
+    _C.check_status()
+    want = torch.zeros(c_in, c_out, dtype=torch.float64, device="cuda")
+    for part in range(0, n, 250_000):
+        want += x[part:part + 250_000].double().T @ dy[part:part + 250_000].double()
+    assert torch.equal(dw[2], want.to(torch.bfloat16))
+    assert not bool(dw[:2].any()) and not bool(dw[3:].any())
