@@ -546,7 +546,7 @@ int spira_b200_expert_combine_backward_cleared(const void *rows, const void *dou
 /* Ragged products: group e holds the rows [offsets[e], offsets[e + 1]) of x[n][c_in] and has the matrix weight[e][c_in][c_out].
  *   spira_b200_grouped_linear      y[r] = relu?(x[r] W[e] + bias[e]); rows outside every group are zero
  *                                  (mask != NULL: also a bit per element, set where the value before the ReLU is
- *                                  positive; spira_b200_grouped_linear_workspace says how large it is, 0: this call has none)
+ *                                  positive; spira_b200_grouped_linear_workspace says how large it is, 0 without `relu` or rows)
  *   spira_b200_grouped_linear_backward   with dz = dy, with `relu` only where the mask is set (or y > 0 without a mask):
  *                                  dx[r] = dz[r] W[e]^T (rows outside every group are zero), dweight[e] = x_e^T dz_e and
  *                                  dbias[e] = column sums of dz_e (zero for an empty group); NULL outputs are left out.

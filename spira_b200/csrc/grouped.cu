@@ -44,6 +44,7 @@ struct GroupedParams {
   float *partial;                 // dW with several pieces per group: [pieces][c_in][c_out]
   int64_t a_stride, b_stride;
   int n, experts, c_in, c_out, relu, piece;
+  unsigned char *mask;            // forward: a bit per element that the ReLU let through
 };
 
 template <typename T>
@@ -171,7 +172,8 @@ __global__ void __launch_bounds__(kAThreads) grouped_any_kernel(const __grid_con
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) {
+      uint32_t bits[2] = {0, 0};                      // of rows g and g + 8: two columns of this lane's, of a byte
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int m = m0 + wm + 16 * i + g + 8 * (q >> 1), n = n0 + wn + 8 * j + 2 * t4 + (q & 1);
@@ -179,6 +181,7 @@ __global__ void __launch_bounds__(kAThreads) grouped_any_kernel(const __grid_con
         float v = acc[i][j][q];
         if (MODE == kForward) {
           if (P.bias) v += to_f32(static_cast<const T *>(P.bias)[static_cast<int64_t>(expert) * P.c_out + n]);
+          if (v > 0.f) bits[q >> 1] |= 1u << (2 * t4 + (q & 1));
           if (P.relu) v = v < 0.f ? 0.f : v;          // (a NaN stays)
           out[static_cast<int64_t>(m) * P.c_out + n] = from_f32<T>(v);
         } else if (MODE == kDx) {
@@ -189,6 +192,16 @@ __global__ void __launch_bounds__(kAThreads) grouped_any_kernel(const __grid_con
           P.partial[(unit * P.c_in + m) * P.c_out + n] = v;
         }
       }
+      if (MODE == kForward && P.mask) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          bits[h] |= __shfl_xor_sync(0xffffffffu, bits[h], 1);
+          bits[h] |= __shfl_xor_sync(0xffffffffu, bits[h], 2);
+          const int m = m0 + wm + 16 * i + g + 8 * h, n = n0 + wn + 8 * j;
+          if (t4 == 0 && m < m_end && n < n_end) P.mask[static_cast<int64_t>(m) * mask_pitch(P.c_out) + n / 8] = static_cast<unsigned char>(bits[h]);
+        }
+      }
+    }
 }
 
 // Number of the first piece of group e and how many it has, by every warp for itself.
@@ -475,7 +488,7 @@ extern "C" int spira_b200_grouped_linear_workspace(const spira_b200_grouped_desc
   if (desc->n == 0) return SPIRA_B200_OK;
   const ForwardPlan plan = forward_plan(*desc);
   *workspace_bytes = plan.bytes;
-  *mask_bytes = desc->relu && plan.tc ? static_cast<size_t>(desc->n) * mask_pitch(desc->c_out) : 0;
+  *mask_bytes = desc->relu ? static_cast<size_t>(desc->n) * mask_pitch(desc->c_out) : 0;
   return SPIRA_B200_OK;
 }
 
@@ -485,10 +498,11 @@ extern "C" int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, vo
   const spira_b200_grouped_desc &D = *desc;
   SB_CHECK_ARG(D.x && D.weight && D.y, "grouped_linear: null pointer");
   const ForwardPlan plan = forward_plan(D);
-  SB_CHECK_ARG(!D.mask || (D.relu && plan.tc), "grouped_linear: no mask is written for this call (spira_b200_grouped_linear_workspace says 0)");
+  SB_CHECK_ARG(!D.mask || D.relu, "grouped_linear: no mask is written for this call (spira_b200_grouped_linear_workspace says 0)");
   cudaStream_t st = as_stream(stream);
   if (!plan.tc) {
-    GroupedParams P{D.x, D.weight, D.bias, D.offsets, D.y, nullptr, D.x_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, D.relu, 0};
+    GroupedParams P{D.x, D.weight, D.bias, D.offsets, D.y, nullptr, D.x_stride, 0, static_cast<int>(D.n), D.experts, D.c_in, D.c_out, D.relu, 0,
+                    static_cast<unsigned char *>(D.mask)};
     return SB_DISPATCH_HALF(D.dtype, T, return (launch_any<T, kForward>(P, st)););
   }
   rc = check_workspace("grouped_linear", workspace, workspace_bytes, plan.bytes);
@@ -633,7 +647,7 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
         rc = grouped_tc_run(kDx, Z, w_pitch, dx_pitch, 0, nullptr, status, wait_ns(), st);
         if (rc == SPIRA_B200_OK && plan.dx != kNoCopy) rc = repitch(Z.dx, dx_pitch, D.dx, D.c_in, D.n, D.c_in, st);
       } else {
-        GroupedParams P{Z.dy, Z.weight, nullptr, Z.offsets, Z.dx, nullptr, Z.dy_stride, 0, n, Z.experts, Z.c_in, Z.c_out, 0, 0};
+        GroupedParams P{Z.dy, Z.weight, nullptr, Z.offsets, Z.dx, nullptr, Z.dy_stride, 0, n, Z.experts, Z.c_in, Z.c_out, 0, 0, nullptr};
         rc = launch_any<T, kDx>(P, st);
       }
       if (rc != SPIRA_B200_OK) return rc;
@@ -643,7 +657,7 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
       rc = grouped_tc_run(kDw, Z, w_pitch, dw_pitch, plan.dw_rows, partial, status, wait_ns(), st);
       if (rc == SPIRA_B200_OK && plan.dw != kNoCopy) rc = repitch(Z.dweight, dw_pitch, D.dweight, D.c_out, static_cast<int64_t>(D.experts) * D.c_in, D.c_out, st);
     } else {
-      GroupedParams P{Z.x, Z.dy, nullptr, Z.offsets, Z.dweight, partial, Z.x_stride, Z.dy_stride, n, Z.experts, Z.c_in, Z.c_out, 0, plan.dw_rows};
+      GroupedParams P{Z.x, Z.dy, nullptr, Z.offsets, Z.dweight, partial, Z.x_stride, Z.dy_stride, n, Z.experts, Z.c_in, Z.c_out, 0, plan.dw_rows, nullptr};
       rc = launch_any<T, kDw>(P, st);
     }
     if (rc != SPIRA_B200_OK || plan.dw_rows == 0) return rc;

@@ -87,7 +87,7 @@ __device__ __forceinline__ void group_span(const int32_t *offsets, int experts, 
 inline int64_t group_tiles_bound(int64_t n, int experts, int64_t rows) { return n / rows + (experts < n ? experts : n); }
 
 // Bytes per row of the ReLU mask: a bit per column, rows of whole 4-byte words.
-inline int mask_pitch(int c_out) { return (c_out + 31) / 32 * 4; }
+__host__ __device__ __forceinline__ int mask_pitch(int c_out) { return (c_out + 31) / 32 * 4; }
 
 inline int pitch8(int channels) { return (channels + 7) / 8 * 8; }
 

@@ -302,8 +302,8 @@ def _grouped_desc(n, weights, offsets, relu, x=None, bias=None, dy=None, y=None,
 
 
 def _grouped(x, weights, offsets, bias, relu, want_mask=False):
-    """The product and, for a backward pass, what its ReLU let through: the bit mask the kernel writes, or None where the
-    call has none (then the sign of the result says it)."""
+    """The product and, for a backward pass, what its ReLU let through: the bit mask the kernel writes (None without a ReLU or rows).
+    It is the sign of the unrounded values: a positive one that rounds to zero lets its gradient through."""
     index, n = x.get_device(), x.shape[0]
     y = _dense(x, n, weights.shape[2])
     mask, workspace, room = None, 0, 0
@@ -337,13 +337,13 @@ class _Grouped(torch.autograd.Function):
     def forward(ctx, x, weights, offsets, bias, relu):
         y, mask = _grouped(x, weights, offsets, bias, relu, want_mask=True)
         ctx.relu, ctx.has_bias = relu, bias is not None
-        ctx.save_for_backward(x, weights, offsets, y if relu and mask is None else None, mask)
+        ctx.save_for_backward(x, weights, offsets, mask)
         return y
 
     @staticmethod
     def backward(ctx, dy):
         _once(dy)
-        x, weights, offsets, y, mask = ctx.saved_tensors
+        x, weights, offsets, mask = ctx.saved_tensors
         dy = _rows(dy)
         need = ctx.needs_input_grad
         index, n = x.get_device(), x.shape[0]
@@ -351,7 +351,7 @@ class _Grouped(torch.autograd.Function):
         dw = torch.empty_like(weights) if need[1] else None            # (dense: the call made it so)
         db = _dense(weights, weights.shape[0], weights.shape[2]) if ctx.has_bias and need[3] else None
         _with_workspace(index, dy, "spira_b200_grouped_linear_backward",
-                        _grouped_desc(n, weights, offsets, 1 if ctx.relu else 0, x, None, dy, y, mask, dx, dw, db), _status(index))
+                        _grouped_desc(n, weights, offsets, 1 if ctx.relu else 0, x, None, dy, None, mask, dx, dw, db), _status(index))
         return dx, dw, None, db, None
 
 

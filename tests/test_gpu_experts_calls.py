@@ -246,3 +246,42 @@ def test_a_long_group_does_not_run_out_of_a_bounded_wait(c_in, c_out):
         want += x[part:part + 250_000].double().T @ dy[part:part + 250_000].double()
     assert torch.equal(dw[2], want.to(torch.bfloat16))
     assert not bool(dw[:2].any()) and not bool(dw[3:].any())
+
+
+# ------------------------------------------------------------------------------------------------ what the ReLU lets through
+@pytest.mark.parametrize("ci,co", [(64, 64), (20, 30), (33, 72), (200, 152)])
+def test_relu_gradient_goes_by_the_unrounded_value(ci, co):
+    """Positive values that round to zero in fp16 let the gradient through on every kernel, as max(z, 0) does before its rounding."""
+    from spira_b200.nn import functional as F
+    n = 40
+    sign = torch.where(torch.arange(n, device="cuda") % 3 == 0, -1.0, 1.0)
+    x = (2.0 ** -14 * sign[:, None].expand(n, ci)).half().requires_grad_(True)
+    w = torch.full((2, ci, co), 2.0 ** -21, device="cuda").half().requires_grad_(True)         # (a subnormal: ci 2^-35 rounds to zero)
+    o = torch.tensor([0, 10, n - 1], dtype=torch.int32, device="cuda")
+    b = torch.zeros(2, co, dtype=torch.float16, device="cuda").requires_grad_(True)
+    y = F.grouped_linear(x, w, o, b, relu=True)
+    assert not bool(y.any())
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.ones_like(y))
+    live = (sign > 0) & (torch.arange(n, device="cuda") < n - 1)
+    assert torch.equal(dx, torch.where(live[:, None], float(co) * 2.0 ** -21, 0.0).half().expand(n, ci))
+    counts = torch.stack([live[:10].sum(), live[10:].sum()])
+    assert torch.equal(db, counts[:, None].half().expand(2, co)) and torch.equal(dw, (counts[:, None, None] * 2.0 ** -14).half().expand(2, ci, co))
+
+
+@pytest.mark.parametrize("ci,co", [(64, 64), (20, 30)])
+def test_library_backward_without_a_mask_goes_by_the_result(ci, co):
+    """A caller of the library that kept y and no mask: y > 0 says what the ReLU let through."""
+    from spira_b200 import _lib
+    from spira_b200.nn import functional as F
+    from spira_b200.nn.functional import experts
+    n = 300
+    o = torch.tensor([3, 100, 290], dtype=torch.int32, device="cuda")
+    x, w, dy = whole(n, ci, dtype=torch.float16), whole(2, ci, co, dtype=torch.float16, seed=1), whole(n, co, dtype=torch.float16, top=1, seed=2)
+    xg, wg = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = F.grouped_linear(xg, wg, o, relu=True)
+    want = torch.autograd.grad(y, [xg, wg], dy)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty(2, co, dtype=torch.float16, device="cuda")
+    desc = experts._grouped_desc(n, w, o, 1, x, None, dy, y.detach(), None, dx, dw, db)
+    experts._with_workspace(x.get_device(), x, "spira_b200_grouped_linear_backward", desc, experts._status(x.get_device()))
+    dz = torch.where(y.detach() > 0, dy, 0.0).double()
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1]) and torch.equal(db, torch.stack([dz[3:100].sum(0), dz[100:290].sum(0)]).half())
