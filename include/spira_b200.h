@@ -566,6 +566,10 @@ int spira_b200_grouped_linear(const spira_b200_grouped_desc *desc, void *workspa
 int spira_b200_grouped_linear_backward_workspace(const spira_b200_grouped_desc *desc, size_t *bytes);
 int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status,
                                        void *stream);
+/* Which kernels the calls of a descriptor take, for measurements and tests (the choice depends on sizes, strides and alignment
+ * alone): paths[0] forward, [1] dx, [2] dweight: 0 the general kernel, 1 tensor cores, 2 tensor cores with pairs of CTAs;
+ * [3] rows of a unit of dweight (0: a whole group).  -1: the descriptor has no such result. */
+int spira_b200_grouped_linear_paths(const spira_b200_grouped_desc *desc, int32_t paths[4]);
 
 /* Norms around a block, its gate and the residual, in one pass over the rows:
  *   p = post ? norm(block) * post_weight + post_bias : block

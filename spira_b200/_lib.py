@@ -181,6 +181,7 @@ SIGNATURES = {
     "spira_b200_grouped_linear": [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p],
     "spira_b200_grouped_linear_backward_workspace": [c_void_p, C.POINTER(c_size_t)],
     "spira_b200_grouped_linear_backward": [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p],
+    "spira_b200_grouped_linear_paths": [c_void_p, C.POINTER(c_int32)],
     "spira_b200_residual_norm": [c_void_p, c_void_p],
     "spira_b200_residual_norm_backward_workspace": [c_void_p, C.POINTER(c_size_t)],
     "spira_b200_residual_norm_backward": [c_void_p, c_void_p, c_size_t, c_void_p],

@@ -585,6 +585,20 @@ extern "C" int spira_b200_grouped_linear_backward_workspace(const spira_b200_gro
   return SPIRA_B200_OK;
 }
 
+extern "C" int spira_b200_grouped_linear_paths(const spira_b200_grouped_desc *desc, int32_t *paths) {
+  int rc = grouped_check("grouped_linear_paths", desc);
+  if (rc != SPIRA_B200_OK) return rc;
+  SB_CHECK_ARG(paths && desc->n > 0, "grouped_linear_paths: null pointer, or no rows");
+  const spira_b200_grouped_desc &D = *desc;
+  auto path = [&](int mode, bool tc) { return !tc ? 0 : grouped_tc_pair(mode, D) ? 2 : 1; };
+  const BackwardPlan plan = backward_plan(D);
+  paths[0] = path(kForward, forward_plan(D).tc);
+  paths[1] = D.dx ? path(kDx, plan.tc) : -1;
+  paths[2] = D.dweight ? path(kDw, plan.tc) : -1;
+  paths[3] = D.dweight ? plan.dw_rows : -1;
+  return SPIRA_B200_OK;
+}
+
 extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc *desc, void *workspace, size_t workspace_bytes, int32_t *status,
                                                   void *stream) {
   int rc = backward_check(desc);

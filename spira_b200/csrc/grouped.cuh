@@ -95,6 +95,7 @@ inline int pitch8(int channels) { return (channels + 7) / 8 * 8; }
 // results have pitches (elements per row) in whole units of 8.
 enum { kForward = 0, kDx = 1, kDw = 2 };
 bool grouped_tc_available();
+bool grouped_tc_pair(int mode, const spira_b200_grouped_desc &D);      // whether pairs of CTAs share its tiles
 bool grouped_tc_rows_ok(const void *p, int64_t stride, int channels, int64_t n);
 int grouped_tc_dw_tiles(int c_in, int c_out);
 int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int w_pitch, int out_pitch, int piece, float *partial, int32_t *status,

@@ -721,7 +721,7 @@ int grouped_tc_dw_tiles(int c_in, int c_out) {
 // Two CTAs per tile where it has the rows and columns for both, enough work to fill the SMs in pairs and a reduction long
 // enough for the fuller pipeline to matter.  Measured pair / single: 80 026 rows in 16 groups, 512 -> 2048: forward 146 /
 // 155 us, dx 111 / 131 us, dW 127 / 147 us; 40 000 rows in 8 groups, 256 -> 1024: forward 62 / 44 us.
-static bool use_pair(int mode, const spira_b200_grouped_desc &D) {
+bool grouped_tc_pair(int mode, const spira_b200_grouped_desc &D) {
   if (mode == kDw) return D.c_in > kGRows && D.c_out >= 128 && D.n / D.experts >= 256;
   const int n = mode == kForward ? D.c_out : D.c_in, k = mode == kForward ? D.c_in : D.c_out;
   return n >= 128 && k >= 384 && D.n / D.experts >= 512 && D.n / 256 * div_up(n, kGMaxN) >= sm_count() / 2;
@@ -737,7 +737,7 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int w_pitch, int 
   P.piece = piece;
   P.wait_ns = wait_ns;
   P.out_pitch = out_pitch;
-  const bool pair = use_pair(mode, D);
+  const bool pair = grouped_tc_pair(mode, D);
   P.tile_rows = pair ? 2 * kGRows : kGRows;
   int64_t units;
   if (mode == kDw) {

@@ -110,3 +110,15 @@ def test_library_refuses_bad_arguments_of_the_cleared_forms(lib):
     assert backward(None, None, 0, 0, 8, 8, 8, None, 0, 0, None, None, 2, None, None, None) == 0
     assert backward(None, None, 0, 4, 8, 8, 8, None, 0, 0, None, None, 2, None, None, None) != 0 and b"null pointer" in err()
     assert backward(None, None, 0, 4, 8, 8, 8, None, 0, 0, None, None, 0, None, None, None) != 0 and b"top_k=0" in err()
+
+
+def test_paths_call_checks_its_arguments(lib):
+    from spira_b200 import _lib
+    paths, err = (ctypes.c_int32 * 4)(), lib.spira_b200_last_error
+    g = _lib.GroupedDesc(dtype=_lib.F16, experts=2, c_in=8, c_out=8, n=0)
+    assert lib.spira_b200_grouped_linear_paths(ctypes.byref(g), paths) != 0 and b"no rows" in err()
+    g.n, g.offsets = 4, 4096
+    assert lib.spira_b200_grouped_linear_paths(ctypes.byref(g), None) != 0 and b"null pointer" in err()
+    assert lib.spira_b200_grouped_linear_paths(None, paths) != 0
+    g.x_stride, g.c_in = 7, 7
+    assert lib.spira_b200_grouped_linear_paths(ctypes.byref(g), paths) == 0 and list(paths) == [0, -1, -1, -1]

@@ -7,7 +7,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from test_gpu_experts import ANY, rand, whole
+from test_gpu_experts import ANY, HALF, plain_products, rand, whole
 
 pytestmark = pytest.mark.gpu
 
@@ -285,3 +285,55 @@ def test_library_backward_without_a_mask_goes_by_the_result(ci, co):
     experts._with_workspace(x.get_device(), x, "spira_b200_grouped_linear_backward", desc, experts._status(x.get_device()))
     dz = torch.where(y.detach() > 0, dy, 0.0).double()
     assert torch.equal(dx, want[0]) and torch.equal(dw, want[1]) and torch.equal(db, torch.stack([dz[3:100].sum(0), dz[100:290].sum(0)]).half())
+
+
+# ------------------------------------------------------------------------------------------------ every kernel the sizes choose between
+def cut(n, e, seed, first=0, behind=0, empty=(), most=0.0):
+    """Offsets of uneven groups: random cuts, some groups empty, a share `most` of the rows in group 1."""
+    g = torch.Generator().manual_seed(seed)
+    share = torch.rand(e, generator=g) + 0.05
+    share[list(empty)] = 0.0
+    share = share / share.sum() * (1 - most)
+    share[1] += most
+    ends = first + ((n - first - behind) * share.cumsum(0)).round().long()
+    ends[-1] = n - behind
+    return torch.cat([torch.tensor([first]), ends]).to(torch.int32).cuda()
+
+
+GENERAL, SINGLE, PAIR = 0, 1, 2
+#         rows    groups  c_in  c_out  forward dx      dW      rows of a unit of dW: whole groups or pieces
+PATHS = [(40000,  16,     512,  2048,  PAIR,   PAIR,   PAIR,   "whole"),       # long reductions: staged stores forward, direct ones in dx
+         (20003,  7,      520,  1992,  PAIR,   PAIR,   PAIR,   "whole"),       # channels and rows that no tile divides, direct stores forward
+         (24001,  20,     1992, 520,   PAIR,   PAIR,   PAIR,   "whole"),
+         (20000,  80,     136,  264,   SINGLE, SINGLE, SINGLE, "whole"),       # more groups than are sorted by length
+         (24007,  80,     136,  264,   SINGLE, SINGLE, PAIR,   "whole"),
+         (9000,   50,     128,  520,   SINGLE, SINGLE, SINGLE, "whole"),       # sorted by length: 50 x 3 tiles fill 148 SMs
+         (9000,   40,     128,  520,   SINGLE, SINGLE, SINGLE, "pieces"),      # 40 x 3 do not
+         (30001,  2,      200,  136,   SINGLE, SINGLE, PAIR,   "pieces"),
+         (9001,   5,      96,   192,   SINGLE, SINGLE, SINGLE, "pieces"),
+         (500,    3,      33,   70,    GENERAL, GENERAL, GENERAL, "pieces"),
+         (500,    90,     65,   70,    GENERAL, GENERAL, GENERAL, "whole")]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n,e,ci,co,forward,dx,dw,unit", PATHS)
+def test_products_exact_on_every_path(dtype, n, e, ci, co, forward, dx, dw, unit):
+    """Whole numbers on uneven, empty and dominating groups, with and without bias and ReLU: the bits of the 64-bit values; and the
+    sizes take the kernels that the list says."""
+    from spira_b200 import _lib
+    from spira_b200.nn import functional as F
+    from spira_b200.nn.functional import experts
+    x, w, b = whole(n, ci, dtype=dtype, seed=1), whole(e, ci, co, dtype=dtype, seed=2), whole(e, co, dtype=dtype, seed=3)
+    dy = whole(n, co, dtype=dtype, top=1, seed=4)
+    paths = (ctypes.c_int32 * 4)()
+    _lib.call("spira_b200_grouped_linear_paths", experts._grouped_desc(n, w, torch.zeros(e + 1, dtype=torch.int32, device="cuda"), 1, x, b, dy, None, None, x, w, b), paths)
+    assert list(paths)[:3] == [forward, dx, dw] and (paths[3] == 0) == (unit == "whole"), list(paths)
+    variants = [(cut(n, e, 1, first=3, behind=5, empty=(0, e // 2)), True, True), (cut(n, e, 2, behind=1, empty=(e - 1,), most=0.8), False, False),
+                (cut(n, e, 3, empty=(0,), most=0.97), True, False)]
+    for offsets, bias, relu in variants:
+        leaves = [t.clone().requires_grad_(True) for t in ([x, w, b] if bias else [x, w])]
+        y = F.grouped_linear(leaves[0], leaves[1], offsets, leaves[2] if bias else None, relu=relu)
+        grads = torch.autograd.grad(y, leaves, dy)
+        want = plain_products(x, w, offsets, b if bias else None, relu, dy, y.detach())
+        for name, got, ref in zip(("y", "dx", "dw", "db"), (y,) + grads, want):
+            assert torch.equal(got, ref.to(dtype)), (name, bias, relu, float((got.double() - ref).abs().max()))
