@@ -953,9 +953,9 @@ def measure(engine, host, dev, args, l2buf, dist_ctx, device):
         step_resident(i)
         step_e2e(i)
     torch.cuda.synchronize()
-    launches0 = _lib.launch_count
+    launches0 = _lib.launches()
     res = timed_loop(step_resident, args.steps, args.warmup, l2buf, dist_ctx)
-    launches = _lib.launch_count - launches0
+    launches = _lib.launches() - launches0
     e2e = timed_loop(step_e2e, args.steps, args.warmup, l2buf, dist_ctx, drain_e2e)
     return {"median_ms": res["median_ms"], "mean_ms": res["mean_ms"], "steps": res["steps"], "enqueue_ms": res["enqueue_ms"],
             "rank_median_ms": res["rank_median_ms"], "rank_enqueue_ms": res["rank_enqueue_ms"],

@@ -504,6 +504,9 @@ int spira_b200_conv_ws_static(const void *feats, const void *weights, const void
 #define SPIRA_B200_BF16 1
 #define SPIRA_B200_F32 2
 
+/* Kernels that the calls below have launched in this process so far. */
+int spira_b200_operator_launches(int64_t *count);
+
 /* The k experts of every row of logits[n][experts] (rows `row_stride` elements apart): the k largest, ties to the lowest
  * index, -inf never (chosen = -1, weight 0).  weights[n][k] fp32: softmax over the chosen (renormalize != 0) or over all
  * experts.  slots[n][k]: place of every (row, j) in the order (expert, row, j), -1 where there is none; order[n * k]: the

@@ -165,6 +165,7 @@ SIGNATURES = {
     "spira_b200_conv_ws_static": [c_void_p, c_void_p, c_void_p, C.POINTER(Epilogue), c_void_p, c_void_p, c_void_p, c_void_p,
                                   c_int, c_int64, c_int, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p,
                                   c_void_p],
+    "spira_b200_operator_launches": [C.POINTER(c_int64)],
     "spira_b200_expert_route_workspace": [c_int64, c_int, c_int, C.POINTER(c_size_t)],
     "spira_b200_expert_route": [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_size_t, c_void_p],
@@ -218,19 +219,17 @@ def check(code: int) -> None:
         raise RuntimeError(f"[spira_b200] {msg} (code {code})")
 
 
-# kernels of this library launched per successful call (library kernels such as the radix sort are not counted)
+# kernels of this library launched per successful call (library kernels such as the radix sort are not counted); the library
+# counts those of the expert and norm operators itself, their number depends on the sizes
 KERNELS_PER_CALL = {
     "spira_b200_pack": 1, "spira_b200_unpack": 1, "spira_b200_flatten_sort": 1, "spira_b200_permute_rows": 1,
     "spira_b200_downsample": 1, "spira_b200_pointwise": 1, "spira_b200_downsample_sorted": 1, "spira_b200_kmap_search": 1, "spira_b200_kmap_ws_sizes": 2, "spira_b200_kmap_ws_pairs": 1, "spira_b200_kmap_ws_lists": 3,
     "spira_b200_kmap_masks": 1, "spira_b200_kmap_masks_half": 1, "spira_b200_kmap_lists_from_masks": 3, "spira_b200_convert_transposed_os": 1, "spira_b200_transpose_map": 1,
     "spira_b200_pack_weights": 1, "spira_b200_conv_os": 1, "spira_b200_conv_os_grouped": 1, "spira_b200_conv_os_split": 1,
     "spira_b200_kmap_group": 2,
-    "spira_b200_expert_route": 1, "spira_b200_expert_route_backward": 1, "spira_b200_expert_dispatch_cleared": 2, "spira_b200_expert_combine_backward_cleared": 2, "spira_b200_expert_dispatch": 1, "spira_b200_expert_combine": 1,
-    "spira_b200_expert_combine_backward": 1, "spira_b200_grouped_linear": 1, "spira_b200_grouped_linear_backward": 2,
-    "spira_b200_residual_norm": 1, "spira_b200_residual_norm_backward": 1,
     "spira_b200_conv_ws": 2, "spira_b200_conv_ws_fused": 1, "spira_b200_conv_ws_static": 2,
 }
-launch_count = 0          # kernels launched through `call` since import (or since it was last reset by the caller)
+launch_count = 0          # kernels launched through `call` since import (or since it was last reset by the caller), operators aside
 profile_hook = None       # optional callable(name, args, run) -> None used by the benchmark to time single calls
 
 
@@ -242,3 +241,10 @@ def call(name: str, *args) -> None:
     else:
         check(fn(*args))
     launch_count += KERNELS_PER_CALL.get(name, 0)
+
+
+def launches() -> int:
+    """Kernels of this library launched so far: ``launch_count`` and those of the expert and norm operators."""
+    count = c_int64()
+    check(load().spira_b200_operator_launches(C.byref(count)))
+    return launch_count + count.value

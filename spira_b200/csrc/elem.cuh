@@ -71,6 +71,15 @@ inline int allow_smem(K kernel, size_t most) {
   return SPIRA_B200_OK;
 }
 
+// Kernels of the expert and norm operators launched by this process (how many a call takes depends on its sizes).
+void count_operator_launch();
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_operator(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args &&...args) {
+  const cudaError_t e = launch_dependent(kernel, grid, block, smem, stream, static_cast<Args &&>(args)...);
+  if (e == cudaSuccess) count_operator_launch();
+  return e;
+}
+
 inline int elem_size(int dtype) { return dtype == SPIRA_B200_F32 ? 4 : 2; }
 
 // Runs BODY with T = the element type of the code.

@@ -10,6 +10,7 @@
 // j in order.  Dispatch and combine are bound by memory (127 363 x 96 fp16, k 2: 12 us = 6.0 TB/s there, 14 us = 5.3 TB/s
 // back), routing by the integer instructions of the selection (127 363 x 64 fp16, k 4: 19.2 us for 24 MB), all of it by
 // the launch for a few rows.
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 
@@ -680,6 +681,9 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const MoveParams 
   if (drows && P.offsets) zero_tail<T, V>(P, drows, vecs);
 }
 
+static std::atomic<int64_t> g_operator_launches{0};
+void count_operator_launch() { g_operator_launches.fetch_add(1, std::memory_order_relaxed); }
+
 static unsigned capped_blocks(int64_t work, int per_cta, int ctas_per_sm) {
   const int64_t want = div_up(work, per_cta), cap = static_cast<int64_t>(sm_count()) * ctas_per_sm;
   return static_cast<unsigned>(want < 1 ? 1 : want < cap ? want : cap);
@@ -699,7 +703,7 @@ template <typename... KArgs>
 static int launch_route_kernel(void (*kernel)(KArgs...), int ctas, size_t smem, size_t most, cudaStream_t st, const RouteParams &P) {
   const int rc = allow_smem(kernel, most);
   if (rc != SPIRA_B200_OK) return rc;
-  SB_CHECK_CUDA(launch_dependent(kernel, dim3(ctas), dim3(kRouteThreads), smem, st, P));
+  SB_CHECK_CUDA(launch_operator(kernel, dim3(ctas), dim3(kRouteThreads), smem, st, P));
   return SPIRA_B200_OK;
 }
 
@@ -769,7 +773,7 @@ static int launch_move(MoveParams &P, bool combine, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(div_up(P.rows_per_launch_row * pieces, 256)), static_cast<unsigned>(div_up(P.n, P.rows_per_launch_row)));
   SB_CHECK_ARG(grid.y < 65536, "too many rows x channels");
   auto go = [&](auto kernel) -> int {
-    SB_CHECK_CUDA(launch_dependent(kernel, grid, dim3(256), 0, st, P));
+    SB_CHECK_CUDA(launch_operator(kernel, grid, dim3(256), 0, st, P));
     return SPIRA_B200_OK;
   };
   if (combine) return P.k == 1 ? go(combine_kernel<T, V, 1>) : P.k == 2 ? go(combine_kernel<T, V, 2>) : P.k == 4 ? go(combine_kernel<T, V, 4>) : go(combine_kernel<T, V, 0>);
@@ -785,10 +789,10 @@ static int launch_combine_backward(const MoveParams &P, cudaStream_t st) {
   int lanes = vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
   if (lanes > 4 && vecs <= 32 && P.n * (lanes / 2) >= 4 * 256 * static_cast<int64_t>(sm_count())) lanes /= 2;
   const unsigned blocks = capped_blocks(P.n * lanes, 256, 8);
-  if (lanes == 4) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 4>, dim3(blocks), dim3(256), 0, st, P));
-  else if (lanes == 8) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 8>, dim3(blocks), dim3(256), 0, st, P));
-  else if (lanes == 16) SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 16>, dim3(blocks), dim3(256), 0, st, P));
-  else SB_CHECK_CUDA(launch_dependent(combine_backward_kernel<T, V, 32>, dim3(blocks), dim3(256), 0, st, P));
+  if (lanes == 4) SB_CHECK_CUDA(launch_operator(combine_backward_kernel<T, V, 4>, dim3(blocks), dim3(256), 0, st, P));
+  else if (lanes == 8) SB_CHECK_CUDA(launch_operator(combine_backward_kernel<T, V, 8>, dim3(blocks), dim3(256), 0, st, P));
+  else if (lanes == 16) SB_CHECK_CUDA(launch_operator(combine_backward_kernel<T, V, 16>, dim3(blocks), dim3(256), 0, st, P));
+  else SB_CHECK_CUDA(launch_operator(combine_backward_kernel<T, V, 32>, dim3(blocks), dim3(256), 0, st, P));
   return SPIRA_B200_OK;
 }
 
@@ -796,9 +800,9 @@ static int launch_clear(const MoveParams &P, const int32_t *order, int size, cud
   const int64_t total = P.n * P.k, row_bytes = static_cast<int64_t>(P.channels) * size;
   const dim3 grid(static_cast<unsigned>(div_up(total, 256)));
   unsigned char *rows = static_cast<unsigned char *>(P.out);
-  if (rows_aligned(rows, P.channels, size)) SB_CHECK_CUDA(launch_dependent(clear_kernel<16>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
-  else if (size == 4) SB_CHECK_CUDA(launch_dependent(clear_kernel<4>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
-  else SB_CHECK_CUDA(launch_dependent(clear_kernel<2>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
+  if (rows_aligned(rows, P.channels, size)) SB_CHECK_CUDA(launch_operator(clear_kernel<16>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
+  else if (size == 4) SB_CHECK_CUDA(launch_operator(clear_kernel<4>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
+  else SB_CHECK_CUDA(launch_operator(clear_kernel<2>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
   return SPIRA_B200_OK;
 }
 
@@ -832,6 +836,12 @@ static int run_combine_backward(const MoveParams &P, int dtype, bool clear, cons
 }  // namespace sb
 
 using namespace sb;
+
+extern "C" int spira_b200_operator_launches(int64_t *count) {
+  SB_CHECK_ARG(count, "operator_launches: null pointer");
+  *count = g_operator_launches.load(std::memory_order_relaxed);
+  return SPIRA_B200_OK;
+}
 
 extern "C" int spira_b200_expert_route_workspace(int64_t n, int experts, int k, size_t *bytes) {
   int rc = check_route("expert_route", SPIRA_B200_F32, n, experts, experts, k);
@@ -868,7 +878,7 @@ extern "C" int spira_b200_expert_route_backward(const void *logits, int dtype, i
     const T *l = static_cast<const T *>(logits);
     T *d = static_cast<T *>(dlogits);
     auto go = [&](auto kernel, int lanes) -> int {
-      SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(div_up(n * lanes, 256))), dim3(256), 0, st, l, n, row_stride, experts, k,
+      SB_CHECK_CUDA(launch_operator(kernel, dim3(static_cast<unsigned>(div_up(n * lanes, 256))), dim3(256), 0, st, l, n, row_stride, experts, k,
                                      renormalize != 0 ? 1 : 0, weights, chosen, dweights, dweights_row, dweights_col, d));
       return SPIRA_B200_OK;
     };

@@ -415,7 +415,7 @@ static int launch_any(const GroupedParams &P, cudaStream_t st) {
   const int64_t units = MODE == kDw ? (P.piece ? group_tiles_bound(P.n, P.experts, P.piece) : P.experts) : group_tiles_bound(P.n, P.experts, kATile);
   const int64_t columns = MODE == kForward ? div_up(P.c_out, kATile) : MODE == kDx ? div_up(P.c_in, kATile) : any_tiles(P.c_in, P.c_out);
   SB_CHECK_ARG(columns < 65536 && units < (int64_t(1) << 31), "grouped_linear: too many tiles");
-  SB_CHECK_CUDA(launch_dependent(grouped_any_kernel<T, MODE>, dim3(static_cast<unsigned>(units < 1 ? 1 : units), static_cast<unsigned>(columns)),
+  SB_CHECK_CUDA(launch_operator(grouped_any_kernel<T, MODE>, dim3(static_cast<unsigned>(units < 1 ? 1 : units), static_cast<unsigned>(columns)),
                                  dim3(kAThreads), 0, st, P));
   return SPIRA_B200_OK;
 }
@@ -470,7 +470,7 @@ static int repitch(const void *src, int64_t src_pitch, void *dst, int64_t dst_pi
   P.div_shift = 31 + bits;
   P.div_mul = ((uint64_t(1) << P.div_shift) + columns - 1) / columns;
   const dim3 grid(static_cast<unsigned>(div_up(P.rows_per_group * columns, 1024)), static_cast<unsigned>(div_up(rows, P.rows_per_group)));
-  SB_CHECK_CUDA(launch_dependent(grouped_repitch_kernel, grid, dim3(256), 0, st, P));
+  SB_CHECK_CUDA(launch_operator(grouped_repitch_kernel, grid, dim3(256), 0, st, P));
   return SPIRA_B200_OK;
 }
 
@@ -623,7 +623,7 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
       const unsigned units = static_cast<unsigned>(group_tiles_bound(n, D.experts, plan.dz_rows));
       const bool wide = D.c_out % 8 == 0 && aligned16(D.dy) && (D.dy_stride % 8 == 0 || n == 1) && (D.mask || aligned16(D.y));
       auto go = [&](auto kernel, int columns) -> int {
-        SB_CHECK_CUDA(launch_dependent(kernel, dim3(units, static_cast<unsigned>(div_up(columns, 256))), dim3(256), 0, st, static_cast<const T *>(D.dy),
+        SB_CHECK_CUDA(launch_operator(kernel, dim3(units, static_cast<unsigned>(div_up(columns, 256))), dim3(256), 0, st, static_cast<const T *>(D.dy),
                                        D.dy_stride, static_cast<const T *>(D.y), static_cast<const unsigned char *>(D.mask), mask_pitch(D.c_out), dz,
                                        plan.dz_pitch, D.dbias ? partial : nullptr, D.offsets, n, D.experts, D.c_out, plan.dz_rows));
         return SPIRA_B200_OK;
@@ -633,7 +633,7 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
       else rc = kind == 0 ? go(grouped_dz_kernel<T, 1, 0>, D.c_out) : kind == 1 ? go(grouped_dz_kernel<T, 1, 1>, D.c_out) : go(grouped_dz_kernel<T, 1, 2>, D.c_out);
       if (rc != SPIRA_B200_OK) return rc;
       if (D.dbias)
-        SB_CHECK_CUDA(launch_dependent(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(256), 0, st,
+        SB_CHECK_CUDA(launch_operator(grouped_column_sum_kernel<T>, dim3(static_cast<unsigned>(div_up(D.c_out, 32)), D.experts), dim3(256), 0, st,
                                        static_cast<const float *>(partial), D.offsets, n, D.experts, plan.dz_rows, D.c_out, static_cast<T *>(D.dbias)));
       if (dz) {
         Z.dy = dz;
@@ -676,7 +676,7 @@ extern "C" int spira_b200_grouped_linear_backward(const spira_b200_grouped_desc 
     }
     if (rc != SPIRA_B200_OK || plan.dw_rows == 0) return rc;
     const int64_t want = div_up(static_cast<int64_t>(D.c_in) * dw_pitch, 256);
-    SB_CHECK_CUDA(launch_dependent(grouped_sum_kernel<T>, dim3(static_cast<unsigned>(want < 1024 ? want : 1024), D.experts), dim3(256), 0, st,
+    SB_CHECK_CUDA(launch_operator(grouped_sum_kernel<T>, dim3(static_cast<unsigned>(want < 1024 ? want : 1024), D.experts), dim3(256), 0, st,
                                    static_cast<const float *>(partial), D.offsets, n, D.experts, plan.dw_rows, static_cast<int64_t>(D.c_in), D.c_out, dw_pitch,
                                    static_cast<T *>(D.dweight)));
     return SPIRA_B200_OK;

@@ -834,6 +834,7 @@ int grouped_tc_run(int mode, const spira_b200_grouped_desc &D, int w_pitch, int 
     }
     cfg.attrs = attr;
     SB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, map_a, map_b, map_out));
+    count_operator_launch();
     return SPIRA_B200_OK;
   };
   auto pick = [&](auto type) -> int {

@@ -735,7 +735,7 @@ static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaS
     if (rc != SPIRA_B200_OK) return rc;
     static int resident[4] = {0, 0, 0, 0};
     const int64_t cap = static_cast<int64_t>(sm_count()) * resident_ctas(kernel, kThreads, smem, resident[tensors]);
-    SB_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), smem, st, P));
+    SB_CHECK_CUDA(launch_operator(kernel, dim3(static_cast<unsigned>(rounds < cap ? rounds : cap)), dim3(kThreads), smem, st, P));
     return SPIRA_B200_OK;
   }
   constexpr int RB = L <= 32 && ITEMS == 1 ? 2 : 1, kBackward = kBackwardThreads<V, L, RB>, kBackwardRows = kBackward / L;
@@ -753,7 +753,7 @@ static int launch_norm_kind(const NormParams &P, bool backward, int *ctas, cudaS
   const int64_t cap = static_cast<int64_t>(sm_count()) * (fit < kNormBackwardCtas ? fit : kNormBackwardCtas);
   const int grid = static_cast<int>(rounds < cap ? rounds : cap);
   *ctas = grid;
-  SB_CHECK_CUDA(launch_dependent(kernel, dim3(grid), dim3(kBackward), smem, st, P));
+  SB_CHECK_CUDA(launch_operator(kernel, dim3(grid), dim3(kBackward), smem, st, P));
   return SPIRA_B200_OK;
 }
 
@@ -886,7 +886,7 @@ extern "C" int spira_b200_residual_norm_backward(const spira_b200_norm_desc *des
   S.out[4] = D.gate_kind == kGateChannel ? D.dgate : nullptr;
   S.ctas = ctas; S.channels = D.channels; S.params_f32 = D.params_f32;
   return SB_DISPATCH_ELEM(D.dtype, T, {
-    SB_CHECK_CUDA(launch_dependent(norm_sums_kernel<T>, dim3(static_cast<unsigned>(div_up(D.channels, 32)), kSums), dim3(1024), 0, st, S));
+    SB_CHECK_CUDA(launch_operator(norm_sums_kernel<T>, dim3(static_cast<unsigned>(div_up(D.channels, 32)), kSums), dim3(1024), 0, st, S));
     return SPIRA_B200_OK;
   });
 }

@@ -337,3 +337,41 @@ def test_products_exact_on_every_path(dtype, n, e, ci, co, forward, dx, dw, unit
         want = plain_products(x, w, offsets, b if bias else None, relu, dy, y.detach())
         for name, got, ref in zip(("y", "dx", "dw", "db"), (y,) + grads, want):
             assert torch.equal(got, ref.to(dtype)), (name, bias, relu, float((got.double() - ref).abs().max()))
+
+
+# ------------------------------------------------------------------------------------------------ launch counts
+def test_launches_are_counted():
+    """The counter against the number of kernels each call is made of."""
+    from spira_b200 import _lib
+    from spira_b200.nn import functional as F
+
+    def count(call, *args, **kw):
+        before = _lib.launches()
+        out = call(*args, **kw)
+        return _lib.launches() - before, out
+    few, many = rand(8, 8).requires_grad_(True), rand(5000, 8)
+    one, r = count(F.expert_route, few, 2)
+    assert one == 1 and count(torch.autograd.grad, r.weights, few, torch.ones_like(r.weights))[0] == 1
+    two, r = count(F.expert_route, many, 2)
+    assert two == 2
+    x, y, w = rand(5000, 64, dtype=torch.float16), rand(10000, 64, dtype=torch.float16), r.weights.clone().requires_grad_(True)
+    n, rows = count(F.expert_dispatch, x.requires_grad_(True), r)
+    assert n == 2 and count(torch.autograd.grad, rows, x, rows.detach())[0] == 1                              # clear and write; sums
+    # (a function computes the gradients of all inputs that asked for one when it was called)
+    n, out = count(F.expert_combine, y, r._replace(weights=w))
+    assert n == 1 and count(torch.autograd.grad, out, w, out.detach())[0] == 1                                # no rows to clear
+    n, out = count(F.expert_combine, y.requires_grad_(True), r)
+    assert n == 1 and count(torch.autograd.grad, out, y, out.detach())[0] == 2
+    v, b = rand(8, 64, 64, dtype=torch.float16).requires_grad_(True), rand(8, 64, dtype=torch.float16).requires_grad_(True)
+    n, z = count(F.grouped_linear, y, v, r.offsets, b, relu=True)
+    assert n == 1 and count(torch.autograd.grad, z, [y, v, b], z.detach())[0] == 5                            # dz, db, dx, dW in pieces, their sum
+    n, z = count(F.grouped_linear, y, v.detach(), r.offsets)
+    assert n == 1 and count(torch.autograd.grad, z, y, z.detach())[0] == 1
+    base, u = rand(9000, 203, dtype=torch.float16), rand(3, 200, 151, dtype=torch.float16)
+    o = torch.tensor([0, 3000, 4000, 9000], dtype=torch.int32, device="cuda")
+    assert count(F.grouped_linear, base[:, 1:201], u, o)[0] == 4                                              # copies of x and W, product, copy of y
+    weight = rand(64).requires_grad_(True)
+    n, (_, h) = count(F.residual_norm, x, weight=weight.detach())
+    assert n == 1 and count(torch.autograd.grad, h, x, h.detach())[0] == 1
+    n, (_, h) = count(F.residual_norm, x, weight=weight)
+    assert n == 1 and count(torch.autograd.grad, h, [x, weight], h.detach())[0] == 2
