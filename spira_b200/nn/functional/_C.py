@@ -1191,11 +1191,18 @@ POINTWISE_HEAD = True   # 1x1x1 layers with at most 32 output channels run the e
 def pointwise(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """``feats @ weight (+ bias)`` for a 1x1x1 layer with few output channels (``weight`` ``[c_in, c_out]``), or ``None``
     when the layer is outside what ``spira_b200_pointwise`` takes (the caller then uses the library GEMM, like the
-    reference: spira/nn/conv.py:312-316)."""
+    reference: spira/nn/conv.py:312-316, which also reports tensors that do not fit each other)."""
     c_in, c_out = weight.shape
     if not POINTWISE_HEAD or c_out > 32 or c_in % 8 != 0 or c_in < 8 or c_in > 512 or not feats.is_cuda \
             or feats.dtype != torch.float16 or weight.dtype != torch.float16 or (bias is not None and bias.dtype != torch.float16):
         return None
+    # the kernel gets addresses and trusts them: widths that differ, or a weight in another memory, are not for it
+    if len(feats.shape) != 2 or feats.shape[1] != c_in or weight.device != feats.device \
+            or (bias is not None and (bias.device != feats.device or bias.shape != (c_out,))):
+        return None
+    if feats.device.index != torch.cuda.current_device():
+        with torch.cuda.device(feats.device):
+            return pointwise(feats, weight, bias)
     if not feats.is_contiguous():
         feats = feats.contiguous()
     if not weight.is_contiguous():

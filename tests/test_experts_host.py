@@ -122,3 +122,22 @@ def test_paths_call_checks_its_arguments(lib):
     assert lib.spira_b200_grouped_linear_paths(None, paths) != 0
     g.x_stride, g.c_in = 7, 7
     assert lib.spira_b200_grouped_linear_paths(ctypes.byref(g), paths) == 0 and list(paths) == [0, -1, -1, -1]
+
+
+def test_pointwise_leaves_tensors_that_do_not_fit_to_the_library_product(monkeypatch):
+    """Widths that differ, or a weight that was not moved to the device: None before any launch (the kernel would read outside)."""
+    from types import SimpleNamespace
+    from spira_b200 import _lib
+    from spira_b200.nn.functional import _C
+
+    def device_tensor(*shape, index=0):
+        return SimpleNamespace(shape=torch.Size(shape), dtype=torch.float16, is_cuda=True, device=torch.device("cuda", index))
+    monkeypatch.setattr(_lib, "load", lambda: pytest.fail("the library was called"))
+    weight = device_tensor(64, 8)
+    assert _C.pointwise(device_tensor(5, 32), weight, None) is None
+    assert _C.pointwise(device_tensor(5, 72), weight, None) is None
+    assert _C.pointwise(device_tensor(64), weight, None) is None
+    assert _C.pointwise(device_tensor(5, 64), torch.zeros(64, 8, dtype=torch.float16), None) is None
+    assert _C.pointwise(device_tensor(5, 64), device_tensor(64, 8, index=1), None) is None
+    assert _C.pointwise(device_tensor(5, 64), weight, torch.zeros(8, dtype=torch.float16)) is None
+    assert _C.pointwise(device_tensor(5, 64), weight, device_tensor(7)) is None

@@ -375,3 +375,27 @@ def test_launches_are_counted():
     assert n == 1 and count(torch.autograd.grad, h, x, h.detach())[0] == 1
     n, (_, h) = count(F.residual_norm, x, weight=weight)
     assert n == 1 and count(torch.autograd.grad, h, [x, weight], h.detach())[0] == 2
+
+
+# ------------------------------------------------------------------------------------------------ the modules
+def test_router_refuses_tensors_that_do_not_fit():
+    """Features of another width, and weights that were not moved to the device, end in an error and not in a kernel."""
+    import spira_b200 as sp
+    from spira_b200 import nn as spnn
+    moe = spnn.SparseExperts(64, 128, 8).cuda().half()
+    n = 300
+    coords = torch.arange(n, dtype=torch.int32, device="cuda")
+    for c in (32, 72):
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            moe(sp.SparseTensor(coords, rand(n, c, dtype=torch.float16)))
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        spnn.SparseExperts(64, 128, 8).half()(sp.SparseTensor(coords, rand(n, 64, dtype=torch.float16)))
+    with torch.no_grad():
+        x = rand(n, 64, dtype=torch.float16)
+        y = moe(sp.SparseTensor(coords, x))._features
+        head = spnn.SparseConv(64, 8, 1, bias=True).cuda().half()
+        z = head(sp.SparseTensor(coords, x))._features
+        with pytest.raises(RuntimeError):
+            head(sp.SparseTensor(coords, rand(n, 32, dtype=torch.float16)))
+    assert bool(y.isfinite().all()) and bool(z.isfinite().all())
+    torch.cuda.synchronize()
