@@ -19,7 +19,11 @@ from spira_b200.utils.apply import fapply
 class SparseExperts(Module):
     """``out = sum over the voxel's experts e of weight_e * (relu(x W1[e] + b1[e]) W2[e] + b2[e])``, experts and weights from
     ``expert_route(x @ router, top_k)``.  ``forward(inputs, mask)``: voxels where the boolean ``mask [N]`` is False go to no
-    expert and come out as zeros; what they hold (also NaN) shows nowhere.  Weights are laid out like ``SparseConv.kernel``: ``[E, c_in, c_out]``."""
+    expert and come out as zeros; what they hold (also NaN) shows nowhere.  Weights are laid out like ``SparseConv.kernel``: ``[E, c_in, c_out]``.
+
+    Runs in float16 or bfloat16, module and features alike (``module.cuda().half()``).  The router's logits have that type too;
+    for logits of another precision call ``expert_route`` and the functions behind it.  ``compile_model`` replays a network
+    that holds this module operator by operator (the library's tape executor takes convolutions only)."""
 
     def __init__(self, in_channels: int, hidden_channels: int, num_experts: int, top_k: int = 2, out_channels: Optional[int] = None,
                  bias: bool = True, renormalize: bool = True):
@@ -56,6 +60,10 @@ class SparseExperts(Module):
         return torch.mm(feats, self.router)
 
     def _run(self, feats: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        for p in (self.router, self.kernel1, self.kernel2):
+            if feats.dtype not in (torch.float16, torch.bfloat16) or p.dtype != feats.dtype:
+                raise RuntimeError(f"[spira_b200] SparseExperts runs in float16 or bfloat16, module and features alike (module.cuda().half()), "
+                                   f"got features {feats.dtype} and weights {p.dtype}")
         if mask is not None and torch.is_grad_enabled():      # (0 * NaN would reach the router's gradient)
             feats = feats.masked_fill(~mask[:, None], 0)
         logits = self.logits(feats)

@@ -141,3 +141,15 @@ def test_pointwise_leaves_tensors_that_do_not_fit_to_the_library_product(monkeyp
     assert _C.pointwise(device_tensor(5, 64), device_tensor(64, 8, index=1), None) is None
     assert _C.pointwise(device_tensor(5, 64), weight, torch.zeros(8, dtype=torch.float16)) is None
     assert _C.pointwise(device_tensor(5, 64), weight, device_tensor(7)) is None
+
+
+def test_experts_module_says_which_types_it_runs_in():
+    import spira_b200 as sp
+    from spira_b200 import nn as spnn
+    x, coords = torch.zeros(4, 16), torch.arange(4, dtype=torch.int32)
+    for module, feats in ((spnn.SparseExperts(16, 32, 4), x), (spnn.SparseExperts(16, 32, 4), x.half()), (spnn.SparseExperts(16, 32, 4).half(), x),
+                          (spnn.SparseExperts(16, 32, 4).half(), x.bfloat16()), (spnn.SparseExperts(16, 32, 4).double(), x.double())):
+        with pytest.raises(RuntimeError, match="float16 or bfloat16, module and features alike"):
+            module(sp.SparseTensor(coords, feats))
+    with pytest.raises(NotImplementedError, match="CUDA"):
+        spnn.SparseExperts(16, 32, 4).half()(sp.SparseTensor(coords, x.half()))
