@@ -6,7 +6,8 @@
     feats = expert_combine(rows, routing)                      # [N, C_out]
 
 No reference counterpart (the reference stops at convolutions, BatchNorm and ReLU).  All calls run on the current stream
-of their tensors' device, never synchronise, and may be captured into a CUDA graph.  Results do not depend on scheduling:
+of their tensors' device, never synchronise, and may be captured into a CUDA graph (``grouped_linear`` after one call outside
+of it: the device's status word has to exist).  Results do not depend on scheduling:
 the same inputs give the same bits.  Gradients once and in reverse mode only; anything else is refused.
 """
 from __future__ import annotations
@@ -361,7 +362,8 @@ def grouped_linear(feats: torch.Tensor, weights: torch.Tensor, offsets: torch.Te
 
     ``feats [N, C_in]`` and ``weights [E, C_in, C_out]`` are fp16 or bf16 (sums in fp32, one rounding), ``offsets [E + 1]``
     is int32 on the device and is never read by the host; ``bias`` is ``[E, C_out]``.  Groups may be empty; rows outside
-    every group are zero in the result and have no gradient."""
+    every group are zero in the result and have no gradient.  A kernel that gives up on an internal wait raises the device's
+    status word, which ``_C.check_status()`` reports (it synchronises)."""
     index = _device_of(feats, weights, offsets, bias)
     if feats.dim() != 2 or weights.dim() != 3:
         _fail(f"feats is expected to be [N, C_in] and weights [E, C_in, C_out], got {tuple(feats.shape)} and {tuple(weights.shape)}")

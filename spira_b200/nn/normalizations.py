@@ -21,7 +21,8 @@ class ResidualNorm(torch.nn.Module):
     ``stream = residual_scale * inputs + block_scale * gate * p`` with ``p = norm(block)`` if ``post`` else ``block``, and
     ``normed = norm(stream)``.  ``kind`` is ``"rms"`` or ``"layer"`` (then with biases); ``gate=True`` learns one factor per
     channel (initial value ``gate_init``).  Without a block (the first norm of a network) the stream is ``inputs`` itself;
-    ``post``, gate and scales then have nothing to act on and are left out."""
+    ``post``, gate and scales then have nothing to act on and are left out.  ``compile_model`` replays a network that holds this
+    module operator by operator (the library's tape executor takes convolutions only)."""
 
     def __init__(self, channels: int, kind: str = "rms", post: bool = False, gate: bool = False, gate_init: float = 1.0,
                  residual_scale: float = 1.0, block_scale: float = 1.0, eps: float = 1e-6):

@@ -399,3 +399,19 @@ def test_router_refuses_tensors_that_do_not_fit():
             head(sp.SparseTensor(coords, rand(n, 32, dtype=torch.float16)))
     assert bool(y.isfinite().all()) and bool(z.isfinite().all())
     torch.cuda.synchronize()
+
+
+def test_the_readme_runs():
+    """Its Python blocks, one after the other, on a small scene; the modules of the second one train."""
+    import re
+    from helpers import surface
+    blocks = re.findall(r"```python\n(.*?)```", (ROOT / "README.md").read_text(), flags=re.S)
+    assert len(blocks) >= 2 and "SparseExperts" in blocks[1]
+    coords = torch.from_numpy(surface(3, 3000)).cuda()
+    names = {"coords_int32_cuda": coords, "feats_fp16_cuda": rand(len(coords), 4, dtype=torch.float16)}
+    for block in blocks:
+        exec(block, names)
+    stream, h = names["stream"]._features, names["h"]._features
+    assert stream.shape == h.shape == (len(coords), 96) and bool(h.isfinite().all())
+    h.float().square().mean().backward()
+    assert all(p.grad is not None and bool(p.grad.isfinite().all()) for m in ("moe", "last") for p in names[m].parameters())
