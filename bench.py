@@ -459,8 +459,20 @@ def profile_kernels(engine, scene):
     return out, layers
 
 
-# sources that no kernel of the benchmarked workloads includes (the expert and norm operators)
-OTHER_SOURCES = {"elem.cuh", "experts.cu", "grouped.cu", "grouped.cuh", "grouped_tc.cu", "norm.cu"}
+# translation units without a kernel of the benchmarked workloads (the expert and norm operators)
+OTHER_UNITS = {"experts.cu", "grouped.cu", "grouped_tc.cu", "norm.cu"}
+
+
+def kernel_sources(csrc: Path = ROOT / "spira_b200" / "csrc"):
+    """The CUDA sources behind the benchmarked kernels: their translation units and every file of the folder that these include."""
+    import re
+    todo, found = [f for f in csrc.glob("*.cu") if f.name not in OTHER_UNITS], set()
+    while todo:
+        f = todo.pop()
+        if f not in found and f.exists():
+            found.add(f)
+            todo += [csrc / name for name in re.findall(r'^\s*#\s*include\s*"([^"]+)"', f.read_text(), flags=re.M)]
+    return sorted(found)
 
 
 def kernel_source_sha() -> str:
@@ -469,9 +481,7 @@ def kernel_source_sha() -> str:
     import hashlib
     import re
     h = hashlib.sha256()
-    for f in sorted((ROOT / "spira_b200" / "csrc").glob("*.cu*")):
-        if f.name in OTHER_SOURCES:
-            continue
+    for f in kernel_sources():
         text = f.read_text()
         text = re.sub(r"/\*.*?\*/", " ", text, flags=re.S)       # block comments
         text = re.sub(r"//[^\n]*", " ", text)                     # line comments (no string literal of the sources holds "//")

@@ -153,3 +153,14 @@ def test_experts_module_says_which_types_it_runs_in():
             module(sp.SparseTensor(coords, feats))
     with pytest.raises(NotImplementedError, match="CUDA"):
         spnn.SparseExperts(16, 32, 4).half()(sp.SparseTensor(coords, x.half()))
+
+
+def test_traffic_hash_follows_the_includes(tmp_path):
+    """A header that a benchmarked kernel starts to include counts towards the hash of its sources; the operators' units do not."""
+    import bench
+    names = {f.name for f in bench.kernel_sources()}
+    assert {"conv.cu", "common.cuh", "ptx.cuh"} <= names and not names & (bench.OTHER_UNITS | {"elem.cuh", "grouped.cuh"})
+    for name, text in (("conv.cu", '#include "a.cuh"\n#include <cuda.h>\n'), ("a.cuh", '  #  include "elem.cuh"\n'), ("elem.cuh", '#include "a.cuh"\n'),
+                       ("norm.cu", '#include "only.cuh"\n'), ("only.cuh", "")):
+        (tmp_path / name).write_text(text)
+    assert [f.name for f in bench.kernel_sources(tmp_path)] == ["a.cuh", "conv.cu", "elem.cuh"]
