@@ -7,9 +7,9 @@
 //   combine   out[t] = sum_j weights[t][j] * rows[slots[t][j]]
 //
 // Every result is a function of the inputs alone: counts are integers, places follow from counts and ranks, sums run over
-// j in order.  Dispatch and combine are bound by memory (127 363 x 96 fp16, k 2: 12 us = 6.0 TB/s there, 14 us = 5.3 TB/s
-// back), routing by the integer instructions of the selection (127 363 x 64 fp16, k 4: 19.2 us for 24 MB), all of it by
-// the launch for a few rows.
+// j in order.  Dispatch and combine are bound by memory (127 363 x 96 fp16, k 2: 11 us = 6.8 TB/s there, 14 us = 5.3 TB/s
+// back), routing by its two launches, the selection (127 363 x 64 fp16, k 4: 13 us) and the sort (11 us) for 24 MB, all of it
+// by the launch for a few rows.
 #include <atomic>
 #include <cfloat>
 #include <cmath>

@@ -18,9 +18,9 @@
 // memory.  Every CTA reads the group boundaries once into shared memory.  Every wait is bounded; an expired one raises the
 // status word.
 //
-// Measured: 254 726 rows in 8 groups 96 -> 384 fp16 with bias and ReLU 60 us: its 196 MB of results alone take 52 us at the
-// 3.8 TB/s at which this memory takes writes; 80 026 rows in 16 groups 512 -> 2048 bf16: forward with bias, ReLU and mask
-// 147 us, dx 106 us = 1590 TFLOP/s, dW 128 us (one dense library product of the size: 135, 109, 118 us).
+// Measured one at a time behind an L2 flush: 254 726 rows in 8 groups 96 -> 384 fp16 with bias 61 us (a fill of its
+// 196 MB of results alone: 53 us); 80 026 rows in 16 groups 512 -> 2048 bf16: forward with bias, ReLU and mask 162 us, dx
+// 119 us = 1410 TFLOP/s, dW 136 us (one dense library product of the size on the same board: 139, 115, 126).
 #include <cuda.h>
 
 #include <type_traits>

@@ -11,9 +11,9 @@
 // cancellation).  The backward pass reads x, block and the gate again and rebuilds the stream in fp32 from them and from
 // the saved row statistics, so it needs neither output of the forward pass.  Parameter gradients are column sums: a thread
 // owns its columns for all rows its CTA visits, CTAs write partial sums, a second launch adds those in a fixed order.
-// Bound by memory and instructions together: forward 2 row reads + 2 row writes, backward 4 + 2 (one more of each with a
-// gate per element).  127 363 x 256 bf16, layer norms on both sides, a gate per element, fp32 parameters: forward 62 us =
-// 5.3 TB/s, backward 107 us = 4.9 TB/s; 127 363 x 96 fp16 with one rms norm: 22 us = 4.4 TB/s.
+// Bound by memory and by the latency of a row's chain at the warps that registers leave room for: forward 2 row reads + 2 row writes, backward 4 + 2 (one more of each with a
+// gate per element).  127 363 x 256 bf16, layer norms on both sides, a gate per element, fp32 parameters: forward 60 us =
+// 5.4 TB/s, backward 105 us = 5.0 TB/s; 127 363 x 96 fp16 with one rms norm: 20 us = 4.9 TB/s.
 #include "common.cuh"
 #include "elem.cuh"
 #include "ptx.cuh"

@@ -361,7 +361,7 @@ def grouped_linear(feats: torch.Tensor, weights: torch.Tensor, offsets: torch.Te
     """``relu?(feats[r] @ weights[e] + bias[e])`` for the rows ``offsets[e] <= r < offsets[e + 1]`` of every expert ``e``.
 
     ``feats [N, C_in]`` and ``weights [E, C_in, C_out]`` are fp16 or bf16 (sums in fp32, one rounding), ``offsets [E + 1]``
-    is int32 on the device and is never read by the host; ``bias`` is ``[E, C_out]``.  Groups may be empty; rows outside
+    is int32 on the device and is never read by the host; ``bias`` is ``[E, C_out]``; ``E <= 1024``, channels up to 65 536.  Groups may be empty; rows outside
     every group are zero in the result and have no gradient.  A kernel that gives up on an internal wait raises the device's
     status word, which ``_C.check_status()`` reports (it synchronises)."""
     index = _device_of(feats, weights, offsets, bias)

@@ -99,9 +99,10 @@ def residual_norm(feats: torch.Tensor, block: Optional[torch.Tensor] = None, *, 
     with ``pre=False``).
 
     ``norm`` is ``v / sqrt(mean(v^2) + eps)`` for ``kind="rms"``, ``(v - mean) / sqrt(var + eps)`` for ``kind="layer"``, in
-    fp32 on the unrounded stream.  ``feats`` and ``block`` are ``[N, C]`` in fp16, bf16 or fp32, ``C <= 8192``; ``gate`` is a
-    parameter ``[C]``, or ``[N, 1]`` or ``[N, C]`` in the type of ``feats``.  Parameters are all fp32 or all of the type of
-    ``feats``; a missing one counts as ones (weights) or zeros (biases).  The two scales are constants."""
+    fp32 on the unrounded stream.  ``feats`` and ``block`` are ``[N, C]`` in fp16, bf16 or fp32, ``C <= 8192`` (rows
+    less than 2^31 elements apart); ``gate`` is a parameter ``[C]``, or ``[N, 1]`` or ``[N, C]`` in the type of ``feats``.
+    Parameters are all fp32 or all of the type of ``feats``; a missing one counts as ones (weights) or zeros (biases).  The two
+    scales are constants."""
     _device_of(feats, block, weight, bias, post_weight, post_bias, gate)
     if feats.dim() != 2 or feats.dtype not in _DTYPES:
         _fail(f"Tensor feats is expected to be a float16, bfloat16 or float32 matrix [N, C], got {feats.dtype} {tuple(feats.shape)}")
