@@ -509,11 +509,12 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const T *logits, in
 struct MoveParams {
   const void *x, *y;
   const float *weights;
-  const int32_t *slots, *offsets;
+  const int32_t *slots, *offsets, *order;
   void *out;
   float *dweights;
   int64_t n, x_stride, y_stride, w_row, w_col;
   int channels, k, experts;
+  int clear, clear_here;             // rows of places that no slot names are cleared / by the one CTA that writes the rows
   int64_t rows_per_launch_row;       // rows of one blockIdx.y: rows * pieces stays below 2^31
   uint64_t div_mul;                  // i / pieces = (i * div_mul) >> div_shift for 0 <= i < 2^31
   int div_shift;
@@ -530,17 +531,14 @@ __device__ __forceinline__ void zero_tail(const MoveParams &P, T *rows, int vecs
     store_f32<T, V>(rows + (tail + i / vecs) * P.channels + (i % vecs) * V, zero);
 }
 
-// Places that no slot names, in a launch of its own before the rows are written: `order` says which pair a place belongs to, and
-// a place whose pair says the same needs nothing.  All others get zeros, so whatever `order` holds (it may be older than
-// the slots, or absent) costs writes and never a wrong row.  A warp looks at 32 places; their rows are neighbours.  Bound by two
-// dependent loads (127 363 x 96 fp16, k 2: 27.9 -> 29.5 us for dispatch and combine together).
+// Zeros for the places that no slot names, before the rows are written: `order` says which pair a place belongs to, and a place
+// whose pair says the same needs nothing.  All others get zeros, so whatever `order` holds (it may be older than the
+// slots, or absent) costs writes and never a wrong row.  A warp looks at 32 places, whose rows are neighbours.
 template <int BYTES>
-__global__ void __launch_bounds__(256) clear_kernel(const int32_t *slots, const int32_t *order, int64_t total, int64_t row_bytes, unsigned char *rows) {
+__device__ __forceinline__ void clear_places(const int32_t *slots, const int32_t *order, int64_t total, int64_t row_bytes, unsigned char *rows, int64_t p0) {
   typedef typename std::conditional<BYTES == 16, uint4, typename std::conditional<BYTES == 4, uint32_t, unsigned short>::type>::type Word;
-  pdl_trigger();
-  pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t p0 = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) & ~static_cast<int64_t>(31), p = p0 + lane;
+  const int64_t p = p0 + lane;
   bool named = p >= total;
   if (!named && order) {
     const int32_t pair = order[p];
@@ -559,6 +557,22 @@ __global__ void __launch_bounds__(256) clear_kernel(const int32_t *slots, const 
   }
 }
 
+// In a launch of its own (bound by two dependent loads: 3.5 us for 254 726 places), or, where the rows are written by one CTA,
+// in that CTA (few rows: dispatch 9.7 us at the host, 12.1 with two launches).
+template <int BYTES>
+__global__ void __launch_bounds__(256) clear_kernel(const int32_t *slots, const int32_t *order, int64_t total, int64_t row_bytes, unsigned char *rows) {
+  pdl_trigger();
+  pdl_wait();
+  clear_places<BYTES>(slots, order, total, row_bytes, rows, (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) & ~static_cast<int64_t>(31));
+}
+template <typename T, int V>
+__device__ __forceinline__ void clear_here(const MoveParams &P) {
+  const int64_t total = P.n * P.k;
+  for (int64_t p0 = threadIdx.x & ~31u; p0 < total; p0 += 256)
+    clear_places<V * static_cast<int>(sizeof(T))>(P.slots, P.order, total, P.channels * static_cast<int64_t>(sizeof(T)), static_cast<unsigned char *>(P.out), p0);
+  __syncthreads();
+}
+
 // The row and the first channel of a thread; false behind the last row.
 template <int V>
 __device__ __forceinline__ bool my_piece(const MoveParams &P, int64_t &row, int &c) {
@@ -574,6 +588,7 @@ template <typename T, int V, int K>
 __global__ void __launch_bounds__(256) dispatch_kernel(const MoveParams P) {
   pdl_trigger();
   pdl_wait();
+  if (P.clear_here) clear_here<T, V>(P);
   const int64_t total = P.n * P.k;
   T *rows = static_cast<T *>(P.out);
   int64_t row;
@@ -629,6 +644,7 @@ template <typename T, int V, int G>
 __global__ void __launch_bounds__(256) combine_backward_kernel(const MoveParams P) {
   pdl_trigger();
   pdl_wait();
+  if (P.clear_here) clear_here<T, V>(P);
   const int g = threadIdx.x & (G - 1);
   const int vecs = P.channels / V;
   constexpr int kRows = 256 / G;
@@ -761,6 +777,22 @@ static bool rows_aligned(const void *p, int64_t stride, int size) {
   return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0);
 }
 
+// For `ctas` CTAs that write the rows: by that one CTA, or by a launch before them.
+static int launch_clear(MoveParams &P, int64_t ctas, int size, cudaStream_t st) {
+  if (!P.clear || !P.out) return SPIRA_B200_OK;
+  if (ctas == 1) {
+    P.clear_here = 1;
+    return SPIRA_B200_OK;
+  }
+  const int64_t total = P.n * P.k, row_bytes = static_cast<int64_t>(P.channels) * size;
+  const dim3 grid(static_cast<unsigned>(div_up(total, 256)));
+  unsigned char *rows = static_cast<unsigned char *>(P.out);
+  if (rows_aligned(rows, P.channels, size)) SB_CHECK_CUDA(launch_operator(clear_kernel<16>, grid, dim3(256), 0, st, P.slots, P.order, total, row_bytes, rows));
+  else if (size == 4) SB_CHECK_CUDA(launch_operator(clear_kernel<4>, grid, dim3(256), 0, st, P.slots, P.order, total, row_bytes, rows));
+  else SB_CHECK_CUDA(launch_operator(clear_kernel<2>, grid, dim3(256), 0, st, P.slots, P.order, total, row_bytes, rows));
+  return SPIRA_B200_OK;
+}
+
 template <typename T, int V>
 static int launch_move(MoveParams &P, bool combine, cudaStream_t st) {
   const int64_t pieces = P.channels / V;
@@ -772,6 +804,10 @@ static int launch_move(MoveParams &P, bool combine, cudaStream_t st) {
   P.div_mul = ((uint64_t(1) << P.div_shift) + pieces - 1) / pieces;
   const dim3 grid(static_cast<unsigned>(div_up(P.rows_per_launch_row * pieces, 256)), static_cast<unsigned>(div_up(P.n, P.rows_per_launch_row)));
   SB_CHECK_ARG(grid.y < 65536, "too many rows x channels");
+  if (!combine) {
+    const int rc = launch_clear(P, static_cast<int64_t>(grid.x) * grid.y, sizeof(T), st);
+    if (rc != SPIRA_B200_OK) return rc;
+  }
   auto go = [&](auto kernel) -> int {
     SB_CHECK_CUDA(launch_operator(kernel, grid, dim3(256), 0, st, P));
     return SPIRA_B200_OK;
@@ -781,7 +817,7 @@ static int launch_move(MoveParams &P, bool combine, cudaStream_t st) {
 }
 
 template <typename T, int V>
-static int launch_combine_backward(const MoveParams &P, cudaStream_t st) {
+static int launch_combine_backward(MoveParams &P, cudaStream_t st) {
   const int vecs = P.channels / V;
   // as many lanes as the row has pieces, half of them where the rows fill the SMs all the same: two pieces per lane are in
   // flight together (127 363 x 96, k 2: 28 instead of 33 us; 20 000 x 64, k 8: 13 with all lanes, 20 us with half).  No
@@ -789,6 +825,8 @@ static int launch_combine_backward(const MoveParams &P, cudaStream_t st) {
   int lanes = vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
   if (lanes > 4 && vecs <= 32 && P.n * (lanes / 2) >= 4 * 256 * static_cast<int64_t>(sm_count())) lanes /= 2;
   const unsigned blocks = capped_blocks(P.n * lanes, 256, 8);
+  const int rc = launch_clear(P, blocks, sizeof(T), st);
+  if (rc != SPIRA_B200_OK) return rc;
   if (lanes == 4) SB_CHECK_CUDA(launch_operator(combine_backward_kernel<T, V, 4>, dim3(blocks), dim3(256), 0, st, P));
   else if (lanes == 8) SB_CHECK_CUDA(launch_operator(combine_backward_kernel<T, V, 8>, dim3(blocks), dim3(256), 0, st, P));
   else if (lanes == 16) SB_CHECK_CUDA(launch_operator(combine_backward_kernel<T, V, 16>, dim3(blocks), dim3(256), 0, st, P));
@@ -796,22 +834,8 @@ static int launch_combine_backward(const MoveParams &P, cudaStream_t st) {
   return SPIRA_B200_OK;
 }
 
-static int launch_clear(const MoveParams &P, const int32_t *order, int size, cudaStream_t st) {
-  const int64_t total = P.n * P.k, row_bytes = static_cast<int64_t>(P.channels) * size;
-  const dim3 grid(static_cast<unsigned>(div_up(total, 256)));
-  unsigned char *rows = static_cast<unsigned char *>(P.out);
-  if (rows_aligned(rows, P.channels, size)) SB_CHECK_CUDA(launch_operator(clear_kernel<16>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
-  else if (size == 4) SB_CHECK_CUDA(launch_operator(clear_kernel<4>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
-  else SB_CHECK_CUDA(launch_operator(clear_kernel<2>, grid, dim3(256), 0, st, P.slots, order, total, row_bytes, rows));
-  return SPIRA_B200_OK;
-}
-
-static int run_dispatch(MoveParams &P, int dtype, bool clear, const int32_t *order, cudaStream_t st) {
+static int run_dispatch(MoveParams &P, int dtype, cudaStream_t st) {
   const int size = elem_size(dtype);
-  if (clear) {
-    const int rc = launch_clear(P, order, size, st);
-    if (rc != SPIRA_B200_OK) return rc;
-  }
   const bool wide = P.channels * size % 16 == 0 && rows_aligned(P.x, P.x_stride, size) && rows_aligned(P.out, P.channels, size);
   return SB_DISPATCH_ELEM(dtype, T, {
     if (wide) return launch_move<T, 16 / static_cast<int>(sizeof(T))>(P, false, st);
@@ -819,12 +843,8 @@ static int run_dispatch(MoveParams &P, int dtype, bool clear, const int32_t *ord
   });
 }
 
-static int run_combine_backward(const MoveParams &P, int dtype, bool clear, const int32_t *order, cudaStream_t st) {
+static int run_combine_backward(MoveParams &P, int dtype, cudaStream_t st) {
   const int size = elem_size(dtype);
-  if (clear && P.out) {
-    const int rc = launch_clear(P, order, size, st);
-    if (rc != SPIRA_B200_OK) return rc;
-  }
   const bool wide = P.channels * size % 16 == 0 && rows_aligned(P.y, P.y_stride, size) && rows_aligned(P.x, P.x_stride, size) &&
                     rows_aligned(P.out, P.channels, size);
   return SB_DISPATCH_ELEM(dtype, T, {
@@ -899,18 +919,18 @@ extern "C" int spira_b200_expert_dispatch(const void *x, int dtype, int64_t n, i
   int rc = check_move("expert_dispatch", P, dtype, x_stride, 0);
   if (rc != SPIRA_B200_OK || n == 0) return rc;
   SB_CHECK_ARG(x && slots && offsets && rows && experts >= 1, "expert_dispatch: null pointer");
-  return run_dispatch(P, dtype, false, nullptr, as_stream(stream));
+  return run_dispatch(P, dtype, as_stream(stream));
 }
 
 extern "C" int spira_b200_expert_dispatch_cleared(const void *x, int dtype, int64_t n, int64_t x_stride, int channels, const int32_t *slots,
                                                   const int32_t *order, int k, void *rows, void *stream) {
   MoveParams P{};
-  P.x = x; P.slots = slots; P.out = rows;
+  P.x = x; P.slots = slots; P.order = order; P.out = rows; P.clear = 1;
   P.n = n; P.x_stride = x_stride; P.channels = channels; P.k = k;
   int rc = check_move("expert_dispatch_cleared", P, dtype, x_stride, 0);
   if (rc != SPIRA_B200_OK || n == 0) return rc;
   SB_CHECK_ARG(x && slots && rows, "expert_dispatch_cleared: null pointer");
-  return run_dispatch(P, dtype, true, order, as_stream(stream));
+  return run_dispatch(P, dtype, as_stream(stream));
 }
 
 extern "C" int spira_b200_expert_combine(const void *rows, int dtype, int64_t n, int64_t row_stride, int channels, const float *weights,
@@ -941,7 +961,7 @@ extern "C" int spira_b200_expert_combine_backward(const void *rows, const void *
   int rc = check_move("expert_combine_backward", P, dtype, row_stride, dout_stride);
   if (rc != SPIRA_B200_OK || n == 0) return rc;
   SB_CHECK_ARG(dout && slots && offsets && experts >= 1 && (rows || !dweights) && (drows || dweights), "expert_combine_backward: null pointer");
-  return run_combine_backward(P, dtype, false, nullptr, as_stream(stream));
+  return run_combine_backward(P, dtype, as_stream(stream));
 }
 
 extern "C" int spira_b200_expert_combine_backward_cleared(const void *rows, const void *dout, int dtype, int64_t n, int64_t row_stride,
@@ -949,11 +969,11 @@ extern "C" int spira_b200_expert_combine_backward_cleared(const void *rows, cons
                                                           int64_t weights_col, const int32_t *slots, const int32_t *order, int k, void *drows,
                                                           float *dweights, void *stream) {
   MoveParams P{};
-  P.x = dout; P.y = rows; P.weights = weights; P.slots = slots; P.out = drows; P.dweights = dweights;
+  P.x = dout; P.y = rows; P.weights = weights; P.slots = slots; P.order = order; P.out = drows; P.dweights = dweights; P.clear = 1;
   P.n = n; P.x_stride = dout_stride; P.y_stride = row_stride; P.w_row = weights_row; P.w_col = weights_col;
   P.channels = channels; P.k = k;
   int rc = check_move("expert_combine_backward_cleared", P, dtype, row_stride, dout_stride);
   if (rc != SPIRA_B200_OK || n == 0) return rc;
   SB_CHECK_ARG(dout && slots && (rows || !dweights) && (drows || dweights), "expert_combine_backward_cleared: null pointer");
-  return run_combine_backward(P, dtype, true, order, as_stream(stream));
+  return run_combine_backward(P, dtype, as_stream(stream));
 }

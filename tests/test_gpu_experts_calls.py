@@ -415,3 +415,24 @@ def test_the_readme_runs():
     assert stream.shape == h.shape == (len(coords), 96) and bool(h.isfinite().all())
     h.float().square().mean().backward()
     assert all(p.grad is not None and bool(p.grad.isfinite().all()) for m in ("moe", "last") for p in names[m].parameters())
+
+
+def test_few_rows_are_cleared_and_written_in_one_launch():
+    """21 rows of 96 channels are the work of one CTA (256 pieces of 16 bytes), 22 are not; the rows are right on both sides."""
+    from spira_b200 import _lib
+    from spira_b200.nn import functional as F
+    c, k = 96, 2
+    for n, launches in ((1, 1), (21, 1), (22, 2)):
+        r = F.expert_route(rand(n, 4), k)
+        slots = r.slots.clone()
+        slots[n // 2, 0] = -1
+        x = whole(n, c, dtype=torch.float16)
+        stale_memory(n * k, c, torch.float16)
+        before = _lib.launches()
+        rows = F.expert_dispatch(x, r._replace(slots=slots))
+        assert _lib.launches() - before == launches
+        want = torch.zeros_like(rows)
+        for j in range(k):
+            t = (slots[:, j] >= 0).nonzero()[:, 0]
+            want[slots[t, j].long()] = x[t]
+        assert torch.equal(rows, want)
